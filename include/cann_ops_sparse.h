@@ -381,6 +381,78 @@ aclsparseStatus_t aclsparseSpMMOp_setGlobalUserData(aclsparseHandle_t handle, ac
 aclsparseStatus_t aclsparseSpMMOp(aclsparseHandle_t handle, aclsparseSpMMOpPlan_t plan, const void* alpha,
                                   const void* beta, aclsparseConstDnMatDescr_t matB, aclsparseDnMatDescr_t matC);
 
+/* ---------------- Experts' operators (no counterpart in the reference) ----------------
+ *
+ * The products of a layer whose tokens each choose k of a number of experts.
+ * The choice is a CSR matrix of k entries per row, kept as arrays of int32:
+ *   ids[t*k + j]       the j-th choice of token t (-1: none)
+ *   offsets[e]         first row of expert e among the assignments sorted by
+ *                      expert, offsets[experts] their number: the column
+ *                      pointers of the matrix's CSC form
+ *   rowTokens[r]       the token of sorted row r (-1 past the last)
+ *   places[t*k + j]    the sorted row of assignment (t, j), or -1
+ * All arrays are in device memory and are read when the work runs on the
+ * handle's stream; no call waits, allocates or copies to the host, so every
+ * call may be captured in a HIP graph.  Results do not change from run to run.
+ * Matrices are row by row; a leading dimension counts elements.
+ */
+
+/* Bytes of the buffer that aclsparseRoute and aclsparseExpertPlan work in (calls that share one must not overlap). */
+aclsparseStatus_t aclsparseRoute_bufferSize(aclsparseHandle_t handle, int64_t tokens, int64_t experts, int64_t k,
+                                            size_t* bufferSize);
+/* The k largest logits of each row (ties: the lowest index; -inf is never chosen, NaN counts as the largest), their
+ * weights w_j = exp(l_j - max) / sum, the sum over the chosen (normalize != 0) or over the row, and the plan above.
+ * logits: ACL_FLOAT, ACL_FLOAT16 or ACL_BF16; experts <= 1024, k <= 64. */
+aclsparseStatus_t aclsparseRoute(aclsparseHandle_t handle, int64_t tokens, int64_t experts, int64_t k,
+                                 const void* logits, int64_t ldLogits, aclDataType logitsType, int32_t normalize,
+                                 float* weights, int32_t* ids, int32_t* offsets, int32_t* rowTokens, int32_t* places,
+                                 void* buffer);
+/* The plan of a given choice; ids outside [0, experts) are assignments that are dropped. */
+aclsparseStatus_t aclsparseExpertPlan(aclsparseHandle_t handle, int64_t tokens, int64_t experts, int64_t k,
+                                      const int32_t* ids, int32_t* offsets, int32_t* rowTokens, int32_t* places,
+                                      void* buffer);
+/* Gradient of aclsparseRoute's weights with respect to the logits, in their type; logits may be null when
+ * normalize != 0. */
+aclsparseStatus_t aclsparseRouteGrad(aclsparseHandle_t handle, int64_t tokens, int64_t experts, int64_t k,
+                                     const void* logits, int64_t ldLogits, aclDataType logitsType, int32_t normalize,
+                                     const float* weights, const int32_t* ids, const float* gradWeights,
+                                     void* gradLogits, int64_t ldGrad);
+/* C_r = A_i(r) op(B_g) for the rows r in [offsets[g], offsets[g+1]) of every group g, i(r) = rowIndex[r] (rowIndex
+ * null: i(r) = r), and C_r = 0 for rows past offsets[groups]; offsets null: one group of all rows.  op(B_g) is k x n:
+ * ACL_SPARSE_OP_NON_TRANSPOSE takes B_g [k, n], ACL_SPARSE_OP_TRANSPOSE takes B_g [n, k]; B_g starts strideB elements
+ * after B_(g-1).  A and B ACL_FLOAT16 or ACL_BF16, C their type or ACL_FLOAT; sums in fp32.  offsets start at 0 and do
+ * not decrease and indices lie in [0, rowsA): others give values without meaning, never an access outside the
+ * operands. */
+aclsparseStatus_t aclsparseGroupedMM(aclsparseHandle_t handle, aclsparseOperation_t opB, int64_t groups, int64_t rows,
+                                     int64_t n, int64_t k, const int32_t* offsets, const int32_t* rowIndex,
+                                     int64_t rowsA, const void* A, int64_t lda, const void* B, int64_t ldb,
+                                     int64_t strideB, aclDataType abType, void* C, int64_t ldc, aclDataType cType);
+/* W_g = sum over the rows r of group g of gradC_r^T X_i(r), [n, k] each (zero for an empty group): the gradient of
+ * aclsparseGroupedMM with ACL_SPARSE_OP_TRANSPOSE with respect to B. */
+aclsparseStatus_t aclsparseGroupedMMGrad(aclsparseHandle_t handle, int64_t groups, int64_t rows, int64_t n, int64_t k,
+                                         const int32_t* offsets, const int32_t* rowIndex, int64_t rowsX,
+                                         const void* gradC, int64_t ldg, const void* X, int64_t ldx, aclDataType type,
+                                         void* W, int64_t ldw, int64_t strideW, aclDataType wType);
+/* aclsparseGroupedMM with ACL_SPARSE_OP_TRANSPOSE on 8-bit integers: C_r[n] = scaleA[i(r)] * scaleB[g*N + n] * (the
+ * exact integer product), N the n given; k <= 131071.  C ACL_FLOAT, ACL_FLOAT16 or ACL_BF16. */
+aclsparseStatus_t aclsparseGroupedMMScaled(aclsparseHandle_t handle, int64_t groups, int64_t rows, int64_t n,
+                                           int64_t k, const int32_t* offsets, const int32_t* rowIndex, int64_t rowsA,
+                                           const int8_t* A, int64_t lda, const float* scaleA, const int8_t* B,
+                                           int64_t ldb, int64_t strideB, const float* scaleB, void* C, int64_t ldc,
+                                           aclDataType cType);
+/* out_t = sum_j weights[t*k + j] * Y[places[t*k + j]] (weights null: ones; places outside [0, rows) add nothing),
+ * summed in fp32.  out ACL_FLOAT16 or ACL_BF16, Y its type or ACL_FLOAT. */
+aclsparseStatus_t aclsparseCombine(aclsparseHandle_t handle, int64_t tokens, int64_t k, int64_t width, int64_t rows,
+                                   const int32_t* places, const float* weights, const void* Y, int64_t ldy,
+                                   aclDataType yType, void* out, int64_t ldOut, aclDataType outType);
+/* gradY[places[t*k + j]] = weights[t*k + j] * gradOut_t, zero for the rows past offsets[groups], and
+ * gradWeights[t*k + j] = <gradOut_t, Y[places[t*k + j]]>; either may be null when it is not wanted. */
+aclsparseStatus_t aclsparseCombineGrad(aclsparseHandle_t handle, int64_t tokens, int64_t k, int64_t width,
+                                       int64_t rows, int64_t groups, const int32_t* offsets, const int32_t* places,
+                                       const float* weights, const void* Y, int64_t ldy, const void* gradOut,
+                                       int64_t ldOut, aclDataType type, void* gradY, int64_t ldGradY,
+                                       float* gradWeights);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,134 @@
+// Device helpers of the experts' kernels: 16-bit types, sums and maxima over
+// a 64-lane wave, and the search of a tile's group.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace aclsp {
+
+using Half = _Float16;
+using Bf16 = __bf16;
+
+template <typename T>
+__device__ __forceinline__ float ToFloat(T v)
+{
+    return static_cast<float>(v);
+}
+// Rounds to nearest even (one instruction for bfloat16 on gfx950).
+template <typename T>
+__device__ __forceinline__ T FromFloat(float v)
+{
+    return static_cast<T>(v);
+}
+
+// Moves within a wave by DPP: lanes that have no source keep `old`.
+template <int kCtrl, int kRowMask>
+__device__ __forceinline__ uint32_t Dpp(uint32_t old, uint32_t v)
+{
+    return static_cast<uint32_t>(
+        __builtin_amdgcn_update_dpp(static_cast<int>(old), static_cast<int>(v), kCtrl, kRowMask, 0xF, false));
+}
+constexpr int kDppShr1 = 0x111, kDppShr2 = 0x112, kDppShr4 = 0x114, kDppShr8 = 0x118;
+constexpr int kDppBcast15 = 0x142, kDppBcast31 = 0x143;
+
+// Inclusive scan over the wave: within rows of 16 lanes, then row 15 -> next, then lane 31 -> upper half.
+template <typename F>
+__device__ __forceinline__ uint32_t WaveScan(uint32_t x, uint32_t identity, F op)
+{
+    x = op(x, Dpp<kDppShr1, 0xF>(identity, x));
+    x = op(x, Dpp<kDppShr2, 0xF>(identity, x));
+    x = op(x, Dpp<kDppShr4, 0xF>(identity, x));
+    x = op(x, Dpp<kDppShr8, 0xF>(identity, x));
+    x = op(x, Dpp<kDppBcast15, 0xA>(identity, x));
+    x = op(x, Dpp<kDppBcast31, 0xC>(identity, x));
+    return x;
+}
+
+__device__ __forceinline__ uint32_t LastLane(uint32_t x)
+{
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), 63));
+}
+
+__device__ __forceinline__ uint32_t WaveMaxU32(uint32_t x)
+{
+    return LastLane(WaveScan(x, 0U, [](uint32_t a, uint32_t b) { return a > b ? a : b; }));
+}
+
+__device__ __forceinline__ int32_t WaveInclusiveSum(int32_t x)
+{
+    return static_cast<int32_t>(WaveScan(static_cast<uint32_t>(x), 0U, [](uint32_t a, uint32_t b) { return a + b; }));
+}
+
+__device__ __forceinline__ float WaveSum(float x)
+{
+    return __uint_as_float(LastLane(WaveScan(__float_as_uint(x), 0U, [](uint32_t a, uint32_t b) {
+        return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+    })));
+}
+
+__device__ __forceinline__ float WaveMax(float x)
+{
+    return __uint_as_float(LastLane(WaveScan(__float_as_uint(x), 0xFF800000U, [](uint32_t a, uint32_t b) {
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    })));
+}
+
+// Rows [begin, end) of a group, whatever the offsets hold: within [0, rows] and not negative in length.
+__device__ __forceinline__ void GroupRows(const int32_t* offsets, int64_t rows, int group, int32_t& begin, int32_t& end)
+{
+    if (offsets == nullptr) {
+        begin = 0;
+        end = static_cast<int32_t>(rows);
+        return;
+    }
+    const int32_t r = static_cast<int32_t>(rows);
+    const int32_t b = offsets[group], e = offsets[group + 1];
+    begin = b < 0 ? 0 : b > r ? r : b;
+    end = e < begin ? begin : e > r ? r : e;
+}
+
+// A tile of a ragged product: rows [row, end) of `group`; group == groups is
+// the tail of rows that belong to no group, group < 0 no tile.
+struct RaggedTile {
+    int32_t group;
+    int32_t row;
+    int32_t end;
+    int32_t tiles;  // of all groups
+};
+
+// The tile-th tile of `height` rows, counted through the groups and the tail.
+// Called by whole waves with a uniform tile; 64 groups a turn.
+__device__ __forceinline__ RaggedTile FindTile(const int32_t* offsets, int64_t rows, int64_t groups, int32_t height,
+                                               int32_t tile)
+{
+    const int lane = threadIdx.x & 63;
+    const int32_t all = static_cast<int32_t>(groups) + 1;
+    RaggedTile t{-1, 0, 0, 0};
+    for (int32_t g0 = 0; g0 < all; g0 += 64) {
+        const int32_t g = g0 + lane;
+        int32_t begin = 0, end = 0;
+        if (g < all - 1) {
+            GroupRows(offsets, rows, g, begin, end);
+        } else if (g == all - 1 && offsets != nullptr) {
+            int32_t unused;
+            GroupRows(offsets, rows, g - 1, unused, begin);
+            end = static_cast<int32_t>(rows);
+        }
+        const int32_t n = (end - begin + height - 1) / height;
+        const int32_t incl = WaveInclusiveSum(n);
+        const uint64_t hit = __ballot(t.tiles + incl > tile);
+        if (t.group < 0 && hit != 0) {
+            const int src = __builtin_ctzll(hit);
+            t.group = g0 + src;
+            const int32_t before = t.tiles + __builtin_amdgcn_readlane(incl - n, src);
+            t.row = __builtin_amdgcn_readlane(begin, src) + (tile - before) * height;
+            t.end = __builtin_amdgcn_readlane(end, src);
+        }
+        t.tiles += __builtin_amdgcn_readlane(incl, 63);
+    }
+    return t;
+}
+
+}  // namespace aclsp

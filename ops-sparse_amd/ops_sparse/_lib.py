@@ -176,6 +176,19 @@ SIGNATURES = {
     "aclsparseSpMMOp_destroyPlan": [_vp],
     "aclsparseSpMMOp_setGlobalUserData": [_vp, _vp, ctypes.c_char_p, _vp, _sz],
     "aclsparseSpMMOp": [_vp, _vp, _vp, _vp, _vp, _vp],
+    "aclsparseRoute_bufferSize": [_vp, _i64, _i64, _i64, ctypes.POINTER(_sz)],
+    "aclsparseRoute": [_vp, _i64, _i64, _i64, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp],
+    "aclsparseExpertPlan": [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp],
+    "aclsparseRouteGrad": [_vp, _i64, _i64, _i64, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _i64],
+    "aclsparseGroupedMM": [_vp, _i32, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _vp,
+                           _i64, _i32],
+    "aclsparseGroupedMMGrad": [_vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _vp, _i64,
+                               _i64, _i32],
+    "aclsparseGroupedMMScaled": [_vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _vp,
+                                 _vp, _i64, _i32],
+    "aclsparseCombine": [_vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i32, _vp, _i64, _i32],
+    "aclsparseCombineGrad": [_vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i32, _vp, _i64,
+                             _vp],
 }
 
 _LIB = None

@@ -1,0 +1,667 @@
+"""The experts' operators on the GPU against plain implementations in 64 bits.
+
+Tolerances follow from the arithmetic: a sum of n products in fp32 is off by at most (n + 1) * 2^-24 times the sum of
+the products' magnitudes, and the result is rounded once to a type of p significant bits (2^-p relative, 2^-11 for
+float16 and 2^-8 for bfloat16; float16 results below its normal range by up to 2^-25).  Integers are exact.
+"""
+import numpy as np
+import pytest
+import torch
+
+from ops_sparse import ExpertPlan, combine, expert_plan, grouped_mm, grouped_mm_scaled, route
+
+pytestmark = pytest.mark.gpu
+
+U32 = 2.0**-24
+U = {torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8, torch.float32: U32}
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+def close(got, want, magnitude, terms):
+    """got against want (float64), a sum of `terms` products whose magnitudes sum to `magnitude`."""
+    assert got.shape == want.shape
+    bound = U[got.dtype] * want.abs() + (terms + 1) * U32 * magnitude * (1 + U[got.dtype]) + 2.0**-25
+    err = (got.double() - want).abs()
+    bad = ~(err <= bound)
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} off, worst by {float((err / bound).max()):.3g} bounds"
+
+
+def gen(seed, device="cuda"):
+    g = torch.Generator(device=device)
+    g.manual_seed(seed)
+    return g
+
+
+def lengths_to_plan(lens, tail=0, tokens=None, seed=0):
+    """offsets of the given lengths, and `tail` rows past the last group; with tokens, a drawn gather index."""
+    off = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device="cuda")
+    rows = int(off[-1]) + tail
+    idx = None
+    if tokens is not None:
+        idx = torch.randint(0, tokens, (rows,), generator=gen(seed), device="cuda", dtype=torch.int32)
+        if tail:
+            idx[-tail:] = -1
+    return ExpertPlan(off, idx, None), rows
+
+
+def strided(shape, dtype, seed, pad, scale=1.0, offset=0):
+    """Random values in rows longer than they need be, NaN (or -128) between them."""
+    full = list(shape[:-1]) + [shape[-1] + pad]
+    n = int(np.prod(full)) + offset
+    if dtype == torch.int8:
+        buf = torch.full((n,), -128, dtype=dtype, device="cuda")
+        v = torch.randint(-127, 128, shape, generator=gen(seed), device="cuda", dtype=torch.int8)
+    else:
+        buf = torch.full((n,), float("nan"), dtype=dtype, device="cuda")
+        v = (torch.randn(shape, generator=gen(seed), device="cuda") * scale).to(dtype)
+    view = buf[offset:].view(full)[..., :shape[-1]]
+    view.copy_(v)
+    return view
+
+
+# ------------------------------------------------------------------------------------------------------- routing
+
+
+def plain_route(logits, k, normalize):
+    """(weights, ids) of CPU logits in float64, one row at a time."""
+    l = logits.double().cpu().numpy()
+    t, e = l.shape
+    w, ids = np.zeros((t, k)), np.full((t, k), -1, np.int64)
+    for r in range(t):
+        order = sorted((i for i in range(e) if l[r, i] != -np.inf), key=lambda i: (-l[r, i], i))[:k]
+        if not order:
+            continue
+        top = l[r, order[0]]
+        total = sum(np.exp(l[r, i] - top) for i in (order if normalize else range(e)))
+        for j, i in enumerate(order):
+            ids[r, j], w[r, j] = i, np.exp(l[r, i] - top) / total
+    return w, ids
+
+
+def plain_plan(ids, experts):
+    flat = ids.reshape(-1)
+    keep = (flat >= 0) & (flat < experts)
+    order = np.argsort(np.where(keep, flat, experts), kind="stable")[:int(keep.sum())]
+    offsets = np.concatenate([[0], np.cumsum(np.bincount(flat[keep], minlength=experts))])
+    tokens = np.full(flat.size, -1, np.int64)
+    tokens[:order.size] = order // ids.shape[1]
+    places = np.full(flat.size, -1, np.int64)
+    places[order] = np.arange(order.size)
+    return offsets, tokens, places.reshape(ids.shape)
+
+
+def check_plan(plan, ids, experts):
+    offsets, tokens, places = plain_plan(ids, experts)
+    assert np.array_equal(plan.offsets.cpu().numpy(), offsets)
+    assert np.array_equal(plan.places.cpu().numpy(), places)
+    assert np.array_equal(plan.tokens.cpu().numpy(), tokens)
+
+
+def check_weights(got, want, terms):
+    # exp to 2 ulp of an argument rounded in 32 bits (|argument| * 2^-24), the sum, and the division
+    err = (got.double().cpu() - torch.from_numpy(want)).abs()
+    bound = torch.from_numpy(want) * (terms + 40) * 2 * U32 + 1e-38
+    assert bool((err <= bound).all()), float((err / bound).max())
+
+
+@pytest.mark.parametrize("normalize", [True, False])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("tokens,experts,k", [(1, 1, 1), (1, 64, 8), (2, 4, 4), (7, 60, 4), (33, 128, 8), (65, 129, 2),
+                                              (200, 257, 6), (130, 1000, 64), (17, 64, 64), (2100, 16, 2),
+                                              (9000, 96, 3)])
+def test_route(dev, tokens, experts, k, dtype, normalize):
+    logits = (torch.randn(tokens, experts, generator=gen(tokens + experts), device=dev) * 2).to(dtype)
+    weights, ids, plan = route(logits, k, normalize=normalize)
+    w, want = plain_route(logits, k, normalize)
+    assert np.array_equal(ids.cpu().numpy(), want)
+    check_weights(weights, w, experts)
+    check_plan(plan, want, experts)
+
+
+def test_route_ties_masks_and_strides(dev):
+    inf = float("inf")
+    lowest = float(torch.finfo(F32).min)
+    rows = torch.tensor([[1.0, 1.0, 1.0, 1.0, 1.0], [-inf] * 5, [-inf, 2.0, -inf, -inf, 2.0],
+                         [lowest] * 5, [lowest, 0.0, lowest, -inf, lowest], [0.0, -0.0, 0.0, -0.0, -1.0],
+                         [3e38, -3e38, 3e38, 1.0, 2.0]], device=dev)
+    for normalize in (True, False):
+        buf = torch.full((7, 9), 1e30, device=dev)
+        view = buf[:, 2:7]
+        view.copy_(rows)
+        weights, ids, plan = route(view, 3, normalize=normalize)
+        w, want = plain_route(rows, 3, normalize)
+        assert np.array_equal(ids.cpu().numpy(), want)
+        assert np.array_equal(want[1], [-1, -1, -1]) and np.array_equal(want[2], [1, 4, -1])
+        check_weights(weights, w, 5)
+        assert weights[1].abs().max() == 0
+        check_plan(plan, want, 5)
+
+
+def test_route_nan_and_infinity_stay_in_their_row(dev):
+    logits = torch.zeros(4, 6, device=dev)
+    logits[1, 3] = float("nan")
+    logits[2, 5] = float("inf")
+    weights, ids, _ = route(logits, 2)
+    assert ids.cpu().tolist() == [[0, 1], [3, 0], [5, 0], [0, 1]]
+    assert weights[1].isnan().all() and weights[2, 0].isnan()
+    assert weights[0].tolist() == [0.5, 0.5] and weights[3].tolist() == [0.5, 0.5]
+
+
+def test_route_no_tokens(dev):
+    weights, ids, plan = route(torch.empty(0, 8, device=dev), 2)
+    assert weights.shape == (0, 2) and ids.shape == (0, 2) and plan.places.shape == (0, 2)
+    assert plan.offsets.cpu().tolist() == [0] * 9
+
+
+@pytest.mark.parametrize("tokens,experts,k", [(1, 3, 1), (5, 8, 3), (1000, 70, 4), (20000, 1024, 2), (300, 2, 2)])
+def test_expert_plan_with_dropped_assignments(dev, tokens, experts, k):
+    ids = torch.randint(-2, experts + 2, (tokens, k), generator=gen(k), device=dev, dtype=torch.int32)
+    check_plan(expert_plan(ids, experts), ids.cpu().numpy().astype(np.int64), experts)
+
+
+def test_expert_plan_of_one_expert(dev):
+    ids = torch.full((3000, 2), 5, dtype=torch.int32, device=dev)
+    check_plan(expert_plan(ids, 9), ids.cpu().numpy().astype(np.int64), 9)
+
+
+def plain_route_grad(logits, ids, grad, normalize):
+    """The softmax's gradient in float64 by autograd on the CPU, for the given choice."""
+    l = logits.detach().double().cpu().requires_grad_(True)
+    chosen = torch.zeros(l.shape, dtype=torch.bool)
+    safe = torch.where(ids < 0, 0, ids).long()
+    for r, row in enumerate(ids.tolist()):
+        chosen[r, [i for i in row if i >= 0]] = True
+    base = l.masked_fill(~chosen, -float("inf")) if normalize else l
+    empty = (ids < 0).all(1, keepdim=True)
+    p = torch.softmax(torch.where(empty, torch.zeros_like(base), base), 1)
+    w = torch.where(ids < 0, torch.zeros_like(grad), p.gather(1, safe))
+    (w * grad).sum().backward()
+    return torch.where(empty, torch.zeros_like(l), l.grad)
+
+
+@pytest.mark.parametrize("normalize", [True, False])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("tokens,experts,k", [(1, 1, 1), (3, 64, 8), (7, 60, 4), (65, 129, 2), (50, 1000, 64)])
+def test_route_gradient(dev, tokens, experts, k, dtype, normalize):
+    logits = torch.randn(tokens, experts, generator=gen(1), device=dev).to(dtype)
+    if tokens > 5 and experts > 8:
+        logits[1, 3:] = -float("inf")   # fewer than k experts left
+        logits[2] = -float("inf")       # none left
+    logits.requires_grad_(True)
+    weights, ids, _ = route(logits, k, normalize=normalize)
+    grad = torch.randn(tokens, k, generator=gen(2), device=dev)
+    got, = torch.autograd.grad(weights, logits, grad)
+    want = plain_route_grad(logits, ids.cpu().long(), grad.double().cpu(), normalize)
+    # p (g - sum): a few roundings of each factor, each relative to max |g| times p
+    p = weights.detach().double().cpu().max() if normalize else 1.0
+    bound = U[dtype] * want.abs() + (experts + 60) * 2 * U32 * float(grad.abs().max()) * k * float(p) + 2.0**-25
+    assert got.dtype == dtype and bool(((got.double().cpu() - want).abs() <= bound).all())
+
+
+def test_route_gradient_against_differences(dev):
+    logits = torch.randn(4, 12, generator=gen(3), device=dev).requires_grad_(True)
+    grad = torch.randn(4, 3, generator=gen(4), device=dev)
+    for normalize in (True, False):
+        weights, ids, _ = route(logits, 3, normalize=normalize)
+        got, = torch.autograd.grad(weights, logits, grad)
+        step = 2.0**-7
+        for t, e in ((0, int(ids[0, 0])), (1, int(ids[1, 2])), (2, 5), (3, 0)):
+            moved = []
+            for s in (step, -step):
+                l = logits.detach().clone()
+                l[t, e] += s
+                w, i, _ = route(l, 3, normalize=normalize)
+                moved.append(float((w.double() * grad.double()).sum()) if torch.equal(i, ids) else None)
+            if None in moved:
+                continue  # the choice itself changed
+            # third derivatives of a softmax are below 1; rounding 2^-22 over the step
+            bound = step**2 * float(grad.abs().sum()) + 2.0**-20 / step * float(grad.abs().sum())
+            assert abs((moved[0] - moved[1]) / (2 * step) - float(got[t, e])) <= bound
+
+
+# ------------------------------------------------------------------------------------------------------- products
+
+
+def plain_grouped(a, w, plan, rows):
+    """(y, magnitudes) in float64."""
+    off = plan.offsets.tolist()
+    y = torch.zeros(rows, w.shape[1], dtype=torch.float64, device="cuda")
+    m = torch.zeros_like(y)
+    for e in range(w.shape[0]):
+        lo, hi = off[e], off[e + 1]
+        if lo < hi and a.shape[1]:
+            r = a[plan.tokens[lo:hi].long()] if plan.tokens is not None else a[lo:hi]
+            y[lo:hi] = r.double() @ w[e].double().t()
+            m[lo:hi] = r.double().abs() @ w[e].double().abs().t()
+    return y, m
+
+
+GROUPS = {
+    "one": [1], "one_of_many": [0, 0, 1, 0], "empty": [0, 0, 0], "single_rows": [1, 1, 0, 1, 1],
+    "ragged": [5, 0, 17, 64, 1, 33], "tile_ends": [64, 128, 16, 256, 32, 0], "over": [65, 129, 17, 257],
+    "many": [(i * 7) % 5 for i in range(130)], "long": [700, 3, 1100, 0, 260],
+}
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("n,k", [(1, 1), (8, 8), (64, 64), (65, 33), (256, 264), (300, 40), (520, 1032), (40, 2048),
+                                 (129, 1001)])
+@pytest.mark.parametrize("groups", list(GROUPS))
+def test_grouped_mm(dev, groups, n, k, dtype):
+    lens = GROUPS[groups]
+    gather = (n + k + len(lens)) % 2 == 0
+    tokens = 97
+    plan, rows = lengths_to_plan(lens, tail=3, tokens=tokens if gather else None)
+    a = torch.randn(tokens if gather else rows, k, generator=gen(1), device=dev).to(dtype)
+    w = torch.randn(len(lens), n, k, generator=gen(2), device=dev).to(dtype)
+    y = grouped_mm(a, w, plan, gather=gather)
+    want, magnitude = plain_grouped(a, w, plan, rows)
+    close(y, want, magnitude, k)
+    assert not y[rows - 3:].any()
+
+
+@pytest.mark.parametrize("pad,offset", [(0, 0), (8, 0), (1, 0), (0, 1), (24, 8), (3, 5)])
+@pytest.mark.parametrize("groups", ["ragged", "long", "single_rows"])
+def test_grouped_mm_strides_and_alignment(dev, groups, pad, offset):
+    lens = GROUPS[groups]
+    plan, rows = lengths_to_plan(lens, tokens=50)
+    a = strided((50, 136), BF16, 1, pad, offset=offset)
+    w = strided((len(lens), 72, 136), BF16, 2, pad, offset=offset)
+    want, magnitude = plain_grouped(a, w, plan, rows)
+    close(grouped_mm(a, w, plan, gather=True), want, magnitude, 136)
+    # every other expert of a larger tensor, and columns of it that are not contiguous
+    big = strided((2 * len(lens), 72, 136), BF16, 3, pad, offset=offset)
+    close(grouped_mm(a, big[::2], plan, gather=True), *plain_grouped(a, big[::2], plan, rows), 136)
+    turned = strided((len(lens), 136, 72), BF16, 4, pad).transpose(1, 2)
+    close(grouped_mm(a, turned, plan, gather=True), *plain_grouped(a, turned, plan, rows), 136)
+
+
+def test_grouped_mm_no_rows_no_width(dev):
+    plan, _ = lengths_to_plan([0, 0])
+    w = torch.ones(2, 16, 8, dtype=F16, device=dev)
+    assert grouped_mm(torch.empty(0, 8, dtype=F16, device=dev), w, plan).shape == (0, 16)
+    plan, rows = lengths_to_plan([2, 1])
+    y = grouped_mm(torch.empty(3, 0, dtype=F16, device=dev), w[:, :, :0], plan)
+    assert y.shape == (3, 16) and not y.any()
+    assert grouped_mm(torch.ones(3, 8, dtype=F16, device=dev), w[:, :0], plan).shape == (3, 0)
+
+
+@pytest.mark.parametrize("k", [64, 72, 1000, 33])
+def test_grouped_mm_non_finite_values_stay_in_their_rows(dev, k):
+    lens = [20, 70, 3]
+    plan, rows = lengths_to_plan(lens)
+    a = torch.randn(rows, k, generator=gen(1), device=dev).to(BF16)
+    w = torch.randn(3, 48, k, generator=gen(2), device=dev).to(BF16)
+    clean = grouped_mm(a, w, plan)
+    dirty = a.clone()
+    dirty[19, k - 1] = float("nan")   # the last row of a group, next to another's first
+    dirty[92, 0] = float("inf")
+    wd = w.clone()
+    wd[1, 7] = float("nan")
+    y = grouped_mm(dirty, wd, plan)
+    assert y[19].isnan().all() and not y[92].isfinite().any() and y[20:90, 7].isnan().all()
+    keep = torch.ones(rows, 48, dtype=torch.bool, device=dev)
+    keep[19] = keep[92] = False
+    keep[20:90, 7] = False
+    assert torch.equal(y[keep], clean[keep])
+
+
+@pytest.mark.parametrize("offsets", [[0, 40, 20, 60], [0, -5, 70, 1 << 30], [3, 3, 3, 3], [50, 40, 30, 20]])
+def test_grouped_mm_offsets_without_meaning_stay_in_bounds(dev, offsets):
+    off = torch.tensor(offsets, dtype=torch.int32, device=dev)
+    tokens = torch.full((60,), 1 << 20, dtype=torch.int32, device=dev)
+    a = torch.ones(60, 64, dtype=F16, device=dev, requires_grad=True)
+    w = torch.ones(3, 64, 64, dtype=F16, device=dev, requires_grad=True)
+    y = grouped_mm(a.detach(), w, ExpertPlan(off, tokens, None), gather=True)
+    assert y.shape == (60, 64)
+    dw, = torch.autograd.grad(y, w, torch.ones_like(y))
+    assert dw.shape == w.shape
+    torch.cuda.synchronize()
+
+
+def plain_grads(a, w, plan, grad):
+    """(da, its magnitudes, dw, its magnitudes) in float64."""
+    off = plan.offsets.tolist()
+    index = plan.tokens.long() if plan.tokens is not None else torch.arange(a.shape[0], device="cuda")
+    da, dw = (torch.zeros(t.shape, dtype=torch.float64, device="cuda") for t in (a, w))
+    ma, mw = torch.zeros_like(da), torch.zeros_like(dw)
+    for e in range(w.shape[0]):
+        s = slice(off[e], off[e + 1])
+        if s.start < s.stop:
+            g, x, b = grad[s].double(), a[index[s]].double(), w[e].double()
+            da.index_add_(0, index[s], g @ b)
+            ma.index_add_(0, index[s], g.abs() @ b.abs())
+            dw[e], mw[e] = g.t() @ x, g.abs().t() @ x.abs()
+    return da, ma, dw, mw
+
+
+def routed(tokens, experts, k, seed, drop=0.0, taken=None):
+    ids = torch.stack([torch.randperm(taken or experts, generator=gen(seed * 1000 + t, "cpu"))[:k]
+                       for t in range(tokens)]).to(torch.int32)
+    ids[torch.rand(tokens, k, generator=gen(seed, "cpu")) < drop] = -1
+    return ids.cuda()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("tokens,experts,k,n,width,drop", [
+    (1, 4, 2, 64, 64, 0.0), (9, 8, 3, 40, 72, 0.3), (70, 5, 2, 129, 33, 0.0), (300, 6, 2, 264, 520, 0.1),
+    (513, 3, 3, 256, 256, 0.0), (40, 100, 4, 96, 128, 0.0), (700, 2, 1, 72, 1000, 0.5), (12, 3, 1, 64, 64, 1.0)])
+def test_grouped_mm_gradients(dev, tokens, experts, k, n, width, drop, dtype):
+    plan = expert_plan(routed(tokens, experts, k, 5, drop, taken=max(experts - 1, k)), experts)
+    a = torch.randn(tokens, width, generator=gen(1), device=dev).to(dtype).requires_grad_(True)
+    w = torch.randn(experts, n, width, generator=gen(2), device=dev).to(dtype).requires_grad_(True)
+    y = grouped_mm(a, w, plan, gather=True)
+    grad = torch.randn(y.shape, generator=gen(3), device=dev).to(dtype)
+    da, dw = torch.autograd.grad(y, (a, w), grad)
+    wa, ma, ww, mw = plain_grads(a.detach(), w.detach(), plan, grad)
+    close(da, wa, ma, n + k)
+    close(dw, ww, mw, tokens)
+    assert not dw[experts - 1].any() or experts == k  # an expert that nobody chose
+
+
+@pytest.mark.parametrize("n,width", [(64, 64), (129, 65), (256, 320)])
+@pytest.mark.parametrize("groups", ["one_of_many", "ragged", "tile_ends", "over", "many", "long"])
+def test_grouped_mm_gradients_without_gather(dev, groups, n, width):
+    lens = GROUPS[groups]
+    plan, rows = lengths_to_plan(lens)
+    a = torch.randn(rows, width, generator=gen(1), device=dev).to(BF16).requires_grad_(True)
+    w = torch.randn(len(lens), n, width, generator=gen(2), device=dev).to(BF16).requires_grad_(True)
+    y = grouped_mm(a, w, plan)
+    grad = torch.randn(y.shape, generator=gen(3), device=dev).to(BF16)
+    da, dw = torch.autograd.grad(y, (a, w), grad)
+    wa, ma, ww, mw = plain_grads(a.detach(), w.detach(), plan, grad)
+    close(da, wa, ma, n)
+    close(dw, ww, mw, max(lens))
+
+
+def test_grouped_mm_gradients_of_strided_and_broadcast_inputs(dev):
+    lens = [30, 0, 100]
+    plan, rows = lengths_to_plan(lens)
+    a = strided((rows, 72), BF16, 1, 9).requires_grad_(True)
+    shared = torch.randn(1, 40, 72, generator=gen(2), device=dev).to(BF16).requires_grad_(True)
+    y = grouped_mm(a, shared.expand(3, 40, 72), plan)
+    grad = torch.randn(40, generator=gen(3), device=dev).to(BF16).expand(rows, 40)
+    da, dw = torch.autograd.grad(y, (a, shared), grad)
+    wa, ma, ww, mw = plain_grads(a.detach(), shared.detach().expand(3, 40, 72), plan, grad)
+    close(da, wa, ma, 40)
+    # each expert's part is rounded before torch adds them over the broadcast
+    bound = BF16_SUM * ww.abs().sum(0) + (rows + 1) * U32 * mw.sum(0) * 2 + 2 * BF16_SUM * ww.sum(0).abs() + 2.0**-25
+    assert bool(((dw[0].double() - ww.sum(0)).abs() <= bound).all())
+
+
+BF16_SUM = 2.0**-8
+
+
+def test_grouped_mm_gradient_against_differences(dev):
+    plan = expert_plan(routed(12, 3, 2, 1), 3)
+    a = torch.randn(12, 24, generator=gen(1), device=dev).to(F16).requires_grad_(True)
+    w = torch.randn(3, 16, 24, generator=gen(2), device=dev).to(F16).requires_grad_(True)
+    c = torch.randn(24, 16, generator=gen(3), device=dev).to(F16)
+    y = grouped_mm(a, w, plan, gather=True)
+    da, dw = torch.autograd.grad(y, (a, w), c)
+    # the product is linear in each input: differences are exact up to y's rounding
+    for t, grad, at in ((a, da, (3, 5)), (a, da, (11, 23)), (w, dw, (0, 2, 7)), (w, dw, (2, 15, 0))):
+        value, outs = float(t[at].detach()), []
+        for v in (value + 1.0, value - 1.0):
+            moved = t.detach().clone()
+            moved[at] = v
+            args = (moved, w.detach()) if t is a else (a.detach(), moved)
+            outs.append((float(moved[at]), (grouped_mm(*args, plan, gather=True).double() * c.double()).sum()))
+        slope = float(outs[0][1] - outs[1][1]) / (outs[0][0] - outs[1][0])
+        rounding = 2.0**-11 * float((y.detach().double().abs() * c.double().abs()).sum() + 24 * 50)
+        assert abs(slope - float(grad[at])) <= rounding
+
+
+# ------------------------------------------------------------------------------------------------------- 8 bits
+
+
+def plain_scaled(a, sa, w, sw, plan, rows):
+    off = plan.offsets.tolist()
+    y = torch.zeros(rows, w.shape[1], dtype=torch.float64, device="cuda")
+    index = plan.tokens.long() if plan.tokens is not None else torch.arange(rows, device="cuda")
+    for e in range(w.shape[0]):
+        s = slice(off[e], off[e + 1])
+        if s.start < s.stop:
+            y[s] = (a[index[s]].double() @ w[e].double().t()) * sa[index[s]].double()[:, None] * sw[e].double()
+    return y
+
+
+def scaled_close(got, want):
+    # the integer sum is exact; its conversion to fp32, the product of the scales and the product with it round
+    bound = (U[got.dtype] + 4 * U32) * want.abs() + 2.0**-25
+    assert bool(((got.double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("out", [F32, F16, BF16])
+@pytest.mark.parametrize("n,k", [(1, 1), (16, 16), (64, 128), (65, 33), (256, 272), (300, 48), (129, 1001), (512, 1040)])
+@pytest.mark.parametrize("groups", list(GROUPS))
+def test_grouped_mm_scaled(dev, groups, n, k, out):
+    lens = GROUPS[groups]
+    gather = (n + len(lens)) % 2 == 0
+    plan, rows = lengths_to_plan(lens, tail=2, tokens=97 if gather else None)
+    rows_a = 97 if gather else rows
+    a = strided((rows_a, k), torch.int8, 1, 0)
+    w = strided((len(lens), n, k), torch.int8, 2, 0)
+    sa = torch.rand(rows_a, generator=gen(3), device=dev) * 1e-3
+    sw = torch.rand(len(lens), n, generator=gen(4), device=dev) * 1e-2
+    y = grouped_mm_scaled(a, sa, w, sw, plan, gather=gather, out_dtype=out)
+    scaled_close(y, plain_scaled(a, sa, w, sw, plan, rows))
+    assert not y[rows - 2:].any()
+
+
+@pytest.mark.parametrize("rows", [1, 2, 15, 16, 17, 64, 100, 300, 1000])
+@pytest.mark.parametrize("n,k,pad", [(64, 64, 0), (1000, 528, 16), (520, 77, 3), (256, 4096, 0)])
+def test_scaled_dense(dev, rows, n, k, pad):
+    a, w = strided((rows, k), torch.int8, 1, pad), strided((n, k), torch.int8, 2, pad)
+    sa = torch.rand(rows, generator=gen(3), device=dev)
+    sw = torch.rand(n, generator=gen(4), device=dev) * 1e-4
+    y = grouped_mm_scaled(a, sa, w, sw, out_dtype=F32)
+    want = (a.double() @ w.double().t()) * sa.double()[:, None] * sw.double()
+    scaled_close(y, want)
+
+
+def test_scaled_extremes(dev):
+    # the largest magnitudes in the longest contraction: -128 * -128 * 131071 is just within 32 bits
+    a = torch.full((3, 131071), -128, dtype=torch.int8, device=dev)
+    w = torch.full((5, 131071), -128, dtype=torch.int8, device=dev)
+    one = torch.ones(5, device=dev)
+    y = grouped_mm_scaled(a, one[:3], w, one, out_dtype=F32)
+    assert bool((y.double() == float(np.float32(131071 * 16384))).all())
+    with pytest.raises(ValueError):
+        grouped_mm_scaled(torch.zeros(1, 131072, dtype=torch.int8, device=dev), one[:1],
+                          torch.zeros(5, 131072, dtype=torch.int8, device=dev), one)
+
+
+# ------------------------------------------------------------------------------------------------------- combination
+
+
+def plain_combine(y, weights, places):
+    safe = torch.where(places < 0, 0, places).long()
+    rows = y.double()[safe] * (places >= 0)[:, :, None]
+    w = weights.double() if weights is not None else torch.ones(places.shape, dtype=torch.float64, device="cuda")
+    return (rows * w[:, :, None]).sum(1), (rows.abs() * w.abs()[:, :, None]).sum(1)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("weighted", [True, False])
+@pytest.mark.parametrize("tokens,experts,k,width,drop", [
+    (1, 4, 1, 1, 0.0), (5, 8, 3, 33, 0.0), (64, 16, 8, 2048, 0.0), (100, 9, 4, 264, 0.4), (31, 40, 33, 72, 0.1),
+    (7, 3, 2, 5000, 0.0), (6, 3, 2, 4104, 1.0)])
+def test_combine_and_its_gradients(dev, tokens, experts, k, width, drop, weighted, dtype):
+    plan = expert_plan(routed(tokens, experts, k, 3, drop), experts)
+    y = torch.randn(tokens * k, width, generator=gen(1), device=dev).to(dtype).requires_grad_(True)
+    weights = torch.randn(tokens, k, generator=gen(2), device=dev).requires_grad_(True) if weighted else None
+    out = combine(y, plan, weights)
+    want, magnitude = plain_combine(y.detach(), weights.detach() if weighted else None, plan.places)
+    close(out, want, magnitude, k)
+    grad = torch.randn(tokens, width, generator=gen(4), device=dev).to(dtype)
+    grads = torch.autograd.grad(out, (y, weights) if weighted else (y,), grad)
+    places = plan.places
+    wy = torch.zeros(y.shape, dtype=torch.float64, device=dev)
+    w = weights.detach().double() if weighted else torch.ones(tokens, k, dtype=torch.float64, device=dev)
+    used = places >= 0
+    wy[places[used].long()] = (w[:, :, None] * grad.double()[:, None, :])[used]
+    close(grads[0], wy, wy.abs(), 1)
+    if weighted:
+        rows = y.detach().double()[torch.where(used, places, 0).long()] * used[:, :, None]
+        prod = rows * grad.double()[:, None, :]
+        close(grads[1], prod.sum(2), prod.abs().sum(2), width)
+
+
+@pytest.mark.parametrize("pad,offset", [(8, 0), (1, 0), (0, 3)])
+def test_combine_strides(dev, pad, offset):
+    plan = expert_plan(routed(20, 6, 2, 3), 6)
+    y = strided((40, 520), F16, 1, pad, offset=offset).requires_grad_(True)
+    weights = torch.rand(2, 20, generator=gen(2), device=dev).t().requires_grad_(True)
+    out = combine(y, plan, weights)
+    close(out, *plain_combine(y.detach(), weights.detach(), plan.places), 2)
+    dy, dw = torch.autograd.grad(out, (y, weights), torch.ones(1, 1, dtype=F16, device=dev).expand(20, 520))
+    wy = torch.zeros(40, 520, dtype=torch.float64, device=dev)
+    wy[plan.places.long()] = weights.detach().double()[:, :, None]
+    close(dy, wy, wy, 1)
+    rows = y.detach().double()[plan.places.long()]
+    close(dw, rows.sum(2), rows.abs().sum(2), 520)
+
+
+def test_combine_gradient_against_differences(dev):
+    plan = expert_plan(routed(5, 4, 2, 3), 4)
+    y = torch.randn(10, 16, generator=gen(1), device=dev).to(F16).requires_grad_(True)
+    weights = torch.rand(5, 2, generator=gen(2), device=dev).requires_grad_(True)
+    c = torch.randn(5, 16, generator=gen(3), device=dev).to(F16)
+    out = combine(y, plan, weights)
+    dy, dw = torch.autograd.grad(out, (y, weights), c)
+    for t, grad, at in ((y, dy, (2, 3)), (y, dy, (9, 15)), (weights, dw, (4, 1)), (weights, dw, (0, 0))):
+        outs = []
+        for s in (1.0, -1.0):
+            moved = t.detach().clone()
+            moved[at] += s
+            args = (moved, plan, weights.detach()) if t is y else (y.detach(), plan, moved)
+            outs.append((float(moved[at]), float((combine(*args).double() * c.double()).sum())))
+        slope = (outs[0][1] - outs[1][1]) / (outs[0][0] - outs[1][0])
+        rounding = 2.0**-11 * float((out.detach().double().abs() * c.double().abs()).sum() + 16 * 30)
+        assert abs(slope - float(grad[at])) <= rounding
+
+
+# ------------------------------------------------------------------------------------------------------- as a whole
+
+
+def test_results_do_not_change_from_run_to_run(dev):
+    logits = torch.randn(700, 32, generator=gen(1), device=dev).requires_grad_(True)
+    x = torch.randn(700, 264, generator=gen(2), device=dev).to(BF16).requires_grad_(True)
+    w = (torch.randn(32, 264, 264, generator=gen(3), device=dev) / 16).to(BF16).requires_grad_(True)
+
+    def step():
+        weights, _, plan = route(logits, 4)
+        out = combine(grouped_mm(x, w, plan, gather=True), plan, weights)
+        return (out.detach(),) + torch.autograd.grad(out, (logits, x, w), torch.ones_like(out))
+
+    first = step()
+    for _ in range(3):
+        for a, b in zip(first, step()):
+            assert torch.equal(a, b)
+
+
+def test_another_stream(dev):
+    x = torch.randn(256, 512, generator=gen(2), device=dev).to(BF16)
+    w = (torch.randn(8, 512, 512, generator=gen(3), device=dev) / 16).to(BF16)
+    logits = torch.randn(256, 8, generator=gen(1), device=dev)
+    weights, _, plan = route(logits, 2)
+    want = combine(grouped_mm(x, w, plan, gather=True), plan, weights)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(20_000_000)
+        late = torch.zeros_like(x)
+        late.copy_(x)      # the operands exist only once this stream has got here
+        lw, _, lp = route(logits.clone(), 2)
+        got = combine(grouped_mm(late, w, lp, gather=True), lp, lw)
+    stream.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_hip_graph_capture_and_replay(dev):
+    x = torch.randn(48, 256, generator=gen(2), device=dev).to(F16)
+    w = (torch.randn(8, 256, 256, generator=gen(3), device=dev) / 16).to(F16)
+    logits = torch.randn(48, 8, generator=gen(1), device=dev)
+
+    def layer():
+        weights, _, plan = route(logits, 2)
+        return combine(grouped_mm(x, w, plan, gather=True), plan, weights)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer()
+    for seed in range(4):
+        logits.copy_(torch.randn(48, 8, generator=gen(10 + seed), device=dev))
+        x.copy_(torch.randn(48, 256, generator=gen(20 + seed), device=dev))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, layer())
+
+
+def test_offsets_past_32_bits(dev):
+    # an operand of more than 2^32 bytes, read at its far end
+    width, tokens = 4096, 540_000
+    x = torch.empty(tokens, width, dtype=F16, device=dev)
+    x[-64:] = torch.randn(64, width, generator=gen(1), device=dev)
+    x[:64] = 1.0
+    idx = torch.cat([torch.arange(tokens - 64, tokens), torch.arange(64)]).to(torch.int32).to(dev)
+    plan = ExpertPlan(torch.tensor([0, 100, 128], dtype=torch.int32, device=dev), idx, None)
+    w = torch.randn(2, 64, width, generator=gen(2), device=dev).to(F16)
+    y = grouped_mm(x, w, plan, gather=True)
+    close(y, *plain_grouped(x, w, plan, 128), width)
+    y8 = torch.empty(600_000, width, dtype=F16, device=dev)
+    y8[-2:] = 1.0
+    places = torch.tensor([[599_999, 599_998]], dtype=torch.int32, device=dev)
+    out = combine(y8, ExpertPlan(plan.offsets, None, places))
+    assert bool((out == 2.0).all())
+
+
+# ------------------------------------------------------------------------------------------------------- refusals
+
+
+def test_refusals(dev):
+    x = torch.zeros(4, 8, dtype=F16, device=dev)
+    w = torch.zeros(2, 8, 8, dtype=F16, device=dev)
+    plan = ExpertPlan(torch.tensor([0, 2, 4], dtype=torch.int32, device=dev),
+                      torch.zeros(4, dtype=torch.int32, device=dev))
+    for call, error in (
+            (lambda: route(torch.zeros(4, 8, device=dev), 9), ValueError),
+            (lambda: route(torch.zeros(4, 8, device=dev), 0), ValueError),
+            (lambda: route(torch.zeros(4, 1025, device=dev), 2), ValueError),
+            (lambda: route(torch.zeros(4, 200, device=dev), 65), ValueError),
+            (lambda: route(torch.zeros(8, device=dev), 1), ValueError),
+            (lambda: route(torch.zeros(4, 8, device=dev, dtype=torch.float64), 1), TypeError),
+            (lambda: route(torch.zeros(4, 8), 1), ValueError),
+            (lambda: expert_plan(torch.zeros(4, 2, dtype=torch.int64, device=dev), 4), TypeError),
+            (lambda: expert_plan(torch.zeros(4, 2, dtype=torch.int32, device=dev), 1), ValueError),
+            (lambda: grouped_mm(x.float(), w.float(), plan), TypeError),
+            (lambda: grouped_mm(x, w.to(BF16), plan), TypeError),
+            (lambda: grouped_mm(x, w[:, :, :4], plan), ValueError),
+            (lambda: grouped_mm(x, w[0], plan), ValueError),
+            (lambda: grouped_mm(x, w[:1], plan), ValueError),
+            (lambda: grouped_mm(x.cpu(), w, plan), ValueError),
+            (lambda: grouped_mm(x, w.cpu(), plan), ValueError),
+            (lambda: grouped_mm(x, w, ExpertPlan(plan.offsets), gather=True), ValueError),
+            (lambda: grouped_mm(x, w, ExpertPlan(plan.offsets.long(), plan.tokens)), TypeError),
+            (lambda: grouped_mm(x, w, ExpertPlan(plan.offsets.cpu(), plan.tokens)), ValueError),
+            (lambda: grouped_mm(x.requires_grad_(True), w, plan, gather=True), ValueError),
+            (lambda: grouped_mm_scaled(x.detach(), torch.ones(4, device=dev), w, torch.ones(2, 8, device=dev), plan),
+             TypeError),
+            (lambda: grouped_mm_scaled(x.detach().to(torch.int8), torch.ones(3, device=dev), w.to(torch.int8),
+                                       torch.ones(2, 8, device=dev), plan), ValueError),
+            (lambda: grouped_mm_scaled(x.detach().to(torch.int8), torch.ones(4, device=dev), w.to(torch.int8),
+                                       torch.ones(2, 8, device=dev), plan, out_dtype=torch.int32), TypeError),
+            (lambda: grouped_mm_scaled(x.detach().to(torch.int8), torch.ones(4, device=dev), w.to(torch.int8),
+                                       torch.ones(2, 8, device=dev)), ValueError),
+            (lambda: combine(x.detach(), plan), ValueError),
+            (lambda: combine(x.detach().float(), ExpertPlan(plan.offsets, None, plan.tokens.view(2, 2))), TypeError),
+            (lambda: combine(x.detach(), ExpertPlan(plan.offsets, None, plan.tokens.view(2, 2)),
+                             torch.ones(4, 1, device=dev)), ValueError)):
+        with pytest.raises(error):
+            call()
+    torch.cuda.synchronize()

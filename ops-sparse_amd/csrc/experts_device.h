@@ -89,13 +89,39 @@ __device__ __forceinline__ void GroupRows(const int32_t* offsets, int64_t rows, 
     end = e < begin ? begin : e > r ? r : e;
 }
 
+// Group g's tiles of `height` rows for lane g - g0; the tail's for the lane past the last group's.
+__device__ __forceinline__ int32_t LaneTiles(const int32_t* offsets, int64_t rows, int32_t groups, int32_t height,
+                                             int32_t g, int32_t& begin, int32_t& end)
+{
+    begin = end = 0;
+    if (g < groups) {
+        GroupRows(offsets, rows, g, begin, end);
+    } else if (g == groups && offsets != nullptr) {
+        int32_t unused;
+        GroupRows(offsets, rows, g - 1, unused, begin);
+        end = static_cast<int32_t>(rows);
+    }
+    return (end - begin + height - 1) / height;
+}
+
+// All tiles of `height` rows, through the groups and the tail.  Called by whole waves.
+__device__ __forceinline__ int32_t CountTiles(const int32_t* offsets, int64_t rows, int64_t groups, int32_t height)
+{
+    int32_t total = 0, begin, end;
+    for (int32_t g0 = 0; g0 <= static_cast<int32_t>(groups); g0 += 64) {
+        const int32_t n = LaneTiles(offsets, rows, static_cast<int32_t>(groups), height, g0 + (threadIdx.x & 63),
+                                    begin, end);
+        total += __builtin_amdgcn_readlane(WaveInclusiveSum(n), 63);
+    }
+    return total;
+}
+
 // A tile of a ragged product: rows [row, end) of `group`; group == groups is
 // the tail of rows that belong to no group, group < 0 no tile.
 struct RaggedTile {
     int32_t group;
     int32_t row;
     int32_t end;
-    int32_t tiles;  // of all groups
 };
 
 // The tile-th tile of `height` rows, counted through the groups and the tail.
@@ -103,32 +129,22 @@ struct RaggedTile {
 __device__ __forceinline__ RaggedTile FindTile(const int32_t* offsets, int64_t rows, int64_t groups, int32_t height,
                                                int32_t tile)
 {
-    const int lane = threadIdx.x & 63;
-    const int32_t all = static_cast<int32_t>(groups) + 1;
-    RaggedTile t{-1, 0, 0, 0};
-    for (int32_t g0 = 0; g0 < all; g0 += 64) {
-        const int32_t g = g0 + lane;
-        int32_t begin = 0, end = 0;
-        if (g < all - 1) {
-            GroupRows(offsets, rows, g, begin, end);
-        } else if (g == all - 1 && offsets != nullptr) {
-            int32_t unused;
-            GroupRows(offsets, rows, g - 1, unused, begin);
-            end = static_cast<int32_t>(rows);
-        }
-        const int32_t n = (end - begin + height - 1) / height;
+    int32_t before = 0;
+    for (int32_t g0 = 0; g0 <= static_cast<int32_t>(groups); g0 += 64) {
+        int32_t begin, end;
+        const int32_t n = LaneTiles(offsets, rows, static_cast<int32_t>(groups), height, g0 + (threadIdx.x & 63),
+                                    begin, end);
         const int32_t incl = WaveInclusiveSum(n);
-        const uint64_t hit = __ballot(t.tiles + incl > tile);
-        if (t.group < 0 && hit != 0) {
+        const uint64_t hit = __ballot(before + incl > tile);
+        if (hit != 0) {
             const int src = __builtin_ctzll(hit);
-            t.group = g0 + src;
-            const int32_t before = t.tiles + __builtin_amdgcn_readlane(incl - n, src);
-            t.row = __builtin_amdgcn_readlane(begin, src) + (tile - before) * height;
-            t.end = __builtin_amdgcn_readlane(end, src);
+            const int32_t skipped = before + __builtin_amdgcn_readlane(incl - n, src);
+            return {g0 + src, __builtin_amdgcn_readlane(begin, src) + (tile - skipped) * height,
+                    __builtin_amdgcn_readlane(end, src)};
         }
-        t.tiles += __builtin_amdgcn_readlane(incl, 63);
+        before += __builtin_amdgcn_readlane(incl, 63);
     }
-    return t;
+    return {-1, 0, 0};
 }
 
 }  // namespace aclsp

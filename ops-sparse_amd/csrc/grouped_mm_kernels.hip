@@ -9,6 +9,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "experts_device.h"
 #include "experts_internal.h"
@@ -212,7 +213,380 @@ __global__ __launch_bounds__(256) void GroupedGradAnyKernel(GroupedGradLaunch p,
     }
 }
 
+// ---------------------------------------------------------------------------
+// Kernels for operands whose rows are aligned to 16 bytes: large tiles, copied
+// from memory to LDS without passing registers, 32x32 matrix instructions.
+//
+// A tile's contraction advances by 128 bytes per turn.  Two buffers in LDS:
+// while one is multiplied the next is copied.  Each wave keeps the operands
+// of one matrix step ahead of the one it multiplies in registers.
+// ---------------------------------------------------------------------------
+using Float16 = float __attribute__((ext_vector_type(16)));
+using Int16 = int __attribute__((ext_vector_type(16)));
+using Short4 = short __attribute__((ext_vector_type(4)));
+
+constexpr int kTurnBytes = 128;
+constexpr int kStepsPerTurn = 4;  // of 32 bytes (16 elements of 16 bits) per row
+
+// 32x32 matrix instructions: lane l holds row l % 32 of its operand,
+// contraction bytes (l / 32) * 16 on.  The result's lane l holds column l % 32
+// (row of the second operand) and, in register i, row 8 * (i / 4) +
+// 4 * (l / 32) + i % 4 (of the first).
+template <typename T>
+struct Mma32;
+template <>
+struct Mma32<Half> {
+    using Acc = Float16;
+    static __device__ __forceinline__ Acc Run(Int4 a, Int4 b, Acc c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(Half8, a), __builtin_bit_cast(Half8, b), c, 0,
+                                                      0, 0);
+    }
+};
+template <>
+struct Mma32<Bf16> {
+    using Acc = Float16;
+    static __device__ __forceinline__ Acc Run(Int4 a, Int4 b, Acc c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(Bf168, a), __builtin_bit_cast(Bf168, b), c,
+                                                       0, 0, 0);
+    }
+};
+template <>
+struct Mma32<int8_t> {
+    using Acc = Int16;
+    static __device__ __forceinline__ Acc Run(Int4 a, Int4 b, Acc c)
+    {
+        return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
+    }
+};
+
+// What lanes copy that have nothing to copy: both operands read as zero past
+// the contraction's end, so that no value beyond it, NaN among them, counts.
+__device__ const Int4 kZeros = {0, 0, 0, 0};
+
+__device__ __forceinline__ void CopyToLds(const char* from, char* to)
+{
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from),
+                                     (__attribute__((address_space(3))) void*)(to), 16, 0, 0);
+}
+
+// An operand whose rows run along the contraction: R rows of 128 bytes per
+// turn.  Its 16-byte chunk c of row r lies at slot c ^ (r & 7), so that the
+// lanes that read one chunk of eight rows touch every bank once.
+template <int R, int kThreads>
+struct RowOperand {
+    static constexpr int kLoads = R * 8 / kThreads;
+    static constexpr int kRowsPerLoad = kThreads / 8;
+    static constexpr int kBytes = R * kTurnBytes;
+    const char* ptr[kLoads];
+    int64_t left;  // bytes of the contraction from the next turn on
+
+    // This thread's rows are Row(i); its chunk of each is the same.
+    static __device__ __forceinline__ int Row(int i) { return i * kRowsPerLoad + (threadIdx.x >> 3); }
+    static __device__ __forceinline__ int Chunk() { return (threadIdx.x & 7) ^ ((threadIdx.x >> 3) & 7); }
+
+    __device__ __forceinline__ void Issue(char* lds)
+    {
+        const char* zero = reinterpret_cast<const char*>(&kZeros);
+        char* to = lds + (threadIdx.x >> 6) * 1024;
+        if (left >= kTurnBytes) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                CopyToLds(ptr[i], to + i * kThreads * 16);
+                ptr[i] += kTurnBytes;
+            }
+        } else {
+            const bool in = Chunk() * 16 < left;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) CopyToLds(in ? ptr[i] : zero, to + i * kThreads * 16);
+        }
+        left -= kTurnBytes;
+    }
+
+    // The operand of one matrix step: 32 rows from `row` on.
+    static __device__ __forceinline__ Int4 Read(const char* lds, int row, int step)
+    {
+        const int lane = threadIdx.x & 63;
+        const int chunk = (step * 2 + (lane >> 5)) ^ (lane & 7);
+        return *reinterpret_cast<const Int4*>(lds + (row + (lane & 31)) * kTurnBytes + chunk * 16);
+    }
+};
+
+// An operand of 16-bit elements whose rows run across the contraction: 64
+// rows of C columns per turn, read through the transposing LDS load: of the
+// 16 lanes that work together lane j supplies 4 columns (j % 4) of row j / 4,
+// and lane i receives the 4 rows of column i.  Chunk c of row r lies at slot
+// c ^ 4 (r & 3): the four rows of 64 bytes that 32 lanes read then touch
+// every bank once.
+template <int C, int kThreads>
+struct ColumnOperand {
+    static constexpr int kChunks = C / 8;
+    static constexpr int kRowsPerLoad = kThreads / kChunks;
+    static constexpr int kLoads = 64 / kRowsPerLoad;
+    static constexpr int kBytes = 64 * C * 2;
+    const char* base;  // chunk of row 0, or null when the chunk lies past the last column
+    int64_t ld;        // bytes
+    const int32_t* index;
+    int64_t count;     // rows that an index may name
+    int32_t row, end;  // of this thread's first load in the next turn, and of all
+    int32_t next[kLoads];
+
+    static __device__ __forceinline__ int Row(int i) { return i * kRowsPerLoad + threadIdx.x / kChunks; }
+    static __device__ __forceinline__ int Chunk()
+    {
+        return (threadIdx.x % kChunks) ^ (((threadIdx.x / kChunks) & 3) << 2);
+    }
+
+    __device__ __forceinline__ void Init(const void* p, int64_t ldBytes, int64_t column, int64_t columns,
+                                         const int32_t* rowIndex, int64_t rowCount, int32_t first, int32_t last)
+    {
+        const int64_t c = column + Chunk() * 8;
+        base = c < columns ? static_cast<const char*>(p) + c * 2 : nullptr;
+        ld = ldBytes;
+        index = rowIndex;
+        count = rowCount;
+        row = first + Row(0);
+        end = last;
+        Fetch();
+    }
+
+    // The rows of the next turn: their indices are read a turn ahead.
+    __device__ __forceinline__ void Fetch()
+    {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int32_t r = row + i * kRowsPerLoad;
+            next[i] = r < end ? (index != nullptr ? index[r] : r) : -1;
+        }
+    }
+
+    __device__ __forceinline__ void Issue(char* lds)
+    {
+        const char* zero = reinterpret_cast<const char*>(&kZeros);
+        char* to = lds + (threadIdx.x >> 6) * 1024;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            int32_t r = next[i];
+            if (index != nullptr && row + i * kRowsPerLoad < end && (r < 0 || r >= count)) r = 0;
+            const char* from = base + r * ld;
+            CopyToLds(base != nullptr && r >= 0 ? from : zero, to + i * kThreads * 16);
+        }
+        row += 64;
+        Fetch();
+    }
+
+    static __device__ __forceinline__ Int4 Read(const char* lds, int column, int step)
+    {
+        using LdsShort4 = __attribute__((address_space(3))) Short4;
+        const int lane = threadIdx.x & 63, j = lane & 15;
+        const int r = step * 16 + (lane >> 5) * 8 + (j >> 2);
+        const int c = column + ((lane >> 4) & 1) * 16 + (j & 3) * 4;
+        const char* p = lds + r * (C * 2) + ((((c >> 3) ^ ((r & 3) << 2)) << 4) | ((c & 4) << 1));
+        struct Pair {
+            Short4 lo, hi;
+        } v;
+        v.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsShort4*)(p));
+        v.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsShort4*)(p + 4 * (C * 2)));
+        return __builtin_bit_cast(Int4, v);
+    }
+};
+
+// Waits for this wave's copies and reads, then for the other waves'.
+__device__ __forceinline__ void WaitAll()
+{
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// acc += the product over `turns` turns; MI x NI tiles of 32x32 per wave from
+// rows (columns of the output) rowA and rowB on.
+template <typename T, int MI, int NI, typename OperandA, typename OperandB>
+__device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds, int64_t turns, int rowA, int rowB,
+                                             typename Mma32<T>::Acc (&acc)[MI][NI])
+{
+    constexpr int kBuffer = OperandA::kBytes + OperandB::kBytes;
+    Int4 fa[2][MI], fb[2][NI];
+    a.Issue(lds);
+    b.Issue(lds + OperandA::kBytes);
+    WaitAll();
+#pragma unroll
+    for (int i = 0; i < MI; ++i) fa[0][i] = OperandA::Read(lds, rowA + i * 32, 0);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) fb[0][i] = OperandB::Read(lds + OperandA::kBytes, rowB + i * 32, 0);
+    char* cur = lds;
+    char* other = lds + kBuffer;
+    for (int64_t t = 0; t < turns; ++t) {
+        if (t + 1 < turns) {
+            a.Issue(other);
+            b.Issue(other + OperandA::kBytes);
+        }
+#pragma unroll
+        for (int s = 0; s < kStepsPerTurn; ++s) {
+            const int next = (s + 1) & 1;
+            if (s + 1 == kStepsPerTurn) {
+                WaitAll();
+                char* swap = cur;
+                cur = other;
+                other = swap;
+            }
+            const int step = (s + 1) % kStepsPerTurn;
+#pragma unroll
+            for (int i = 0; i < MI; ++i) fa[next][i] = OperandA::Read(cur, rowA + i * 32, step);
+#pragma unroll
+            for (int i = 0; i < NI; ++i) fb[next][i] = OperandB::Read(cur + OperandA::kBytes, rowB + i * 32, step);
+#pragma unroll
+            for (int i = 0; i < MI; ++i) {
+#pragma unroll
+                for (int j = 0; j < NI; ++j) acc[i][j] = Mma32<T>::Run(fb[s & 1][j], fa[s & 1][i], acc[i][j]);
+            }
+        }
+    }
+}
+
+// Four consecutive values of a row of the output.
+template <typename TOut>
+__device__ __forceinline__ void StoreFour(TOut* p, int64_t left, bool wide, const float (&v)[4])
+{
+    TOut o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = FromFloat<TOut>(v[i]);
+    if (wide && left >= 4) {
+        __builtin_memcpy(__builtin_assume_aligned(p, sizeof(o)), o, sizeof(o));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (i < left) p[i] = o[i];
+        }
+    }
+}
+
+// The workgroup's place among `total` tiles: neighbours in number share an L2
+// (workgroups are dealt to the 8 dies in turn), -1 when there is none.
+__device__ __forceinline__ int64_t TileOfWorkgroup(int64_t total)
+{
+    const int64_t per = (total + 7) / 8;
+    const int64_t at = blockIdx.x / 8;
+    const int64_t id = (blockIdx.x % 8) * per + at;
+    return at < per && id < total ? id : -1;
+}
+
+template <typename T, typename TOut, bool kBTrans, int MI, int NI, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64, 1) void GroupedTileKernel(GroupedLaunch p, int32_t tilesN, bool wideC)
+{
+    constexpr int kThreads = WM * WN * 64, BM = MI * WM * 32, BN = NI * WN * 32;
+    using OperandA = RowOperand<BM, kThreads>;
+    using OperandB = std::conditional_t<kBTrans, RowOperand<BN, kThreads>, ColumnOperand<BN, kThreads>>;
+    __shared__ __align__(128) char lds[2 * (OperandA::kBytes + OperandB::kBytes)];
+    const int64_t id = TileOfWorkgroup(static_cast<int64_t>(CountTiles(p.offsets, p.rows, p.groups, BM)) * tilesN);
+    if (id < 0) return;
+    const RaggedTile tile = FindTile(p.offsets, p.rows, p.groups, BM, static_cast<int32_t>(id / tilesN));
+    if (tile.group < 0) return;
+    const int64_t n0 = id % tilesN * BN;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int rowA = (wave % WM) * MI * 32, rowB = (wave / WM) * NI * 32;
+    typename Mma32<T>::Acc acc[MI][NI] = {};
+    const bool real = tile.group < p.groups;
+    if (real && p.k > 0) {
+        const T* bg = static_cast<const T*>(p.b) + tile.group * p.stride_b;
+        OperandA a;
+        OperandB b;
+#pragma unroll
+        for (int i = 0; i < OperandA::kLoads; ++i) {
+            // rows past the tile's end repeat its first: they are computed and not stored
+            const int32_t r = tile.row + OperandA::Row(i);
+            const int64_t row = IndexedRow(p.row_index, r < tile.end ? r : tile.row, p.rows_a);
+            a.ptr[i] = reinterpret_cast<const char*>(static_cast<const T*>(p.a) + row * p.lda) + OperandA::Chunk() * 16;
+        }
+        a.left = p.k * static_cast<int64_t>(sizeof(T));
+        if constexpr (kBTrans) {
+#pragma unroll
+            for (int i = 0; i < OperandB::kLoads; ++i) {
+                const int64_t n = n0 + OperandB::Row(i);
+                b.ptr[i] = reinterpret_cast<const char*>(bg + (n < p.n ? n : n0) * p.ldb) + OperandB::Chunk() * 16;
+            }
+            b.left = a.left;
+        } else {
+            b.Init(bg, p.ldb * 2, n0, p.n, nullptr, p.k, 0, static_cast<int32_t>(p.k));
+        }
+        MultiplyTile<T, MI, NI>(a, b, lds, (a.left + kTurnBytes - 1) / kTurnBytes, rowA, rowB, acc);
+    }
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+        const int32_t r = tile.row + rowA + i * 32 + (lane & 31);
+        if (r >= tile.end) continue;
+        float sa = 0.0f;
+        if constexpr (sizeof(T) == 1) {
+            if (real) sa = p.scale_a[IndexedRow(p.row_index, r, p.rows_a)];
+        }
+        TOut* c = static_cast<TOut*>(p.c) + r * p.ldc;
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int64_t n = n0 + rowB + j * 32 + q * 8 + (lane >> 5) * 4;
+                float v[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    v[x] = static_cast<float>(acc[i][j][q * 4 + x]);
+                    if constexpr (sizeof(T) == 1) {
+                        if (real && n + x < p.n) v[x] *= sa * p.scale_b[tile.group * p.n + n + x];
+                    }
+                }
+                StoreFour<TOut>(c + n, p.n - n, wideC, v);
+            }
+        }
+    }
+}
+
+template <typename T, typename TOut, int MI, int NI, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64, 1) void GroupedGradTileKernel(GroupedGradLaunch p, int32_t tilesN,
+                                                                        int32_t tilesK, bool wideW)
+{
+    constexpr int kThreads = WM * WN * 64, BM = MI * WM * 32, BN = NI * WN * 32;
+    using OperandA = ColumnOperand<BM, kThreads>;
+    using OperandB = ColumnOperand<BN, kThreads>;
+    __shared__ __align__(128) char lds[2 * (OperandA::kBytes + OperandB::kBytes)];
+    int64_t id = TileOfWorkgroup(static_cast<int64_t>(tilesN) * tilesK * p.groups);
+    if (id < 0) return;
+    const int64_t k0 = id % tilesK * BN;
+    id /= tilesK;
+    const int64_t n0 = id % tilesN * BM;
+    const int64_t g = id / tilesN;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int rowA = (wave % WM) * MI * 32, rowB = (wave / WM) * NI * 32;
+    int32_t begin, end;
+    GroupRows(p.offsets, p.rows, static_cast<int>(g), begin, end);
+    typename Mma32<T>::Acc acc[MI][NI] = {};
+    if (begin < end) {
+        OperandA a;
+        OperandB b;
+        a.Init(p.grad, p.ldg * 2, n0, p.n, nullptr, p.rows, begin, end);
+        b.Init(p.x, p.ldx * 2, k0, p.k, p.row_index, p.rows_x, begin, end);
+        MultiplyTile<T, MI, NI>(a, b, lds, (end - begin + 63) / 64, rowA, rowB, acc);
+    }
+    TOut* w = static_cast<TOut*>(p.w) + g * p.stride_w;
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+        const int64_t n = n0 + rowA + i * 32 + (lane & 31);
+        if (n >= p.n) continue;
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int64_t k = k0 + rowB + j * 32 + q * 8 + (lane >> 5) * 4;
+                const float v[4] = {acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2],
+                                    acc[i][j][q * 4 + 3]};
+                StoreFour<TOut>(w + n * p.ldw + k, p.k - k, wideW, v);
+            }
+        }
+    }
+}
+
 int64_t CeilDiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+bool Aligned16(const void* p, int64_t strideBytes) { return (reinterpret_cast<uintptr_t>(p) | strideBytes) % 16 == 0; }
 
 // The most tiles of `height` rows: every group, and the tail, may end inside one.
 int64_t MaxRowTiles(const int32_t* offsets, int64_t rows, int64_t groups, int64_t height)
@@ -222,9 +596,36 @@ int64_t MaxRowTiles(const int32_t* offsets, int64_t rows, int64_t groups, int64_
     return most < rows ? most : rows;
 }
 
+template <typename T, typename TOut, bool kBTrans, int MI, int NI, int WM, int WN>
+int LaunchTiles(const GroupedLaunch& l, hipStream_t s)
+{
+    const int64_t tilesN = CeilDiv(l.n, NI * WN * 32);
+    const int64_t grid = CeilDiv(MaxRowTiles(l.offsets, l.rows, l.groups, MI * WM * 32) * tilesN, 8) * 8;
+    if (grid > INT32_MAX) return kTooLarge;
+    const bool wideC = reinterpret_cast<uintptr_t>(l.c) % (4 * sizeof(TOut)) == 0 && l.ldc % 4 == 0;
+    GroupedTileKernel<T, TOut, kBTrans, MI, NI, WM, WN>
+        <<<static_cast<uint32_t>(grid), WM * WN * 64, 0, s>>>(l, static_cast<int32_t>(tilesN), wideC);
+    return 0;
+}
+
+template <typename T, typename TOut, bool kBTrans>
+int GroupedAligned(const GroupedLaunch& l, hipStream_t s)
+{
+    return LaunchTiles<T, TOut, kBTrans, 4, 4, 2, 2>(l, s);
+}
+
 template <typename T, typename TOut>
 int GroupedTyped(const GroupedLaunch& l, hipStream_t s)
 {
+    constexpr int64_t kSize = sizeof(T);
+    const int64_t inner = l.b_trans ? l.k : l.n;  // what a row of B holds
+    if (Aligned16(l.a, l.lda * kSize) && Aligned16(l.b, l.ldb * kSize) && Aligned16(l.b, l.stride_b * kSize) &&
+        l.k * kSize % 16 == 0 && inner * kSize % 16 == 0) {
+        if constexpr (kSize == 2) {
+            if (!l.b_trans) return GroupedAligned<T, TOut, false>(l, s);
+        }
+        return GroupedAligned<T, TOut, true>(l, s);
+    }
     const int64_t tilesN = CeilDiv(l.n, kAnyTile);
     const int64_t grid = MaxRowTiles(l.offsets, l.rows, l.groups, kAnyTile) * tilesN;
     if (grid > INT32_MAX) return kTooLarge;
@@ -238,9 +639,25 @@ int GroupedTyped(const GroupedLaunch& l, hipStream_t s)
     return 0;
 }
 
+template <typename T, typename TOut, int MI, int NI, int WM, int WN>
+int LaunchGradTiles(const GroupedGradLaunch& l, hipStream_t s)
+{
+    const int64_t tilesN = CeilDiv(l.n, MI * WM * 32), tilesK = CeilDiv(l.k, NI * WN * 32);
+    if (tilesN * tilesK > (INT32_MAX - 7) / l.groups) return kTooLarge;
+    const int64_t grid = CeilDiv(tilesN * tilesK * l.groups, 8) * 8;
+    const bool wideW = reinterpret_cast<uintptr_t>(l.w) % (4 * sizeof(TOut)) == 0 && l.ldw % 4 == 0 &&
+                       (l.groups == 1 || l.stride_w % 4 == 0);
+    GroupedGradTileKernel<T, TOut, MI, NI, WM, WN><<<static_cast<uint32_t>(grid), WM * WN * 64, 0, s>>>(
+        l, static_cast<int32_t>(tilesN), static_cast<int32_t>(tilesK), wideW);
+    return 0;
+}
+
 template <typename T, typename TOut>
 int GroupedGradTyped(const GroupedGradLaunch& l, hipStream_t s)
 {
+    if (Aligned16(l.grad, l.ldg * 2) && Aligned16(l.x, l.ldx * 2) && l.n % 8 == 0 && l.k % 8 == 0) {
+        return LaunchGradTiles<T, TOut, 4, 4, 2, 2>(l, s);
+    }
     const int64_t tilesN = CeilDiv(l.n, kAnyTile), tilesK = CeilDiv(l.k, kAnyTile);
     if (tilesN * tilesK > INT32_MAX / l.groups) return kTooLarge;
     GroupedGradAnyKernel<T, TOut><<<static_cast<uint32_t>(tilesN * tilesK * l.groups), 256, 0, s>>>(

@@ -226,7 +226,6 @@ using Int16 = int __attribute__((ext_vector_type(16)));
 using Short4 = short __attribute__((ext_vector_type(4)));
 
 constexpr int kTurnBytes = 128;
-constexpr int kStepsPerTurn = 4;  // of 32 bytes (16 elements of 16 bits) per row
 
 // 32x32 matrix instructions: lane l holds row l % 32 of its operand,
 // contraction bytes (l / 32) * 16 on.  The result's lane l holds column l % 32
@@ -271,44 +270,43 @@ __device__ __forceinline__ void CopyToLds(const char* from, char* to)
                                      (__attribute__((address_space(3))) void*)(to), 16, 0, 0);
 }
 
+__device__ __forceinline__ int WaveNumber() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
 // An operand whose rows run along the contraction: R rows of 128 bytes per
-// turn.  Its 16-byte chunk c of row r lies at slot c ^ (r & 7), so that the
-// lanes that read one chunk of eight rows touch every bank once.
+// turn.  Its 16-byte chunk c of row r lies at slot c ^ (r / 2 & 7), so that the
+// lanes that read one chunk of 16 rows touch each of the 64 banks once.
 template <int R, int kThreads>
 struct RowOperand {
     static constexpr int kLoads = R * 8 / kThreads;
     static constexpr int kRowsPerLoad = kThreads / 8;
     static constexpr int kBytes = R * kTurnBytes;
+    static constexpr int kReads = 1;  // LDS loads per operand of a matrix step
     const char* ptr[kLoads];
-    int64_t left;  // bytes of the contraction from the next turn on
 
     // This thread's rows are Row(i); its chunk of each is the same.
     static __device__ __forceinline__ int Row(int i) { return i * kRowsPerLoad + (threadIdx.x >> 3); }
-    static __device__ __forceinline__ int Chunk() { return (threadIdx.x & 7) ^ ((threadIdx.x >> 3) & 7); }
+    static __device__ __forceinline__ int Chunk() { return (threadIdx.x & 7) ^ ((threadIdx.x >> 4) & 7); }
 
-    __device__ __forceinline__ void Issue(char* lds)
+    // Copies this thread's chunks of the next turn (every row's first `bytes` of 128 hold operands).
+    __device__ __forceinline__ void Prepare(int64_t bytes)
     {
-        const char* zero = reinterpret_cast<const char*>(&kZeros);
-        char* to = lds + (threadIdx.x >> 6) * 1024;
-        if (left >= kTurnBytes) {
+        if (bytes < kTurnBytes && Chunk() * 16 >= bytes) {
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                CopyToLds(ptr[i], to + i * kThreads * 16);
-                ptr[i] += kTurnBytes;
-            }
-        } else {
-            const bool in = Chunk() * 16 < left;
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) CopyToLds(in ? ptr[i] : zero, to + i * kThreads * 16);
+            for (int i = 0; i < kLoads; ++i) ptr[i] = reinterpret_cast<const char*>(&kZeros);
         }
-        left -= kTurnBytes;
     }
+    __device__ __forceinline__ void Issue(char* lds, int i)
+    {
+        CopyToLds(ptr[i], lds + WaveNumber() * 1024 + i * kThreads * 16);
+        ptr[i] += kTurnBytes;
+    }
+    __device__ __forceinline__ void LookUp() {}
 
     // The operand of one matrix step: 32 rows from `row` on.
     static __device__ __forceinline__ Int4 Read(const char* lds, int row, int step)
     {
         const int lane = threadIdx.x & 63;
-        const int chunk = (step * 2 + (lane >> 5)) ^ (lane & 7);
+        const int chunk = (step * 2 + (lane >> 5)) ^ ((lane >> 1) & 7);
         return *reinterpret_cast<const Int4*>(lds + (row + (lane & 31)) * kTurnBytes + chunk * 16);
     }
 };
@@ -319,18 +317,20 @@ struct RowOperand {
 // and lane i receives the 4 rows of column i.  Chunk c of row r lies at slot
 // c ^ 4 (r & 3): the four rows of 64 bytes that 32 lanes read then touch
 // every bank once.
-template <int C, int kThreads>
+template <int C, int kThreads, bool kIndexed>
 struct ColumnOperand {
     static constexpr int kChunks = C / 8;
     static constexpr int kRowsPerLoad = kThreads / kChunks;
     static constexpr int kLoads = 64 / kRowsPerLoad;
     static constexpr int kBytes = 64 * C * 2;
-    const char* base;  // chunk of row 0, or null when the chunk lies past the last column
+    static constexpr int kReads = 2;
+    const char* ptr[kLoads];
+    const char* base;  // this thread's chunk of row 0
     int64_t ld;        // bytes
     const int32_t* index;
     int64_t count;     // rows that an index may name
     int32_t row, end;  // of this thread's first load in the next turn, and of all
-    int32_t next[kLoads];
+    int32_t next[kIndexed ? kLoads : 1];
 
     static __device__ __forceinline__ int Row(int i) { return i * kRowsPerLoad + threadIdx.x / kChunks; }
     static __device__ __forceinline__ int Chunk()
@@ -342,38 +342,56 @@ struct ColumnOperand {
                                          const int32_t* rowIndex, int64_t rowCount, int32_t first, int32_t last)
     {
         const int64_t c = column + Chunk() * 8;
-        base = c < columns ? static_cast<const char*>(p) + c * 2 : nullptr;
+        const bool in = c < columns;
+        base = static_cast<const char*>(p) + c * 2;
         ld = ldBytes;
         index = rowIndex;
         count = rowCount;
         row = first + Row(0);
         end = last;
-        Fetch();
-    }
-
-    // The rows of the next turn: their indices are read a turn ahead.
-    __device__ __forceinline__ void Fetch()
-    {
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int32_t r = row + i * kRowsPerLoad;
-            next[i] = r < end ? (index != nullptr ? index[r] : r) : -1;
+        for (int i = 0; i < kLoads; ++i) ptr[i] = base + (row + i * kRowsPerLoad) * ld;
+        LookUp();
+        if (!in) {
+            ld = 0;
+            base = reinterpret_cast<const char*>(&kZeros);
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) ptr[i] = base;
         }
     }
 
-    __device__ __forceinline__ void Issue(char* lds)
+    // The next turn's rows; those past the end, which only the last turn has, read as zero.
+    __device__ __forceinline__ void Prepare(int64_t bytes)
     {
-        const char* zero = reinterpret_cast<const char*>(&kZeros);
-        char* to = lds + (threadIdx.x >> 6) * 1024;
+        if constexpr (kIndexed) {
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            int32_t r = next[i];
-            if (index != nullptr && row + i * kRowsPerLoad < end && (r < 0 || r >= count)) r = 0;
-            const char* from = base + r * ld;
-            CopyToLds(base != nullptr && r >= 0 ? from : zero, to + i * kThreads * 16);
+            for (int i = 0; i < kLoads; ++i) {
+                ptr[i] = base + (next[i] < 0 || next[i] >= count ? 0 : next[i]) * ld;
+            }
+        }
+        if (bytes < kTurnBytes) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                if (row + i * kRowsPerLoad >= end) ptr[i] = reinterpret_cast<const char*>(&kZeros);
+            }
         }
         row += 64;
-        Fetch();
+    }
+    __device__ __forceinline__ void Issue(char* lds, int i)
+    {
+        CopyToLds(ptr[i], lds + WaveNumber() * 1024 + i * kThreads * 16);
+        if constexpr (!kIndexed) ptr[i] += 64 * ld;
+    }
+    // The indices of the turn after: they arrive while this one is multiplied.
+    __device__ __forceinline__ void LookUp()
+    {
+        if constexpr (kIndexed) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int32_t r = row + i * kRowsPerLoad;
+                next[i] = index[r < end ? r : end - 1];
+            }
+        }
     }
 
     static __device__ __forceinline__ Int4 Read(const char* lds, int column, int step)
@@ -392,73 +410,176 @@ struct ColumnOperand {
     }
 };
 
+// Orders a step's instructions: its LDS reads follow its first matrix
+// instructions, so that they have arrived when the next step starts, and its
+// copies the others.
+template <int kProducts, int kReads, int kCopies>
+__device__ __forceinline__ void Interleave()
+{
+    constexpr int kMfma = 0x8, kVmem = 0x10, kDsRead = 0x100;
+    constexpr int kHalf = kProducts / 2 > 0 ? kProducts / 2 : 1;
+    constexpr int kReadsPer = (kReads + kHalf - 1) / kHalf, kCopiesPer = (kCopies + kHalf - 1) / kHalf;
+#pragma unroll
+    for (int i = 0; i < kHalf; ++i) {
+        __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kDsRead, kReadsPer, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < kProducts - kHalf; ++i) {
+        __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+        if constexpr (kCopies > 0) __builtin_amdgcn_sched_group_barrier(kVmem, kCopiesPer, 0);
+    }
+}
+
 // Waits for this wave's copies and reads, then for the other waves'.
 __device__ __forceinline__ void WaitAll()
 {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
 
-// acc += the product over `turns` turns; MI x NI tiles of 32x32 per wave from
-// rows (columns of the output) rowA and rowB on.
+// acc += the product over `bytes` of the contraction (of 16-bit elements when
+// an operand's rows run across it); MI x NI tiles of 32x32 per wave from rows
+// (columns of the output) rowA and rowB on.
+//
+// One turn is four matrix steps.  While a step is multiplied the next one's
+// operands are read from LDS (the group barriers below keep the compiler from
+// moving the reads behind the products they are meant to overlap), and in its
+// first two steps a turn issues the copies of the next.  One barrier per turn,
+// before its last step: by then every wave has read this turn's operands
+// and the next turn's have arrived.
 template <typename T, int MI, int NI, typename OperandA, typename OperandB>
-__device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds, int64_t turns, int rowA, int rowB,
+__device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds, int64_t bytes, int rowA, int rowB,
                                              typename Mma32<T>::Acc (&acc)[MI][NI])
 {
     constexpr int kBuffer = OperandA::kBytes + OperandB::kBytes;
+    constexpr int kCopies = OperandA::kLoads + OperandB::kLoads;
+    constexpr int kReads = MI * OperandA::kReads + NI * OperandB::kReads;
     Int4 fa[2][MI], fb[2][NI];
-    a.Issue(lds);
-    b.Issue(lds + OperandA::kBytes);
+    auto read = [&](int to, const char* from, int step) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) fa[to][i] = OperandA::Read(from, rowA + i * 32, step);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) fb[to][i] = OperandB::Read(from + OperandA::kBytes, rowB + i * 32, step);
+    };
+    auto multiply = [&](int with) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+#pragma unroll
+            for (int j = 0; j < NI; ++j) acc[i][j] = Mma32<T>::Run(fb[with][j], fa[with][i], acc[i][j]);
+        }
+    };
+    auto copy = [&](char* to, int first, int last) {
+#pragma unroll
+        for (int i = first; i < last; ++i) {
+            if (i < OperandA::kLoads) {
+                a.Issue(to, i);
+            } else {
+                b.Issue(to + OperandA::kBytes, i - OperandA::kLoads);
+            }
+        }
+    };
+    int cur = 0;
+    auto turn = [&](auto copies) {
+        constexpr int kHalf = decltype(copies)::value / 2, kAll = decltype(copies)::value;
+        char* now = lds + cur;
+        cur ^= kBuffer;
+        char* next = lds + cur;
+        read(1, now, 1);
+        copy(next, 0, kHalf);
+        multiply(0);
+        Interleave<MI * NI, kReads, kHalf>();
+        read(0, now, 2);
+        copy(next, kHalf, kAll);
+        multiply(1);
+        Interleave<MI * NI, kReads, kAll - kHalf>();
+        if constexpr (kAll > 0) {
+            a.LookUp();
+            b.LookUp();
+        }
+        read(1, now, 3);
+        multiply(0);
+        Interleave<MI * NI, kReads, 0>();
+        WaitAll();
+        if constexpr (kAll > 0) read(0, next, 0);
+        multiply(1);
+        if constexpr (kAll > 0) Interleave<MI * NI, kReads, 0>();
+    };
+    a.Prepare(bytes);
+    b.Prepare(bytes);
+    copy(lds, 0, kCopies);
+    a.LookUp();
+    b.LookUp();
     WaitAll();
-#pragma unroll
-    for (int i = 0; i < MI; ++i) fa[0][i] = OperandA::Read(lds, rowA + i * 32, 0);
-#pragma unroll
-    for (int i = 0; i < NI; ++i) fb[0][i] = OperandB::Read(lds + OperandA::kBytes, rowB + i * 32, 0);
-    char* cur = lds;
-    char* other = lds + kBuffer;
-    for (int64_t t = 0; t < turns; ++t) {
-        if (t + 1 < turns) {
-            a.Issue(other);
-            b.Issue(other + OperandA::kBytes);
-        }
-#pragma unroll
-        for (int s = 0; s < kStepsPerTurn; ++s) {
-            const int next = (s + 1) & 1;
-            if (s + 1 == kStepsPerTurn) {
-                WaitAll();
-                char* swap = cur;
-                cur = other;
-                other = swap;
-            }
-            const int step = (s + 1) % kStepsPerTurn;
-#pragma unroll
-            for (int i = 0; i < MI; ++i) fa[next][i] = OperandA::Read(cur, rowA + i * 32, step);
-#pragma unroll
-            for (int i = 0; i < NI; ++i) fb[next][i] = OperandB::Read(cur + OperandA::kBytes, rowB + i * 32, step);
-#pragma unroll
-            for (int i = 0; i < MI; ++i) {
-#pragma unroll
-                for (int j = 0; j < NI; ++j) acc[i][j] = Mma32<T>::Run(fb[s & 1][j], fa[s & 1][i], acc[i][j]);
-            }
-        }
+    read(0, lds, 0);
+    for (bytes -= kTurnBytes; bytes > 0; bytes -= kTurnBytes) {
+        a.Prepare(bytes);
+        b.Prepare(bytes);
+        turn(std::integral_constant<int, kCopies>{});
     }
+    turn(std::integral_constant<int, 0>{});
 }
 
-// Four consecutive values of a row of the output.
-template <typename TOut>
-__device__ __forceinline__ void StoreFour(TOut* p, int64_t left, bool wide, const float (&v)[4])
+// Writes a wave's MI*32 x NI*32 tile of the output, rows [0, rows) and columns
+// [0, columns) of it, at c.  A result's lanes hold neighbouring rows: stored
+// from there, each store would touch 32 rows by 8 bytes (a 256x256 tile then
+// took 68 us).  The wave passes its tile through its own part of LDS instead
+// and stores whole rows, 16 bytes per lane.  value(i, j, q, v) gives the four
+// values of tile (i, j) in registers 4q on.  Chunk c of row r lies at slot
+// c ^ r, which spreads the rows of a write over the banks.
+template <typename TOut, int MI, int NI, int kLdsBytes, typename Value>
+__device__ __forceinline__ void StoreTile(char* lds, TOut* c, int64_t ldc, int64_t rows, int64_t columns, bool wide,
+                                          Value value)
 {
-    TOut o[4];
+    constexpr int kRowBytes = NI * 32 * static_cast<int>(sizeof(TOut));
+    constexpr int kChunks = kRowBytes / 16, kPer = 16 / static_cast<int>(sizeof(TOut));
+    constexpr int kTiles = kLdsBytes / (32 * kRowBytes) < MI ? kLdsBytes / (32 * kRowBytes) : MI;  // at a time
+    constexpr int kRowsPerStore = 64 / kChunks;
+    static_assert(kTiles > 0 && kChunks <= 64, "a row of tiles must fit the wave's LDS");
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = FromFloat<TOut>(v[i]);
-    if (wide && left >= 4) {
-        __builtin_memcpy(__builtin_assume_aligned(p, sizeof(o)), o, sizeof(o));
-    } else {
+    for (int first = 0; first < MI; first += kTiles) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (i < left) p[i] = o[i];
+        for (int i = first; i < first + kTiles && i < MI; ++i) {
+            const int r = (i - first) * 32 + (lane & 31);
+#pragma unroll
+            for (int j = 0; j < NI; ++j) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    float v[4];
+                    value(i, j, q, v);
+                    TOut o[4];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) o[x] = FromFloat<TOut>(v[x]);
+                    const int byte = (j * 32 + q * 8 + (lane >> 5) * 4) * static_cast<int>(sizeof(TOut));
+                    char* to = lds + r * kRowBytes + (((byte >> 4) ^ (r & (kChunks - 1))) << 4) + (byte & 8);
+                    __builtin_memcpy(__builtin_assume_aligned(to, sizeof(o)), o, sizeof(o));
+                }
+            }
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const int base = first * 32;
+#pragma unroll 4
+        for (int r = lane / kChunks; r < kTiles * 32; r += kRowsPerStore) {
+            const int chunk = (lane % kChunks) ^ (r & (kChunks - 1));
+            const int64_t left = columns - chunk * kPer;
+            if (base + r >= rows || left <= 0) continue;
+            const Int4 v = *reinterpret_cast<const Int4*>(lds + r * kRowBytes + (lane % kChunks) * 16);
+            TOut* to = c + (base + r) * ldc + chunk * kPer;
+            if (wide && left >= kPer) {
+                *reinterpret_cast<Int4*>(to) = v;
+            } else {
+                TOut o[kPer];
+                __builtin_memcpy(o, &v, 16);
+#pragma unroll
+                for (int x = 0; x < kPer; ++x) {
+                    if (x < left) to[x] = o[x];
+                }
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 }
 
@@ -477,14 +598,15 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void GroupedTileKernel(GroupedLaun
 {
     constexpr int kThreads = WM * WN * 64, BM = MI * WM * 32, BN = NI * WN * 32;
     using OperandA = RowOperand<BM, kThreads>;
-    using OperandB = std::conditional_t<kBTrans, RowOperand<BN, kThreads>, ColumnOperand<BN, kThreads>>;
-    __shared__ __align__(128) char lds[2 * (OperandA::kBytes + OperandB::kBytes)];
+    using OperandB = std::conditional_t<kBTrans, RowOperand<BN, kThreads>, ColumnOperand<BN, kThreads, false>>;
+    constexpr int kLds = 2 * (OperandA::kBytes + OperandB::kBytes);
+    __shared__ __align__(128) char lds[kLds];
     const int64_t id = TileOfWorkgroup(static_cast<int64_t>(CountTiles(p.offsets, p.rows, p.groups, BM)) * tilesN);
     if (id < 0) return;
     const RaggedTile tile = FindTile(p.offsets, p.rows, p.groups, BM, static_cast<int32_t>(id / tilesN));
     if (tile.group < 0) return;
     const int64_t n0 = id % tilesN * BN;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = WaveNumber();
     const int rowA = (wave % WM) * MI * 32, rowB = (wave / WM) * NI * 32;
     typename Mma32<T>::Acc acc[MI][NI] = {};
     const bool real = tile.group < p.groups;
@@ -499,62 +621,62 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void GroupedTileKernel(GroupedLaun
             const int64_t row = IndexedRow(p.row_index, r < tile.end ? r : tile.row, p.rows_a);
             a.ptr[i] = reinterpret_cast<const char*>(static_cast<const T*>(p.a) + row * p.lda) + OperandA::Chunk() * 16;
         }
-        a.left = p.k * static_cast<int64_t>(sizeof(T));
         if constexpr (kBTrans) {
 #pragma unroll
             for (int i = 0; i < OperandB::kLoads; ++i) {
                 const int64_t n = n0 + OperandB::Row(i);
                 b.ptr[i] = reinterpret_cast<const char*>(bg + (n < p.n ? n : n0) * p.ldb) + OperandB::Chunk() * 16;
             }
-            b.left = a.left;
         } else {
             b.Init(bg, p.ldb * 2, n0, p.n, nullptr, p.k, 0, static_cast<int32_t>(p.k));
         }
-        MultiplyTile<T, MI, NI>(a, b, lds, (a.left + kTurnBytes - 1) / kTurnBytes, rowA, rowB, acc);
+        MultiplyTile<T, MI, NI>(a, b, lds, p.k * static_cast<int64_t>(sizeof(T)), rowA, rowB, acc);
     }
+    const int64_t n = n0 + rowB;
+    TOut* c = static_cast<TOut*>(p.c) + (tile.row + rowA) * p.ldc + n;
+    char* part = lds + wave * (kLds / (WM * WN));
+    if constexpr (sizeof(T) == 1) {
+        float sa[MI], sb[NI][4][4];
 #pragma unroll
-    for (int i = 0; i < MI; ++i) {
-        const int32_t r = tile.row + rowA + i * 32 + (lane & 31);
-        if (r >= tile.end) continue;
-        float sa = 0.0f;
-        if constexpr (sizeof(T) == 1) {
-            if (real) sa = p.scale_a[IndexedRow(p.row_index, r, p.rows_a)];
+        for (int i = 0; i < MI; ++i) {
+            const int32_t r = tile.row + rowA + i * 32 + (lane & 31);
+            sa[i] = real && r < tile.end ? p.scale_a[IndexedRow(p.row_index, r, p.rows_a)] : 0.0f;
         }
-        TOut* c = static_cast<TOut*>(p.c) + r * p.ldc;
 #pragma unroll
-        for (int j = 0; j < NI; ++j) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int64_t n = n0 + rowB + j * 32 + q * 8 + (lane >> 5) * 4;
-                float v[4];
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    v[x] = static_cast<float>(acc[i][j][q * 4 + x]);
-                    if constexpr (sizeof(T) == 1) {
-                        if (real && n + x < p.n) v[x] *= sa * p.scale_b[tile.group * p.n + n + x];
-                    }
-                }
-                StoreFour<TOut>(c + n, p.n - n, wideC, v);
-            }
+        for (int j = 0; j < NI * 16; ++j) {
+            const int64_t at = n + j / 4 * 8 + (lane >> 5) * 4 + j % 4;
+            sb[j / 16][j / 4 % 4][j % 4] = real && at < p.n ? p.scale_b[tile.group * p.n + at] : 0.0f;
         }
+        StoreTile<TOut, MI, NI, kLds / (WM * WN)>(
+            part, c, p.ldc, tile.end - tile.row - rowA, p.n - n, wideC, [&](int i, int j, int q, float(&v)[4]) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) v[x] = static_cast<float>(acc[i][j][q * 4 + x]) * (sa[i] * sb[j][q][x]);
+            });
+    } else {
+        StoreTile<TOut, MI, NI, kLds / (WM * WN)>(
+            part, c, p.ldc, tile.end - tile.row - rowA, p.n - n, wideC, [&](int i, int j, int q, float(&v)[4]) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) v[x] = acc[i][j][q * 4 + x];
+            });
     }
 }
 
-template <typename T, typename TOut, int MI, int NI, int WM, int WN>
+template <typename T, typename TOut, bool kIndexed, int MI, int NI, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64, 1) void GroupedGradTileKernel(GroupedGradLaunch p, int32_t tilesN,
                                                                         int32_t tilesK, bool wideW)
 {
     constexpr int kThreads = WM * WN * 64, BM = MI * WM * 32, BN = NI * WN * 32;
-    using OperandA = ColumnOperand<BM, kThreads>;
-    using OperandB = ColumnOperand<BN, kThreads>;
-    __shared__ __align__(128) char lds[2 * (OperandA::kBytes + OperandB::kBytes)];
+    using OperandA = ColumnOperand<BM, kThreads, false>;
+    using OperandB = ColumnOperand<BN, kThreads, kIndexed>;
+    constexpr int kLds = 2 * (OperandA::kBytes + OperandB::kBytes);
+    __shared__ __align__(128) char lds[kLds];
     int64_t id = TileOfWorkgroup(static_cast<int64_t>(tilesN) * tilesK * p.groups);
     if (id < 0) return;
     const int64_t k0 = id % tilesK * BN;
     id /= tilesK;
     const int64_t n0 = id % tilesN * BM;
     const int64_t g = id / tilesN;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = WaveNumber();
     const int rowA = (wave % WM) * MI * 32, rowB = (wave / WM) * NI * 32;
     int32_t begin, end;
     GroupRows(p.offsets, p.rows, static_cast<int>(g), begin, end);
@@ -564,24 +686,15 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void GroupedGradTileKernel(Grouped
         OperandB b;
         a.Init(p.grad, p.ldg * 2, n0, p.n, nullptr, p.rows, begin, end);
         b.Init(p.x, p.ldx * 2, k0, p.k, p.row_index, p.rows_x, begin, end);
-        MultiplyTile<T, MI, NI>(a, b, lds, (end - begin + 63) / 64, rowA, rowB, acc);
+        MultiplyTile<T, MI, NI>(a, b, lds, static_cast<int64_t>(end - begin) * 2, rowA, rowB, acc);
     }
-    TOut* w = static_cast<TOut*>(p.w) + g * p.stride_w;
+    const int64_t n = n0 + rowA, k = k0 + rowB;
+    StoreTile<TOut, MI, NI, kLds / (WM * WN)>(lds + wave * (kLds / (WM * WN)),
+                                              static_cast<TOut*>(p.w) + g * p.stride_w + n * p.ldw + k, p.ldw, p.n - n,
+                                              p.k - k, wideW, [&](int i, int j, int q, float(&v)[4]) {
 #pragma unroll
-    for (int i = 0; i < MI; ++i) {
-        const int64_t n = n0 + rowA + i * 32 + (lane & 31);
-        if (n >= p.n) continue;
-#pragma unroll
-        for (int j = 0; j < NI; ++j) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int64_t k = k0 + rowB + j * 32 + q * 8 + (lane >> 5) * 4;
-                const float v[4] = {acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2],
-                                    acc[i][j][q * 4 + 3]};
-                StoreFour<TOut>(w + n * p.ldw + k, p.k - k, wideW, v);
-            }
-        }
-    }
+                                                  for (int x = 0; x < 4; ++x) v[x] = acc[i][j][q * 4 + x];
+                                              });
 }
 
 int64_t CeilDiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -602,7 +715,7 @@ int LaunchTiles(const GroupedLaunch& l, hipStream_t s)
     const int64_t tilesN = CeilDiv(l.n, NI * WN * 32);
     const int64_t grid = CeilDiv(MaxRowTiles(l.offsets, l.rows, l.groups, MI * WM * 32) * tilesN, 8) * 8;
     if (grid > INT32_MAX) return kTooLarge;
-    const bool wideC = reinterpret_cast<uintptr_t>(l.c) % (4 * sizeof(TOut)) == 0 && l.ldc % 4 == 0;
+    const bool wideC = Aligned16(l.c, l.ldc * static_cast<int64_t>(sizeof(TOut)));
     GroupedTileKernel<T, TOut, kBTrans, MI, NI, WM, WN>
         <<<static_cast<uint32_t>(grid), WM * WN * 64, 0, s>>>(l, static_cast<int32_t>(tilesN), wideC);
     return 0;
@@ -645,10 +758,12 @@ int LaunchGradTiles(const GroupedGradLaunch& l, hipStream_t s)
     const int64_t tilesN = CeilDiv(l.n, MI * WM * 32), tilesK = CeilDiv(l.k, NI * WN * 32);
     if (tilesN * tilesK > (INT32_MAX - 7) / l.groups) return kTooLarge;
     const int64_t grid = CeilDiv(tilesN * tilesK * l.groups, 8) * 8;
-    const bool wideW = reinterpret_cast<uintptr_t>(l.w) % (4 * sizeof(TOut)) == 0 && l.ldw % 4 == 0 &&
-                       (l.groups == 1 || l.stride_w % 4 == 0);
-    GroupedGradTileKernel<T, TOut, MI, NI, WM, WN><<<static_cast<uint32_t>(grid), WM * WN * 64, 0, s>>>(
-        l, static_cast<int32_t>(tilesN), static_cast<int32_t>(tilesK), wideW);
+    constexpr int64_t kOut = sizeof(TOut);
+    const bool wideW = Aligned16(l.w, l.ldw * kOut) && (l.groups == 1 || Aligned16(l.w, l.stride_w * kOut));
+    const auto kernel = l.row_index != nullptr ? GroupedGradTileKernel<T, TOut, true, MI, NI, WM, WN>
+                                               : GroupedGradTileKernel<T, TOut, false, MI, NI, WM, WN>;
+    kernel<<<static_cast<uint32_t>(grid), WM * WN * 64, 0, s>>>(l, static_cast<int32_t>(tilesN),
+                                                                static_cast<int32_t>(tilesK), wideW);
     return 0;
 }
 

@@ -122,6 +122,9 @@ struct RaggedTile {
     int32_t group;
     int32_t row;
     int32_t end;
+    int32_t begin;   // the group's first row,
+    int32_t before;  // the tiles before it
+    int32_t tiles;   // and its own
 };
 
 // The tile-th tile of `height` rows, counted through the groups and the tail.
@@ -139,12 +142,13 @@ __device__ __forceinline__ RaggedTile FindTile(const int32_t* offsets, int64_t r
         if (hit != 0) {
             const int src = __builtin_ctzll(hit);
             const int32_t skipped = before + __builtin_amdgcn_readlane(incl - n, src);
-            return {g0 + src, __builtin_amdgcn_readlane(begin, src) + (tile - skipped) * height,
-                    __builtin_amdgcn_readlane(end, src)};
+            const int32_t first = __builtin_amdgcn_readlane(begin, src);
+            return {g0 + src,  first + (tile - skipped) * height, __builtin_amdgcn_readlane(end, src), first, skipped,
+                    __builtin_amdgcn_readlane(n, src)};
         }
         before += __builtin_amdgcn_readlane(incl, 63);
     }
-    return {-1, 0, 0};
+    return {-1, 0, 0, 0, 0, 0};
 }
 
 }  // namespace aclsp

@@ -55,66 +55,6 @@ struct Mma<int8_t> {
     }
 };
 
-// ---------------------------------------------------------------------------
-// Kernels for every size, stride and alignment: tiles of 64x64, loaded element
-// by element through registers, zeros beyond the ends.
-// ---------------------------------------------------------------------------
-constexpr int kAnyTile = 64;
-constexpr int kAnyRowBytes = 64;                 // of the contraction per turn
-constexpr int kAnyLdsStride = kAnyRowBytes + 16;  // keeps the 16 rows of a read in different banks
-
-template <typename T>
-struct AnyTiles {
-    static constexpr int kDepth = kAnyRowBytes / static_cast<int>(sizeof(T));
-    static constexpr int kPer = 16 / static_cast<int>(sizeof(T));  // elements per thread and operand
-    typename Mma<T>::Acc acc[2][2];
-
-    // Adds the product of two 64-row tiles held in LDS as [row][contraction].
-    __device__ __forceinline__ void Multiply(const char* a, const char* b)
-    {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        Int4 fa[2], fb[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int ra = (wave & 1) * 32 + i * 16 + (lane & 15), rb = (wave >> 1) * 32 + i * 16 + (lane & 15);
-            fa[i] = *reinterpret_cast<const Int4*>(a + ra * kAnyLdsStride + (lane >> 4) * 16);
-            fb[i] = *reinterpret_cast<const Int4*>(b + rb * kAnyLdsStride + (lane >> 4) * 16);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) acc[i][j] = Mma<T>::Run(fb[j], fa[i], acc[i][j]);
-        }
-    }
-};
-
-// Rows of 64 bytes: thread t holds 16 bytes of row t / 4.
-template <typename T>
-__device__ __forceinline__ void AnyLoadRows(char* lds, const T* row, bool rowOk, int64_t depth, int64_t at)
-{
-    constexpr int kPer = AnyTiles<T>::kPer;
-    const int chunk = threadIdx.x & 3;
-    T v[kPer];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int64_t c = at + chunk * kPer + i;
-        v[i] = rowOk && c < depth ? row[c] : static_cast<T>(0);
-    }
-    __builtin_memcpy(lds + (threadIdx.x >> 2) * kAnyLdsStride + chunk * 16, v, 16);
-}
-
-// The transposed tile: thread t holds 8 columns of contraction row t / 8.
-template <typename T>
-__device__ __forceinline__ void AnyLoadColumns(char* lds, const T* row, bool rowOk, int64_t width, int64_t at)
-{
-    const int kk = threadIdx.x >> 3, c0 = (threadIdx.x & 7) * 8;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const T v = rowOk && at + c0 + i < width ? row[at + c0 + i] : static_cast<T>(0);
-        *reinterpret_cast<T*>(lds + (c0 + i) * kAnyLdsStride + kk * sizeof(T)) = v;
-    }
-}
-
 __device__ __forceinline__ int64_t IndexedRow(const int32_t* index, int64_t r, int64_t count)
 {
     if (index == nullptr) return r;
@@ -122,104 +62,12 @@ __device__ __forceinline__ int64_t IndexedRow(const int32_t* index, int64_t r, i
     return i < 0 || i >= count ? 0 : i;  // stays within the operand whatever the index holds
 }
 
-template <typename T, typename TOut, bool kBTrans>
-__global__ __launch_bounds__(256) void GroupedAnyKernel(GroupedLaunch p, int32_t tilesN)
-{
-    __shared__ __align__(16) char lds[2][kAnyTile * kAnyLdsStride];
-    const RaggedTile tile = FindTile(p.offsets, p.rows, p.groups, kAnyTile, static_cast<int32_t>(blockIdx.x / tilesN));
-    if (tile.group < 0) return;
-    const int64_t n0 = static_cast<int64_t>(blockIdx.x % tilesN) * kAnyTile;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    AnyTiles<T> t{};
-    if (tile.group < p.groups) {
-        const T* b = static_cast<const T*>(p.b) + tile.group * p.stride_b;
-        const int64_t r = tile.row + (threadIdx.x >> 2), nb = n0 + (threadIdx.x >> 2);
-        const bool aOk = r < tile.end, bOk = nb < p.n;
-        const T* aRow = static_cast<const T*>(p.a) + (aOk ? IndexedRow(p.row_index, r, p.rows_a) : 0) * p.lda;
-        for (int64_t k0 = 0; k0 < p.k; k0 += AnyTiles<T>::kDepth) {
-            AnyLoadRows<T>(lds[0], aRow, aOk, p.k, k0);
-            if constexpr (kBTrans) {
-                AnyLoadRows<T>(lds[1], b + nb * p.ldb, bOk, p.k, k0);
-            } else {
-                const int64_t kk = k0 + (threadIdx.x >> 3);
-                AnyLoadColumns<T>(lds[1], b + kk * p.ldb, kk < p.k, p.n, n0);
-            }
-            __syncthreads();
-            t.Multiply(lds[0], lds[1]);
-            __syncthreads();
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int64_t r = tile.row + (wave & 1) * 32 + i * 16 + (lane & 15);
-        if (r >= tile.end) continue;
-        float sa = 1.0f;
-        if constexpr (sizeof(T) == 1) {
-            if (tile.group < p.groups) sa = p.scale_a[IndexedRow(p.row_index, r, p.rows_a)];
-        }
-        TOut* c = static_cast<TOut*>(p.c) + r * p.ldc;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int64_t n = n0 + (wave >> 1) * 32 + j * 16 + (lane >> 4) * 4 + x;
-                if (n >= p.n) continue;
-                float v = static_cast<float>(t.acc[i][j][x]);
-                if constexpr (sizeof(T) == 1) {
-                    if (tile.group < p.groups) v = v * (sa * p.scale_b[tile.group * p.n + n]);
-                }
-                c[n] = FromFloat<TOut>(v);
-            }
-        }
-    }
-}
-
-template <typename T, typename TOut>
-__global__ __launch_bounds__(256) void GroupedGradAnyKernel(GroupedGradLaunch p, int32_t tilesN, int32_t tilesK)
-{
-    __shared__ __align__(16) char lds[2][kAnyTile * kAnyLdsStride];
-    uint32_t id = blockIdx.x;
-    const int64_t k0 = static_cast<int64_t>(id % tilesK) * kAnyTile;
-    id /= tilesK;
-    const int64_t n0 = static_cast<int64_t>(id % tilesN) * kAnyTile;
-    const int64_t g = id / tilesN;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int32_t begin, end;
-    GroupRows(p.offsets, p.rows, static_cast<int>(g), begin, end);
-    AnyTiles<T> t{};
-    for (int64_t r0 = begin; r0 < end; r0 += AnyTiles<T>::kDepth) {
-        const int64_t r = r0 + (threadIdx.x >> 3);
-        const bool ok = r < end;
-        AnyLoadColumns<T>(lds[0], static_cast<const T*>(p.grad) + r * p.ldg, ok, p.n, n0);
-        AnyLoadColumns<T>(lds[1], static_cast<const T*>(p.x) + (ok ? IndexedRow(p.row_index, r, p.rows_x) : 0) * p.ldx,
-                          ok, p.k, k0);
-        __syncthreads();
-        t.Multiply(lds[0], lds[1]);
-        __syncthreads();
-    }
-    TOut* w = static_cast<TOut*>(p.w) + g * p.stride_w;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int64_t n = n0 + (wave & 1) * 32 + i * 16 + (lane & 15);
-        if (n >= p.n) continue;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int64_t k = k0 + (wave >> 1) * 32 + j * 16 + (lane >> 4) * 4 + x;
-                if (k < p.k) w[n * p.ldw + k] = FromFloat<TOut>(t.acc[i][j][x]);
-            }
-        }
-    }
-}
-
 // ---------------------------------------------------------------------------
-// Kernels for operands whose rows are aligned to 16 bytes: large tiles, copied
-// from memory to LDS without passing registers, 32x32 matrix instructions.
-//
-// A tile's contraction advances by 128 bytes per turn.  Two buffers in LDS:
-// while one is multiplied the next is copied.  Each wave keeps the operands
-// of one matrix step ahead of the one it multiplies in registers.
+// Tiles through LDS, 32x32 matrix instructions.  A tile's contraction advances
+// by 128 bytes per turn.  Two buffers in LDS: while one is multiplied the next
+// is copied, straight from memory where every row is aligned to 16 bytes,
+// through registers by loads of any alignment where not.  Each wave keeps the
+// operands of one matrix step ahead of the one it multiplies in registers.
 // ---------------------------------------------------------------------------
 using Float16 = float __attribute__((ext_vector_type(16)));
 using Int16 = int __attribute__((ext_vector_type(16)));
@@ -270,35 +118,88 @@ __device__ __forceinline__ void CopyToLds(const char* from, char* to)
                                      (__attribute__((address_space(3))) void*)(to), 16, 0, 0);
 }
 
+// The first `valid` bytes at `from` of any alignment (of T's at least), zeros after them.
+template <typename T>
+__device__ __forceinline__ Int4 LoadUnaligned(const char* from, int valid)
+{
+    Int4 v;
+    if (valid >= 16) {
+        __builtin_memcpy(&v, from, 16);
+        return v;
+    }
+    T e[16 / sizeof(T)];
+#pragma unroll
+    for (int i = 0; i < 16 / static_cast<int>(sizeof(T)); ++i) {
+        e[i] = static_cast<T>(0);
+        if (i * static_cast<int>(sizeof(T)) < valid) __builtin_memcpy(&e[i], from + i * sizeof(T), sizeof(T));
+    }
+    __builtin_memcpy(&v, e, 16);
+    return v;
+}
+
+// All of a thread's chunks of a turn; whole ones without a branch between them.
+template <typename T, int N>
+__device__ __forceinline__ void LoadAll(const char* const (&ptr)[N], int valid, Int4 (&held)[N])
+{
+    if (__all(valid >= 16)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) __builtin_memcpy(&held[i], ptr[i], 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) held[i] = LoadUnaligned<T>(ptr[i], valid);
+    }
+}
+
 __device__ __forceinline__ int WaveNumber() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 // An operand whose rows run along the contraction: R rows of 128 bytes per
 // turn.  Its 16-byte chunk c of row r lies at slot c ^ (r / 2 & 7), so that the
 // lanes that read one chunk of 16 rows touch each of the 64 banks once.
-template <int R, int kThreads>
+template <typename T, int R, int kThreads, bool kAligned>
 struct RowOperand {
     static constexpr int kLoads = R * 8 / kThreads;
     static constexpr int kRowsPerLoad = kThreads / 8;
     static constexpr int kBytes = R * kTurnBytes;
     static constexpr int kReads = 1;  // LDS loads per operand of a matrix step
+    static constexpr bool kDirect = kAligned;
     const char* ptr[kLoads];
+    Int4 held[kLoads];
+    int valid = 16;  // bytes of this thread's chunks before the contraction's end
 
     // This thread's rows are Row(i); its chunk of each is the same.
     static __device__ __forceinline__ int Row(int i) { return i * kRowsPerLoad + (threadIdx.x >> 3); }
     static __device__ __forceinline__ int Chunk() { return (threadIdx.x & 7) ^ ((threadIdx.x >> 4) & 7); }
 
-    // Copies this thread's chunks of the next turn (every row's first `bytes` of 128 hold operands).
+    // Before a turn's copies: `bytes` of the contraction are left.
     __device__ __forceinline__ void Prepare(int64_t bytes)
     {
-        if (bytes < kTurnBytes && Chunk() * 16 >= bytes) {
+        if (bytes >= kTurnBytes) return;
+        const int here = static_cast<int>(bytes) - Chunk() * 16;
+        if constexpr (!kAligned) valid = here < 0 ? 0 : here < 16 ? here : 16;
+        if (here > 0) return;
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) ptr[i] = reinterpret_cast<const char*>(&kZeros);
-        }
+        for (int i = 0; i < kLoads; ++i) ptr[i] = reinterpret_cast<const char*>(&kZeros);
     }
     __device__ __forceinline__ void Issue(char* lds, int i)
     {
         CopyToLds(ptr[i], lds + WaveNumber() * 1024 + i * kThreads * 16);
         ptr[i] += kTurnBytes;
+    }
+    // The same through registers, for rows of any alignment.
+    __device__ __forceinline__ void Load()
+    {
+        LoadAll<T>(ptr, valid, held);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) ptr[i] += kTurnBytes;
+    }
+    __device__ __forceinline__ void Commit(char* lds)
+    {
+        if constexpr (!kAligned) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                *reinterpret_cast<Int4*>(lds + (i * kThreads + static_cast<int>(threadIdx.x)) * 16) = held[i];
+            }
+        }
     }
 
     // The operand of one matrix step: 32 rows from `row` on.
@@ -315,14 +216,16 @@ struct RowOperand {
 // 16 lanes that work together lane j supplies 4 columns (j % 4) of row j / 4,
 // and lane i receives the 4 rows of column i.  Chunk c of row r lies at slot
 // c ^ 4 (r & 3): the four rows of 64 bytes that 32 lanes read then touch
-// every bank once.
-template <int C, int kThreads, bool kIndexed>
+// every bank once.  (Rows of 128 bytes lie in one half of the banks or the
+// other by themselves: c ^ 4 (r / 2 & 1).)
+template <typename T, int C, int kThreads, bool kIndexed, bool kAligned>
 struct ColumnOperand {
     static constexpr int kChunks = C / 8;
     static constexpr int kRowsPerLoad = kThreads / kChunks;
     static constexpr int kLoads = 64 / kRowsPerLoad;
     static constexpr int kBytes = 64 * C * 2;
     static constexpr int kReads = 2;
+    static constexpr bool kDirect = kAligned;
     const char* ptr[kLoads];
     const char* base;  // this thread's chunk of row 0
     int64_t ld;        // bytes
@@ -330,11 +233,14 @@ struct ColumnOperand {
     int64_t count;     // rows that an index may name
     int32_t row, end;  // of this thread's first load in the next turn, and of all
     int32_t next[kIndexed ? kLoads : 1];
+    Int4 held[kLoads];
+    int valid;         // bytes of the chunk before the last column
 
+    static __device__ __forceinline__ int Swizzle(int r) { return kChunks == 8 ? (r & 2) << 1 : (r & 3) << 2; }
     static __device__ __forceinline__ int Row(int i) { return i * kRowsPerLoad + threadIdx.x / kChunks; }
     static __device__ __forceinline__ int Chunk()
     {
-        return (threadIdx.x % kChunks) ^ (((threadIdx.x / kChunks) & 3) << 2);
+        return (threadIdx.x % kChunks) ^ Swizzle(threadIdx.x / kChunks);
     }
 
     __device__ __forceinline__ void Init(const void* p, int64_t ldBytes, int64_t column, int64_t columns,
@@ -342,6 +248,7 @@ struct ColumnOperand {
     {
         const int64_t c = column + Chunk() * 8;
         const bool in = c < columns;
+        valid = columns - c >= 8 ? 16 : static_cast<int>(columns - c) * 2;
         base = static_cast<const char*>(p) + c * 2;
         ld = ldBytes;
         index = rowIndex;
@@ -352,6 +259,7 @@ struct ColumnOperand {
         for (int i = 0; i < kLoads; ++i) ptr[i] = base + (row + i * kRowsPerLoad) * ld;
         LookUp();
         if (!in) {
+            valid = 16;
             ld = 0;
             base = reinterpret_cast<const char*>(&kZeros);
 #pragma unroll
@@ -382,6 +290,23 @@ struct ColumnOperand {
         CopyToLds(ptr[i], lds + WaveNumber() * 1024 + i * kThreads * 16);
         if constexpr (!kIndexed) ptr[i] += 64 * ld;
     }
+    __device__ __forceinline__ void Load()
+    {
+        LoadAll<T>(ptr, valid, held);
+        if constexpr (!kIndexed) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) ptr[i] += 64 * ld;
+        }
+    }
+    __device__ __forceinline__ void Commit(char* lds)
+    {
+        if constexpr (!kAligned) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                *reinterpret_cast<Int4*>(lds + (i * kThreads + static_cast<int>(threadIdx.x)) * 16) = held[i];
+            }
+        }
+    }
     // The indices of the turn after: they arrive while this one is multiplied.
     __device__ __forceinline__ void LookUp()
     {
@@ -400,7 +325,7 @@ struct ColumnOperand {
         const int lane = threadIdx.x & 63, j = lane & 15;
         const int r = step * 16 + (lane >> 5) * 8 + (j >> 2);
         const int c = column + ((lane >> 4) & 1) * 16 + (j & 3) * 4;
-        const char* p = lds + r * (C * 2) + ((((c >> 3) ^ ((r & 3) << 2)) << 4) | ((c & 4) << 1));
+        const char* p = lds + r * (C * 2) + ((((c >> 3) ^ Swizzle(r)) << 4) | ((c & 4) << 1));
         struct Pair {
             Short4 lo, hi;
         } v;
@@ -474,13 +399,18 @@ __device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds
         }
     };
     auto copy = [&](char* to, int first, int last) {
+        if constexpr (OperandA::kDirect) {
 #pragma unroll
-        for (int i = first; i < last; ++i) {
-            if (i < OperandA::kLoads) {
-                a.Issue(to, i);
-            } else {
-                b.Issue(to + OperandA::kBytes, i - OperandA::kLoads);
+            for (int i = first; i < last; ++i) {
+                if (i < OperandA::kLoads) {
+                    a.Issue(to, i);
+                } else {
+                    b.Issue(to + OperandA::kBytes, i - OperandA::kLoads);
+                }
             }
+        } else if (first == 0 && last > 0) {  // through registers: all at once, written to LDS by commit
+            a.Load();
+            b.Load();
         }
     };
     auto prepare = [&] {
@@ -488,8 +418,13 @@ __device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds
         b.Prepare(bytes);
         bytes -= kTurnBytes;
     };
+    auto commit = [&](char* to) {
+        a.Commit(to);
+        b.Commit(to + OperandA::kBytes);
+    };
     prepare();
     copy(lds, 0, kCopies);
+    commit(lds);
     WaitAll();
     read(0, lds, 0);
     int cur = 0;
@@ -513,6 +448,7 @@ __device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds
         read(1, now, 3);
         multiply(0);
         Interleave<MI * NI, kReads, 0>();
+        if constexpr (kLate > 0) commit(next);
         WaitAll();
         if constexpr (decltype(more)::value) read(0, next, 0);
         copy(now, 0, kEarly);
@@ -536,7 +472,7 @@ __device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds
 // values of tile (i, j) in registers 4q on.  Chunk c of row r lies at slot
 // c ^ r, which spreads the rows of a write over the banks.
 template <typename TOut, int MI, int NI, int kLdsBytes, typename Value>
-__device__ __forceinline__ void StoreTile(char* lds, TOut* c, int64_t ldc, int64_t rows, int64_t columns, bool wide,
+__device__ __forceinline__ void StoreTile(char* lds, TOut* c, int64_t ldc, int64_t rows, int64_t columns,
                                           Value value)
 {
     constexpr int kRowBytes = NI * 32 * static_cast<int>(sizeof(TOut));
@@ -574,8 +510,8 @@ __device__ __forceinline__ void StoreTile(char* lds, TOut* c, int64_t ldc, int64
             if (base + r >= rows || left <= 0) continue;
             const Int4 v = *reinterpret_cast<const Int4*>(lds + r * kRowBytes + (lane % kChunks) * 16);
             TOut* to = c + (base + r) * ldc + chunk * kPer;
-            if (wide && left >= kPer) {
-                *reinterpret_cast<Int4*>(to) = v;
+            if (left >= kPer) {
+                __builtin_memcpy(to, &v, 16);  // whatever C's alignment
             } else {
                 TOut o[kPer];
                 __builtin_memcpy(o, &v, 16);
@@ -607,44 +543,55 @@ __device__ __forceinline__ TilePlace PlaceInBands(int64_t id, int32_t m, int32_t
     return {rest / w, first + rest % w};
 }
 
-// The workgroup's place among `total` tiles: neighbours in number share an L2
-// (workgroups are dealt to the 8 dies in turn), -1 when there is none.
-__device__ __forceinline__ int64_t TileOfWorkgroup(int64_t total)
+// What a workgroup of GroupedTileKernel does: a tile of the list of 256x256
+// tiles, or one of `parts` slices of its rows; tile < 0: nothing.
+//
+// Workgroups are dealt to the 8 dies in turn, so those of one remainder take
+// one run of the list: neighbours then share an L2.  A die works on a tile per
+// CU at a time; when the last round of its run would fill half or a quarter
+// of the CUs, its tiles are cut into two or four slices.
+struct TileShare {
+    int64_t tile;
+    int32_t part, parts;
+};
+__device__ __forceinline__ TileShare ShareOfWorkgroup(int64_t total, int32_t cus)
 {
-    const int64_t per = (total + 7) / 8;
-    const int64_t at = blockIdx.x / 8;
-    const int64_t id = (blockIdx.x % 8) * per + at;
-    return at < per && id < total ? id : -1;
+    const int32_t die = static_cast<int32_t>(blockIdx.x % 8);
+    const int64_t per = (total + 7) / 8, at = blockIdx.x / 8;
+    const int64_t first = die * per;
+    const int64_t mine = total - first < per ? total - first : per;
+    if (mine <= 0) return {-1, 0, 1};
+    const int64_t whole = mine / cus * cus, rest = mine - whole;
+    const int32_t parts = rest * 4 <= cus ? 4 : rest * 2 <= cus ? 2 : 1;
+    if (at < whole) return {first + at, 0, 1};
+    const int64_t tile = whole + (at - whole) / parts;
+    return {tile < mine ? first + tile : -1, static_cast<int32_t>((at - whole) % parts), parts};
 }
 
-template <typename T, typename TOut, bool kBTrans, int MI, int NI, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * 64, 1) void GroupedTileKernel(GroupedLaunch p, int32_t tilesN, bool wideC)
+constexpr int kTileRows = 256;  // of a whole tile
+
+template <typename T, typename TOut, bool kBTrans, bool kAligned, int MI, int NI, int WM, int WN>
+__device__ __forceinline__ void GroupedTile(const GroupedLaunch& p, char* lds, int32_t group, int32_t firstRow,
+                                            int32_t endRow, int64_t n0)
 {
     constexpr int kThreads = WM * WN * 64, BM = MI * WM * 32, BN = NI * WN * 32;
-    using OperandA = RowOperand<BM, kThreads>;
-    using OperandB = std::conditional_t<kBTrans, RowOperand<BN, kThreads>, ColumnOperand<BN, kThreads, false>>;
+    using OperandA = RowOperand<T, BM, kThreads, kAligned>;
+    using OperandB = std::conditional_t<kBTrans, RowOperand<T, BN, kThreads, kAligned>,
+                                        ColumnOperand<T, BN, kThreads, false, kAligned>>;
     constexpr int kLds = 2 * (OperandA::kBytes + OperandB::kBytes);
-    __shared__ __align__(128) char lds[kLds];
-    const int64_t id = TileOfWorkgroup(static_cast<int64_t>(CountTiles(p.offsets, p.rows, p.groups, BM)) * tilesN);
-    if (id < 0) return;
-    RaggedTile tile = FindTile(p.offsets, p.rows, p.groups, BM, static_cast<int32_t>(id / tilesN));
-    if (tile.group < 0) return;
-    const TilePlace place = PlaceInBands(id - static_cast<int64_t>(tile.before) * tilesN, tile.tiles, tilesN);
-    tile.row = tile.begin + place.m * BM;
-    const int64_t n0 = static_cast<int64_t>(place.n) * BN;
     const int lane = threadIdx.x & 63, wave = WaveNumber();
     const int rowA = (wave % WM) * MI * 32, rowB = (wave / WM) * NI * 32;
     typename Mma32<T>::Acc acc[MI][NI] = {};
-    const bool real = tile.group < p.groups;
+    const bool real = group < p.groups;
     if (real && p.k > 0) {
-        const T* bg = static_cast<const T*>(p.b) + tile.group * p.stride_b;
+        const T* bg = static_cast<const T*>(p.b) + group * p.stride_b;
         OperandA a;
         OperandB b;
 #pragma unroll
         for (int i = 0; i < OperandA::kLoads; ++i) {
             // rows past the tile's end repeat its first: they are computed and not stored
-            const int32_t r = tile.row + OperandA::Row(i);
-            const int64_t row = IndexedRow(p.row_index, r < tile.end ? r : tile.row, p.rows_a);
+            const int32_t r = firstRow + OperandA::Row(i);
+            const int64_t row = IndexedRow(p.row_index, r < endRow ? r : firstRow, p.rows_a);
             a.ptr[i] = reinterpret_cast<const char*>(static_cast<const T*>(p.a) + row * p.lda) + OperandA::Chunk() * 16;
         }
         if constexpr (kBTrans) {
@@ -659,52 +606,99 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void GroupedTileKernel(GroupedLaun
         MultiplyTile<T, MI, NI>(a, b, lds, p.k * static_cast<int64_t>(sizeof(T)), rowA, rowB, acc);
     }
     const int64_t n = n0 + rowB;
-    TOut* c = static_cast<TOut*>(p.c) + (tile.row + rowA) * p.ldc + n;
+    TOut* c = static_cast<TOut*>(p.c) + (firstRow + rowA) * p.ldc + n;
     char* part = lds + wave * (kLds / (WM * WN));
     if constexpr (sizeof(T) == 1) {
         float sa[MI], sb[NI][4][4];
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
-            const int32_t r = tile.row + rowA + i * 32 + (lane & 31);
-            sa[i] = real && r < tile.end ? p.scale_a[IndexedRow(p.row_index, r, p.rows_a)] : 0.0f;
+            const int32_t r = firstRow + rowA + i * 32 + (lane & 31);
+            sa[i] = real && r < endRow ? p.scale_a[IndexedRow(p.row_index, r, p.rows_a)] : 0.0f;
         }
 #pragma unroll
         for (int j = 0; j < NI * 16; ++j) {
             const int64_t at = n + j / 4 * 8 + (lane >> 5) * 4 + j % 4;
-            sb[j / 16][j / 4 % 4][j % 4] = real && at < p.n ? p.scale_b[tile.group * p.n + at] : 0.0f;
+            sb[j / 16][j / 4 % 4][j % 4] = real && at < p.n ? p.scale_b[group * p.n + at] : 0.0f;
         }
         StoreTile<TOut, MI, NI, kLds / (WM * WN)>(
-            part, c, p.ldc, tile.end - tile.row - rowA, p.n - n, wideC, [&](int i, int j, int q, float(&v)[4]) {
+            part, c, p.ldc, endRow - firstRow - rowA, p.n - n, [&](int i, int j, int q, float(&v)[4]) {
 #pragma unroll
                 for (int x = 0; x < 4; ++x) v[x] = static_cast<float>(acc[i][j][q * 4 + x]) * (sa[i] * sb[j][q][x]);
             });
     } else {
         StoreTile<TOut, MI, NI, kLds / (WM * WN)>(
-            part, c, p.ldc, tile.end - tile.row - rowA, p.n - n, wideC, [&](int i, int j, int q, float(&v)[4]) {
+            part, c, p.ldc, endRow - firstRow - rowA, p.n - n, [&](int i, int j, int q, float(&v)[4]) {
 #pragma unroll
                 for (int x = 0; x < 4; ++x) v[x] = acc[i][j][q * 4 + x];
             });
     }
 }
 
-template <typename T, typename TOut, bool kIndexed, int MI, int NI, int WM, int WN>
+// Tiles of 256x256, or fewer rows where the group's end or a share leaves
+// fewer: a tile of 64 or 128 rows costs about that part of a whole one.
+template <typename T, typename TOut, bool kBTrans>
+__global__ __launch_bounds__(512, 1) void GroupedTileKernel(GroupedLaunch p, int32_t tilesN, int32_t cus)
+{
+    __shared__ __align__(128) char lds[2 * (kTileRows + 256) * kTurnBytes];
+    const int64_t total = static_cast<int64_t>(CountTiles(p.offsets, p.rows, p.groups, kTileRows)) * tilesN;
+    const TileShare share = ShareOfWorkgroup(total, cus);
+    if (share.tile < 0) return;
+    const RaggedTile tile =
+        FindTile(p.offsets, p.rows, p.groups, kTileRows, static_cast<int32_t>(share.tile / tilesN));
+    if (tile.group < 0) return;
+    const TilePlace place = PlaceInBands(share.tile - static_cast<int64_t>(tile.before) * tilesN, tile.tiles, tilesN);
+    const int32_t height = kTileRows / share.parts;
+    const int32_t row = tile.begin + place.m * kTileRows + share.part * height;
+    if (row >= tile.end) return;
+    const int32_t end = tile.end - row < height ? tile.end : row + height;
+    const int64_t n0 = static_cast<int64_t>(place.n) * 256;
+    if (end - row <= 64) {
+        GroupedTile<T, TOut, kBTrans, true, 1, 2, 2, 4>(p, lds, tile.group, row, end, n0);
+    } else if (end - row <= 128) {
+        GroupedTile<T, TOut, kBTrans, true, 2, 2, 2, 4>(p, lds, tile.group, row, end, n0);
+    } else {
+        GroupedTile<T, TOut, kBTrans, true, 4, 2, 2, 4>(p, lds, tile.group, row, end, n0);
+    }
+}
+
+// Tiles of 64x128 for groups of few rows or few tiles: three workgroups per CU.
+template <typename T, typename TOut, bool kBTrans, bool kAligned>
+__global__ __launch_bounds__(256, 1) void GroupedSmallTileKernel(GroupedLaunch p, int32_t tilesN)
+{
+    __shared__ __align__(128) char lds[2 * (64 + 128) * kTurnBytes];
+    const int64_t total = static_cast<int64_t>(CountTiles(p.offsets, p.rows, p.groups, 64)) * tilesN;
+    const TileShare share = ShareOfWorkgroup(total, 1);
+    if (share.tile < 0) return;
+    const RaggedTile tile = FindTile(p.offsets, p.rows, p.groups, 64, static_cast<int32_t>(share.tile / tilesN));
+    if (tile.group < 0) return;
+    const TilePlace place = PlaceInBands(share.tile - static_cast<int64_t>(tile.before) * tilesN, tile.tiles, tilesN);
+    const int32_t row = tile.begin + place.m * 64;
+    GroupedTile<T, TOut, kBTrans, kAligned, 1, 2, 2, 2>(p, lds, tile.group, row,
+                                                        tile.end - row < 64 ? tile.end : row + 64,
+                                                        static_cast<int64_t>(place.n) * 128);
+}
+
+template <typename T, typename TOut, bool kIndexed, bool kAligned, int MI, int NI, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64, 1) void GroupedGradTileKernel(GroupedGradLaunch p, int32_t tilesN,
-                                                                        int32_t tilesK, bool wideW)
+                                                                        int32_t tilesK)
 {
     constexpr int kThreads = WM * WN * 64, BM = MI * WM * 32, BN = NI * WN * 32;
-    using OperandA = ColumnOperand<BM, kThreads, false>;
-    using OperandB = ColumnOperand<BN, kThreads, kIndexed>;
+    using OperandA = ColumnOperand<T, BM, kThreads, false, kAligned>;
+    using OperandB = ColumnOperand<T, BN, kThreads, kIndexed, kAligned>;
     constexpr int kLds = 2 * (OperandA::kBytes + OperandB::kBytes);
     __shared__ __align__(128) char lds[kLds];
-    const int64_t id = TileOfWorkgroup(static_cast<int64_t>(tilesN) * tilesK * p.groups);
-    if (id < 0) return;
-    const int64_t g = id / (static_cast<int64_t>(tilesN) * tilesK);
-    const TilePlace place = PlaceInBands(id - g * tilesN * tilesK, tilesN, tilesK);
+    // Every die takes an eighth of each group's tiles, so that a long group is no die's alone; which
+    // eighth turns with the group, so that the last, shorter ones go round too.
+    const int32_t per = (tilesN * tilesK + 7) / 8, at = static_cast<int32_t>(blockIdx.x / 8);
+    const int32_t g = at / per;
+    const int32_t id = static_cast<int32_t>((blockIdx.x + g) % 8) * per + at % per;
+    if (id >= tilesN * tilesK) return;
+    const TilePlace place = PlaceInBands(id, tilesN, tilesK);
     const int64_t n0 = static_cast<int64_t>(place.m) * BM, k0 = static_cast<int64_t>(place.n) * BN;
     const int wave = WaveNumber();
     const int rowA = (wave % WM) * MI * 32, rowB = (wave / WM) * NI * 32;
     int32_t begin, end;
-    GroupRows(p.offsets, p.rows, static_cast<int>(g), begin, end);
+    GroupRows(p.offsets, p.rows, g, begin, end);
     typename Mma32<T>::Acc acc[MI][NI] = {};
     if (begin < end) {
         OperandA a;
@@ -716,10 +710,116 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void GroupedGradTileKernel(Grouped
     const int64_t n = n0 + rowA, k = k0 + rowB;
     StoreTile<TOut, MI, NI, kLds / (WM * WN)>(lds + wave * (kLds / (WM * WN)),
                                               static_cast<TOut*>(p.w) + g * p.stride_w + n * p.ldw + k, p.ldw, p.n - n,
-                                              p.k - k, wideW, [&](int i, int j, int q, float(&v)[4]) {
+                                              p.k - k, [&](int i, int j, int q, float(&v)[4]) {
 #pragma unroll
                                                   for (int x = 0; x < 4; ++x) v[x] = acc[i][j][q * 4 + x];
                                               });
+}
+
+// ---------------------------------------------------------------------------
+// Few rows per group: the weights are read once and bound the time.  A
+// workgroup multiplies MT*16 rows by NT*16 columns; its waves split the
+// contraction, each lane loading its operands of 16x16 instructions straight
+// from memory (16 rows of 64 bytes per load), and add their sums through LDS
+// in the order of the waves.
+// ---------------------------------------------------------------------------
+template <typename T, typename TOut, bool kAligned, int MT, int NT, int kWaves>
+__global__ __launch_bounds__(kWaves * 64) void GroupedRowsKernel(GroupedLaunch p, int32_t tilesN)
+{
+    using Acc = typename Mma<T>::Acc;
+    constexpr int kAhead = 16 / (MT + NT) > 4 ? 8 : 4;  // steps loaded before they are multiplied
+    __shared__ Acc part[kWaves][MT * NT][64];
+    const RaggedTile tile =
+        FindTile(p.offsets, p.rows, p.groups, MT * 16, static_cast<int32_t>(blockIdx.x / static_cast<uint32_t>(tilesN)));
+    const int32_t n0 = static_cast<int32_t>(blockIdx.x % static_cast<uint32_t>(tilesN)) * NT * 16;
+    const int32_t width = static_cast<int32_t>(p.n);
+    if (tile.group < 0 || n0 >= width) return;
+    const int lane = threadIdx.x & 63, wave = WaveNumber();
+    const bool real = tile.group < p.groups;
+    Acc acc[MT][NT] = {};
+    if (real) {
+        const int32_t bytes = static_cast<int32_t>(p.k) * static_cast<int32_t>(sizeof(T));
+        const char* b[NT];
+        const char* a[MT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int32_t n = n0 + j * 16 + (lane & 15);
+            b[j] = reinterpret_cast<const char*>(static_cast<const T*>(p.b) + tile.group * p.stride_b +
+                                                 (n < width ? n : width - 1) * p.ldb);
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const int32_t r = tile.row + i * 16 + (lane & 15);
+            a[i] = reinterpret_cast<const char*>(
+                static_cast<const T*>(p.a) + IndexedRow(p.row_index, r < tile.end ? r : tile.row, p.rows_a) * p.lda);
+        }
+        // step s is 64 bytes; a wave takes two neighbouring ones, a memory line, at a time
+        auto at = [&](int s) { return ((s >> 1) * kWaves + wave) * 128 + (s & 1) * 64 + (lane >> 4) * 16; };
+        for (int s0 = 0; ((s0 >> 1) * kWaves + wave) * 128 < bytes; s0 += kAhead) {
+            Int4 fb[kAhead][NT], fa[kAhead][MT];
+            auto loadAll = [&](auto load) {
+#pragma unroll
+                for (int s = 0; s < kAhead; ++s) {
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) fb[s][j] = load(b[j], at(s0 + s));
+                }
+#pragma unroll
+                for (int s = 0; s < kAhead; ++s) {
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) fa[s][i] = load(a[i], at(s0 + s));
+                }
+            };
+            if (kAligned || (((s0 + kAhead - 1) >> 1) * kWaves + wave + 1) * 128 <= bytes) {
+                loadAll([&](const char* row, int32_t byte) {
+                    Int4 v;
+                    if constexpr (kAligned) {
+                        v = *reinterpret_cast<const Int4*>(row + (byte < bytes ? byte : 0));
+                        if (byte >= bytes) v = Int4{0, 0, 0, 0};
+                    } else {
+                        __builtin_memcpy(&v, row + byte, 16);
+                    }
+                    return v;
+                });
+            } else {
+                loadAll([&](const char* row, int32_t byte) {
+                    return LoadUnaligned<T>(row + (byte < bytes ? byte : 0), bytes - byte);
+                });
+            }
+#pragma unroll
+            for (int s = 0; s < kAhead; ++s) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) acc[i][j] = Mma<T>::Run(fb[s][j], fa[s][i], acc[i][j]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT * NT; ++i) part[wave][i][lane] = acc[i / NT][i % NT];
+    __syncthreads();
+    for (int t = wave; t < MT * NT; t += kWaves) {
+        Acc sum = part[0][t][lane];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) sum += part[w][t][lane];
+        const int32_t r = tile.row + t / NT * 16 + (lane & 15);
+        const int32_t n = n0 + t % NT * 16 + (lane >> 4) * 4;
+        if (r >= tile.end) continue;
+        float sa = 1.0f;
+        if constexpr (sizeof(T) == 1) {
+            if (real) sa = p.scale_a[IndexedRow(p.row_index, r, p.rows_a)];
+        }
+        TOut* c = static_cast<TOut*>(p.c) + r * p.ldc;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            if (n + x >= width) continue;
+            float v = static_cast<float>(sum[x]);
+            if constexpr (sizeof(T) == 1) {
+                if (real) v *= sa * p.scale_b[tile.group * p.n + n + x];
+            }
+            c[n + x] = FromFloat<TOut>(v);
+        }
+    }
 }
 
 int64_t CeilDiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -734,22 +834,70 @@ int64_t MaxRowTiles(const int32_t* offsets, int64_t rows, int64_t groups, int64_
     return most < rows ? most : rows;
 }
 
-template <typename T, typename TOut, bool kBTrans, int MI, int NI, int WM, int WN>
-int LaunchTiles(const GroupedLaunch& l, hipStream_t s)
+int CusPerDie()
 {
-    const int64_t tilesN = CeilDiv(l.n, NI * WN * 32);
-    const int64_t grid = CeilDiv(MaxRowTiles(l.offsets, l.rows, l.groups, MI * WM * 32) * tilesN, 8) * 8;
-    if (grid > INT32_MAX) return kTooLarge;
-    const bool wideC = Aligned16(l.c, l.ldc * static_cast<int64_t>(sizeof(TOut)));
-    GroupedTileKernel<T, TOut, kBTrans, MI, NI, WM, WN>
-        <<<static_cast<uint32_t>(grid), WM * WN * 64, 0, s>>>(l, static_cast<int32_t>(tilesN), wideC);
-    return 0;
+    static const int cus = [] {
+        int dev = 0, n = 0;
+        const bool ok = hipGetDevice(&dev) == hipSuccess &&
+                        hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && n >= 8;
+        return ok ? n / 8 : 32;
+    }();
+    return cus;
 }
 
 template <typename T, typename TOut, bool kBTrans>
-int GroupedAligned(const GroupedLaunch& l, hipStream_t s)
+int LaunchTiles(const GroupedLaunch& l, hipStream_t s)
 {
-    return LaunchTiles<T, TOut, kBTrans, 4, 2, 2, 4>(l, s);
+    const int64_t tilesN = CeilDiv(l.n, 256);
+    // a die may cut the tiles of its last round into four
+    const int64_t grid = CeilDiv(MaxRowTiles(l.offsets, l.rows, l.groups, kTileRows) * tilesN, 8) * 8 + 8 * CusPerDie();
+    if (grid > INT32_MAX) return kTooLarge;
+    GroupedTileKernel<T, TOut, kBTrans>
+        <<<static_cast<uint32_t>(grid), 512, 0, s>>>(l, static_cast<int32_t>(tilesN), CusPerDie());
+    return 0;
+}
+
+template <typename T, typename TOut, bool kBTrans, bool kAligned>
+int LaunchSmallTiles(const GroupedLaunch& l, hipStream_t s)
+{
+    const int64_t tilesN = CeilDiv(l.n, 128);
+    const int64_t grid = CeilDiv(MaxRowTiles(l.offsets, l.rows, l.groups, 64) * tilesN, 8) * 8;
+    if (grid > INT32_MAX) return kTooLarge;
+    GroupedSmallTileKernel<T, TOut, kBTrans, kAligned>
+        <<<static_cast<uint32_t>(grid), 256, 0, s>>>(l, static_cast<int32_t>(tilesN));
+    return 0;
+}
+
+template <typename T, typename TOut, bool kAligned, int MT, int NT>
+int LaunchRows(const GroupedLaunch& l, hipStream_t s)
+{
+    constexpr int kWaves = 4;
+    // the row tiles of a group then read a column's weights on one die, whose L2 holds them
+    const int64_t tilesN = CeilDiv(CeilDiv(l.n, NT * 16), 8) * 8;
+    const int64_t grid = MaxRowTiles(l.offsets, l.rows, l.groups, MT * 16) * tilesN;
+    if (grid > INT32_MAX) return kTooLarge;
+    GroupedRowsKernel<T, TOut, kAligned, MT, NT, kWaves>
+        <<<static_cast<uint32_t>(grid), kWaves * 64, 0, s>>>(l, static_cast<int32_t>(tilesN));
+    return 0;
+}
+
+template <typename T, typename TOut, bool kBTrans, bool kAligned>
+int GroupedBySize(const GroupedLaunch& l, hipStream_t s)
+{
+    const int64_t cus = 8 * CusPerDie();
+    const int64_t smallTiles = (l.rows / 64 + (l.offsets != nullptr ? CeilDiv(l.groups, 2) : 1)) * CeilDiv(l.n, 128);
+    if constexpr (kBTrans) {
+        const bool few = l.rows <= 12 * l.groups || (l.rows <= 64 * l.groups && smallTiles < cus / 2);
+        if (few && l.k * static_cast<int64_t>(sizeof(T)) <= INT32_MAX / 2) {
+            const int64_t groups = l.rows < l.groups ? l.rows : l.groups;
+            const bool narrow = groups * CeilDiv(l.n, 32) < 2 * cus && l.rows <= 16 * l.groups;
+            return narrow ? LaunchRows<T, TOut, kAligned, 1, 1>(l, s) : LaunchRows<T, TOut, kAligned, 2, 2>(l, s);
+        }
+    }
+    if constexpr (kAligned) {
+        if (l.rows >= 160 * l.groups && smallTiles > 3 * cus) return LaunchTiles<T, TOut, kBTrans>(l, s);
+    }
+    return LaunchSmallTiles<T, TOut, kBTrans, kAligned>(l, s);
 }
 
 template <typename T, typename TOut>
@@ -757,52 +905,36 @@ int GroupedTyped(const GroupedLaunch& l, hipStream_t s)
 {
     constexpr int64_t kSize = sizeof(T);
     const int64_t inner = l.b_trans ? l.k : l.n;  // what a row of B holds
-    if (Aligned16(l.a, l.lda * kSize) && Aligned16(l.b, l.ldb * kSize) && Aligned16(l.b, l.stride_b * kSize) &&
-        l.k * kSize % 16 == 0 && inner * kSize % 16 == 0) {
-        if constexpr (kSize == 2) {
-            if (!l.b_trans) return GroupedAligned<T, TOut, false>(l, s);
-        }
-        return GroupedAligned<T, TOut, true>(l, s);
-    }
-    const int64_t tilesN = CeilDiv(l.n, kAnyTile);
-    const int64_t grid = MaxRowTiles(l.offsets, l.rows, l.groups, kAnyTile) * tilesN;
-    if (grid > INT32_MAX) return kTooLarge;
-    if constexpr (sizeof(T) == 2) {
+    const bool aligned = Aligned16(l.a, l.lda * kSize) && Aligned16(l.b, l.ldb * kSize) &&
+                         Aligned16(l.b, l.stride_b * kSize) && l.k * kSize % 16 == 0 && inner * kSize % 16 == 0;
+    if constexpr (kSize == 2) {
         if (!l.b_trans) {
-            GroupedAnyKernel<T, TOut, false><<<static_cast<uint32_t>(grid), 256, 0, s>>>(l, static_cast<int32_t>(tilesN));
-            return 0;
+            return aligned ? GroupedBySize<T, TOut, false, true>(l, s) : GroupedBySize<T, TOut, false, false>(l, s);
         }
     }
-    GroupedAnyKernel<T, TOut, true><<<static_cast<uint32_t>(grid), 256, 0, s>>>(l, static_cast<int32_t>(tilesN));
-    return 0;
+    return aligned ? GroupedBySize<T, TOut, true, true>(l, s) : GroupedBySize<T, TOut, true, false>(l, s);
 }
 
-template <typename T, typename TOut, int MI, int NI, int WM, int WN>
+template <typename T, typename TOut, bool kAligned, int MI>
 int LaunchGradTiles(const GroupedGradLaunch& l, hipStream_t s)
 {
-    const int64_t tilesN = CeilDiv(l.n, MI * WM * 32), tilesK = CeilDiv(l.k, NI * WN * 32);
-    if (tilesN * tilesK > (INT32_MAX - 7) / l.groups) return kTooLarge;
-    const int64_t grid = CeilDiv(tilesN * tilesK * l.groups, 8) * 8;
-    constexpr int64_t kOut = sizeof(TOut);
-    const bool wideW = Aligned16(l.w, l.ldw * kOut) && (l.groups == 1 || Aligned16(l.w, l.stride_w * kOut));
-    const auto kernel = l.row_index != nullptr ? GroupedGradTileKernel<T, TOut, true, MI, NI, WM, WN>
-                                               : GroupedGradTileKernel<T, TOut, false, MI, NI, WM, WN>;
-    kernel<<<static_cast<uint32_t>(grid), WM * WN * 64, 0, s>>>(l, static_cast<int32_t>(tilesN),
-                                                                static_cast<int32_t>(tilesK), wideW);
+    const int64_t tilesN = CeilDiv(l.n, MI * 64), tilesK = CeilDiv(l.k, 256);
+    if (tilesN * tilesK + 7 > INT32_MAX / l.groups) return kTooLarge;
+    const int64_t grid = CeilDiv(tilesN * tilesK, 8) * 8 * l.groups;
+    const auto kernel = l.row_index != nullptr ? GroupedGradTileKernel<T, TOut, true, kAligned, MI, 2, 2, 4>
+                                               : GroupedGradTileKernel<T, TOut, false, kAligned, MI, 2, 2, 4>;
+    kernel<<<static_cast<uint32_t>(grid), 512, 0, s>>>(l, static_cast<int32_t>(tilesN), static_cast<int32_t>(tilesK));
     return 0;
 }
 
 template <typename T, typename TOut>
 int GroupedGradTyped(const GroupedGradLaunch& l, hipStream_t s)
 {
-    if (Aligned16(l.grad, l.ldg * 2) && Aligned16(l.x, l.ldx * 2) && l.n % 8 == 0 && l.k % 8 == 0) {
-        return LaunchGradTiles<T, TOut, 4, 2, 2, 4>(l, s);
-    }
-    const int64_t tilesN = CeilDiv(l.n, kAnyTile), tilesK = CeilDiv(l.k, kAnyTile);
-    if (tilesN * tilesK > INT32_MAX / l.groups) return kTooLarge;
-    GroupedGradAnyKernel<T, TOut><<<static_cast<uint32_t>(tilesN * tilesK * l.groups), 256, 0, s>>>(
-        l, static_cast<int32_t>(tilesN), static_cast<int32_t>(tilesK));
-    return 0;
+    const bool aligned =
+        Aligned16(l.grad, l.ldg * 2) && Aligned16(l.x, l.ldx * 2) && l.n % 8 == 0 && l.k % 8 == 0;
+    if (!aligned) return LaunchGradTiles<T, TOut, false, 1>(l, s);
+    const bool many = CeilDiv(l.n, 256) * CeilDiv(l.k, 256) * l.groups >= 6 * CusPerDie();
+    return many ? LaunchGradTiles<T, TOut, true, 4>(l, s) : LaunchGradTiles<T, TOut, true, 1>(l, s);
 }
 
 }  // namespace

@@ -56,6 +56,30 @@ __device__ __forceinline__ uint32_t WaveMaxU32(uint32_t x)
     return LastLane(WaveScan(x, 0U, [](uint32_t a, uint32_t b) { return a > b ? a : b; }));
 }
 
+// The same over each row of 16 lanes, in all of its lanes: rotations by 8, 4, 2 and 1.
+constexpr int kDppRor8 = 0x128, kDppRor4 = 0x124, kDppRor2 = 0x122, kDppRor1 = 0x121;
+template <typename F>
+__device__ __forceinline__ uint32_t RowReduce(uint32_t x, F op)
+{
+    x = op(x, Dpp<kDppRor8, 0xF>(x, x));
+    x = op(x, Dpp<kDppRor4, 0xF>(x, x));
+    x = op(x, Dpp<kDppRor2, 0xF>(x, x));
+    x = op(x, Dpp<kDppRor1, 0xF>(x, x));
+    return x;
+}
+
+__device__ __forceinline__ uint32_t RowMaxU32(uint32_t x)
+{
+    return RowReduce(x, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+}
+
+__device__ __forceinline__ float RowSum(float x)
+{
+    return __uint_as_float(RowReduce(__float_as_uint(x), [](uint32_t a, uint32_t b) {
+        return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+    }));
+}
+
 __device__ __forceinline__ int32_t WaveInclusiveSum(int32_t x)
 {
     return static_cast<int32_t>(WaveScan(static_cast<uint32_t>(x), 0U, [](uint32_t a, uint32_t b) { return a + b; }));

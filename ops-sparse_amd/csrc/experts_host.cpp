@@ -41,9 +41,9 @@ aclsparseStatus_t CheckRouteShape(int64_t tokens, int64_t experts, int64_t k)
     return ACL_SPARSE_STATUS_SUCCESS;
 }
 
-size_t RouteBytes(int64_t tokens, int64_t experts, int64_t k)
+size_t RouteBytes(int64_t tokens, int64_t experts)
 {
-    const size_t bytes = static_cast<size_t>(aclsp::RouteBlocks(tokens, experts, k) * experts) * sizeof(int32_t);
+    const size_t bytes = static_cast<size_t>(aclsp::RouteBlocks(tokens) * experts) * sizeof(int32_t);
     return aclsp::AlignUp(bytes < aclsp::kWsAlign ? aclsp::kWsAlign : bytes);
 }
 
@@ -80,7 +80,7 @@ aclsparseStatus_t aclsparseRoute_bufferSize(aclsparseHandle_t handle, int64_t to
     st = CheckRouteShape(tokens, experts, k);
     if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
     if (bufferSize == nullptr) return ACL_SPARSE_STATUS_INVALID_VALUE;
-    *bufferSize = RouteBytes(tokens, experts, k);
+    *bufferSize = RouteBytes(tokens, experts);
     return ACL_SPARSE_STATUS_SUCCESS;
 }
 

@@ -9,8 +9,8 @@
 
 namespace aclsp {
 
-// The most experts a router's row may have (16 per lane of a wave) and the
-// most of them a token may choose (one per lane).
+// The most experts a router's row may have (64 for each of 16 lanes) and the
+// most of them a token may choose (one per lane of a wave).
 constexpr int64_t kMaxRouteExperts = 1024;
 constexpr int64_t kMaxRouteK = 64;
 // The longest contraction of 8-bit products whose sum cannot leave 32 bits:
@@ -35,7 +35,7 @@ struct RouteLaunch {
 };
 
 // Workgroups of the routing kernels, and so rows of their histogram.
-int64_t RouteBlocks(int64_t tokens, int64_t experts, int64_t k);
+int64_t RouteBlocks(int64_t tokens);
 int LaunchRoute(const RouteLaunch& l, void* stream);
 
 struct RouteGradLaunch {

@@ -18,6 +18,7 @@ namespace {
 
 constexpr int kRouteThreads = 1024;
 constexpr int kRouteWaves = kRouteThreads / 64;
+constexpr int64_t kTokensPerTurn = kRouteThreads / 16;  // a quarter of that beyond 256 experts
 
 // A logit as an unsigned key of the same order.  NaN is above everything, as
 // in torch.topk; -0 and +0 are one value; 0 is below every value.
@@ -29,103 +30,99 @@ __device__ __forceinline__ uint32_t OrderKey(float v)
 }
 constexpr uint32_t kKeyMinusInf = 0x007FFFFFU;
 
-// One token's choice by one wave: lane j < k ends with the j-th largest logit
-// and its index (-1 when the row has no j-th logit above -inf).  Each of the
-// k rounds takes the wave's largest key and, among equal ones, the lowest
-// index: value i of lane l is expert 64 i + l.
-template <int V>
-__device__ __forceinline__ void ChooseTopK(const float (&v)[V], int experts, int k, int lane, float& value, int& index)
+__device__ __forceinline__ float KeyValue(uint32_t key)
 {
+    return key == 0xFFFFFFFFU ? __uint_as_float(0x7FC00000U)
+                              : __uint_as_float(key ^ ((key >> 31) ? 0x80000000U : 0xFFFFFFFFU));
+}
+
+// The choices of a wave's tokens, L = 16 lanes each (64 beyond 256 experts,
+// whose values would not fit the registers): lane l of a token holds its
+// logits l*V to l*V + V - 1.  Each of the k rounds takes the largest key of
+// the L lanes and, among equal ones, the lowest lane and its lowest value,
+// which is the lowest index; that lane notes the choice in LDS and drops the
+// value.  The rounds are a chain of dependent steps, which four tokens share.
+struct Choice {
+    uint32_t key;
+    int32_t index;
+};
+
+template <typename T, int V, int L>
+__device__ __forceinline__ void GateTokens(const RouteLaunch& p, int64_t t, bool valid, Choice* choices)
+{
+    const int lane = threadIdx.x & 63, sub = lane & (L - 1), row = lane / L;
+    const int experts = static_cast<int>(p.experts), k = static_cast<int>(p.k);
+    const T* logits = static_cast<const T*>(p.logits) + (valid ? t : 0) * p.ld;
     uint32_t key[V];
+    float v[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) key[i] = 64 * i + lane < experts ? OrderKey(v[i]) : 0U;
-    value = -INFINITY;
-    index = -1;
+    for (int i = 0; i < V; ++i) {
+        const int e = sub * V + i;
+        v[i] = valid && e < experts ? ToFloat(logits[e]) : -INFINITY;
+        key[i] = e < experts ? OrderKey(v[i]) : 0U;
+    }
+    uint32_t top = 0;
+    int32_t count = 0;
     for (int j = 0; j < k; ++j) {
         uint32_t best = key[0];
+        int at = 0;
 #pragma unroll
-        for (int i = 1; i < V; ++i) best = best > key[i] ? best : key[i];
-        best = WaveMaxU32(best);
-        if (best <= kKeyMinusInf) break;  // uniform
-        int who = -1;
+        for (int i = 1; i < V; ++i) {
+            at = key[i] > best ? i : at;
+            best = key[i] > best ? key[i] : best;
+        }
+        const uint32_t most = L == 16 ? RowMaxU32(best) : WaveMaxU32(best);
+        if (__all(most <= kKeyMinusInf)) break;
+        const uint64_t who = __ballot(best == most) >> (row * L) & (~uint64_t{0} >> (64 - L));
+        if (most > kKeyMinusInf) {
+            if (j == 0) top = most;
+            count = j + 1;
+            if (sub == __builtin_ctzll(who)) {
+                choices[j] = {most, sub * V + at};
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const uint64_t m = __ballot(key[i] == best);
-            if (who < 0 && m != 0) {
-                who = 64 * i + __builtin_ctzll(m);
-                if (lane == (who & 63)) key[i] = 0U;
+                for (int i = 0; i < V; ++i) key[i] = i == at ? 0U : key[i];
             }
         }
-        if (lane == j) {
-            index = who;
-            const uint32_t u = best == 0xFFFFFFFFU ? 0x7FC00000U
-                                                   : best ^ ((best >> 31) ? 0x80000000U : 0xFFFFFFFFU);
-            value = __uint_as_float(u);
-        }
     }
-}
-
-template <typename T, int V>
-__device__ __forceinline__ void LoadRow(const T* row, int experts, int lane, float (&v)[V])
-{
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = 64 * i + lane < experts ? ToFloat(row[64 * i + lane]) : -INFINITY;
-}
-
-// Weights and ids of one token by one wave: w_j = exp(l_j - m) / sum, the sum
-// over the chosen or over the whole row, all in 32 bits.
-template <typename T, int V>
-__device__ __forceinline__ int GateToken(const RouteLaunch& p, int64_t t, int lane)
-{
-    float v[V];
-    const int experts = static_cast<int>(p.experts), k = static_cast<int>(p.k);
-    LoadRow<T, V>(static_cast<const T*>(p.logits) + t * p.ld, experts, lane, v);
-    float value;
-    int index;
-    ChooseTopK<V>(v, experts, k, lane, value, index);
-    const float top = __shfl(value, 0);
-    const float e = index >= 0 ? expf(value - top) : 0.0f;
-    float sum;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the choices of other lanes
+    const float peak = KeyValue(top);
+    float sum = 0.0f;
     if (p.normalize) {
-        sum = WaveSum(e);
-    } else {
-        float s = 0.0f;
+        for (int j = sub; j < count; j += L) sum += expf(KeyValue(choices[j].key) - peak);
+    } else if (count > 0) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) s += 64 * i + lane < experts && v[i] != -INFINITY ? expf(v[i] - top) : 0.0f;
-        sum = WaveSum(s);
+        for (int i = 0; i < V; ++i) sum += v[i] != -INFINITY ? expf(v[i] - peak) : 0.0f;
     }
-    if (lane < k) {
-        p.weights[t * k + lane] = index >= 0 ? e / sum : 0.0f;
-        p.ids[t * k + lane] = index;
+    sum = L == 16 ? RowSum(sum) : WaveSum(sum);
+    if (!valid) return;
+    for (int j = sub; j < k; j += L) {
+        const bool chosen = j < count;
+        p.weights[t * k + j] = chosen ? expf(KeyValue(choices[j].key) - peak) / sum : 0.0f;
+        p.ids[t * k + j] = chosen ? choices[j].index : -1;
     }
-    return index;
 }
 
-// The experts' assignment counts of one workgroup's tokens, with their choice
-// where logits are given.
-template <typename T, int V>
-__global__ __launch_bounds__(kRouteThreads) void RouteGateKernel(RouteLaunch p, int64_t tokensPerBlock)
+// Counts of one workgroup's assignments by expert, with their choice where
+// logits are given.
+template <typename T, int V, int L>
+__device__ __forceinline__ void GateAndCount(const RouteLaunch& p, int64_t t0, int64_t t1, int32_t* hist)
 {
-    __shared__ int32_t hist[kMaxRouteExperts];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int kTokens = kRouteThreads / L;
+    __shared__ Choice choices[kTokens][kMaxRouteK];
     const int experts = static_cast<int>(p.experts), k = static_cast<int>(p.k);
     for (int e = threadIdx.x; e < experts; e += kRouteThreads) hist[e] = 0;
-    __syncthreads();
-    const int64_t t0 = blockIdx.x * tokensPerBlock;
-    const int64_t t1 = t0 + tokensPerBlock < p.tokens ? t0 + tokensPerBlock : p.tokens;
     if (p.logits != nullptr) {
-        for (int64_t t = t0 + wave; t < t1; t += kRouteWaves) {
-            const int index = GateToken<T, V>(p, t, lane);
-            if (lane < k && index >= 0) atomicAdd(&hist[index], 1);
-        }
-    } else {
-        for (int64_t a = t0 * k + threadIdx.x; a < t1 * k; a += kRouteThreads) {
-            const int id = p.ids[a];
-            if (id >= 0 && id < experts) atomicAdd(&hist[id], 1);
+        for (int64_t t = t0; t < t1; t += kTokens) {
+            const int slot = threadIdx.x / L;
+            GateTokens<T, V, L>(p, t + slot, t + slot < t1, choices[slot]);
         }
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < experts; e += kRouteThreads) p.hist[blockIdx.x * p.experts + e] = hist[e];
+    for (int64_t a = t0 * k + threadIdx.x; a < t1 * k; a += kRouteThreads) {
+        const int id = p.ids[a];
+        if (id >= 0 && id < experts) atomicAdd(&hist[id], 1);
+    }
+    __syncthreads();
 }
 
 // Places of one workgroup's assignments.  base[e] starts as the place of the
@@ -190,72 +187,106 @@ __device__ int32_t ScanExperts(const int32_t* total, int32_t* base, int experts)
     return before;
 }
 
-// Rows of row_tokens that no assignment took (dropped ones) read -1.
-__device__ void FillTail(const RouteLaunch& p, int32_t used, int64_t start, int64_t step)
-{
-    for (int64_t r = used + start; r < p.tokens * p.k; r += step) p.row_tokens[r] = -1;
-}
-
-// Every workgroup sums the histograms itself (at most 256 of them, from L2):
-// those before it give its base within each expert, all of them the experts' totals.
-__global__ __launch_bounds__(kRouteThreads) void RoutePlaceKernel(RouteLaunch p, int64_t tokensPerBlock, int blocks,
-                                                                  int bits)
+// The plan from every expert's total and, in before[e], its assignments in
+// earlier workgroups.
+__device__ void PlacePart(const RouteLaunch& p, int64_t t0, int64_t t1, const int32_t* total, int32_t* before, int bits)
 {
     __shared__ WaveCounts waveCount;
-    __shared__ int32_t base[kMaxRouteExperts], total[kMaxRouteExperts], first[kMaxRouteExperts];
+    __shared__ int32_t first[kMaxRouteExperts];
     __shared__ int32_t used;
     const int experts = static_cast<int>(p.experts);
-    for (int e = threadIdx.x; e < experts; e += kRouteThreads) {
-        int32_t before = 0, all = 0;
-        for (int b = 0; b < blocks; ++b) {
-            const int32_t c = p.hist[static_cast<int64_t>(b) * experts + e];
-            before += b < static_cast<int>(blockIdx.x) ? c : 0;
-            all += c;
-        }
-        base[e] = before;
-        total[e] = all;
-    }
-    __syncthreads();
     if (threadIdx.x < 64) {
         const int32_t n = ScanExperts(total, first, experts);
         if (threadIdx.x == 0) used = n;
     }
     __syncthreads();
     for (int e = threadIdx.x; e < experts; e += kRouteThreads) {
-        base[e] += first[e];
+        before[e] += first[e];
         if (blockIdx.x == 0) p.offsets[e] = first[e];
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) p.offsets[experts] = used;
+    // rows that no assignment took (dropped ones) read -1
+    for (int64_t r = used + static_cast<int64_t>(blockIdx.x) * kRouteThreads + threadIdx.x; r < p.tokens * p.k;
+         r += static_cast<int64_t>(gridDim.x) * kRouteThreads) {
+        p.row_tokens[r] = -1;
+    }
     __syncthreads();
-    FillTail(p, used, static_cast<int64_t>(blockIdx.x) * kRouteThreads + threadIdx.x,
-             static_cast<int64_t>(blocks) * kRouteThreads);
-    const int64_t t0 = blockIdx.x * tokensPerBlock;
-    const int64_t t1 = t0 + tokensPerBlock < p.tokens ? t0 + tokensPerBlock : p.tokens;
-    PlaceAssignments(p, t0 * p.k, t1 * p.k, base, waveCount, bits);
+    PlaceAssignments(p, t0 * p.k, t1 * p.k, before, waveCount, bits);
 }
 
-// Gradient of the weights with respect to the logits of one token, by one wave.
+// Few tokens: everything in one workgroup and one launch.
+template <typename T, int V, int L>
+__global__ __launch_bounds__(kRouteThreads) void RouteOneKernel(RouteLaunch p, int bits)
+{
+    __shared__ int32_t total[kMaxRouteExperts], before[kMaxRouteExperts];
+    GateAndCount<T, V, L>(p, 0, p.tokens, total);
+    for (int e = threadIdx.x; e < p.experts; e += kRouteThreads) before[e] = 0;
+    PlacePart(p, 0, p.tokens, total, before, bits);
+}
+
+template <typename T, int V, int L>
+__global__ __launch_bounds__(kRouteThreads) void RouteGateKernel(RouteLaunch p, int64_t tokensPerBlock)
+{
+    __shared__ int32_t hist[kMaxRouteExperts];
+    const int64_t t0 = blockIdx.x * tokensPerBlock;
+    GateAndCount<T, V, L>(p, t0, t0 + tokensPerBlock < p.tokens ? t0 + tokensPerBlock : p.tokens, hist);
+    for (int e = threadIdx.x; e < p.experts; e += kRouteThreads) p.hist[blockIdx.x * p.experts + e] = hist[e];
+}
+
+// Every workgroup sums the histograms itself (at most 256 of them, from L2):
+// those before it give its base within each expert, all of them the experts'
+// totals.  The threads of one expert take turns at the histograms.
+__global__ __launch_bounds__(kRouteThreads) void RoutePlaceKernel(RouteLaunch p, int64_t tokensPerBlock, int bits)
+{
+    __shared__ int32_t total[kMaxRouteExperts], before[kMaxRouteExperts];
+    const int experts = static_cast<int>(p.experts), blocks = static_cast<int>(gridDim.x);
+    const int width = 1 << (bits < 6 ? 6 : bits);  // whole waves per histogram
+    for (int e = threadIdx.x; e < experts; e += kRouteThreads) total[e] = before[e] = 0;
+    __syncthreads();
+    const int e = threadIdx.x & (width - 1);
+    if (e < experts) {
+        int32_t mine = 0, all = 0;
+#pragma unroll 8
+        for (int b = static_cast<int>(threadIdx.x) / width; b < blocks; b += kRouteThreads / width) {
+            const int32_t c = p.hist[static_cast<int64_t>(b) * experts + e];
+            mine += b < static_cast<int>(blockIdx.x) ? c : 0;
+            all += c;
+        }
+        atomicAdd(&before[e], mine);
+        atomicAdd(&total[e], all);
+    }
+    __syncthreads();
+    const int64_t t0 = blockIdx.x * tokensPerBlock;
+    PlacePart(p, t0, t0 + tokensPerBlock < p.tokens ? t0 + tokensPerBlock : p.tokens, total, before, bits);
+}
+
+// Gradient of the weights with respect to the logits of one token, by one
+// wave: the row is put together in LDS, which the chosen entries enter by index.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void RouteGradKernel(RouteGradLaunch p)
 {
+    __shared__ float rows[4][V * 64];
     const int lane = threadIdx.x & 63;
     const int64_t t = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (t >= p.tokens) return;
+    if (t >= p.tokens) return;  // whole waves
+    float* row = rows[threadIdx.x >> 6];
     const int experts = static_cast<int>(p.experts), k = static_cast<int>(p.k);
     const float w = lane < k ? p.weights[t * k + lane] : 0.0f;
     const float g = lane < k ? p.grad_weights[t * k + lane] : 0.0f;
     const int id = lane < k ? p.ids[t * k + lane] : -1;
     const float dot = WaveSum(id >= 0 ? w * g : 0.0f);
-    float d[V];
-    float prob[V];
     if (p.normalize) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) d[i] = 0.0f;
+        for (int i = 0; i < V; ++i) row[64 * i + lane] = 0.0f;
     } else {
-        LoadRow<T, V>(static_cast<const T*>(p.logits) + t * p.ld, experts, lane, prob);
+        float prob[V];
+        const T* logits = static_cast<const T*>(p.logits) + t * p.ld;
         float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < V; ++i) top = fmaxf(top, prob[i]);
+        for (int i = 0; i < V; ++i) {
+            prob[i] = 64 * i + lane < experts ? ToFloat(logits[64 * i + lane]) : -INFINITY;
+            top = fmaxf(top, prob[i]);
+        }
         top = WaveMax(top);
         float s = 0.0f;
 #pragma unroll
@@ -265,35 +296,23 @@ __global__ __launch_bounds__(256) void RouteGradKernel(RouteGradLaunch p)
         }
         s = WaveSum(s);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            prob[i] = s == 0.0f ? 0.0f : prob[i] / s;
-            d[i] = -prob[i] * dot;
-        }
+        for (int i = 0; i < V; ++i) row[64 * i + lane] = s == 0.0f ? 0.0f : -(prob[i] / s) * dot;
     }
-    // the k chosen entries: those of lane l are taken up by the lane that holds expert id
-    for (int j = 0; j < k; ++j) {
-        const int idj = __shfl(id, j);
-        const float wj = __shfl(w, j), gj = __shfl(g, j);
-        if (idj >= 0 && lane == (idj & 63)) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                if (i == (idj >> 6)) d[i] = wj * (gj - dot);
-            }
-        }
-    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (id >= 0 && id < experts) row[id] = w * (g - dot);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     T* out = static_cast<T*>(p.grad_logits) + t * p.ld_grad;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        if (64 * i + lane < experts) out[64 * i + lane] = FromFloat<T>(d[i]);
+        if (64 * i + lane < experts) out[64 * i + lane] = FromFloat<T>(row[64 * i + lane]);
     }
 }
 
-int64_t TokensPerBlock(int64_t tokens, int64_t k)
+// Whole turns of 64 tokens, and no more than 256 workgroups.
+int64_t TokensPerBlock(int64_t tokens)
 {
-    // 16 tokens at least (one per wave), and no more than 256 workgroups
-    const int64_t even = (tokens + 255) / 256;
-    const int64_t least = (kRouteThreads + k - 1) / k;
-    return even > least ? even : least;
+    const int64_t turns = (tokens + 256 * kTokensPerTurn - 1) / (256 * kTokensPerTurn);
+    return (turns > 0 ? turns : 1) * kTokensPerTurn;
 }
 
 int Bits(int64_t experts)
@@ -303,14 +322,17 @@ int Bits(int64_t experts)
     return b;
 }
 
-template <typename T, int V>
+template <typename T, int V, int L>
 int RouteTyped(const RouteLaunch& l, hipStream_t s)
 {
-    const int64_t per = TokensPerBlock(l.tokens, l.k);
-    const int64_t blocks = RouteBlocks(l.tokens, l.experts, l.k);
-    RouteGateKernel<T, V><<<static_cast<uint32_t>(blocks), kRouteThreads, 0, s>>>(l, per);
-    RoutePlaceKernel<<<static_cast<uint32_t>(blocks), kRouteThreads, 0, s>>>(l, per, static_cast<int>(blocks),
-                                                                            Bits(l.experts));
+    const int64_t per = TokensPerBlock(l.tokens);
+    const int64_t blocks = RouteBlocks(l.tokens);
+    if (blocks == 1) {
+        RouteOneKernel<T, V, L><<<1, kRouteThreads, 0, s>>>(l, Bits(l.experts));
+        return 0;
+    }
+    RouteGateKernel<T, V, L><<<static_cast<uint32_t>(blocks), kRouteThreads, 0, s>>>(l, per);
+    RoutePlaceKernel<<<static_cast<uint32_t>(blocks), kRouteThreads, 0, s>>>(l, per, Bits(l.experts));
     return 0;
 }
 
@@ -321,38 +343,45 @@ int RouteGradTyped(const RouteGradLaunch& l, hipStream_t s)
     return 0;
 }
 
+template <typename T>
+int RouteByExperts(const RouteLaunch& l, hipStream_t s)
+{
+    if (l.experts <= 64) return RouteTyped<T, 4, 16>(l, s);
+    if (l.experts <= 128) return RouteTyped<T, 8, 16>(l, s);
+    if (l.experts <= 256) return RouteTyped<T, 16, 16>(l, s);
+    return RouteTyped<T, 16, 64>(l, s);
+}
+
+template <typename T>
+int RouteGradByExperts(const RouteGradLaunch& l, hipStream_t s)
+{
+    if (l.experts <= 64) return RouteGradTyped<T, 1>(l, s);
+    if (l.experts <= 128) return RouteGradTyped<T, 2>(l, s);
+    if (l.experts <= 256) return RouteGradTyped<T, 4>(l, s);
+    return RouteGradTyped<T, 16>(l, s);
+}
+
 }  // namespace
 
-int64_t RouteBlocks(int64_t tokens, int64_t experts, int64_t k)
+int64_t RouteBlocks(int64_t tokens)
 {
-    (void)experts;
-    const int64_t per = TokensPerBlock(tokens, k);
+    const int64_t per = TokensPerBlock(tokens);
     const int64_t b = (tokens + per - 1) / per;
     return b > 0 ? b : 1;
 }
 
-#define ROUTE_BY_EXPERTS(T, FN)                         \
-    if (l.experts <= 64) return FN<T, 1>(l, s);         \
-    if (l.experts <= 128) return FN<T, 2>(l, s);        \
-    if (l.experts <= 256) return FN<T, 4>(l, s);        \
-    if (l.experts <= 512) return FN<T, 8>(l, s);        \
-    return FN<T, 16>(l, s);
-
 int LaunchRoute(const RouteLaunch& l, void* stream)
 {
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (l.logits == nullptr) return RouteTyped<float, 1>(l, s);  // the choice is given: V is not used
-    if (l.type == ACL_FLOAT16) { ROUTE_BY_EXPERTS(Half, RouteTyped) }
-    if (l.type == ACL_BF16) { ROUTE_BY_EXPERTS(Bf16, RouteTyped) }
-    ROUTE_BY_EXPERTS(float, RouteTyped)
+    if (l.logits == nullptr || l.type == ACL_FLOAT) return RouteByExperts<float>(l, s);
+    return l.type == ACL_FLOAT16 ? RouteByExperts<Half>(l, s) : RouteByExperts<Bf16>(l, s);
 }
 
 int LaunchRouteGrad(const RouteGradLaunch& l, void* stream)
 {
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (l.type == ACL_FLOAT16) { ROUTE_BY_EXPERTS(Half, RouteGradTyped) }
-    if (l.type == ACL_BF16) { ROUTE_BY_EXPERTS(Bf16, RouteGradTyped) }
-    ROUTE_BY_EXPERTS(float, RouteGradTyped)
+    if (l.type == ACL_FLOAT) return RouteGradByExperts<float>(l, s);
+    return l.type == ACL_FLOAT16 ? RouteGradByExperts<Half>(l, s) : RouteGradByExperts<Bf16>(l, s);
 }
 
 }  // namespace aclsp

@@ -11,13 +11,14 @@ pattern by columns, which the products read.  One layer is::
 the current torch stream; nothing waits for the device.  There is no CPU path.  The reference has no counterpart.
 """
 import ctypes
+import functools
 from typing import NamedTuple, Optional
 
 import torch
 
 from . import _lib
 from ._lib import Operation, check
-from .spmv import Handle, _stream_ptr, acl_dtype
+from .spmv import Handle, acl_dtype
 
 _MAX_EXPERTS, _MAX_K = 1024, 64
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
@@ -36,27 +37,49 @@ class ExpertPlan(NamedTuple):
     places: Optional[torch.Tensor] = None
 
 
+# the C enumeration's value of each type (a dictionary look-up costs less than an enumeration's conversion)
+_TYPE = {t: int(acl_dtype(t)) for t in (torch.float32, torch.float16, torch.bfloat16, torch.int8)}
+_NN, _NT = int(Operation.NON_TRANSPOSE), int(Operation.TRANSPOSE)
+
+# torch's own look-ups of the current stream and device without the objects that its public ones build around
+# them (4 us of a call's 14); the public ones where a version has not got them
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
 _HANDLES = {}
-
-
-def _handle(device):
-    """The handle of a device's current stream; a handle holds nothing but the stream."""
-    stream = _stream_ptr(device)
-    key = (device.index, stream)
-    h = _HANDLES.get(key)
-    if h is None:
-        h = _HANDLES[key] = Handle(stream)
-    return h.h
+_FUNCTIONS = {}
 
 
 def _call(device, name, *args):
-    """Calls a C function on the device's current stream, with that device current."""
-    fn = getattr(_lib.lib(), name)
-    if torch.cuda.current_device() == device.index:
-        check(name, fn(_handle(device), *args))
+    """Calls a C function on the device's current stream, with that device current.
+
+    Handles are kept per stream: one holds nothing but the stream.
+    """
+    index = device.index
+    stream = _raw_stream(index) or _lib.HIP_NULL_STREAM
+    handle = _HANDLES.get((index, stream))
+    if handle is None:
+        handle = _HANDLES[(index, stream)] = Handle(stream)
+    fn = _FUNCTIONS.get(name)
+    if fn is None:
+        fn = _FUNCTIONS[name] = getattr(_lib.lib(), name)
+    if _current_device() == index:
+        status = fn(handle.h, *args)
     else:
         with torch.cuda.device(device):
-            check(name, fn(_handle(device), *args))
+            status = fn(handle.h, *args)
+    if status:
+        check(name, status)
+
+
+def _tracked(*tensors):
+    """Whether autograd has to see the call."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _on_device(first, **others):
@@ -111,41 +134,61 @@ def _route_shape(tokens, experts, k):
         raise ValueError("tokens * k must fit int32")
 
 
-def _plan_tensors(tokens, experts, k, device):
-    """Plan and buffer of a routing call, cut from two allocations."""
+@functools.lru_cache(maxsize=256)
+def _buffer_size(device, tokens, experts, k):
     size = ctypes.c_size_t(0)
     _call(device, "aclsparseRoute_bufferSize", tokens, experts, k, ctypes.byref(size))
-    buffer = torch.empty(size.value, dtype=torch.uint8, device=device)
-    return (torch.empty(experts + 1, dtype=torch.int32, device=device),
-            torch.empty(tokens * k, dtype=torch.int32, device=device),
-            torch.empty(tokens, k, dtype=torch.int32, device=device), buffer)
+    return size.value
+
+
+def _plan_tensors(tokens, experts, k, device, ids):
+    """Plan tensors (with the choice's where ``ids``) and the buffer of a routing call, in one allocation."""
+    n = tokens * k
+    sizes = [n, n, n if ids else 0, experts + 1, _buffer_size(device, tokens, experts, k) // 4]
+    starts = [0]
+    for size in sizes:
+        starts.append(starts[-1] + (size + 15) // 16 * 16)  # each part at a multiple of 64 bytes
+    data = torch.empty(starts[-1], dtype=torch.int32, device=device)
+    row_tokens = data.as_strided((n,), (1,), starts[0])
+    places = data.as_strided((tokens, k), (k, 1), starts[1])
+    chosen = data.as_strided((tokens, k), (k, 1), starts[2]) if ids else None
+    offsets = data.as_strided((experts + 1,), (1,), starts[3])
+    return offsets, row_tokens, places, chosen, data.data_ptr() + 4 * starts[4]
+
+
+def _route(logits, k, normalize):
+    tokens, experts = logits.shape
+    offsets, row_tokens, places, ids, buffer = _plan_tensors(tokens, experts, k, logits.device, True)
+    weights = torch.empty(tokens, k, dtype=torch.float32, device=logits.device)
+    _call(logits.device, "aclsparseRoute", tokens, experts, k, logits.data_ptr(), _ld(logits), _TYPE[logits.dtype],
+          int(normalize), weights.data_ptr(), ids.data_ptr(), offsets.data_ptr(), row_tokens.data_ptr(),
+          places.data_ptr(), buffer)
+    return weights, ids, offsets, row_tokens, places
 
 
 class _Route(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, k, normalize):
         logits = _rows(logits)
-        tokens, experts = logits.shape
-        offsets, row_tokens, places, buffer = _plan_tensors(tokens, experts, k, logits.device)
-        weights = torch.empty(tokens, k, dtype=torch.float32, device=logits.device)
-        ids = torch.empty(tokens, k, dtype=torch.int32, device=logits.device)
-        _call(logits.device, "aclsparseRoute", tokens, experts, k, logits.data_ptr(), _ld(logits),
-              int(acl_dtype(logits.dtype)), int(normalize), weights.data_ptr(), ids.data_ptr(), offsets.data_ptr(),
-              row_tokens.data_ptr(), places.data_ptr(), buffer.data_ptr())
+        weights, ids, offsets, row_tokens, places = _route(logits, k, normalize)
         ctx.mark_non_differentiable(ids, offsets, row_tokens, places)
-        ctx.save_for_backward(logits, weights, ids)
-        ctx.normalize = normalize
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(None if normalize else logits, weights, ids)
+        ctx.dtype, ctx.shape, ctx.normalize = logits.dtype, logits.shape, normalize
         return weights, ids, offsets, row_tokens, places
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad, *_unused):
+        if grad is None:
+            return None, None, None
         logits, weights, ids = ctx.saved_tensors
-        tokens, experts = logits.shape
+        tokens, experts = ctx.shape
         grad = grad.to(torch.float32).contiguous()
-        out = torch.empty(tokens, experts, dtype=logits.dtype, device=logits.device)
-        _call(logits.device, "aclsparseRouteGrad", tokens, experts, weights.shape[1], logits.data_ptr(), _ld(logits),
-              int(acl_dtype(logits.dtype)), int(ctx.normalize), weights.data_ptr(), ids.data_ptr(), grad.data_ptr(),
+        out = torch.empty(tokens, experts, dtype=ctx.dtype, device=ids.device)
+        _call(ids.device, "aclsparseRouteGrad", tokens, experts, ids.shape[1],
+              logits.data_ptr() if logits is not None else None, _ld(logits) if logits is not None else 0,
+              _TYPE[ctx.dtype], int(ctx.normalize), weights.data_ptr(), ids.data_ptr(), grad.data_ptr(),
               out.data_ptr(), experts)
         return out, None, None
 
@@ -163,7 +206,10 @@ def route(logits, k, normalize=True):
         raise TypeError(f"logits must be float32, float16 or bfloat16, got {logits.dtype}")
     _on_device(logits)
     _route_shape(logits.shape[0], logits.shape[1], k)
-    weights, ids, offsets, tokens, places = _Route.apply(logits, int(k), bool(normalize))
+    if _tracked(logits):
+        weights, ids, offsets, tokens, places = _Route.apply(logits, k, bool(normalize))
+    else:
+        weights, ids, offsets, tokens, places = _route(_rows(logits), k, bool(normalize))
     return weights, ids, ExpertPlan(offsets, tokens, places)
 
 
@@ -178,9 +224,9 @@ def expert_plan(ids, experts):
         raise ValueError("there must be one choice and one expert at least")
     if k > min(experts, _MAX_K) or experts > _MAX_EXPERTS or tokens * k > 2**31 - 1:
         raise ValueError(f"at most {_MAX_EXPERTS} experts and k <= {_MAX_K} and the experts, got {experts} and {k}")
-    offsets, row_tokens, places, buffer = _plan_tensors(tokens, experts, k, ids.device)
+    offsets, row_tokens, places, _, buffer = _plan_tensors(tokens, experts, k, ids.device, False)
     _call(ids.device, "aclsparseExpertPlan", tokens, experts, k, ids.data_ptr(), offsets.data_ptr(),
-          row_tokens.data_ptr(), places.data_ptr(), buffer.data_ptr())
+          row_tokens.data_ptr(), places.data_ptr(), buffer)
     return ExpertPlan(offsets, row_tokens, places)
 
 
@@ -189,10 +235,10 @@ def expert_plan(ids, experts):
 
 def _grouped(op, a, b, offsets, index, rows, n, k, out_dtype):
     out = torch.empty(rows, n, dtype=out_dtype, device=a.device)
-    _call(a.device, "aclsparseGroupedMM", int(op), b.shape[0], rows, n, k, offsets.data_ptr(),
+    _call(a.device, "aclsparseGroupedMM", op, b.shape[0], rows, n, k, offsets.data_ptr(),
           index.data_ptr() if index is not None else None, a.shape[0], a.data_ptr(), _ld(a), b.data_ptr(), _ld(b),
-          b.stride(0) if b.shape[0] > 1 else 0, int(acl_dtype(a.dtype)), out.data_ptr(), max(n, 1),
-          int(acl_dtype(out_dtype)))
+          b.stride(0) if b.shape[0] > 1 else 0, _TYPE[a.dtype], out.data_ptr(), max(n, 1),
+          _TYPE[out_dtype])
     return out
 
 
@@ -200,8 +246,8 @@ def _combine(y, places, weights, dtype):
     tokens, k = places.shape
     out = torch.empty(tokens, y.shape[1], dtype=dtype, device=y.device)
     _call(y.device, "aclsparseCombine", tokens, k, y.shape[1], y.shape[0], places.data_ptr(),
-          weights.data_ptr() if weights is not None else None, y.data_ptr(), _ld(y), int(acl_dtype(y.dtype)),
-          out.data_ptr(), max(y.shape[1], 1), int(acl_dtype(dtype)))
+          weights.data_ptr() if weights is not None else None, y.data_ptr(), _ld(y), _TYPE[y.dtype],
+          out.data_ptr(), max(y.shape[1], 1), _TYPE[dtype])
     return out
 
 
@@ -211,7 +257,7 @@ class _GroupedMM(torch.autograd.Function):
         a, w = _rows(a), _rows(w)
         rows = a.shape[0] if tokens is None else tokens.numel()
         ctx.save_for_backward(a, w, offsets, tokens, places)
-        return _grouped(Operation.TRANSPOSE, a, w, offsets, tokens, rows, w.shape[1], w.shape[2], a.dtype)
+        return _grouped(_NT, a, w, offsets, tokens, rows, w.shape[1], w.shape[2], a.dtype)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -222,17 +268,17 @@ class _GroupedMM(torch.autograd.Function):
         da = dw = None
         if ctx.needs_input_grad[0]:
             if tokens is None:
-                da = _grouped(Operation.NON_TRANSPOSE, grad, w, offsets, None, rows, k, n, a.dtype)
+                da = _grouped(_NN, grad, w, offsets, None, rows, k, n, a.dtype)
             else:
                 # a token's rows are summed in fp32 and rounded once
-                part = _grouped(Operation.NON_TRANSPOSE, grad, w, offsets, None, rows, k, n, torch.float32)
+                part = _grouped(_NN, grad, w, offsets, None, rows, k, n, torch.float32)
                 da = _combine(part, places, None, a.dtype)
         if ctx.needs_input_grad[1]:
             dw = torch.empty(groups, n, k, dtype=w.dtype, device=w.device)
             _call(a.device, "aclsparseGroupedMMGrad", groups, rows, n, k, offsets.data_ptr(),
                   tokens.data_ptr() if tokens is not None else None, a.shape[0], grad.data_ptr(), _ld(grad),
-                  a.data_ptr(), _ld(a), int(acl_dtype(a.dtype)), dw.data_ptr(), max(k, 1), n * k,
-                  int(acl_dtype(dw.dtype)))
+                  a.data_ptr(), _ld(a), _TYPE[a.dtype], dw.data_ptr(), max(k, 1), n * k,
+                  _TYPE[dw.dtype])
         return da, dw, None, None, None
 
 
@@ -250,6 +296,10 @@ def grouped_mm(a, w, plan, gather=False):
     offsets, tokens = _plan_args(plan, gather, a.device)
     if offsets.numel() != w.shape[0] + 1:
         raise ValueError(f"the plan has {offsets.numel() - 1} experts, w {w.shape[0]}")
+    if not _tracked(a, w):
+        a, w = _rows(a), _rows(w)
+        return _grouped(_NT, a, w, offsets, tokens, a.shape[0] if tokens is None else tokens.shape[0], w.shape[1],
+                        w.shape[2], a.dtype)
     places = None
     if gather and a.requires_grad:
         if plan.places is None or plan.places.numel() != tokens.numel() or plan.places.shape[0] != a.shape[0]:
@@ -295,7 +345,7 @@ def grouped_mm_scaled(a, a_scale, w, w_scale, plan=None, gather=False, out_dtype
     _call(a.device, "aclsparseGroupedMMScaled", groups, rows, n, k, offsets.data_ptr() if offsets is not None else None,
           tokens.data_ptr() if tokens is not None else None, a.shape[0], a.data_ptr(), _ld(a), a_scale.data_ptr(),
           w.data_ptr(), _ld(w), w.stride(0) if groups > 1 else 0, w_scale.data_ptr(), out.data_ptr(), max(n, 1),
-          int(acl_dtype(out_dtype)))
+          _TYPE[out_dtype])
     return out
 
 
@@ -320,7 +370,7 @@ class _Combine(torch.autograd.Function):
         dw = torch.empty(tokens, k, dtype=torch.float32, device=y.device) if ctx.needs_input_grad[1] else None
         _call(y.device, "aclsparseCombineGrad", tokens, k, width, rows, offsets.numel() - 1, offsets.data_ptr(),
               places.data_ptr(), weights.data_ptr() if weights is not None else None, y.data_ptr(), _ld(y),
-              grad.data_ptr(), _ld(grad), int(acl_dtype(y.dtype)), dy.data_ptr() if dy is not None else None,
+              grad.data_ptr(), _ld(grad), _TYPE[y.dtype], dy.data_ptr() if dy is not None else None,
               max(width, 1), dw.data_ptr() if dw is not None else None)
         return dy, dw, None, None
 
@@ -346,4 +396,7 @@ def combine(y, plan, weights=None):
         if weights.shape != plan.places.shape:
             raise ValueError(f"weights must be {tuple(plan.places.shape)}, got {tuple(weights.shape)}")
         weights = weights.contiguous()
-    return _Combine.apply(y, weights, _index(plan.offsets, "offsets"), _index(plan.places, "places"))
+    places = _index(plan.places, "places")
+    if not _tracked(y, weights):
+        return _combine(_rows(y), places, weights, y.dtype)
+    return _Combine.apply(y, weights, _index(plan.offsets, "offsets"), places)

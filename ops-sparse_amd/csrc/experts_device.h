@@ -113,33 +113,6 @@ __device__ __forceinline__ void GroupRows(const int32_t* offsets, int64_t rows, 
     end = e < begin ? begin : e > r ? r : e;
 }
 
-// Group g's tiles of `height` rows for lane g - g0; the tail's for the lane past the last group's.
-__device__ __forceinline__ int32_t LaneTiles(const int32_t* offsets, int64_t rows, int32_t groups, int32_t height,
-                                             int32_t g, int32_t& begin, int32_t& end)
-{
-    begin = end = 0;
-    if (g < groups) {
-        GroupRows(offsets, rows, g, begin, end);
-    } else if (g == groups && offsets != nullptr) {
-        int32_t unused;
-        GroupRows(offsets, rows, g - 1, unused, begin);
-        end = static_cast<int32_t>(rows);
-    }
-    return (end - begin + height - 1) / height;
-}
-
-// All tiles of `height` rows, through the groups and the tail.  Called by whole waves.
-__device__ __forceinline__ int32_t CountTiles(const int32_t* offsets, int64_t rows, int64_t groups, int32_t height)
-{
-    int32_t total = 0, begin, end;
-    for (int32_t g0 = 0; g0 <= static_cast<int32_t>(groups); g0 += 64) {
-        const int32_t n = LaneTiles(offsets, rows, static_cast<int32_t>(groups), height, g0 + (threadIdx.x & 63),
-                                    begin, end);
-        total += __builtin_amdgcn_readlane(WaveInclusiveSum(n), 63);
-    }
-    return total;
-}
-
 // A tile of a ragged product: rows [row, end) of `group`; group == groups is
 // the tail of rows that belong to no group, group < 0 no tile.
 struct RaggedTile {
@@ -151,28 +124,88 @@ struct RaggedTile {
     int32_t tiles;   // and its own
 };
 
-// The tile-th tile of `height` rows, counted through the groups and the tail.
-// Called by whole waves with a uniform tile; 64 groups a turn.
-__device__ __forceinline__ RaggedTile FindTile(const int32_t* offsets, int64_t rows, int64_t groups, int32_t height,
-                                               int32_t tile)
-{
-    int32_t before = 0;
-    for (int32_t g0 = 0; g0 <= static_cast<int32_t>(groups); g0 += 64) {
-        int32_t begin, end;
-        const int32_t n = LaneTiles(offsets, rows, static_cast<int32_t>(groups), height, g0 + (threadIdx.x & 63),
-                                    begin, end);
-        const int32_t incl = WaveInclusiveSum(n);
-        const uint64_t hit = __ballot(before + incl > tile);
-        if (hit != 0) {
-            const int src = __builtin_ctzll(hit);
-            const int32_t skipped = before + __builtin_amdgcn_readlane(incl - n, src);
-            const int32_t first = __builtin_amdgcn_readlane(begin, src);
-            return {g0 + src,  first + (tile - skipped) * height, __builtin_amdgcn_readlane(end, src), first, skipped,
-                    __builtin_amdgcn_readlane(n, src)};
-        }
-        before += __builtin_amdgcn_readlane(incl, 63);
+// The tiles of `height` rows of all groups and then of the tail, for whole
+// waves: 64 groups at a time, one per lane.  The first 64 are read once for
+// both the count and the search, which every workgroup waits for.
+struct RaggedTiles {
+    const int32_t* offsets;
+    int32_t rows, groups, height;
+    int32_t begin, end, tiles, upTo;  // this lane's group of the first 64; upTo: tiles through it
+    int32_t tail;                     // its first row
+    int32_t total;
+
+    __device__ __forceinline__ int32_t Count(int32_t from, int32_t to) const
+    {
+        return (to - from + height - 1) / height;
     }
-    return {-1, 0, 0, 0, 0, 0};
+
+    __device__ __forceinline__ void Lane(int32_t g, int32_t& from, int32_t& to) const
+    {
+        from = to = 0;
+        if (g < groups) GroupRows(offsets, rows, g, from, to);
+    }
+
+    __device__ __forceinline__ RaggedTiles(const int32_t* o, int64_t r, int64_t g, int32_t h)
+        : offsets(o), rows(static_cast<int32_t>(r)), groups(static_cast<int32_t>(g)), height(h)
+    {
+        const int lane = threadIdx.x & 63;
+        Lane(lane, begin, end);
+        tiles = Count(begin, end);
+        upTo = WaveInclusiveSum(tiles);
+        total = __builtin_amdgcn_readlane(upTo, 63);
+        int32_t last = end, lastLane = (groups < 64 ? groups : 64) - 1;
+        for (int32_t g0 = 64; g0 < groups; g0 += 64) {
+            int32_t from;
+            Lane(g0 + lane, from, last);
+            total += __builtin_amdgcn_readlane(WaveInclusiveSum(Count(from, last)), 63);
+            lastLane = (groups - g0 < 64 ? groups - g0 : 64) - 1;
+        }
+        tail = offsets != nullptr ? __builtin_amdgcn_readlane(last, lastLane) : rows;
+        total += Count(tail, rows);
+    }
+
+    // The tile-th tile; `tile` is uniform.
+    __device__ __forceinline__ RaggedTile Find(int32_t tile) const
+    {
+        int32_t before = 0, from = begin, to = end, n = tiles, through = upTo;
+        for (int32_t g0 = 0; g0 < groups; g0 += 64) {
+            if (g0 > 0) {
+                Lane(g0 + static_cast<int32_t>(threadIdx.x & 63), from, to);
+                n = Count(from, to);
+                through = WaveInclusiveSum(n);
+            }
+            const uint64_t hit = __ballot(before + through > tile);
+            if (hit != 0) {
+                const int src = __builtin_ctzll(hit);
+                const int32_t skipped = before + __builtin_amdgcn_readlane(through - n, src);
+                const int32_t first = __builtin_amdgcn_readlane(from, src);
+                return {g0 + src, first + (tile - skipped) * height, __builtin_amdgcn_readlane(to, src), first, skipped,
+                        __builtin_amdgcn_readlane(n, src)};
+            }
+            before += __builtin_amdgcn_readlane(through, 63);
+        }
+        const int32_t n0 = Count(tail, rows);
+        if (tile - before >= n0) return {-1, 0, 0, 0, 0, 0};
+        return {groups, tail + (tile - before) * height, rows, tail, before, n0};
+    }
+};
+
+// The `nth`-longest group (equal ones by number), by whole waves: work handed
+// out in this order leaves no long group for the end.  Beyond 64 groups, where
+// one weighs less, their own order.
+__device__ __forceinline__ int32_t LongestGroup(const int32_t* offsets, int64_t rows, int32_t groups, int32_t nth)
+{
+    if (groups > 64 || offsets == nullptr) return nth;
+    const int lane = threadIdx.x & 63;
+    int32_t begin = 0, end = -1;
+    if (lane < groups) GroupRows(offsets, rows, lane, begin, end);
+    const int32_t length = end - begin;
+    int32_t rank = 0;
+    for (int i = 0; i < groups; ++i) {
+        const int32_t other = __builtin_amdgcn_readlane(length, i);
+        rank += other > length || (other == length && i < lane) ? 1 : 0;
+    }
+    return __builtin_ctzll(__ballot(lane < groups && rank == nth));
 }
 
 }  // namespace aclsp

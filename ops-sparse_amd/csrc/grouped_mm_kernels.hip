@@ -640,11 +640,10 @@ template <typename T, typename TOut, bool kBTrans>
 __global__ __launch_bounds__(512, 1) void GroupedTileKernel(GroupedLaunch p, int32_t tilesN, int32_t cus)
 {
     __shared__ __align__(128) char lds[2 * (kTileRows + 256) * kTurnBytes];
-    const int64_t total = static_cast<int64_t>(CountTiles(p.offsets, p.rows, p.groups, kTileRows)) * tilesN;
-    const TileShare share = ShareOfWorkgroup(total, cus);
+    const RaggedTiles tiles(p.offsets, p.rows, p.groups, kTileRows);
+    const TileShare share = ShareOfWorkgroup(static_cast<int64_t>(tiles.total) * tilesN, cus);
     if (share.tile < 0) return;
-    const RaggedTile tile =
-        FindTile(p.offsets, p.rows, p.groups, kTileRows, static_cast<int32_t>(share.tile / tilesN));
+    const RaggedTile tile = tiles.Find(static_cast<int32_t>(share.tile / tilesN));
     if (tile.group < 0) return;
     const TilePlace place = PlaceInBands(share.tile - static_cast<int64_t>(tile.before) * tilesN, tile.tiles, tilesN);
     const int32_t height = kTileRows / share.parts;
@@ -666,10 +665,10 @@ template <typename T, typename TOut, bool kBTrans, bool kAligned>
 __global__ __launch_bounds__(256, 1) void GroupedSmallTileKernel(GroupedLaunch p, int32_t tilesN)
 {
     __shared__ __align__(128) char lds[2 * (64 + 128) * kTurnBytes];
-    const int64_t total = static_cast<int64_t>(CountTiles(p.offsets, p.rows, p.groups, 64)) * tilesN;
-    const TileShare share = ShareOfWorkgroup(total, 1);
+    const RaggedTiles tiles(p.offsets, p.rows, p.groups, 64);
+    const TileShare share = ShareOfWorkgroup(static_cast<int64_t>(tiles.total) * tilesN, 1);
     if (share.tile < 0) return;
-    const RaggedTile tile = FindTile(p.offsets, p.rows, p.groups, 64, static_cast<int32_t>(share.tile / tilesN));
+    const RaggedTile tile = tiles.Find(static_cast<int32_t>(share.tile / tilesN));
     if (tile.group < 0) return;
     const TilePlace place = PlaceInBands(share.tile - static_cast<int64_t>(tile.before) * tilesN, tile.tiles, tilesN);
     const int32_t row = tile.begin + place.m * 64;
@@ -690,9 +689,10 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void GroupedGradTileKernel(Grouped
     // Every die takes an eighth of each group's tiles, so that a long group is no die's alone; which
     // eighth turns with the group, so that the last, shorter ones go round too.
     const int32_t per = (tilesN * tilesK + 7) / 8, at = static_cast<int32_t>(blockIdx.x / 8);
-    const int32_t g = at / per;
-    const int32_t id = static_cast<int32_t>((blockIdx.x + g) % 8) * per + at % per;
+    const int32_t nth = at / per;
+    const int32_t id = static_cast<int32_t>((blockIdx.x + nth) % 8) * per + at % per;
     if (id >= tilesN * tilesK) return;
+    const int32_t g = LongestGroup(p.offsets, p.rows, static_cast<int32_t>(p.groups), nth);
     const TilePlace place = PlaceInBands(id, tilesN, tilesK);
     const int64_t n0 = static_cast<int64_t>(place.m) * BM, k0 = static_cast<int64_t>(place.n) * BN;
     const int wave = WaveNumber();
@@ -729,8 +729,8 @@ __global__ __launch_bounds__(kWaves * 64) void GroupedRowsKernel(GroupedLaunch p
     using Acc = typename Mma<T>::Acc;
     constexpr int kAhead = 16 / (MT + NT) > 4 ? 8 : 4;  // steps loaded before they are multiplied
     __shared__ Acc part[kWaves][MT * NT][64];
-    const RaggedTile tile =
-        FindTile(p.offsets, p.rows, p.groups, MT * 16, static_cast<int32_t>(blockIdx.x / static_cast<uint32_t>(tilesN)));
+    const RaggedTile tile = RaggedTiles(p.offsets, p.rows, p.groups, MT * 16)
+                                .Find(static_cast<int32_t>(blockIdx.x / static_cast<uint32_t>(tilesN)));
     const int32_t n0 = static_cast<int32_t>(blockIdx.x % static_cast<uint32_t>(tilesN)) * NT * 16;
     const int32_t width = static_cast<int32_t>(p.n);
     if (tile.group < 0 || n0 >= width) return;

@@ -21,6 +21,9 @@ SOURCES = ["handle_descr.cpp", "spmv_host.cpp", "spmv_kernels.hip", "spmv_csc_so
            "experts_host.cpp", "experts_route.hip", "experts_combine.hip", "grouped_mm_kernels.hip"]
 OUT = os.path.join(PKG_ROOT, "lib", "libaclsparse_hip.so")
 OBJ_DIR = os.path.join(PKG_ROOT, "lib", "obj")
+# the experts' operators on torch tensors: a Python module next to the library, which itself needs no torch
+TORCH_SOURCE = "experts_torch.cpp"
+TORCH_OUT = os.path.join(PKG_ROOT, "lib", "_ops_sparse_experts.so")
 
 HIPCC_FLAGS = [
     "-std=c++17", "-O3", "--offload-arch=gfx950", "-fPIC", "-shared",
@@ -65,8 +68,25 @@ def file_build_id(path):
     return data[j:j + 32].decode(errors="replace")
 
 
+def torch_module_command(bid):
+    """The command that compiles and links the torch module (host code only)."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], "/opt/rocm/include",
+                os.path.join(REPO_ROOT, "include")]
+    libs = cpp_extension.library_paths()
+    return ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            f"-DACLSPARSE_HIP_BUILD_ID=\"{bid}\"", *["-isystem" + i for i in includes],
+            os.path.join(CSRC, TORCH_SOURCE), *["-L" + d for d in libs], "-lc10", "-lc10_hip", "-ltorch_cpu",
+            "-ltorch", "-ltorch_python", "-ldl", "-o", TORCH_OUT + ".tmp"]
+
+
 def build_library(verbose=False):
-    """Compiles every source to an object in parallel (ops-sparse_amd/lib/obj), then links."""
+    """Compiles every source to an object in parallel (ops-sparse_amd/lib/obj), then links; the torch module beside them."""
     from concurrent.futures import ThreadPoolExecutor
 
     os.makedirs(OBJ_DIR, exist_ok=True)
@@ -84,10 +104,13 @@ def build_library(verbose=False):
             raise RuntimeError("hipcc failed:\n" + " ".join(cmd) + "\n" + res.stdout + res.stderr)
         return cmd
 
-    with ThreadPoolExecutor(max_workers=min(len(cmds), 8)) as ex:
+    with ThreadPoolExecutor(max_workers=min(len(cmds) + 1, 8)) as ex:
+        module = ex.submit(run, torch_module_command(bid))
         for cmd in ex.map(run, cmds):
             if verbose:
                 print(" ".join(cmd))
+        module.result()
+    os.replace(TORCH_OUT + ".tmp", TORCH_OUT)
     link = ["hipcc", *HIPCC_FLAGS, *[c[-1] for c in cmds], "-o", OUT + ".tmp"]
     run(link)
     os.replace(OUT + ".tmp", OUT)

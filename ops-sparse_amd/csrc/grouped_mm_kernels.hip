@@ -112,10 +112,16 @@ struct Mma32<int8_t> {
 // the contraction's end, so that no value beyond it, NaN among them, counts.
 __device__ const Int4 kZeros = {0, 0, 0, 0};
 
+// Copies 16 bytes per lane to 1024 bytes of LDS.  Written as assembly, without
+// an output: the compiler would count the copy against every later LDS read
+// that it cannot tell from the copy's target, and wait for it right there.
+// WaitAll waits for the copies.  m0 is the copy's target and is set for each;
+// nothing that the compiler makes of these kernels uses it.
 __device__ __forceinline__ void CopyToLds(const char* from, char* to)
 {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from),
-                                     (__attribute__((address_space(3))) void*)(to), 16, 0, 0);
+    const uint32_t lds = static_cast<uint32_t>(
+        reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)(to)));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from));
 }
 
 // The first `valid` bytes at `from` of any alignment (of T's at least), zeros after them.
@@ -335,34 +341,10 @@ struct ColumnOperand {
     }
 };
 
-// Orders a step's instructions: its LDS reads follow its first matrix
-// instructions, so that they have arrived when the next step starts; its
-// copies are spread over all of them, since a wave that issues copies faster
-// than the memory pipeline takes them (64 bytes per clock) waits with its
-// products behind them.
-template <int kProducts, int kReads, int kCopies>
-__device__ __forceinline__ void Interleave()
-{
-    constexpr int kMfma = 0x8, kVmem = 0x10, kDsRead = 0x100;
-    constexpr int kHalf = kProducts / 2 > 0 ? kProducts / 2 : 1;
-    constexpr int kReadsPer = (kReads + kHalf - 1) / kHalf;
-    int copied = 0;
-#pragma unroll
-    for (int i = 0; i < kProducts; ++i) {
-        __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-        if (i < kHalf) __builtin_amdgcn_sched_group_barrier(kDsRead, kReadsPer, 0);
-        const int upTo = (i + 1) * kCopies / kProducts;
-        if (upTo - copied == 1) __builtin_amdgcn_sched_group_barrier(kVmem, 1, 0);
-        if (upTo - copied == 2) __builtin_amdgcn_sched_group_barrier(kVmem, 2, 0);
-        copied = upTo;
-    }
-}
-
 // Waits for this wave's copies and reads, then for the other waves'.
 __device__ __forceinline__ void WaitAll()
 {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
@@ -372,30 +354,27 @@ __device__ __forceinline__ void WaitAll()
 // (columns of the output) rowA and rowB on.
 //
 // One turn is four matrix steps.  While a step is multiplied the next one's
-// operands are read from LDS (the group barriers below keep the compiler from
-// moving the reads behind the products they are meant to overlap).  One
-// barrier per turn, before its last step: by then every wave has read this
-// turn's operands and the next turn's have arrived, so the last step issues
-// the copies of the turn after that, which then have a turn's time.
+// operands are read from LDS.  One barrier per turn, before its last step: by
+// then every wave has read this turn's operands and the next turn's have
+// arrived, so the last step issues the first copies of the turn after that,
+// which then have a turn's time.
 template <typename T, int MI, int NI, typename OperandA, typename OperandB>
 __device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds, int64_t bytes, int rowA, int rowB,
                                              typename Mma32<T>::Acc (&acc)[MI][NI])
 {
     constexpr int kBuffer = OperandA::kBytes + OperandB::kBytes;
     constexpr int kCopies = OperandA::kLoads + OperandB::kLoads;
-    constexpr int kReads = MI * OperandA::kReads + NI * OperandB::kReads;
+    constexpr int kProducts = MI * NI, kOperands = MI + NI;
     Int4 fa[2][MI], fb[2][NI];
-    auto read = [&](int to, const char* from, int step) {
-#pragma unroll
-        for (int i = 0; i < MI; ++i) fa[to][i] = OperandA::Read(from, rowA + i * 32, step);
-#pragma unroll
-        for (int i = 0; i < NI; ++i) fb[to][i] = OperandB::Read(from + OperandA::kBytes, rowB + i * 32, step);
-    };
-    auto multiply = [&](int with) {
-#pragma unroll
-        for (int i = 0; i < MI; ++i) {
-#pragma unroll
-            for (int j = 0; j < NI; ++j) acc[i][j] = Mma32<T>::Run(fb[with][j], fa[with][i], acc[i][j]);
+    // The f-th operand of a step, in the order in which its products use them: b0, a0, b1, ..., then a1, ...
+    auto read = [&](int to, const char* from, int step, int f) {
+        if (f == 1) {
+            fa[to][0] = OperandA::Read(from, rowA, step);
+        } else if (f == 0 || f <= NI) {
+            const int j = f == 0 ? 0 : f - 1;
+            fb[to][j] = OperandB::Read(from + OperandA::kBytes, rowB + j * 32, step);
+        } else {
+            fa[to][f - NI] = OperandA::Read(from, rowA + (f - NI) * 32, step);
         }
     };
     auto copy = [&](char* to, int first, int last) {
@@ -413,6 +392,25 @@ __device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds
             b.Load();
         }
     };
+    // One step's products, in this order to the instruction: the next step's reads follow the first of them, so
+    // that they have arrived when it starts; copies [first, last) are spread over all, since a wave that issues
+    // copies faster than the memory pipeline takes them (64 bytes per clock) waits with its products behind them.
+    auto step = [&](int with, const char* from, int next, char* to, int first, int last) {
+        constexpr int kHalf = (kProducts + 1) / 2;
+        if constexpr (!OperandA::kDirect) copy(to, first, last);
+#pragma unroll
+        for (int m = 0; m < kProducts; ++m) {
+            acc[m / NI][m % NI] = Mma32<T>::Run(fb[with][m % NI], fa[with][m / NI], acc[m / NI][m % NI]);
+            if (from != nullptr && m < kHalf) {
+#pragma unroll
+                for (int f = m * kOperands / kHalf; f < (m + 1) * kOperands / kHalf; ++f) read(with ^ 1, from, next, f);
+            }
+            if constexpr (OperandA::kDirect) {
+                copy(to, first + m * (last - first) / kProducts, first + (m + 1) * (last - first) / kProducts);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
     auto prepare = [&] {
         a.Prepare(bytes);
         b.Prepare(bytes);
@@ -426,34 +424,22 @@ __device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds
     copy(lds, 0, kCopies);
     commit(lds);
     WaitAll();
-    read(0, lds, 0);
+#pragma unroll
+    for (int f = 0; f < kOperands; ++f) read(0, lds, 0, f);
     int cur = 0;
-    // kNow of the next copies go out in a turn's last step, the others in the next turn's first two.
-    constexpr int kNow = kCopies / 2, kThen = kCopies;
-    auto turn = [&](auto late, auto copies, auto more) {
-        constexpr int kLate = decltype(late)::value ? kCopies : 0, kEarly = decltype(copies)::value ? kNow : 0;
-        constexpr int kFirst = kLate > 0 ? kNow : 0, kSecond = kLate > 0 ? kThen : 0;
+    constexpr int kNow = kCopies / 2;  // of a turn's copies go out in the turn before the last's last step
+    auto turn = [&](auto late, auto early, auto more) {
+        constexpr int kFirst = decltype(late)::value ? kNow : 0, kLast = decltype(late)::value ? kCopies : 0;
         char* now = lds + cur;
         cur ^= kBuffer;
         char* next = lds + cur;
-        read(1, now, 1);
-        copy(next, kFirst, kSecond);
-        multiply(0);
-        Interleave<MI * NI, kReads, kSecond - kFirst>();
-        read(0, now, 2);
-        copy(next, kSecond, kLate);
-        multiply(1);
-        Interleave<MI * NI, kReads, kLate - kSecond>();
-        if constexpr (kEarly > 0) prepare();
-        read(1, now, 3);
-        multiply(0);
-        Interleave<MI * NI, kReads, 0>();
-        if constexpr (kLate > 0) commit(next);
+        step(0, now, 1, next, kFirst, kLast);
+        step(1, now, 2, next, 0, 0);
+        if constexpr (decltype(early)::value) prepare();
+        step(0, now, 3, next, 0, 0);
+        if constexpr (decltype(late)::value) commit(next);
         WaitAll();
-        if constexpr (decltype(more)::value) read(0, next, 0);
-        copy(now, 0, kEarly);
-        multiply(1);
-        if constexpr (decltype(more)::value) Interleave<MI * NI, kReads, kEarly>();
+        step(1, decltype(more)::value ? next : nullptr, 0, now, 0, decltype(early)::value ? kNow : 0);
     };
     if (bytes > 0) {
         prepare();

@@ -64,8 +64,8 @@ __device__ __forceinline__ int64_t IndexedRow(const int32_t* index, int64_t r, i
 
 // ---------------------------------------------------------------------------
 // Tiles through LDS, 32x32 matrix instructions.  A tile's contraction advances
-// by 128 bytes per turn.  Two buffers in LDS: while one is multiplied the next
-// is copied, straight from memory where every row is aligned to 16 bytes,
+// by 128 bytes per turn.  While one turn's
+// operands are multiplied the next ones' are copied to LDS, straight from memory where every row is aligned to 16 bytes,
 // through registers by loads of any alignment where not.  Each wave keeps the
 // operands of one matrix step ahead of the one it multiplies in registers.
 // ---------------------------------------------------------------------------
@@ -115,7 +115,7 @@ __device__ const Int4 kZeros = {0, 0, 0, 0};
 // Copies 16 bytes per lane to 1024 bytes of LDS.  Written as assembly, without
 // an output: the compiler would count the copy against every later LDS read
 // that it cannot tell from the copy's target, and wait for it right there.
-// WaitAll waits for the copies.  m0 is the copy's target and is set for each;
+// Wait waits for the copies.  m0 is the copy's target and is set for each;
 // nothing that the compiler makes of these kernels uses it.
 __device__ __forceinline__ void CopyToLds(const char* from, char* to)
 {
@@ -341,10 +341,11 @@ struct ColumnOperand {
     }
 };
 
-// Waits for this wave's copies and reads, then for the other waves'.
-__device__ __forceinline__ void WaitAll()
+// Waits for this wave's reads and its copies but the last kLeft of them, then for the other waves'.
+template <int kLeft>
+__device__ __forceinline__ void Wait()
 {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kLeft) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
@@ -356,98 +357,132 @@ __device__ __forceinline__ void WaitAll()
 // One turn is four matrix steps.  While a step is multiplied the next one's
 // operands are read from LDS.  One barrier per turn, before its last step: by
 // then every wave has read this turn's operands and the next turn's have
-// arrived, so the last step issues the first copies of the turn after that,
-// which then have a turn's time.
-template <typename T, int MI, int NI, typename OperandA, typename OperandB>
+// arrived.  B has two places in LDS, A kPlacesA: the last step copies B of the
+// turn after the next to where this turn's was; the first step copies A of the
+// turn kPlacesA - 1 ahead.  With three places the barrier need not wait for
+// the A copied last, and the memory has two turns for it: the copies alone
+// take most of a turn, and with two places both operands' were waited for
+// within three steps.
+template <typename T, int MI, int NI, int kPlacesA, typename OperandA, typename OperandB>
 __device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds, int64_t bytes, int rowA, int rowB,
                                              typename Mma32<T>::Acc (&acc)[MI][NI])
 {
-    constexpr int kBuffer = OperandA::kBytes + OperandB::kBytes;
-    constexpr int kCopies = OperandA::kLoads + OperandB::kLoads;
-    constexpr int kProducts = MI * NI, kOperands = MI + NI;
+    constexpr bool kDirect = OperandA::kDirect;
+    constexpr int kCopiesA = OperandA::kLoads, kCopiesB = OperandB::kLoads;
+    constexpr int kProducts = MI * NI, kOperands = MI + NI, kAhead = kPlacesA - 1;
+    constexpr int kLeft = kAhead == 2 ? kCopiesA : 0;  // copies that a barrier need not wait for
+    static_assert(kAhead == 1 || (kAhead == 2 && kDirect), "copies through registers are kept for one turn");
+    char* const placesB = lds + kPlacesA * OperandA::kBytes;
     Int4 fa[2][MI], fb[2][NI];
     // The f-th operand of a step, in the order in which its products use them: b0, a0, b1, ..., then a1, ...
-    auto read = [&](int to, const char* from, int step, int f) {
+    auto read = [&](int to, const char* fromA, const char* fromB, int step, int f) {
         if (f == 1) {
-            fa[to][0] = OperandA::Read(from, rowA, step);
+            fa[to][0] = OperandA::Read(fromA, rowA, step);
         } else if (f == 0 || f <= NI) {
             const int j = f == 0 ? 0 : f - 1;
-            fb[to][j] = OperandB::Read(from + OperandA::kBytes, rowB + j * 32, step);
+            fb[to][j] = OperandB::Read(fromB, rowB + j * 32, step);
         } else {
-            fa[to][f - NI] = OperandA::Read(from, rowA + (f - NI) * 32, step);
-        }
-    };
-    auto copy = [&](char* to, int first, int last) {
-        if constexpr (OperandA::kDirect) {
-#pragma unroll
-            for (int i = first; i < last; ++i) {
-                if (i < OperandA::kLoads) {
-                    a.Issue(to, i);
-                } else {
-                    b.Issue(to + OperandA::kBytes, i - OperandA::kLoads);
-                }
-            }
-        } else if (first == 0 && last > 0) {  // through registers: all at once, written to LDS by commit
-            a.Load();
-            b.Load();
+            fa[to][f - NI] = OperandA::Read(fromA, rowA + (f - NI) * 32, step);
         }
     };
     // One step's products, in this order to the instruction: the next step's reads follow the first of them, so
-    // that they have arrived when it starts; copies [first, last) are spread over all, since a wave that issues
+    // that they have arrived when it starts; `copies` calls of copy are spread over all, since a wave that issues
     // copies faster than the memory pipeline takes them (64 bytes per clock) waits with its products behind them.
-    auto step = [&](int with, const char* from, int next, char* to, int first, int last) {
+    auto step = [&](int with, const char* fromA, const char* fromB, int next, int copies, auto copy) {
         constexpr int kHalf = (kProducts + 1) / 2;
-        if constexpr (!OperandA::kDirect) copy(to, first, last);
 #pragma unroll
         for (int m = 0; m < kProducts; ++m) {
             acc[m / NI][m % NI] = Mma32<T>::Run(fb[with][m % NI], fa[with][m / NI], acc[m / NI][m % NI]);
-            if (from != nullptr && m < kHalf) {
+            if (fromA != nullptr && m < kHalf) {
 #pragma unroll
-                for (int f = m * kOperands / kHalf; f < (m + 1) * kOperands / kHalf; ++f) read(with ^ 1, from, next, f);
+                for (int f = m * kOperands / kHalf; f < (m + 1) * kOperands / kHalf; ++f) {
+                    read(with ^ 1, fromA, fromB, next, f);
+                }
             }
-            if constexpr (OperandA::kDirect) {
-                copy(to, first + m * (last - first) / kProducts, first + (m + 1) * (last - first) / kProducts);
-            }
+#pragma unroll
+            for (int i = m * copies / kProducts; i < (m + 1) * copies / kProducts; ++i) copy(i);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    auto prepare = [&] {
-        a.Prepare(bytes);
-        b.Prepare(bytes);
-        bytes -= kTurnBytes;
+    int64_t leftA = bytes, leftB = bytes;
+    int toA = 0, toB = 0;  // places of the next copies, in bytes
+    // straight to LDS one at a time, or through registers all at once (written by commit)
+    auto copyA = [&](int i) { a.Issue(lds + toA, i); };
+    auto copyB = [&](int i) { b.Issue(placesB + toB, i); };
+    auto prepareA = [&] {
+        a.Prepare(leftA);
+        leftA -= kTurnBytes;
+        if constexpr (!kDirect) a.Load();
     };
-    auto commit = [&](char* to) {
-        a.Commit(to);
-        b.Commit(to + OperandA::kBytes);
+    auto prepareB = [&] {
+        b.Prepare(leftB);
+        leftB -= kTurnBytes;
+        if constexpr (!kDirect) b.Load();
     };
-    prepare();
-    copy(lds, 0, kCopies);
-    commit(lds);
-    WaitAll();
+    auto doneA = [&] { toA = toA == (kPlacesA - 1) * OperandA::kBytes ? 0 : toA + OperandA::kBytes; };
+    auto doneB = [&] { toB ^= OperandB::kBytes; };
+    auto copyAllA = [&] {
+        prepareA();
+        if constexpr (kDirect) {
 #pragma unroll
-    for (int f = 0; f < kOperands; ++f) read(0, lds, 0, f);
-    int cur = 0;
-    constexpr int kNow = kCopies / 2;  // of a turn's copies go out in the turn before the last's last step
-    auto turn = [&](auto late, auto early, auto more) {
-        constexpr int kFirst = decltype(late)::value ? kNow : 0, kLast = decltype(late)::value ? kCopies : 0;
-        char* now = lds + cur;
-        cur ^= kBuffer;
-        char* next = lds + cur;
-        step(0, now, 1, next, kFirst, kLast);
-        step(1, now, 2, next, 0, 0);
-        if constexpr (decltype(early)::value) prepare();
-        step(0, now, 3, next, 0, 0);
-        if constexpr (decltype(late)::value) commit(next);
-        WaitAll();
-        step(1, decltype(more)::value ? next : nullptr, 0, now, 0, decltype(early)::value ? kNow : 0);
+            for (int i = 0; i < kCopiesA; ++i) copyA(i);
+        } else {
+            a.Commit(lds + toA);
+        }
+        doneA();
     };
-    if (bytes > 0) {
-        prepare();
-        copy(lds + kBuffer, 0, kNow);
-        while (bytes > 0) turn(std::true_type{}, std::true_type{}, std::true_type{});
-        turn(std::true_type{}, std::false_type{}, std::true_type{});
+    const int64_t turns = (bytes + kTurnBytes - 1) / kTurnBytes;
+    auto copyTurnB = [&] {
+        prepareB();
+        if constexpr (kDirect) {
+#pragma unroll
+            for (int i = 0; i < kCopiesB; ++i) copyB(i);
+        }
+    };
+    copyAllA();
+    copyTurnB();
+    if constexpr (!kDirect) b.Commit(placesB);
+    doneB();
+    if (kAhead == 2 && turns > 1) {
+        copyAllA();
+        Wait<kLeft>();
+    } else {
+        Wait<0>();
     }
-    turn(std::false_type{}, std::false_type{}, std::false_type{});
+    if (turns > 1) copyTurnB();
+#pragma unroll
+    for (int f = 0; f < kOperands; ++f) read(0, lds, placesB, 0, f);
+    int nowA = 0, nowB = 0;
+    // copiesA, copiesB: A of the turn kAhead on and B of the one after the next exist; more: the next one does
+    auto turn = [&](auto copiesA, auto copiesB, auto more) {
+        constexpr bool kA = decltype(copiesA)::value, kB = decltype(copiesB)::value, kMore = decltype(more)::value;
+        const char* fromA = lds + nowA;
+        const char* fromB = placesB + nowB;
+        if constexpr (kA) prepareA();
+        step(0, fromA, fromB, 1, kA && kDirect ? kCopiesA : 0, copyA);
+        step(1, fromA, fromB, 2, 0, copyA);
+        step(0, fromA, fromB, 3, 0, copyA);
+        if constexpr (!kDirect && kMore) {
+            a.Commit(lds + toA);
+            b.Commit(placesB + toB);
+        }
+        if constexpr (kA) doneA();
+        if constexpr (kMore) doneB();
+        nowA = nowA == (kPlacesA - 1) * OperandA::kBytes ? 0 : nowA + OperandA::kBytes;
+        nowB ^= OperandB::kBytes;
+        if constexpr (kB) {
+            Wait<kLeft>();
+            prepareB();
+        } else {
+            Wait<0>();
+        }
+        step(1, kMore ? lds + nowA : nullptr, placesB + nowB, 0, kB && kDirect ? kCopiesB : 0, copyB);
+    };
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
+    for (int64_t t = 2; t < turns; ++t) turn(yes, yes, yes);
+    if (turns > 1) turn(std::bool_constant<kAhead == 1>{}, no, yes);
+    turn(no, no, no);
 }
 
 // Writes a wave's MI*32 x NI*32 tile of the output, rows [0, rows) and columns
@@ -556,7 +591,7 @@ __device__ __forceinline__ TileShare ShareOfWorkgroup(int64_t total, int32_t cus
 
 constexpr int kTileRows = 256;  // of a whole tile
 
-template <typename T, typename TOut, bool kBTrans, bool kAligned, int MI, int NI, int WM, int WN>
+template <typename T, typename TOut, bool kBTrans, bool kAligned, int kPlacesA, int MI, int NI, int WM, int WN>
 __device__ __forceinline__ void GroupedTile(const GroupedLaunch& p, char* lds, int32_t group, int32_t firstRow,
                                             int32_t endRow, int64_t n0)
 {
@@ -564,7 +599,7 @@ __device__ __forceinline__ void GroupedTile(const GroupedLaunch& p, char* lds, i
     using OperandA = RowOperand<T, BM, kThreads, kAligned>;
     using OperandB = std::conditional_t<kBTrans, RowOperand<T, BN, kThreads, kAligned>,
                                         ColumnOperand<T, BN, kThreads, false, kAligned>>;
-    constexpr int kLds = 2 * (OperandA::kBytes + OperandB::kBytes);
+    constexpr int kLds = kPlacesA * OperandA::kBytes + 2 * OperandB::kBytes;
     const int lane = threadIdx.x & 63, wave = WaveNumber();
     const int rowA = (wave % WM) * MI * 32, rowB = (wave / WM) * NI * 32;
     typename Mma32<T>::Acc acc[MI][NI] = {};
@@ -589,7 +624,7 @@ __device__ __forceinline__ void GroupedTile(const GroupedLaunch& p, char* lds, i
         } else {
             b.Init(bg, p.ldb * 2, n0, p.n, nullptr, p.k, 0, static_cast<int32_t>(p.k));
         }
-        MultiplyTile<T, MI, NI>(a, b, lds, p.k * static_cast<int64_t>(sizeof(T)), rowA, rowB, acc);
+        MultiplyTile<T, MI, NI, kPlacesA>(a, b, lds, p.k * static_cast<int64_t>(sizeof(T)), rowA, rowB, acc);
     }
     const int64_t n = n0 + rowB;
     TOut* c = static_cast<TOut*>(p.c) + (firstRow + rowA) * p.ldc + n;
@@ -625,7 +660,7 @@ __device__ __forceinline__ void GroupedTile(const GroupedLaunch& p, char* lds, i
 template <typename T, typename TOut, bool kBTrans>
 __global__ __launch_bounds__(512, 1) void GroupedTileKernel(GroupedLaunch p, int32_t tilesN, int32_t cus)
 {
-    __shared__ __align__(128) char lds[2 * (kTileRows + 256) * kTurnBytes];
+    __shared__ __align__(128) char lds[(3 * kTileRows + 2 * 256) * kTurnBytes];  // all of a CU's
     const RaggedTiles tiles(p.offsets, p.rows, p.groups, kTileRows);
     const TileShare share = ShareOfWorkgroup(static_cast<int64_t>(tiles.total) * tilesN, cus);
     if (share.tile < 0) return;
@@ -638,11 +673,11 @@ __global__ __launch_bounds__(512, 1) void GroupedTileKernel(GroupedLaunch p, int
     const int32_t end = tile.end - row < height ? tile.end : row + height;
     const int64_t n0 = static_cast<int64_t>(place.n) * 256;
     if (end - row <= 64) {
-        GroupedTile<T, TOut, kBTrans, true, 1, 2, 2, 4>(p, lds, tile.group, row, end, n0);
+        GroupedTile<T, TOut, kBTrans, true, 3, 1, 2, 2, 4>(p, lds, tile.group, row, end, n0);
     } else if (end - row <= 128) {
-        GroupedTile<T, TOut, kBTrans, true, 2, 2, 2, 4>(p, lds, tile.group, row, end, n0);
+        GroupedTile<T, TOut, kBTrans, true, 3, 2, 2, 2, 4>(p, lds, tile.group, row, end, n0);
     } else {
-        GroupedTile<T, TOut, kBTrans, true, 4, 2, 2, 4>(p, lds, tile.group, row, end, n0);
+        GroupedTile<T, TOut, kBTrans, true, 3, 4, 2, 2, 4>(p, lds, tile.group, row, end, n0);
     }
 }
 
@@ -658,7 +693,7 @@ __global__ __launch_bounds__(256, 1) void GroupedSmallTileKernel(GroupedLaunch p
     if (tile.group < 0) return;
     const TilePlace place = PlaceInBands(share.tile - static_cast<int64_t>(tile.before) * tilesN, tile.tiles, tilesN);
     const int32_t row = tile.begin + place.m * 64;
-    GroupedTile<T, TOut, kBTrans, kAligned, 1, 2, 2, 2>(p, lds, tile.group, row,
+    GroupedTile<T, TOut, kBTrans, kAligned, 2, 1, 2, 2, 2>(p, lds, tile.group, row,
                                                         tile.end - row < 64 ? tile.end : row + 64,
                                                         static_cast<int64_t>(place.n) * 128);
 }
@@ -670,7 +705,8 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void GroupedGradTileKernel(Grouped
     constexpr int kThreads = WM * WN * 64, BM = MI * WM * 32, BN = NI * WN * 32;
     using OperandA = ColumnOperand<T, BM, kThreads, false, kAligned>;
     using OperandB = ColumnOperand<T, BN, kThreads, kIndexed, kAligned>;
-    constexpr int kLds = 2 * (OperandA::kBytes + OperandB::kBytes);
+    constexpr int kPlacesA = kAligned ? 3 : 2;
+    constexpr int kLds = kPlacesA * OperandA::kBytes + 2 * OperandB::kBytes;
     __shared__ __align__(128) char lds[kLds];
     // Every die takes an eighth of each group's tiles, so that a long group is no die's alone; which
     // eighth turns with the group, so that the last, shorter ones go round too.
@@ -691,7 +727,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void GroupedGradTileKernel(Grouped
         OperandB b;
         a.Init(p.grad, p.ldg * 2, n0, p.n, nullptr, p.rows, begin, end);
         b.Init(p.x, p.ldx * 2, k0, p.k, p.row_index, p.rows_x, begin, end);
-        MultiplyTile<T, MI, NI>(a, b, lds, static_cast<int64_t>(end - begin) * 2, rowA, rowB, acc);
+        MultiplyTile<T, MI, NI, kPlacesA>(a, b, lds, static_cast<int64_t>(end - begin) * 2, rowA, rowB, acc);
     }
     const int64_t n = n0 + rowA, k = k0 + rowB;
     StoreTile<TOut, MI, NI, kLds / (WM * WN)>(lds + wave * (kLds / (WM * WN)),

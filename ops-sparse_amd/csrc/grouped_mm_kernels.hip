@@ -25,7 +25,9 @@ using Bf168 = __bf16 __attribute__((ext_vector_type(8)));
 // 16x16 matrix instructions on operands of 16 bytes per lane: lane l holds
 // row l % 16 of its operand, contraction elements (l / 16) * (16 bytes) on.
 // The result's lane l holds column l % 16 (row of the second operand) and
-// rows 4 * (l / 16) + i (of the first).
+// rows 4 * (l / 16) + i (of the first).  The 32x32 ones have the same rate, but
+// draw more power on random operands: alone they sustain 1.82 PFLOP/s of
+// bfloat16 where these do 2.05.
 template <typename T>
 struct Mma;
 template <>
@@ -63,50 +65,16 @@ __device__ __forceinline__ int64_t IndexedRow(const int32_t* index, int64_t r, i
 }
 
 // ---------------------------------------------------------------------------
-// Tiles through LDS, 32x32 matrix instructions.  A tile's contraction advances
+// Tiles through LDS.  A tile's contraction advances
 // by 128 bytes per turn.  While one turn's
 // operands are multiplied the next ones' are copied to LDS, straight from memory where every row is aligned to 16 bytes,
 // through registers by loads of any alignment where not.  Each wave keeps the
 // operands of one matrix step ahead of the one it multiplies in registers.
 // ---------------------------------------------------------------------------
-using Float16 = float __attribute__((ext_vector_type(16)));
-using Int16 = int __attribute__((ext_vector_type(16)));
 using Short4 = short __attribute__((ext_vector_type(4)));
 
 constexpr int kTurnBytes = 128;
-
-// 32x32 matrix instructions: lane l holds row l % 32 of its operand,
-// contraction bytes (l / 32) * 16 on.  The result's lane l holds column l % 32
-// (row of the second operand) and, in register i, row 8 * (i / 4) +
-// 4 * (l / 32) + i % 4 (of the first).
-template <typename T>
-struct Mma32;
-template <>
-struct Mma32<Half> {
-    using Acc = Float16;
-    static __device__ __forceinline__ Acc Run(Int4 a, Int4 b, Acc c)
-    {
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(Half8, a), __builtin_bit_cast(Half8, b), c, 0,
-                                                      0, 0);
-    }
-};
-template <>
-struct Mma32<Bf16> {
-    using Acc = Float16;
-    static __device__ __forceinline__ Acc Run(Int4 a, Int4 b, Acc c)
-    {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(Bf168, a), __builtin_bit_cast(Bf168, b), c,
-                                                       0, 0, 0);
-    }
-};
-template <>
-struct Mma32<int8_t> {
-    using Acc = Int16;
-    static __device__ __forceinline__ Acc Run(Int4 a, Int4 b, Acc c)
-    {
-        return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
-    }
-};
+constexpr int kSteps = 2;  // matrix instructions take 64 bytes of each row
 
 // What lanes copy that have nothing to copy: both operands read as zero past
 // the contraction's end, so that no value beyond it, NaN among them, counts.
@@ -166,7 +134,6 @@ struct RowOperand {
     static constexpr int kLoads = R * 8 / kThreads;
     static constexpr int kRowsPerLoad = kThreads / 8;
     static constexpr int kBytes = R * kTurnBytes;
-    static constexpr int kReads = 1;  // LDS loads per operand of a matrix step
     static constexpr bool kDirect = kAligned;
     const char* ptr[kLoads];
     Int4 held[kLoads];
@@ -208,29 +175,29 @@ struct RowOperand {
         }
     }
 
-    // The operand of one matrix step: 32 rows from `row` on.
+    // The operand of one matrix instruction: 16 rows from `row` on.
     static __device__ __forceinline__ Int4 Read(const char* lds, int row, int step)
     {
         const int lane = threadIdx.x & 63;
-        const int chunk = (step * 2 + (lane >> 5)) ^ ((lane >> 1) & 7);
-        return *reinterpret_cast<const Int4*>(lds + (row + (lane & 31)) * kTurnBytes + chunk * 16);
+        const int chunk = (step * 4 + (lane >> 4)) ^ ((lane >> 1) & 7);
+        return *reinterpret_cast<const Int4*>(lds + (row + (lane & 15)) * kTurnBytes + chunk * 16);
     }
 };
 
 // An operand of 16-bit elements whose rows run across the contraction: 64
 // rows of C columns per turn, read through the transposing LDS load: of the
 // 16 lanes that work together lane j supplies 4 columns (j % 4) of row j / 4,
-// and lane i receives the 4 rows of column i.  Chunk c of row r lies at slot
-// c ^ 4 (r & 3): the four rows of 64 bytes that 32 lanes read then touch
-// every bank once.  (Rows of 128 bytes lie in one half of the banks or the
-// other by themselves: c ^ 4 (r / 2 & 1).)
+// and lane i receives the 4 rows of column i.  32 lanes read 32 bytes each of
+// rows r to r + 3 and r + 8 to r + 11: chunk c of row r lies at slot
+// c ^ 2 h, h the row's number among those eight, so that they touch every bank
+// once.  (Rows of 128 bytes lie in one half of the banks or the other by
+// themselves: h counts the four of a half.)
 template <typename T, int C, int kThreads, bool kIndexed, bool kAligned>
 struct ColumnOperand {
     static constexpr int kChunks = C / 8;
     static constexpr int kRowsPerLoad = kThreads / kChunks;
     static constexpr int kLoads = 64 / kRowsPerLoad;
     static constexpr int kBytes = 64 * C * 2;
-    static constexpr int kReads = 2;
     static constexpr bool kDirect = kAligned;
     const char* ptr[kLoads];
     const char* base;  // this thread's chunk of row 0
@@ -242,7 +209,11 @@ struct ColumnOperand {
     Int4 held[kLoads];
     int valid;         // bytes of the chunk before the last column
 
-    static __device__ __forceinline__ int Swizzle(int r) { return kChunks == 8 ? (r & 2) << 1 : (r & 3) << 2; }
+    static_assert(kLoads == 1 || kRowsPerLoad % 16 == 0, "a thread's chunk must not change with its rows");
+    static __device__ __forceinline__ int Swizzle(int r)
+    {
+        return kChunks == 8 ? (r & 2) | ((r & 8) >> 1) : ((r & 3) << 1) | (r & 8);
+    }
     static __device__ __forceinline__ int Row(int i) { return i * kRowsPerLoad + threadIdx.x / kChunks; }
     static __device__ __forceinline__ int Chunk()
     {
@@ -329,8 +300,8 @@ struct ColumnOperand {
     {
         using LdsShort4 = __attribute__((address_space(3))) Short4;
         const int lane = threadIdx.x & 63, j = lane & 15;
-        const int r = step * 16 + (lane >> 5) * 8 + (j >> 2);
-        const int c = column + ((lane >> 4) & 1) * 16 + (j & 3) * 4;
+        const int r = step * 32 + (lane >> 4) * 8 + (j >> 2);
+        const int c = column + (j & 3) * 4;
         const char* p = lds + r * (C * 2) + ((((c >> 3) ^ Swizzle(r)) << 4) | ((c & 4) << 1));
         struct Pair {
             Short4 lo, hi;
@@ -351,56 +322,56 @@ __device__ __forceinline__ void Wait()
 }
 
 // acc += the product over `bytes` of the contraction (of 16-bit elements when
-// an operand's rows run across it); MI x NI tiles of 32x32 per wave from rows
+// an operand's rows run across it); MI x NI tiles of 16x16 per wave from rows
 // (columns of the output) rowA and rowB on.
 //
-// One turn is four matrix steps.  While a step is multiplied the next one's
-// operands are read from LDS.  One barrier per turn, before its last step: by
+// A turn is two matrix steps of MI rows of products each.  After a row's
+// products come the reads from LDS of the first operand D rows on, into the
+// registers that the row has left, and of the second operand's next step.  One
+// barrier per turn, before its last D rows, whose reads are the next turn's: by
 // then every wave has read this turn's operands and the next turn's have
-// arrived.  B has two places in LDS, A kPlacesA: the last step copies B of the
-// turn after the next to where this turn's was; the first step copies A of the
+// arrived.  B has two places in LDS, A kPlacesA: the last D rows copy B of the
+// turn after the next to where this turn's was; the rows before copy A of the
 // turn kPlacesA - 1 ahead.  With three places the barrier need not wait for
 // the A copied last, and the memory has two turns for it: the copies alone
-// take most of a turn, and with two places both operands' were waited for
-// within three steps.
+// take most of a turn.
 template <typename T, int MI, int NI, int kPlacesA, typename OperandA, typename OperandB>
 __device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds, int64_t bytes, int rowA, int rowB,
-                                             typename Mma32<T>::Acc (&acc)[MI][NI])
+                                             typename Mma<T>::Acc (&acc)[MI][NI])
 {
     constexpr bool kDirect = OperandA::kDirect;
     constexpr int kCopiesA = OperandA::kLoads, kCopiesB = OperandB::kLoads;
-    constexpr int kProducts = MI * NI, kOperands = MI + NI, kAhead = kPlacesA - 1;
+    constexpr int kAhead = kPlacesA - 1;
     constexpr int kLeft = kAhead == 2 ? kCopiesA : 0;  // copies that a barrier need not wait for
+    constexpr int D = MI >= 4 ? MI / 2 : 2, kRows = kSteps * MI, kBefore = kRows - D;
     static_assert(kAhead == 1 || (kAhead == 2 && kDirect), "copies through registers are kept for one turn");
     char* const placesB = lds + kPlacesA * OperandA::kBytes;
-    Int4 fa[2][MI], fb[2][NI];
-    // The f-th operand of a step, in the order in which its products use them: b0, a0, b1, ..., then a1, ...
-    auto read = [&](int to, const char* fromA, const char* fromB, int step, int f) {
-        if (f == 1) {
-            fa[to][0] = OperandA::Read(fromA, rowA, step);
-        } else if (f == 0 || f <= NI) {
-            const int j = f == 0 ? 0 : f - 1;
-            fb[to][j] = OperandB::Read(fromB, rowB + j * 32, step);
-        } else {
-            fa[to][f - NI] = OperandA::Read(fromA, rowA + (f - NI) * 32, step);
-        }
+    Int4 fa[D], fb[kSteps][NI];
+    auto readA = [&](const char* from, int q) { fa[q % D] = OperandA::Read(from, rowA + q % MI * 16, q / MI); };
+    auto readB = [&](const char* from, int s, int first, int last) {
+#pragma unroll
+        for (int j = first; j < last; ++j) fb[s][j] = OperandB::Read(from, rowB + j * 16, s);
     };
-    // One step's products, in this order to the instruction: the next step's reads follow the first of them, so
-    // that they have arrived when it starts; `copies` calls of copy are spread over all, since a wave that issues
-    // copies faster than the memory pipeline takes them (64 bytes per clock) waits with its products behind them.
-    auto step = [&](int with, const char* fromA, const char* fromB, int next, int copies, auto copy) {
-        constexpr int kHalf = (kProducts + 1) / 2;
+    // Rows [first, last) of a turn, in this order to the instruction; nextA: null, or where the next turn's operands
+    // are.  `copies` calls of copy are spread over the rows, since a wave that issues copies faster than the memory
+    // pipeline takes them (64 bytes per clock) waits with its products behind them.
+    auto rows = [&](int first, int last, const char* fromA, const char* fromB, const char* nextA, const char* nextB,
+                    int copies, auto copy) {
 #pragma unroll
-        for (int m = 0; m < kProducts; ++m) {
-            acc[m / NI][m % NI] = Mma32<T>::Run(fb[with][m % NI], fa[with][m / NI], acc[m / NI][m % NI]);
-            if (fromA != nullptr && m < kHalf) {
+        for (int q = first; q < last; ++q) {
+            const int s = q / MI, i = q % MI;
 #pragma unroll
-                for (int f = m * kOperands / kHalf; f < (m + 1) * kOperands / kHalf; ++f) {
-                    read(with ^ 1, fromA, fromB, next, f);
-                }
+            for (int j = 0; j < NI; ++j) acc[i][j] = Mma<T>::Run(fb[s][j], fa[q % D], acc[i][j]);
+            if (q < kBefore) {
+                readA(fromA, q + D);
+            } else if (nextA != nullptr) {
+                readA(nextA, q - kBefore);
+                readB(nextB, 0, (q - kBefore) * NI / D, (q - kBefore + 1) * NI / D);
             }
+            if (q < MI / 2) readB(fromB, 1, q * NI / (MI / 2), (q + 1) * NI / (MI / 2));
+            const int n = last - first;
 #pragma unroll
-            for (int i = m * copies / kProducts; i < (m + 1) * copies / kProducts; ++i) copy(i);
+            for (int c = (q - first) * copies / n; c < (q - first + 1) * copies / n; ++c) copy(c);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
@@ -450,8 +421,9 @@ __device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds
         Wait<0>();
     }
     if (turns > 1) copyTurnB();
+    readB(placesB, 0, 0, NI);
 #pragma unroll
-    for (int f = 0; f < kOperands; ++f) read(0, lds, placesB, 0, f);
+    for (int q = 0; q < D; ++q) readA(lds, q);
     int nowA = 0, nowB = 0;
     // copiesA, copiesB: A of the turn kAhead on and B of the one after the next exist; more: the next one does
     auto turn = [&](auto copiesA, auto copiesB, auto more) {
@@ -459,9 +431,7 @@ __device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds
         const char* fromA = lds + nowA;
         const char* fromB = placesB + nowB;
         if constexpr (kA) prepareA();
-        step(0, fromA, fromB, 1, kA && kDirect ? kCopiesA : 0, copyA);
-        step(1, fromA, fromB, 2, 0, copyA);
-        step(0, fromA, fromB, 3, 0, copyA);
+        rows(0, kBefore, fromA, fromB, nullptr, nullptr, kA && kDirect ? kCopiesA : 0, copyA);
         if constexpr (!kDirect && kMore) {
             a.Commit(lds + toA);
             b.Commit(placesB + toB);
@@ -476,7 +446,8 @@ __device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds
         } else {
             Wait<0>();
         }
-        step(1, kMore ? lds + nowA : nullptr, placesB + nowB, 0, kB && kDirect ? kCopiesB : 0, copyB);
+        rows(kBefore, kRows, fromA, fromB, kMore ? lds + nowA : nullptr, placesB + nowB,
+             kB && kDirect ? kCopiesB : 0, copyB);
     };
     constexpr std::true_type yes{};
     constexpr std::false_type no{};
@@ -485,52 +456,49 @@ __device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds
     turn(no, no, no);
 }
 
-// Writes a wave's MI*32 x NI*32 tile of the output, rows [0, rows) and columns
+// Writes a wave's MI*16 x NI*16 tile of the output, rows [0, rows) and columns
 // [0, columns) of it, at c.  A result's lanes hold neighbouring rows: stored
-// from there, each store would touch 32 rows by 8 bytes (a 256x256 tile then
+// from there, each store would touch 16 rows by 32 bytes (a 256x256 tile then
 // took 68 us).  The wave passes its tile through its own part of LDS instead
-// and stores whole rows, 16 bytes per lane.  value(i, j, q, v) gives the four
-// values of tile (i, j) in registers 4q on.  Chunk c of row r lies at slot
-// c ^ r, which spreads the rows of a write over the banks.
+// and stores whole rows, 16 bytes per lane.  value(i, j, v) gives the four
+// values of tile (i, j).  Chunk c of row r lies at slot c ^ r (c ^ r / 2 in
+// rows of half the banks), which spreads the rows of a write over the banks.
 template <typename TOut, int MI, int NI, int kLdsBytes, typename Value>
-__device__ __forceinline__ void StoreTile(char* lds, TOut* c, int64_t ldc, int64_t rows, int64_t columns,
-                                          Value value)
+__device__ __forceinline__ void StoreTile(char* lds, TOut* c, int64_t ldc, int64_t rows, int64_t columns, Value value)
 {
-    constexpr int kRowBytes = NI * 32 * static_cast<int>(sizeof(TOut));
-    constexpr int kChunks = kRowBytes / 16, kPer = 16 / static_cast<int>(sizeof(TOut));
-    constexpr int kTiles = kLdsBytes / (32 * kRowBytes) < MI ? kLdsBytes / (32 * kRowBytes) : MI;  // at a time
+    constexpr int kSize = static_cast<int>(sizeof(TOut));
+    constexpr int kRowBytes = NI * 16 * kSize, kChunks = kRowBytes / 16, kPer = 16 / kSize;
+    constexpr int kFit = kLdsBytes / (16 * kRowBytes), kTiles = kFit < MI ? kFit : MI;  // at a time
     constexpr int kRowsPerStore = 64 / kChunks;
-    static_assert(kTiles > 0 && kChunks <= 64, "a row of tiles must fit the wave's LDS");
+    static_assert(kTiles > 0 && kChunks >= 8 && kChunks <= 64, "a row of tiles must fit the wave's LDS");
     const int lane = threadIdx.x & 63;
+    auto slot = [](int r) { return kChunks == 8 ? (r >> 1) & 7 : r & (kChunks - 1); };
 #pragma unroll
     for (int first = 0; first < MI; first += kTiles) {
+        const int tiles = MI - first < kTiles ? MI - first : kTiles;
 #pragma unroll
-        for (int i = first; i < first + kTiles && i < MI; ++i) {
-            const int r = (i - first) * 32 + (lane & 31);
+        for (int i = first; i < first + tiles; ++i) {
+            const int r = (i - first) * 16 + (lane & 15);
 #pragma unroll
             for (int j = 0; j < NI; ++j) {
+                float v[4];
+                value(i, j, v);
+                TOut o[4];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    float v[4];
-                    value(i, j, q, v);
-                    TOut o[4];
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) o[x] = FromFloat<TOut>(v[x]);
-                    const int byte = (j * 32 + q * 8 + (lane >> 5) * 4) * static_cast<int>(sizeof(TOut));
-                    char* to = lds + r * kRowBytes + (((byte >> 4) ^ (r & (kChunks - 1))) << 4) + (byte & 8);
-                    __builtin_memcpy(__builtin_assume_aligned(to, sizeof(o)), o, sizeof(o));
-                }
+                for (int x = 0; x < 4; ++x) o[x] = FromFloat<TOut>(v[x]);
+                const int byte = (j * 16 + (lane >> 4) * 4) * kSize;
+                char* to = lds + r * kRowBytes + (((byte >> 4) ^ slot(r)) << 4) + (byte & 8);
+                __builtin_memcpy(__builtin_assume_aligned(to, sizeof(o)), o, sizeof(o));
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        const int base = first * 32;
 #pragma unroll 4
-        for (int r = lane / kChunks; r < kTiles * 32; r += kRowsPerStore) {
-            const int chunk = (lane % kChunks) ^ (r & (kChunks - 1));
-            const int64_t left = columns - chunk * kPer;
-            if (base + r >= rows || left <= 0) continue;
+        for (int r = lane / kChunks; r < tiles * 16; r += kRowsPerStore) {
+            const int chunk = (lane % kChunks) ^ slot(r);
+            const int64_t row = first * 16 + r, left = columns - chunk * kPer;
+            if (row >= rows || left <= 0) continue;
             const Int4 v = *reinterpret_cast<const Int4*>(lds + r * kRowBytes + (lane % kChunks) * 16);
-            TOut* to = c + (base + r) * ldc + chunk * kPer;
+            TOut* to = c + row * ldc + chunk * kPer;
             if (left >= kPer) {
                 __builtin_memcpy(to, &v, 16);  // whatever C's alignment
             } else {
@@ -595,14 +563,14 @@ template <typename T, typename TOut, bool kBTrans, bool kAligned, int kPlacesA, 
 __device__ __forceinline__ void GroupedTile(const GroupedLaunch& p, char* lds, int32_t group, int32_t firstRow,
                                             int32_t endRow, int64_t n0)
 {
-    constexpr int kThreads = WM * WN * 64, BM = MI * WM * 32, BN = NI * WN * 32;
+    constexpr int kThreads = WM * WN * 64, BM = MI * WM * 16, BN = NI * WN * 16;
     using OperandA = RowOperand<T, BM, kThreads, kAligned>;
     using OperandB = std::conditional_t<kBTrans, RowOperand<T, BN, kThreads, kAligned>,
                                         ColumnOperand<T, BN, kThreads, false, kAligned>>;
     constexpr int kLds = kPlacesA * OperandA::kBytes + 2 * OperandB::kBytes;
     const int lane = threadIdx.x & 63, wave = WaveNumber();
-    const int rowA = (wave % WM) * MI * 32, rowB = (wave / WM) * NI * 32;
-    typename Mma32<T>::Acc acc[MI][NI] = {};
+    const int rowA = (wave % WM) * MI * 16, rowB = (wave / WM) * NI * 16;
+    typename Mma<T>::Acc acc[MI][NI] = {};
     const bool real = group < p.groups;
     if (real && p.k > 0) {
         const T* bg = static_cast<const T*>(p.b) + group * p.stride_b;
@@ -630,27 +598,27 @@ __device__ __forceinline__ void GroupedTile(const GroupedLaunch& p, char* lds, i
     TOut* c = static_cast<TOut*>(p.c) + (firstRow + rowA) * p.ldc + n;
     char* part = lds + wave * (kLds / (WM * WN));
     if constexpr (sizeof(T) == 1) {
-        float sa[MI], sb[NI][4][4];
+        float sa[MI], sb[NI][4];
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
-            const int32_t r = firstRow + rowA + i * 32 + (lane & 31);
+            const int32_t r = firstRow + rowA + i * 16 + (lane & 15);
             sa[i] = real && r < endRow ? p.scale_a[IndexedRow(p.row_index, r, p.rows_a)] : 0.0f;
         }
 #pragma unroll
-        for (int j = 0; j < NI * 16; ++j) {
-            const int64_t at = n + j / 4 * 8 + (lane >> 5) * 4 + j % 4;
-            sb[j / 16][j / 4 % 4][j % 4] = real && at < p.n ? p.scale_b[group * p.n + at] : 0.0f;
+        for (int j = 0; j < NI * 4; ++j) {
+            const int64_t at = n + j / 4 * 16 + (lane >> 4) * 4 + j % 4;
+            sb[j / 4][j % 4] = real && at < p.n ? p.scale_b[group * p.n + at] : 0.0f;
         }
         StoreTile<TOut, MI, NI, kLds / (WM * WN)>(
-            part, c, p.ldc, endRow - firstRow - rowA, p.n - n, [&](int i, int j, int q, float(&v)[4]) {
+            part, c, p.ldc, endRow - firstRow - rowA, p.n - n, [&](int i, int j, float(&v)[4]) {
 #pragma unroll
-                for (int x = 0; x < 4; ++x) v[x] = static_cast<float>(acc[i][j][q * 4 + x]) * (sa[i] * sb[j][q][x]);
+                for (int x = 0; x < 4; ++x) v[x] = static_cast<float>(acc[i][j][x]) * (sa[i] * sb[j][x]);
             });
     } else {
         StoreTile<TOut, MI, NI, kLds / (WM * WN)>(
-            part, c, p.ldc, endRow - firstRow - rowA, p.n - n, [&](int i, int j, int q, float(&v)[4]) {
+            part, c, p.ldc, endRow - firstRow - rowA, p.n - n, [&](int i, int j, float(&v)[4]) {
 #pragma unroll
-                for (int x = 0; x < 4; ++x) v[x] = acc[i][j][q * 4 + x];
+                for (int x = 0; x < 4; ++x) v[x] = acc[i][j][x];
             });
     }
 }
@@ -673,11 +641,11 @@ __global__ __launch_bounds__(512, 1) void GroupedTileKernel(GroupedLaunch p, int
     const int32_t end = tile.end - row < height ? tile.end : row + height;
     const int64_t n0 = static_cast<int64_t>(place.n) * 256;
     if (end - row <= 64) {
-        GroupedTile<T, TOut, kBTrans, true, 3, 1, 2, 2, 4>(p, lds, tile.group, row, end, n0);
+        GroupedTile<T, TOut, kBTrans, true, 3, 2, 4, 2, 4>(p, lds, tile.group, row, end, n0);
     } else if (end - row <= 128) {
-        GroupedTile<T, TOut, kBTrans, true, 3, 2, 2, 2, 4>(p, lds, tile.group, row, end, n0);
+        GroupedTile<T, TOut, kBTrans, true, 3, 4, 4, 2, 4>(p, lds, tile.group, row, end, n0);
     } else {
-        GroupedTile<T, TOut, kBTrans, true, 3, 4, 2, 2, 4>(p, lds, tile.group, row, end, n0);
+        GroupedTile<T, TOut, kBTrans, true, 3, 8, 4, 2, 4>(p, lds, tile.group, row, end, n0);
     }
 }
 
@@ -693,7 +661,7 @@ __global__ __launch_bounds__(256, 1) void GroupedSmallTileKernel(GroupedLaunch p
     if (tile.group < 0) return;
     const TilePlace place = PlaceInBands(share.tile - static_cast<int64_t>(tile.before) * tilesN, tile.tiles, tilesN);
     const int32_t row = tile.begin + place.m * 64;
-    GroupedTile<T, TOut, kBTrans, kAligned, 2, 1, 2, 2, 2>(p, lds, tile.group, row,
+    GroupedTile<T, TOut, kBTrans, kAligned, 2, 2, 4, 2, 2>(p, lds, tile.group, row,
                                                         tile.end - row < 64 ? tile.end : row + 64,
                                                         static_cast<int64_t>(place.n) * 128);
 }
@@ -702,7 +670,7 @@ template <typename T, typename TOut, bool kIndexed, bool kAligned, int MI, int N
 __global__ __launch_bounds__(WM * WN * 64, 1) void GroupedGradTileKernel(GroupedGradLaunch p, int32_t tilesN,
                                                                         int32_t tilesK)
 {
-    constexpr int kThreads = WM * WN * 64, BM = MI * WM * 32, BN = NI * WN * 32;
+    constexpr int kThreads = WM * WN * 64, BM = MI * WM * 16, BN = NI * WN * 16;
     using OperandA = ColumnOperand<T, BM, kThreads, false, kAligned>;
     using OperandB = ColumnOperand<T, BN, kThreads, kIndexed, kAligned>;
     constexpr int kPlacesA = kAligned ? 3 : 2;
@@ -718,10 +686,10 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void GroupedGradTileKernel(Grouped
     const TilePlace place = PlaceInBands(id, tilesN, tilesK);
     const int64_t n0 = static_cast<int64_t>(place.m) * BM, k0 = static_cast<int64_t>(place.n) * BN;
     const int wave = WaveNumber();
-    const int rowA = (wave % WM) * MI * 32, rowB = (wave / WM) * NI * 32;
+    const int rowA = (wave % WM) * MI * 16, rowB = (wave / WM) * NI * 16;
     int32_t begin, end;
     GroupRows(p.offsets, p.rows, g, begin, end);
-    typename Mma32<T>::Acc acc[MI][NI] = {};
+    typename Mma<T>::Acc acc[MI][NI] = {};
     if (begin < end) {
         OperandA a;
         OperandB b;
@@ -732,9 +700,9 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void GroupedGradTileKernel(Grouped
     const int64_t n = n0 + rowA, k = k0 + rowB;
     StoreTile<TOut, MI, NI, kLds / (WM * WN)>(lds + wave * (kLds / (WM * WN)),
                                               static_cast<TOut*>(p.w) + g * p.stride_w + n * p.ldw + k, p.ldw, p.n - n,
-                                              p.k - k, [&](int i, int j, int q, float(&v)[4]) {
+                                              p.k - k, [&](int i, int j, float(&v)[4]) {
 #pragma unroll
-                                                  for (int x = 0; x < 4; ++x) v[x] = acc[i][j][q * 4 + x];
+                                                  for (int x = 0; x < 4; ++x) v[x] = acc[i][j][x];
                                               });
 }
 
@@ -940,11 +908,11 @@ int GroupedTyped(const GroupedLaunch& l, hipStream_t s)
 template <typename T, typename TOut, bool kAligned, int MI>
 int LaunchGradTiles(const GroupedGradLaunch& l, hipStream_t s)
 {
-    const int64_t tilesN = CeilDiv(l.n, MI * 64), tilesK = CeilDiv(l.k, 256);
+    const int64_t tilesN = CeilDiv(l.n, MI * 32), tilesK = CeilDiv(l.k, 256);
     if (tilesN * tilesK + 7 > INT32_MAX / l.groups) return kTooLarge;
     const int64_t grid = CeilDiv(tilesN * tilesK, 8) * 8 * l.groups;
-    const auto kernel = l.row_index != nullptr ? GroupedGradTileKernel<T, TOut, true, kAligned, MI, 2, 2, 4>
-                                               : GroupedGradTileKernel<T, TOut, false, kAligned, MI, 2, 2, 4>;
+    const auto kernel = l.row_index != nullptr ? GroupedGradTileKernel<T, TOut, true, kAligned, MI, 4, 2, 4>
+                                               : GroupedGradTileKernel<T, TOut, false, kAligned, MI, 4, 2, 4>;
     kernel<<<static_cast<uint32_t>(grid), 512, 0, s>>>(l, static_cast<int32_t>(tilesN), static_cast<int32_t>(tilesK));
     return 0;
 }
@@ -954,9 +922,9 @@ int GroupedGradTyped(const GroupedGradLaunch& l, hipStream_t s)
 {
     const bool aligned =
         Aligned16(l.grad, l.ldg * 2) && Aligned16(l.x, l.ldx * 2) && l.n % 8 == 0 && l.k % 8 == 0;
-    if (!aligned) return LaunchGradTiles<T, TOut, false, 1>(l, s);
+    if (!aligned) return LaunchGradTiles<T, TOut, false, 2>(l, s);
     const bool many = CeilDiv(l.n, 256) * CeilDiv(l.k, 256) * l.groups >= 6 * CusPerDie();
-    return many ? LaunchGradTiles<T, TOut, true, 4>(l, s) : LaunchGradTiles<T, TOut, true, 1>(l, s);
+    return many ? LaunchGradTiles<T, TOut, true, 8>(l, s) : LaunchGradTiles<T, TOut, true, 2>(l, s);
 }
 
 }  // namespace

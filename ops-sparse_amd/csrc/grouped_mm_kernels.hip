@@ -165,6 +165,7 @@ struct RowOperand {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) ptr[i] += kTurnBytes;
     }
+    __device__ __forceinline__ void LookUp() {}
     __device__ __forceinline__ void Commit(char* lds)
     {
         if constexpr (!kAligned) {
@@ -205,7 +206,7 @@ struct ColumnOperand {
     const int32_t* index;
     int64_t count;     // rows that an index may name
     int32_t row, end;  // of this thread's first load in the next turn, and of all
-    int32_t next[kIndexed ? kLoads : 1];
+    int32_t next[kIndexed ? kLoads : 1][2];  // of this wave's loads' two rows each
     Int4 held[kLoads];
     int valid;         // bytes of the chunk before the last column
 
@@ -250,7 +251,8 @@ struct ColumnOperand {
         if constexpr (kIndexed) {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                ptr[i] = base + (next[i] < 0 || next[i] >= count ? 0 : next[i]) * ld;
+                const int32_t at = threadIdx.x & 32 ? next[i][1] : next[i][0];
+                ptr[i] = base + (at < 0 || at >= count ? 0 : at) * ld;
             }
         }
         if (bytes < kTurnBytes) {
@@ -260,7 +262,6 @@ struct ColumnOperand {
             }
         }
         row += 64;
-        LookUp();
     }
     __device__ __forceinline__ void Issue(char* lds, int i)
     {
@@ -284,14 +285,22 @@ struct ColumnOperand {
             }
         }
     }
-    // The indices of the turn after: they arrive while this one is multiplied.
+    // The next turn's indices, for Prepare after a wait for reads: each wave's rows are its own, so they come by
+    // scalar loads, which that wait covers.  (As vector loads they were waited for behind all copies in flight:
+    // the training case's gradient took 620 us where rows in order take 527.)
     __device__ __forceinline__ void LookUp()
     {
         if constexpr (kIndexed) {
+            static_assert(kChunks == 32, "a wave copies two rows at a time");
+            const auto* list = (const __attribute__((address_space(4))) int32_t*)(index);
+            const int32_t first = __builtin_amdgcn_readfirstlane(row);
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                const int32_t r = row + i * kRowsPerLoad;
-                next[i] = index[r < end ? r : end - 1];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int32_t r = first + i * kRowsPerLoad + j;
+                    next[i][j] = list[r < end ? r : end - 1];
+                }
             }
         }
     }
@@ -385,7 +394,7 @@ __device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds
         leftA -= kTurnBytes;
         if constexpr (!kDirect) a.Load();
     };
-    auto prepareB = [&] {
+    auto prepareB = [&] {  // after b.LookUp() and a wait
         b.Prepare(leftB);
         leftB -= kTurnBytes;
         if constexpr (!kDirect) b.Load();
@@ -414,6 +423,7 @@ __device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds
     copyTurnB();
     if constexpr (!kDirect) b.Commit(placesB);
     doneB();
+    b.LookUp();
     if (kAhead == 2 && turns > 1) {
         copyAllA();
         Wait<kLeft>();
@@ -441,6 +451,7 @@ __device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds
         nowA = nowA == (kPlacesA - 1) * OperandA::kBytes ? 0 : nowA + OperandA::kBytes;
         nowB ^= OperandB::kBytes;
         if constexpr (kB) {
+            b.LookUp();
             Wait<kLeft>();
             prepareB();
         } else {

@@ -126,6 +126,20 @@ __device__ __forceinline__ void LoadAll(const char* const (&ptr)[N], int valid, 
 
 __device__ __forceinline__ int WaveNumber() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
+// This thread's and wave's number among the kThreads that work on one tile (a
+// workgroup may hold several such teams).
+template <int kThreads>
+__device__ __forceinline__ int TeamThread()
+{
+    static_assert((kThreads & (kThreads - 1)) == 0, "");
+    return static_cast<int>(threadIdx.x) & (kThreads - 1);
+}
+template <int kThreads>
+__device__ __forceinline__ int TeamWave()
+{
+    return WaveNumber() & (kThreads / 64 - 1);
+}
+
 // An operand whose rows run along the contraction: R rows of 128 bytes per
 // turn.  Its 16-byte chunk c of row r lies at slot c ^ (r / 2 & 7), so that the
 // lanes that read one chunk of 16 rows touch each of the 64 banks once.
@@ -140,10 +154,15 @@ struct RowOperand {
     int valid = 16;  // bytes of this thread's chunks before the contraction's end
 
     // This thread's rows are Row(i); its chunk of each is the same.
-    static __device__ __forceinline__ int Row(int i) { return i * kRowsPerLoad + (threadIdx.x >> 3); }
-    static __device__ __forceinline__ int Chunk() { return (threadIdx.x & 7) ^ ((threadIdx.x >> 4) & 7); }
+    static __device__ __forceinline__ int Row(int i) { return i * kRowsPerLoad + (TeamThread<kThreads>() >> 3); }
+    static __device__ __forceinline__ int Chunk() { return (TeamThread<kThreads>() & 7) ^ ((TeamThread<kThreads>() >> 4) & 7); }
 
-    // Before a turn's copies: `bytes` of the contraction are left.
+    __device__ __forceinline__ void Skip(int64_t turns)
+    {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) ptr[i] += turns * kTurnBytes;
+    }
+    // Before a turn's copies: `bytes` of the contraction are left (none, or less, for a turn of zeros).
     __device__ __forceinline__ void Prepare(int64_t bytes)
     {
         if (bytes >= kTurnBytes) return;
@@ -155,7 +174,7 @@ struct RowOperand {
     }
     __device__ __forceinline__ void Issue(char* lds, int i)
     {
-        CopyToLds(ptr[i], lds + WaveNumber() * 1024 + i * kThreads * 16);
+        CopyToLds(ptr[i], lds + TeamWave<kThreads>() * 1024 + i * kThreads * 16);
         ptr[i] += kTurnBytes;
     }
     // The same through registers, for rows of any alignment.
@@ -171,7 +190,7 @@ struct RowOperand {
         if constexpr (!kAligned) {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                *reinterpret_cast<Int4*>(lds + (i * kThreads + static_cast<int>(threadIdx.x)) * 16) = held[i];
+                *reinterpret_cast<Int4*>(lds + (i * kThreads + TeamThread<kThreads>()) * 16) = held[i];
             }
         }
     }
@@ -206,7 +225,8 @@ struct ColumnOperand {
     const int32_t* index;
     int64_t count;     // rows that an index may name
     int32_t row, end;  // of this thread's first load in the next turn, and of all
-    int32_t next[kIndexed ? kLoads : 1][2];  // of this wave's loads' two rows each
+    static constexpr int kWaveRows = 64 / kChunks;  // rows of a wave's load
+    int32_t next[kIndexed ? kLoads : 1][kWaveRows];
     Int4 held[kLoads];
     int valid;         // bytes of the chunk before the last column
 
@@ -215,10 +235,10 @@ struct ColumnOperand {
     {
         return kChunks == 8 ? (r & 2) | ((r & 8) >> 1) : ((r & 3) << 1) | (r & 8);
     }
-    static __device__ __forceinline__ int Row(int i) { return i * kRowsPerLoad + threadIdx.x / kChunks; }
+    static __device__ __forceinline__ int Row(int i) { return i * kRowsPerLoad + TeamThread<kThreads>() / kChunks; }
     static __device__ __forceinline__ int Chunk()
     {
-        return (threadIdx.x % kChunks) ^ Swizzle(threadIdx.x / kChunks);
+        return (TeamThread<kThreads>() % kChunks) ^ Swizzle(TeamThread<kThreads>() / kChunks);
     }
 
     __device__ __forceinline__ void Init(const void* p, int64_t ldBytes, int64_t column, int64_t columns,
@@ -251,7 +271,9 @@ struct ColumnOperand {
         if constexpr (kIndexed) {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                const int32_t at = threadIdx.x & 32 ? next[i][1] : next[i][0];
+                int32_t at = next[i][0];
+#pragma unroll
+                for (int j = 1; j < kWaveRows; ++j) at = (threadIdx.x & 63) / kChunks >= j ? next[i][j] : at;
                 ptr[i] = base + (at < 0 || at >= count ? 0 : at) * ld;
             }
         }
@@ -265,7 +287,7 @@ struct ColumnOperand {
     }
     __device__ __forceinline__ void Issue(char* lds, int i)
     {
-        CopyToLds(ptr[i], lds + WaveNumber() * 1024 + i * kThreads * 16);
+        CopyToLds(ptr[i], lds + TeamWave<kThreads>() * 1024 + i * kThreads * 16);
         if constexpr (!kIndexed) ptr[i] += 64 * ld;
     }
     __device__ __forceinline__ void Load()
@@ -281,7 +303,7 @@ struct ColumnOperand {
         if constexpr (!kAligned) {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                *reinterpret_cast<Int4*>(lds + (i * kThreads + static_cast<int>(threadIdx.x)) * 16) = held[i];
+                *reinterpret_cast<Int4*>(lds + (i * kThreads + TeamThread<kThreads>()) * 16) = held[i];
             }
         }
     }
@@ -291,13 +313,12 @@ struct ColumnOperand {
     __device__ __forceinline__ void LookUp()
     {
         if constexpr (kIndexed) {
-            static_assert(kChunks == 32, "a wave copies two rows at a time");
             const auto* list = (const __attribute__((address_space(4))) int32_t*)(index);
             const int32_t first = __builtin_amdgcn_readfirstlane(row);
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
+                for (int j = 0; j < kWaveRows; ++j) {
                     const int32_t r = first + i * kRowsPerLoad + j;
                     next[i][j] = list[r < end ? r : end - 1];
                 }
@@ -331,7 +352,8 @@ __device__ __forceinline__ void Wait()
 }
 
 // acc += the product over `bytes` of the contraction (of 16-bit elements when
-// an operand's rows run across it); MI x NI tiles of 16x16 per wave from rows
+// an operand's rows run across it) in `turns` turns, those past the bytes of
+// zeros; MI x NI tiles of 16x16 per wave from rows
 // (columns of the output) rowA and rowB on.
 //
 // A turn is two matrix steps of MI rows of products each.  After a row's
@@ -345,8 +367,8 @@ __device__ __forceinline__ void Wait()
 // the A copied last, and the memory has two turns for it: the copies alone
 // take most of a turn.
 template <typename T, int MI, int NI, int kPlacesA, typename OperandA, typename OperandB>
-__device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds, int64_t bytes, int rowA, int rowB,
-                                             typename Mma<T>::Acc (&acc)[MI][NI])
+__device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds, int64_t bytes, int64_t turns, int rowA,
+                                             int rowB, typename Mma<T>::Acc (&acc)[MI][NI])
 {
     constexpr bool kDirect = OperandA::kDirect;
     constexpr int kCopiesA = OperandA::kLoads, kCopiesB = OperandB::kLoads;
@@ -411,7 +433,6 @@ __device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds
         }
         doneA();
     };
-    const int64_t turns = (bytes + kTurnBytes - 1) / kTurnBytes;
     auto copyTurnB = [&] {
         prepareB();
         if constexpr (kDirect) {
@@ -465,6 +486,34 @@ __device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds
     for (int64_t t = 2; t < turns; ++t) turn(yes, yes, yes);
     if (turns > 1) turn(std::bool_constant<kAhead == 1>{}, no, yes);
     turn(no, no, no);
+}
+
+// Adds up what a workgroup's kTeams teams hold of one tile, in their order, in
+// the first one; returns whether this team is that one.  `lds` holds the other
+// teams' operands, which no wave uses any more; the first one's place is left
+// to its store, which may begin before another of its waves has added up.
+template <int kTeams, int kThreads, int kBytes, int MI, int NI, typename Acc>
+__device__ __forceinline__ bool JoinTeams(char* lds, Acc (&acc)[MI][NI])
+{
+    if constexpr (kTeams == 1) return true;
+    constexpr int kTeamBytes = kThreads * MI * NI * static_cast<int>(sizeof(Acc));
+    static_assert(kTeams == 1 || (kTeams - 1) * kTeamBytes <= kBytes, "the sums must fit");
+    const int team = WaveNumber() / (kThreads / 64);
+    Acc* mine = reinterpret_cast<Acc*>(lds) + TeamThread<kThreads>();
+    if (team > 0) {
+#pragma unroll
+        for (int i = 0; i < MI * NI; ++i) {
+            mine[(team - 1) * (kTeamBytes / sizeof(Acc)) + i * kThreads] = acc[i / NI][i % NI];
+        }
+    }
+    Wait<0>();
+    if (team > 0) return false;
+#pragma unroll
+    for (int t = 0; t < kTeams - 1; ++t) {
+#pragma unroll
+        for (int i = 0; i < MI * NI; ++i) acc[i / NI][i % NI] += mine[t * (kTeamBytes / sizeof(Acc)) + i * kThreads];
+    }
+    return true;
 }
 
 // Writes a wave's MI*16 x NI*16 tile of the output, rows [0, rows) and columns
@@ -570,7 +619,7 @@ __device__ __forceinline__ TileShare ShareOfWorkgroup(int64_t total, int32_t cus
 
 constexpr int kTileRows = 256;  // of a whole tile
 
-template <typename T, typename TOut, bool kBTrans, bool kAligned, int kPlacesA, int MI, int NI, int WM, int WN>
+template <typename T, typename TOut, bool kBTrans, bool kAligned, int kTeams, int kPlacesA, int MI, int NI, int WM, int WN>
 __device__ __forceinline__ void GroupedTile(const GroupedLaunch& p, char* lds, int32_t group, int32_t firstRow,
                                             int32_t endRow, int64_t n0)
 {
@@ -579,7 +628,8 @@ __device__ __forceinline__ void GroupedTile(const GroupedLaunch& p, char* lds, i
     using OperandB = std::conditional_t<kBTrans, RowOperand<T, BN, kThreads, kAligned>,
                                         ColumnOperand<T, BN, kThreads, false, kAligned>>;
     constexpr int kLds = kPlacesA * OperandA::kBytes + 2 * OperandB::kBytes;
-    const int lane = threadIdx.x & 63, wave = WaveNumber();
+    const int lane = threadIdx.x & 63, wave = TeamWave<kThreads>();
+    const int team = WaveNumber() / (kThreads / 64);
     const int rowA = (wave % WM) * MI * 16, rowB = (wave / WM) * NI * 16;
     typename Mma<T>::Acc acc[MI][NI] = {};
     const bool real = group < p.groups;
@@ -594,17 +644,25 @@ __device__ __forceinline__ void GroupedTile(const GroupedLaunch& p, char* lds, i
             const int64_t row = IndexedRow(p.row_index, r < endRow ? r : firstRow, p.rows_a);
             a.ptr[i] = reinterpret_cast<const char*>(static_cast<const T*>(p.a) + row * p.lda) + OperandA::Chunk() * 16;
         }
+        // each team takes a run of turns
+        const int64_t bytes = p.k * static_cast<int64_t>(sizeof(T));
+        const int64_t per = ((bytes + kTurnBytes - 1) / kTurnBytes + kTeams - 1) / kTeams;
+        a.Skip(team * per);
         if constexpr (kBTrans) {
 #pragma unroll
             for (int i = 0; i < OperandB::kLoads; ++i) {
                 const int64_t n = n0 + OperandB::Row(i);
                 b.ptr[i] = reinterpret_cast<const char*>(bg + (n < p.n ? n : n0) * p.ldb) + OperandB::Chunk() * 16;
             }
+            b.Skip(team * per);
         } else {
-            b.Init(bg, p.ldb * 2, n0, p.n, nullptr, p.k, 0, static_cast<int32_t>(p.k));
+            b.Init(bg, p.ldb * 2, n0, p.n, nullptr, p.k, static_cast<int32_t>(team * per * 64),
+                   static_cast<int32_t>(p.k));
         }
-        MultiplyTile<T, MI, NI, kPlacesA>(a, b, lds, p.k * static_cast<int64_t>(sizeof(T)), rowA, rowB, acc);
+        MultiplyTile<T, MI, NI, kPlacesA>(a, b, lds + team * kLds, bytes - team * per * kTurnBytes, per, rowA, rowB,
+                                          acc);
     }
+    if (!JoinTeams<kTeams, kThreads, (kTeams - 1) * kLds>(lds + kLds, acc)) return;
     const int64_t n = n0 + rowB;
     TOut* c = static_cast<TOut*>(p.c) + (firstRow + rowA) * p.ldc + n;
     char* part = lds + wave * (kLds / (WM * WN));
@@ -652,19 +710,22 @@ __global__ __launch_bounds__(512, 1) void GroupedTileKernel(GroupedLaunch p, int
     const int32_t end = tile.end - row < height ? tile.end : row + height;
     const int64_t n0 = static_cast<int64_t>(place.n) * 256;
     if (end - row <= 64) {
-        GroupedTile<T, TOut, kBTrans, true, 3, 2, 4, 2, 4>(p, lds, tile.group, row, end, n0);
+        GroupedTile<T, TOut, kBTrans, true, 1, 3, 2, 4, 2, 4>(p, lds, tile.group, row, end, n0);
     } else if (end - row <= 128) {
-        GroupedTile<T, TOut, kBTrans, true, 3, 4, 4, 2, 4>(p, lds, tile.group, row, end, n0);
+        GroupedTile<T, TOut, kBTrans, true, 1, 3, 4, 4, 2, 4>(p, lds, tile.group, row, end, n0);
     } else {
-        GroupedTile<T, TOut, kBTrans, true, 3, 8, 4, 2, 4>(p, lds, tile.group, row, end, n0);
+        GroupedTile<T, TOut, kBTrans, true, 1, 3, 8, 4, 2, 4>(p, lds, tile.group, row, end, n0);
     }
 }
 
-// Tiles of 64x128 for groups of few rows or few tiles: three workgroups per CU.
-template <typename T, typename TOut, bool kBTrans, bool kAligned>
-__global__ __launch_bounds__(256, 1) void GroupedSmallTileKernel(GroupedLaunch p, int32_t tilesN)
+// Tiles of 64x128 for groups of few rows: three workgroups per CU, or, where
+// there are not tiles enough for that, one whose three teams share a tile's
+// contraction.
+constexpr int kSmallTileBytes = 2 * (64 + 128) * kTurnBytes;
+template <typename T, typename TOut, bool kBTrans, bool kAligned, int kTeams>
+__global__ __launch_bounds__(kTeams * 256, 1) void GroupedSmallTileKernel(GroupedLaunch p, int32_t tilesN)
 {
-    __shared__ __align__(128) char lds[2 * (64 + 128) * kTurnBytes];
+    __shared__ __align__(128) char lds[kTeams * kSmallTileBytes];
     const RaggedTiles tiles(p.offsets, p.rows, p.groups, 64);
     const TileShare share = ShareOfWorkgroup(static_cast<int64_t>(tiles.total) * tilesN, 1);
     if (share.tile < 0) return;
@@ -672,21 +733,20 @@ __global__ __launch_bounds__(256, 1) void GroupedSmallTileKernel(GroupedLaunch p
     if (tile.group < 0) return;
     const TilePlace place = PlaceInBands(share.tile - static_cast<int64_t>(tile.before) * tilesN, tile.tiles, tilesN);
     const int32_t row = tile.begin + place.m * 64;
-    GroupedTile<T, TOut, kBTrans, kAligned, 2, 2, 4, 2, 2>(p, lds, tile.group, row,
+    GroupedTile<T, TOut, kBTrans, kAligned, kTeams, 2, 2, 4, 2, 2>(p, lds, tile.group, row,
                                                         tile.end - row < 64 ? tile.end : row + 64,
                                                         static_cast<int64_t>(place.n) * 128);
 }
 
-template <typename T, typename TOut, bool kIndexed, bool kAligned, int MI, int NI, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * 64, 1) void GroupedGradTileKernel(GroupedGradLaunch p, int32_t tilesN,
+template <typename T, typename TOut, bool kIndexed, bool kAligned, int kTeams, int kPlacesA, int MI, int NI, int WM, int WN>
+__global__ __launch_bounds__(kTeams * WM * WN * 64, 1) void GroupedGradTileKernel(GroupedGradLaunch p, int32_t tilesN,
                                                                         int32_t tilesK)
 {
     constexpr int kThreads = WM * WN * 64, BM = MI * WM * 16, BN = NI * WN * 16;
     using OperandA = ColumnOperand<T, BM, kThreads, false, kAligned>;
     using OperandB = ColumnOperand<T, BN, kThreads, kIndexed, kAligned>;
-    constexpr int kPlacesA = kAligned ? 3 : 2;
     constexpr int kLds = kPlacesA * OperandA::kBytes + 2 * OperandB::kBytes;
-    __shared__ __align__(128) char lds[kLds];
+    __shared__ __align__(128) char lds[kTeams * kLds];
     // Every die takes an eighth of each group's tiles, so that a long group is no die's alone; which
     // eighth turns with the group, so that the last, shorter ones go round too.
     const int32_t per = (tilesN * tilesK + 7) / 8, at = static_cast<int32_t>(blockIdx.x / 8);
@@ -696,7 +756,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void GroupedGradTileKernel(Grouped
     const int32_t g = LongestGroup(p.offsets, p.rows, static_cast<int32_t>(p.groups), nth);
     const TilePlace place = PlaceInBands(id, tilesN, tilesK);
     const int64_t n0 = static_cast<int64_t>(place.m) * BM, k0 = static_cast<int64_t>(place.n) * BN;
-    const int wave = WaveNumber();
+    const int wave = TeamWave<kThreads>(), team = WaveNumber() / (kThreads / 64);
     const int rowA = (wave % WM) * MI * 16, rowB = (wave / WM) * NI * 16;
     int32_t begin, end;
     GroupRows(p.offsets, p.rows, g, begin, end);
@@ -704,10 +764,14 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void GroupedGradTileKernel(Grouped
     if (begin < end) {
         OperandA a;
         OperandB b;
-        a.Init(p.grad, p.ldg * 2, n0, p.n, nullptr, p.rows, begin, end);
-        b.Init(p.x, p.ldx * 2, k0, p.k, p.row_index, p.rows_x, begin, end);
-        MultiplyTile<T, MI, NI, kPlacesA>(a, b, lds, static_cast<int64_t>(end - begin) * 2, rowA, rowB, acc);
+        // each team takes a run of turns
+        const int32_t per = ((end - begin + 63) / 64 + kTeams - 1) / kTeams, from = begin + team * per * 64;
+        a.Init(p.grad, p.ldg * 2, n0, p.n, nullptr, p.rows, from, end);
+        b.Init(p.x, p.ldx * 2, k0, p.k, p.row_index, p.rows_x, from, end);
+        MultiplyTile<T, MI, NI, kPlacesA>(a, b, lds + team * kLds, static_cast<int64_t>(end - from) * 2, per, rowA, rowB,
+                                          acc);
     }
+    if (!JoinTeams<kTeams, kThreads, (kTeams - 1) * kLds>(lds + kLds, acc)) return;
     const int64_t n = n0 + rowA, k = k0 + rowB;
     StoreTile<TOut, MI, NI, kLds / (WM * WN)>(lds + wave * (kLds / (WM * WN)),
                                               static_cast<TOut*>(p.w) + g * p.stride_w + n * p.ldw + k, p.ldw, p.n - n,
@@ -858,14 +922,14 @@ int LaunchTiles(const GroupedLaunch& l, hipStream_t s)
     return 0;
 }
 
-template <typename T, typename TOut, bool kBTrans, bool kAligned>
+template <typename T, typename TOut, bool kBTrans, bool kAligned, int kTeams>
 int LaunchSmallTiles(const GroupedLaunch& l, hipStream_t s)
 {
     const int64_t tilesN = CeilDiv(l.n, 128);
     const int64_t grid = CeilDiv(MaxRowTiles(l.offsets, l.rows, l.groups, 64) * tilesN, 8) * 8;
     if (grid > INT32_MAX) return kTooLarge;
-    GroupedSmallTileKernel<T, TOut, kBTrans, kAligned>
-        <<<static_cast<uint32_t>(grid), 256, 0, s>>>(l, static_cast<int32_t>(tilesN));
+    GroupedSmallTileKernel<T, TOut, kBTrans, kAligned, kTeams>
+        <<<static_cast<uint32_t>(grid), kTeams * 256, 0, s>>>(l, static_cast<int32_t>(tilesN));
     return 0;
 }
 
@@ -886,9 +950,9 @@ template <typename T, typename TOut, bool kBTrans, bool kAligned>
 int GroupedBySize(const GroupedLaunch& l, hipStream_t s)
 {
     const int64_t cus = 8 * CusPerDie();
-    const int64_t smallTiles = (l.rows / 64 + (l.offsets != nullptr ? CeilDiv(l.groups, 2) : 1)) * CeilDiv(l.n, 128);
+    const int64_t smallTiles = (CeilDiv(l.rows, 64) + (l.groups - 1) / 2) * CeilDiv(l.n, 128);
     if constexpr (kBTrans) {
-        const bool few = l.rows <= 12 * l.groups || (l.rows <= 64 * l.groups && smallTiles < cus / 2);
+        const bool few = l.rows <= 12 * l.groups || (l.rows <= 64 * l.groups && smallTiles <= cus / 4);
         if (few && l.k * static_cast<int64_t>(sizeof(T)) <= INT32_MAX / 2) {
             const int64_t groups = l.rows < l.groups ? l.rows : l.groups;
             const bool narrow = groups * CeilDiv(l.n, 32) < 2 * cus && l.rows <= 16 * l.groups;
@@ -898,7 +962,9 @@ int GroupedBySize(const GroupedLaunch& l, hipStream_t s)
     if constexpr (kAligned) {
         if (l.rows >= 160 * l.groups && smallTiles > 3 * cus) return LaunchTiles<T, TOut, kBTrans>(l, s);
     }
-    return LaunchSmallTiles<T, TOut, kBTrans, kAligned>(l, s);
+    return smallTiles <= cus && l.k * static_cast<int64_t>(sizeof(T)) >= 12 * kTurnBytes
+               ? LaunchSmallTiles<T, TOut, kBTrans, kAligned, 3>(l, s)
+               : LaunchSmallTiles<T, TOut, kBTrans, kAligned, 1>(l, s);
 }
 
 template <typename T, typename TOut>
@@ -916,15 +982,18 @@ int GroupedTyped(const GroupedLaunch& l, hipStream_t s)
     return aligned ? GroupedBySize<T, TOut, true, true>(l, s) : GroupedBySize<T, TOut, true, false>(l, s);
 }
 
-template <typename T, typename TOut, bool kAligned, int MI>
+template <typename T, typename TOut, bool kAligned, int kTeams, int kPlacesA, int MI, int WN>
 int LaunchGradTiles(const GroupedGradLaunch& l, hipStream_t s)
 {
-    const int64_t tilesN = CeilDiv(l.n, MI * 32), tilesK = CeilDiv(l.k, 256);
+    constexpr int WM = 2, NI = 4, kThreads = kTeams * WM * WN * 64;
+    const int64_t tilesN = CeilDiv(l.n, MI * WM * 16), tilesK = CeilDiv(l.k, NI * WN * 16);
     if (tilesN * tilesK + 7 > INT32_MAX / l.groups) return kTooLarge;
     const int64_t grid = CeilDiv(tilesN * tilesK, 8) * 8 * l.groups;
-    const auto kernel = l.row_index != nullptr ? GroupedGradTileKernel<T, TOut, true, kAligned, MI, 4, 2, 4>
-                                               : GroupedGradTileKernel<T, TOut, false, kAligned, MI, 4, 2, 4>;
-    kernel<<<static_cast<uint32_t>(grid), 512, 0, s>>>(l, static_cast<int32_t>(tilesN), static_cast<int32_t>(tilesK));
+    const auto kernel = l.row_index != nullptr
+                            ? GroupedGradTileKernel<T, TOut, true, kAligned, kTeams, kPlacesA, MI, NI, WM, WN>
+                            : GroupedGradTileKernel<T, TOut, false, kAligned, kTeams, kPlacesA, MI, NI, WM, WN>;
+    kernel<<<static_cast<uint32_t>(grid), kThreads, 0, s>>>(l, static_cast<int32_t>(tilesN),
+                                                            static_cast<int32_t>(tilesK));
     return 0;
 }
 
@@ -933,9 +1002,14 @@ int GroupedGradTyped(const GroupedGradLaunch& l, hipStream_t s)
 {
     const bool aligned =
         Aligned16(l.grad, l.ldg * 2) && Aligned16(l.x, l.ldx * 2) && l.n % 8 == 0 && l.k % 8 == 0;
-    if (!aligned) return LaunchGradTiles<T, TOut, false, 2>(l, s);
+    const bool fewest = CeilDiv(l.n, 64) * CeilDiv(l.k, 128) * l.groups <= 8 * CusPerDie();
+    if (!aligned) {
+        return fewest ? LaunchGradTiles<T, TOut, false, 3, 2, 2, 2>(l, s)
+                      : LaunchGradTiles<T, TOut, false, 1, 2, 2, 4>(l, s);
+    }
+    if (fewest) return LaunchGradTiles<T, TOut, true, 3, 2, 2, 2>(l, s);
     const bool many = CeilDiv(l.n, 256) * CeilDiv(l.k, 256) * l.groups >= 6 * CusPerDie();
-    return many ? LaunchGradTiles<T, TOut, true, 8>(l, s) : LaunchGradTiles<T, TOut, true, 2>(l, s);
+    return many ? LaunchGradTiles<T, TOut, true, 1, 3, 8, 4>(l, s) : LaunchGradTiles<T, TOut, true, 1, 3, 2, 4>(l, s);
 }
 
 }  // namespace

@@ -952,16 +952,21 @@ int GroupedBySize(const GroupedLaunch& l, hipStream_t s)
     const int64_t cus = 8 * CusPerDie();
     const int64_t smallTiles = (CeilDiv(l.rows, 64) + (l.groups - 1) / 2) * CeilDiv(l.n, 128);
     if constexpr (kBTrans) {
-        const bool few = l.rows <= 12 * l.groups || (l.rows <= 64 * l.groups && smallTiles <= cus / 4);
+        // Weights that no cache holds, bf16, us, here / by 64x128 tiles: 8 groups of 4096x4096 with 1 row each 51 /
+        // 56, with 4 55 / 57, with 8 64 / 57; 32 of 2048x2048 with 1 53 / 60, with 8 64 / 60.  One group has too few
+        // tiles: 4096x4096 with 1 row 10 / 38, with 32 19 / 39, with 64 21 (32 rows a time; 33 with 16) / 41.
+        const bool few = l.rows <= 6 * l.groups || (l.rows <= 64 * l.groups && smallTiles <= cus / 4);
         if (few && l.k * static_cast<int64_t>(sizeof(T)) <= INT32_MAX / 2) {
-            const int64_t groups = l.rows < l.groups ? l.rows : l.groups;
-            const bool narrow = groups * CeilDiv(l.n, 32) < 2 * cus && l.rows <= 16 * l.groups;
-            return narrow ? LaunchRows<T, TOut, kAligned, 1, 1>(l, s) : LaunchRows<T, TOut, kAligned, 2, 2>(l, s);
+            return l.rows <= 6 * l.groups || l.rows <= 32 ? LaunchRows<T, TOut, kAligned, 1, 1>(l, s)
+                                                          : LaunchRows<T, TOut, kAligned, 2, 2>(l, s);
         }
     }
+    // 256x256 tiles / 64x128 ones: 32 groups of 2048x2048 with 128 rows each 97 / 90 us, with 160 96 / 97, with 256
+    // 104 / 134; 1 group of 4096x4096 with 1024 rows 51 / 49, with 2048 61 / 95.
     if constexpr (kAligned) {
         if (l.rows >= 160 * l.groups && smallTiles > 3 * cus) return LaunchTiles<T, TOut, kBTrans>(l, s);
     }
+    // three teams a tile / one, us: 256 rows x 4096 x 4096 29 / 43; 1024 rows in 4 groups x 512 x 512 7.6 / 7.1
     return smallTiles <= cus && l.k * static_cast<int64_t>(sizeof(T)) >= 12 * kTurnBytes
                ? LaunchSmallTiles<T, TOut, kBTrans, kAligned, 3>(l, s)
                : LaunchSmallTiles<T, TOut, kBTrans, kAligned, 1>(l, s);
@@ -1002,6 +1007,8 @@ int GroupedGradTyped(const GroupedGradLaunch& l, hipStream_t s)
 {
     const bool aligned =
         Aligned16(l.grad, l.ldg * 2) && Aligned16(l.x, l.ldx * 2) && l.n % 8 == 0 && l.k % 8 == 0;
+    // 64x128 by three teams / 64x256 / 256x256, us: 4 groups of 4096 rows, 512x512 44 / 71 / 112; 8 of 4096, 1024x1024
+    // 253 / 169 / 233; 32 of 256, 2048x2048 - / 261 / 131
     const bool fewest = CeilDiv(l.n, 64) * CeilDiv(l.k, 128) * l.groups <= 8 * CusPerDie();
     if (!aligned) {
         return fewest ? LaunchGradTiles<T, TOut, false, 3, 2, 2, 2>(l, s)

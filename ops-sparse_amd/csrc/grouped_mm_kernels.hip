@@ -966,10 +966,12 @@ int GroupedBySize(const GroupedLaunch& l, hipStream_t s)
     if constexpr (kAligned) {
         if (l.rows >= 160 * l.groups && smallTiles > 3 * cus) return LaunchTiles<T, TOut, kBTrans>(l, s);
     }
-    // three teams a tile / one, us: 256 rows x 4096 x 4096 29 / 43; 1024 rows in 4 groups x 512 x 512 7.6 / 7.1
-    return smallTiles <= cus && l.k * static_cast<int64_t>(sizeof(T)) >= 12 * kTurnBytes
-               ? LaunchSmallTiles<T, TOut, kBTrans, kAligned, 3>(l, s)
-               : LaunchSmallTiles<T, TOut, kBTrans, kAligned, 1>(l, s);
+    // three teams a tile / one, us: 256 rows x 4096 x 4096 29 / 43; 1024 rows in 4 groups x 512 x 512 7.6 / 7.1; with
+    // weights that no cache holds, 512 rows in 32 groups x 2048 x 2048 61 / 72, 816 in 48 x 1024 x 1024 32 / 27
+    const int64_t turns = CeilDiv(l.k * static_cast<int64_t>(sizeof(T)), kTurnBytes);
+    const bool teams = (smallTiles <= cus && turns >= 12) || (smallTiles <= cus + cus / 2 && turns >= 32);
+    return teams ? LaunchSmallTiles<T, TOut, kBTrans, kAligned, 3>(l, s)
+                 : LaunchSmallTiles<T, TOut, kBTrans, kAligned, 1>(l, s);
 }
 
 template <typename T, typename TOut>

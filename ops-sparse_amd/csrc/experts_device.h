@@ -162,6 +162,7 @@ struct RaggedTiles {
         }
         tail = offsets != nullptr ? __builtin_amdgcn_readlane(last, lastLane) : rows;
         total += Count(tail, rows);
+        if (total < 0) total = 0;  // the sum of offsets without meaning
     }
 
     // The tile-th tile; `tile` is uniform.

@@ -706,7 +706,7 @@ __global__ __launch_bounds__(512, 1) void GroupedTileKernel(GroupedLaunch p, int
     const TilePlace place = PlaceInBands(share.tile - static_cast<int64_t>(tile.before) * tilesN, tile.tiles, tilesN);
     const int32_t height = kTileRows / share.parts;
     const int32_t row = tile.begin + place.m * kTileRows + share.part * height;
-    if (row >= tile.end) return;
+    if (row < tile.begin || row >= tile.end) return;  // also whatever offsets without meaning lead to
     const int32_t end = tile.end - row < height ? tile.end : row + height;
     const int64_t n0 = static_cast<int64_t>(place.n) * 256;
     if (end - row <= 64) {
@@ -733,6 +733,7 @@ __global__ __launch_bounds__(kTeams * 256, 1) void GroupedSmallTileKernel(Groupe
     if (tile.group < 0) return;
     const TilePlace place = PlaceInBands(share.tile - static_cast<int64_t>(tile.before) * tilesN, tile.tiles, tilesN);
     const int32_t row = tile.begin + place.m * 64;
+    if (row < tile.begin || row >= tile.end) return;
     GroupedTile<T, TOut, kBTrans, kAligned, kTeams, 2, 2, 4, 2, 2>(p, lds, tile.group, row,
                                                         tile.end - row < 64 ? tile.end : row + 64,
                                                         static_cast<int64_t>(place.n) * 128);
@@ -798,7 +799,7 @@ __global__ __launch_bounds__(kWaves * 64) void GroupedRowsKernel(GroupedLaunch p
                                 .Find(static_cast<int32_t>(blockIdx.x / static_cast<uint32_t>(tilesN)));
     const int32_t n0 = static_cast<int32_t>(blockIdx.x % static_cast<uint32_t>(tilesN)) * NT * 16;
     const int32_t width = static_cast<int32_t>(p.n);
-    if (tile.group < 0 || n0 >= width) return;
+    if (tile.group < 0 || n0 >= width || tile.row < tile.begin || tile.row >= tile.end) return;
     const int lane = threadIdx.x & 63, wave = WaveNumber();
     const bool real = tile.group < p.groups;
     Acc acc[MT][NT] = {};

@@ -412,6 +412,88 @@ def test_grouped_mm_gradient_against_differences(dev):
         assert abs(slope - float(grad[at])) <= rounding
 
 
+# Sizes that reach the 256x256 tiles: whole ones, ends of every height, a last round cut in slices, a tail.
+LARGE = {
+    "whole": [1024, 2048], "ends": [256 + 64, 512 + 1, 768 + 128, 1024 + 129, 255, 257], "one": [3333],
+    "skewed": [2600, 0, 300, 64, 7], "few_rounds": [256 * 21],
+}
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("n,k", [(2304, 64), (2312, 136), (2200, 200), (2560, 512), (4100, 72)])
+@pytest.mark.parametrize("groups", list(LARGE))
+def test_grouped_mm_large_tiles(dev, groups, n, k, dtype):
+    lens = LARGE[groups]
+    gather = k % 16 == 8
+    plan, rows = lengths_to_plan(lens, tail=70, tokens=900 if gather else None)
+    a = torch.randn(900 if gather else rows, k, generator=gen(1), device=dev).to(dtype)
+    w = torch.randn(len(lens), n, k, generator=gen(2), device=dev).to(dtype)
+    y = grouped_mm(a, w, plan, gather=gather)
+    want, magnitude = plain_grouped(a, w, plan, rows)
+    close(y, want, magnitude, k)
+    assert not y[rows - 70:].any()
+
+
+@pytest.mark.parametrize("n,k", [(2304, 128), (2312, 144), (2200, 400), (2560, 1024), (4100, 80)])
+@pytest.mark.parametrize("groups", list(LARGE))
+def test_grouped_mm_scaled_large_tiles(dev, groups, n, k):
+    lens = LARGE[groups]
+    plan, rows = lengths_to_plan(lens, tail=5, tokens=500)
+    a, w = strided((500, k), torch.int8, 1, 16), strided((len(lens), n, k), torch.int8, 2, 0)
+    sa = torch.rand(500, generator=gen(3), device=dev) * 1e-3
+    sw = torch.rand(len(lens), n, generator=gen(4), device=dev) * 1e-2
+    y = grouped_mm_scaled(a, sa, w, sw, plan, gather=True)
+    scaled_close(y, plain_scaled(a, sa, w, sw, plan, rows))
+    assert not y[rows - 5:].any()
+
+
+@pytest.mark.parametrize("groups,n,k", [
+    ("whole", 256, 2304), ("ends", 264, 2200), ("one", 200, 2304), ("skewed", 136, 2312),  # gradient of the input
+    ("ends", 1536, 1544), ("skewed", 1544, 2056),                       # weight gradients of 256x256
+    ("ends", 520, 776), ("skewed", 776, 1032), ("skewed", 777, 1033),   # of 64x256
+    ("few_rounds", 128, 264), ("few_rounds", 129, 263)])                # of 64x128 by three teams
+def test_grouped_mm_gradients_large(dev, groups, n, k):
+    lens = LARGE[groups] * (4 if n >= 1536 else 2 if n >= 520 else 1)
+    plan, rows = lengths_to_plan(lens)
+    tokens = rows // 2 if k % 16 == 8 else rows
+    index = torch.randint(0, tokens, (rows,), generator=gen(7), device=dev, dtype=torch.int32)
+    a = torch.randn(tokens, k, generator=gen(1), device=dev).to(BF16).requires_grad_(True)
+    w = (torch.randn(len(lens), n, k, generator=gen(2), device=dev)).to(BF16).requires_grad_(True)
+    grad = torch.randn(rows, n, generator=gen(3), device=dev).to(BF16)
+    if tokens == rows:
+        y = grouped_mm(a, w, plan)
+        da, dw = torch.autograd.grad(y, (a, w), grad)
+        wa, ma, ww, mw = plain_grads(a.detach(), w.detach(), plan, grad)
+        close(da, wa, ma, n)
+    else:
+        # an index without places serves the weight gradient alone
+        plan = ExpertPlan(plan.offsets, index, None)
+        y = grouped_mm(a.detach(), w, plan, gather=True)
+        dw, = torch.autograd.grad(y, w, grad)
+        _, _, ww, mw = plain_grads(a.detach(), w.detach(), plan, grad)
+    close(dw, ww, mw, max(lens))
+
+
+@pytest.mark.parametrize("rows,n,k,groups", [
+    (1, 64, 4096, 1), (17, 100, 2056, 1), (40, 72, 1544, 1), (64, 520, 776, 1),   # few rows, two heights
+    (200, 136, 4104, 3), (300, 256, 1000, 2), (513, 1000, 2048, 1),               # teams
+    (100, 136, 1001, 2), (513, 1000, 2047, 1)])                                   # and unaligned
+def test_grouped_mm_long_contractions(dev, rows, n, k, groups):
+    lens = [rows // groups] * groups
+    plan, total = lengths_to_plan(lens)
+    a = torch.randn(total, k, generator=gen(1), device=dev).to(F16)
+    w = torch.randn(groups, n, k, generator=gen(2), device=dev).to(F16)
+    close(grouped_mm(a, w, plan), *plain_grouped(a, w, plan, total), k)
+
+
+def test_results_are_differentiable_once(dev):
+    logits = torch.randn(4, 8, generator=gen(1), device=dev).requires_grad_(True)
+    weights, _, _ = route(logits, 2)
+    grad, = torch.autograd.grad((weights ** 2).sum(), logits, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        grad.sum().backward()
+
+
 # ------------------------------------------------------------------------------------------------------- 8 bits
 
 

@@ -98,7 +98,8 @@ CASES = [
         (dict(out=0), INVALID), (dict(ldg=7), INVALID), (dict(ld=7), INVALID), (dict(tokens=0), OK)]),
     ("aclsparseGroupedMM", grouped, [
         (dict(op=2), UNSUPPORTED), (dict(groups=0), INVALID), (dict(rows=-1), INVALID), (dict(n=-1), INVALID),
-        (dict(k=-1), INVALID), (dict(rows=2**31), UNSUPPORTED), (dict(offsets=0), INVALID),
+        (dict(k=-1), INVALID), (dict(rows=2**31 - 64, rows_a=2**31 - 64), UNSUPPORTED), (dict(offsets=0), INVALID),
+        (dict(n=2**31 - 64, ldc=2**31), UNSUPPORTED), (dict(k=2**31 - 64, lda=2**31, ldb=2**31), UNSUPPORTED),
         (dict(index=0, rows_a=3), INVALID), (dict(rows_a=0), INVALID), (dict(type=F32), UNSUPPORTED),
         (dict(type=I8), UNSUPPORTED), (dict(ctype=F16), UNSUPPORTED), (dict(lda=15), INVALID), (dict(ldb=15), INVALID),
         (dict(op=NN, ldb=7), INVALID), (dict(ldc=7), INVALID), (dict(stride=-1), INVALID), (dict(c=0), INVALID),

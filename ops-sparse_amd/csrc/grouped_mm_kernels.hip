@@ -65,11 +65,11 @@ __device__ __forceinline__ int64_t IndexedRow(const int32_t* index, int64_t r, i
 }
 
 // ---------------------------------------------------------------------------
-// Tiles through LDS.  A tile's contraction advances
-// by 128 bytes per turn.  While one turn's
-// operands are multiplied the next ones' are copied to LDS, straight from memory where every row is aligned to 16 bytes,
-// through registers by loads of any alignment where not.  Each wave keeps the
-// operands of one matrix step ahead of the one it multiplies in registers.
+// Tiles through LDS.  A tile's contraction advances by 128 bytes per turn.
+// While one turn's operands are multiplied the next ones' are copied to LDS,
+// straight from memory where every row is aligned to 16 bytes, through
+// registers by loads of any alignment where not.  Each wave keeps the operands
+// of one matrix step ahead of the one it multiplies in registers.
 // ---------------------------------------------------------------------------
 using Short4 = short __attribute__((ext_vector_type(4)));
 
@@ -155,7 +155,10 @@ struct RowOperand {
 
     // This thread's rows are Row(i); its chunk of each is the same.
     static __device__ __forceinline__ int Row(int i) { return i * kRowsPerLoad + (TeamThread<kThreads>() >> 3); }
-    static __device__ __forceinline__ int Chunk() { return (TeamThread<kThreads>() & 7) ^ ((TeamThread<kThreads>() >> 4) & 7); }
+    static __device__ __forceinline__ int Chunk()
+    {
+        return (TeamThread<kThreads>() & 7) ^ ((TeamThread<kThreads>() >> 4) & 7);
+    }
 
     __device__ __forceinline__ void Skip(int64_t turns)
     {
@@ -367,8 +370,8 @@ __device__ __forceinline__ void Wait()
 // the A copied last, and the memory has two turns for it: the copies alone
 // take most of a turn.
 template <typename T, int MI, int NI, int kPlacesA, typename OperandA, typename OperandB>
-__device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds, int64_t bytes, int64_t turns, int rowA,
-                                             int rowB, typename Mma<T>::Acc (&acc)[MI][NI])
+__device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds, int64_t bytes, int64_t turns,
+                                             int rowA, int rowB, typename Mma<T>::Acc (&acc)[MI][NI])
 {
     constexpr bool kDirect = OperandA::kDirect;
     constexpr int kCopiesA = OperandA::kLoads, kCopiesB = OperandB::kLoads;
@@ -619,7 +622,10 @@ __device__ __forceinline__ TileShare ShareOfWorkgroup(int64_t total, int32_t cus
 
 constexpr int kTileRows = 256;  // of a whole tile
 
-template <typename T, typename TOut, bool kBTrans, bool kAligned, int kTeams, int kPlacesA, int MI, int NI, int WM, int WN>
+// One tile: MI*WM*16 rows by NI*WN*16 columns, of which each of a team's WM x
+// WN waves takes MI x NI instructions' results.
+template <typename T, typename TOut, bool kBTrans, bool kAligned, int kTeams, int kPlacesA, int MI, int NI, int WM,
+          int WN>
 __device__ __forceinline__ void GroupedTile(const GroupedLaunch& p, char* lds, int32_t group, int32_t firstRow,
                                             int32_t endRow, int64_t n0)
 {
@@ -694,6 +700,16 @@ __device__ __forceinline__ void GroupedTile(const GroupedLaunch& p, char* lds, i
 
 // Tiles of 256x256, or fewer rows where the group's end or a share leaves
 // fewer: a tile of 64 or 128 rows costs about that part of a whole one.
+//
+// Bound by the matrix instructions, whose clock falls with the power that
+// random operands draw: alone they sustain 2.05 PFLOP/s of bfloat16.  A tile of
+// 256x256 reads each byte of LDS for the most instructions that the registers
+// (128 of sums per lane) allow; the operands' five places of 32 KB fill a CU's
+// LDS, three of them the first operand's, which is copied two turns ahead.
+// 16384 rows in 8 groups, 4096x4096: 454 us, 1.21 PFLOP/s (int8, 32768 rows in
+// 16 groups, 2048x4096: 259 us, 2.12); one group of 8192 rows, 8192x8192: 1.42
+// and 2.67.  Outside its turns a round of tiles takes about 9.5 us: the search,
+// the first copies and the stores.
 template <typename T, typename TOut, bool kBTrans>
 __global__ __launch_bounds__(512, 1) void GroupedTileKernel(GroupedLaunch p, int32_t tilesN, int32_t cus)
 {
@@ -720,7 +736,9 @@ __global__ __launch_bounds__(512, 1) void GroupedTileKernel(GroupedLaunch p, int
 
 // Tiles of 64x128 for groups of few rows: three workgroups per CU, or, where
 // there are not tiles enough for that, one whose three teams share a tile's
-// contraction.
+// contraction.  Bound by the latency of its copies, one turn ahead, and by the
+// weights' bytes: 812 rows in 48 groups, 1001x1000, fp16, 22 us (98 MB, 4.4
+// TB/s).
 constexpr int kSmallTileBytes = 2 * (64 + 128) * kTurnBytes;
 template <typename T, typename TOut, bool kBTrans, bool kAligned, int kTeams>
 __global__ __launch_bounds__(kTeams * 256, 1) void GroupedSmallTileKernel(GroupedLaunch p, int32_t tilesN)
@@ -739,9 +757,17 @@ __global__ __launch_bounds__(kTeams * 256, 1) void GroupedSmallTileKernel(Groupe
                                                         static_cast<int64_t>(place.n) * 128);
 }
 
-template <typename T, typename TOut, bool kIndexed, bool kAligned, int kTeams, int kPlacesA, int MI, int NI, int WM, int WN>
+// Weight gradients, W_g[n, k] = sum over the group's rows of gradC[r, n] *
+// X_index(r)[k]: both operands' rows run across the contraction, so both are
+// read through the transposing LDS loads, and rows are copied by their index
+// as they lie in memory.  Every tile has one workgroup that passes over all of
+// its group's rows: no partial sums, no atomics.  Bound like
+// GroupedTileKernel, and by uneven groups, the longest first: 65536 rows in 32
+// groups, 2048x2048, bfloat16, 552 to 600 us, 0.92 to 1.0 PFLOP/s.
+template <typename T, typename TOut, bool kIndexed, bool kAligned, int kTeams, int kPlacesA, int MI, int NI, int WM,
+          int WN>
 __global__ __launch_bounds__(kTeams * WM * WN * 64, 1) void GroupedGradTileKernel(GroupedGradLaunch p, int32_t tilesN,
-                                                                        int32_t tilesK)
+                                                                                int32_t tilesK)
 {
     constexpr int kThreads = WM * WN * 64, BM = MI * WM * 16, BN = NI * WN * 16;
     using OperandA = ColumnOperand<T, BM, kThreads, false, kAligned>;
@@ -769,8 +795,8 @@ __global__ __launch_bounds__(kTeams * WM * WN * 64, 1) void GroupedGradTileKerne
         const int32_t per = ((end - begin + 63) / 64 + kTeams - 1) / kTeams, from = begin + team * per * 64;
         a.Init(p.grad, p.ldg * 2, n0, p.n, nullptr, p.rows, from, end);
         b.Init(p.x, p.ldx * 2, k0, p.k, p.row_index, p.rows_x, from, end);
-        MultiplyTile<T, MI, NI, kPlacesA>(a, b, lds + team * kLds, static_cast<int64_t>(end - from) * 2, per, rowA, rowB,
-                                          acc);
+        MultiplyTile<T, MI, NI, kPlacesA>(a, b, lds + team * kLds, static_cast<int64_t>(end - from) * 2, per, rowA,
+                                          rowB, acc);
     }
     if (!JoinTeams<kTeams, kThreads, (kTeams - 1) * kLds>(lds + kLds, acc)) return;
     const int64_t n = n0 + rowA, k = k0 + rowB;
@@ -787,7 +813,8 @@ __global__ __launch_bounds__(kTeams * WM * WN * 64, 1) void GroupedGradTileKerne
 // workgroup multiplies MT*16 rows by NT*16 columns; its waves split the
 // contraction, each lane loading its operands of 16x16 instructions straight
 // from memory (16 rows of 64 bytes per load), and add their sums through LDS
-// in the order of the waves.
+// in the order of the waves.  4 groups of 4096x2048 with one row each,
+// bfloat16, call after call: 67 MB in 14.7 us, 4.6 TB/s (17.0 with 8 waves).
 // ---------------------------------------------------------------------------
 template <typename T, typename TOut, bool kAligned, int MT, int NT, int kWaves>
 __global__ __launch_bounds__(kWaves * 64) void GroupedRowsKernel(GroupedLaunch p, int32_t tilesN)

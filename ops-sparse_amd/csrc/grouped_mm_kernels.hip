@@ -78,7 +78,9 @@ constexpr int kSteps = 2;  // matrix instructions take 64 bytes of each row
 
 // What lanes copy that have nothing to copy: both operands read as zero past
 // the contraction's end, so that no value beyond it, NaN among them, counts.
-__device__ const Int4 kZeros = {0, 0, 0, 0};
+// (LoadPart may read up to 15 bytes before what it is given, which are zeros here too.)
+__device__ const Int4 kZeroBytes[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+__device__ __forceinline__ const char* Zeros() { return reinterpret_cast<const char*>(&kZeroBytes[1]); }
 
 // Copies 16 bytes per lane to 1024 bytes of LDS.  Written as assembly, without
 // an output: the compiler would count the copy against every later LDS read
@@ -92,35 +94,58 @@ __device__ __forceinline__ void CopyToLds(const char* from, char* to)
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from));
 }
 
-// The first `valid` bytes at `from` of any alignment (of T's at least), zeros after them.
-template <typename T>
-__device__ __forceinline__ Int4 LoadUnaligned(const char* from, int valid)
+// 16 bytes at any alignment.  The pointer is said to be global memory's: the
+// compiler cannot tell where one that may be Zeros() points, and loads that
+// might be LDS's make every read of LDS wait for them.
+__device__ __forceinline__ Int4 LoadBytes(const char* from)
 {
-    Int4 v;
-    if (valid >= 16) {
-        __builtin_memcpy(&v, from, 16);
+    using Bytes = int __attribute__((ext_vector_type(4), aligned(1)));
+    return *(const __attribute__((address_space(1))) Bytes*)(from);
+}
+
+// The first `valid` bytes of a row's 16-byte chunk at `from`, zeros after them.  A chunk that the row's end cuts is
+// read by the 16 bytes that end there and shifted, which a row of 16 bytes or more holds; `tiny`: it does not, and
+// elements are read one at a time.  (With every cut chunk read so, a load and its wait after the other, 5418 rows
+// in 6 groups x 1144 x 661 took 38 us, now 33; their weight gradient 92, now 59.)
+template <typename T>
+__device__ __forceinline__ Int4 LoadPart(const char* from, int valid, bool tiny)
+{
+    if (tiny) {
+        constexpr int kCount = 16 / static_cast<int>(sizeof(T));
+        const auto* elements = (const __attribute__((address_space(1))) T*)(from);
+        T e[kCount];
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+            e[i] = static_cast<T>(0);
+            if (i * static_cast<int>(sizeof(T)) < valid) e[i] = elements[i];
+        }
+        Int4 v;
+        __builtin_memcpy(&v, e, 16);
         return v;
     }
-    T e[16 / sizeof(T)];
-#pragma unroll
-    for (int i = 0; i < 16 / static_cast<int>(sizeof(T)); ++i) {
-        e[i] = static_cast<T>(0);
-        if (i * static_cast<int>(sizeof(T)) < valid) __builtin_memcpy(&e[i], from + i * sizeof(T), sizeof(T));
-    }
-    __builtin_memcpy(&v, e, 16);
-    return v;
+    const int cut = valid >= 16 || valid <= 0 ? 0 : 16 - valid;
+    const Int4 v = LoadBytes(from - cut);
+    uint64_t half[2];
+    __builtin_memcpy(half, &v, 16);
+    const int bits = cut * 8;
+    const uint64_t down = bits >= 64 ? half[1] >> (bits & 63) : half[0] >> bits | half[1] << 1 << (63 - bits);
+    half[1] = bits >= 64 ? 0 : half[1] >> bits;
+    half[0] = down;
+    Int4 out;
+    __builtin_memcpy(&out, half, 16);
+    return valid <= 0 ? Int4{0, 0, 0, 0} : out;
 }
 
 // All of a thread's chunks of a turn; whole ones without a branch between them.
 template <typename T, int N>
-__device__ __forceinline__ void LoadAll(const char* const (&ptr)[N], int valid, Int4 (&held)[N])
+__device__ __forceinline__ void LoadAll(const char* const (&ptr)[N], int valid, bool tiny, Int4 (&held)[N])
 {
     if (__all(valid >= 16)) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) __builtin_memcpy(&held[i], ptr[i], 16);
+        for (int i = 0; i < N; ++i) held[i] = LoadBytes(ptr[i]);
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) held[i] = LoadUnaligned<T>(ptr[i], valid);
+        for (int i = 0; i < N; ++i) held[i] = LoadPart<T>(ptr[i], valid, tiny);
     }
 }
 
@@ -151,7 +176,8 @@ struct RowOperand {
     static constexpr bool kDirect = kAligned;
     const char* ptr[kLoads];
     Int4 held[kLoads];
-    int valid = 16;  // bytes of this thread's chunks before the contraction's end
+    int valid = 16;     // bytes of this thread's chunks before the contraction's end
+    bool tiny = false;  // whole rows have fewer than 16 bytes
 
     // This thread's rows are Row(i); its chunk of each is the same.
     static __device__ __forceinline__ int Row(int i) { return i * kRowsPerLoad + (TeamThread<kThreads>() >> 3); }
@@ -173,7 +199,7 @@ struct RowOperand {
         if constexpr (!kAligned) valid = here < 0 ? 0 : here < 16 ? here : 16;
         if (here > 0) return;
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) ptr[i] = reinterpret_cast<const char*>(&kZeros);
+        for (int i = 0; i < kLoads; ++i) ptr[i] = Zeros();
     }
     __device__ __forceinline__ void Issue(char* lds, int i)
     {
@@ -183,7 +209,7 @@ struct RowOperand {
     // The same through registers, for rows of any alignment.
     __device__ __forceinline__ void Load()
     {
-        LoadAll<T>(ptr, valid, held);
+        LoadAll<T>(ptr, valid, tiny, held);
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) ptr[i] += kTurnBytes;
     }
@@ -232,6 +258,7 @@ struct ColumnOperand {
     int32_t next[kIndexed ? kLoads : 1][kWaveRows];
     Int4 held[kLoads];
     int valid;         // bytes of the chunk before the last column
+    bool tiny;         // whole rows have fewer than 16 bytes
 
     static_assert(kLoads == 1 || kRowsPerLoad % 16 == 0, "a thread's chunk must not change with its rows");
     static __device__ __forceinline__ int Swizzle(int r)
@@ -250,6 +277,7 @@ struct ColumnOperand {
         const int64_t c = column + Chunk() * 8;
         const bool in = c < columns;
         valid = columns - c >= 8 ? 16 : static_cast<int>(columns - c) * 2;
+        tiny = columns < 8;
         base = static_cast<const char*>(p) + c * 2;
         ld = ldBytes;
         index = rowIndex;
@@ -262,7 +290,7 @@ struct ColumnOperand {
         if (!in) {
             valid = 16;
             ld = 0;
-            base = reinterpret_cast<const char*>(&kZeros);
+            base = Zeros();
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) ptr[i] = base;
         }
@@ -283,7 +311,7 @@ struct ColumnOperand {
         if (bytes < kTurnBytes) {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                if (row + i * kRowsPerLoad >= end) ptr[i] = reinterpret_cast<const char*>(&kZeros);
+                if (row + i * kRowsPerLoad >= end) ptr[i] = Zeros();
             }
         }
         row += 64;
@@ -295,7 +323,7 @@ struct ColumnOperand {
     }
     __device__ __forceinline__ void Load()
     {
-        LoadAll<T>(ptr, valid, held);
+        LoadAll<T>(ptr, valid, tiny, held);
         if constexpr (!kIndexed) {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) ptr[i] += 64 * ld;
@@ -454,7 +482,10 @@ __device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds
     } else {
         Wait<0>();
     }
-    if (turns > 1) copyTurnB();
+    if (turns > 1) {
+        if constexpr (!kDirect) prepareA();
+        copyTurnB();
+    }
     readB(placesB, 0, 0, NI);
 #pragma unroll
     for (int q = 0; q < D; ++q) readA(lds, q);
@@ -464,7 +495,7 @@ __device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds
         constexpr bool kA = decltype(copiesA)::value, kB = decltype(copiesB)::value, kMore = decltype(more)::value;
         const char* fromA = lds + nowA;
         const char* fromB = placesB + nowB;
-        if constexpr (kA) prepareA();
+        if constexpr (kA && kDirect) prepareA();
         rows(0, kBefore, fromA, fromB, nullptr, nullptr, kA && kDirect ? kCopiesA : 0, copyA);
         if constexpr (!kDirect && kMore) {
             a.Commit(lds + toA);
@@ -477,6 +508,7 @@ __device__ __forceinline__ void MultiplyTile(OperandA& a, OperandB& b, char* lds
         if constexpr (kB) {
             b.LookUp();
             Wait<kLeft>();
+            if constexpr (!kDirect) prepareA();  // in registers until the next turn's are multiplied
             prepareB();
         } else {
             Wait<0>();
@@ -653,6 +685,7 @@ __device__ __forceinline__ void GroupedTile(const GroupedLaunch& p, char* lds, i
         // each team takes a run of turns
         const int64_t bytes = p.k * static_cast<int64_t>(sizeof(T));
         const int64_t per = ((bytes + kTurnBytes - 1) / kTurnBytes + kTeams - 1) / kTeams;
+        a.tiny = bytes < 16;
         a.Skip(team * per);
         if constexpr (kBTrans) {
 #pragma unroll
@@ -660,6 +693,7 @@ __device__ __forceinline__ void GroupedTile(const GroupedLaunch& p, char* lds, i
                 const int64_t n = n0 + OperandB::Row(i);
                 b.ptr[i] = reinterpret_cast<const char*>(bg + (n < p.n ? n : n0) * p.ldb) + OperandB::Chunk() * 16;
             }
+            b.tiny = bytes < 16;
             b.Skip(team * per);
         } else {
             b.Init(bg, p.ldb * 2, n0, p.n, nullptr, p.k, static_cast<int32_t>(team * per * 64),
@@ -869,13 +903,13 @@ __global__ __launch_bounds__(kWaves * 64) void GroupedRowsKernel(GroupedLaunch p
                         v = *reinterpret_cast<const Int4*>(row + (byte < bytes ? byte : 0));
                         if (byte >= bytes) v = Int4{0, 0, 0, 0};
                     } else {
-                        __builtin_memcpy(&v, row + byte, 16);
+                        v = LoadBytes(row + byte);
                     }
                     return v;
                 });
             } else {
                 loadAll([&](const char* row, int32_t byte) {
-                    return LoadUnaligned<T>(row + (byte < bytes ? byte : 0), bytes - byte);
+                    return LoadPart<T>(row + (byte < bytes ? byte : 0), bytes - byte, bytes < 16);
                 });
             }
 #pragma unroll

@@ -302,9 +302,15 @@ struct ColumnOperand {
         if constexpr (kIndexed) {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                int32_t at = next[i][0];
+                // by steps from one index to the next: a choice between them the compiler made one between addresses,
+                // of an array in scratch memory
+                uint32_t sum = static_cast<uint32_t>(next[i][0]);
 #pragma unroll
-                for (int j = 1; j < kWaveRows; ++j) at = (threadIdx.x & 63) / kChunks >= j ? next[i][j] : at;
+                for (int j = 1; j < kWaveRows; ++j) {
+                    const uint32_t step = static_cast<uint32_t>(next[i][j]) - static_cast<uint32_t>(next[i][j - 1]);
+                    sum += (threadIdx.x & 63) / kChunks >= j ? step : 0;
+                }
+                const int32_t at = static_cast<int32_t>(sum);
                 ptr[i] = base + (at < 0 || at >= count ? 0 : at) * ld;
             }
         }

@@ -778,10 +778,12 @@ __global__ __launch_bounds__(512, 1) void GroupedTileKernel(GroupedLaunch p, int
 // there are not tiles enough for that, one whose three teams share a tile's
 // contraction.  Bound by the latency of its copies, one turn ahead, and by the
 // weights' bytes: 812 rows in 48 groups, 1001x1000, fp16, 22 us (98 MB, 4.4
-// TB/s).
+// TB/s).  Registers are kept to what three workgroups leave each other (the
+// input's gradient of 5418 rows in 6 groups x 1144 x 660, which would take a
+// few more: 41 us, 51 with two workgroups).
 constexpr int kSmallTileBytes = 2 * (64 + 128) * kTurnBytes;
 template <typename T, typename TOut, bool kBTrans, bool kAligned, int kTeams>
-__global__ __launch_bounds__(kTeams * 256, 1) void GroupedSmallTileKernel(GroupedLaunch p, int32_t tilesN)
+__global__ __launch_bounds__(kTeams * 256, 3) void GroupedSmallTileKernel(GroupedLaunch p, int32_t tilesN)
 {
     __shared__ __align__(128) char lds[kTeams * kSmallTileBytes];
     const RaggedTiles tiles(p.offsets, p.rows, p.groups, 64);

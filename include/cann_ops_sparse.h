@@ -447,12 +447,25 @@ aclsparseStatus_t aclsparseCombine(aclsparseHandle_t handle, int64_t tokens, int
                                    const int32_t* places, const float* weights, const void* Y, int64_t ldy,
                                    aclDataType yType, void* out, int64_t ldOut, aclDataType outType);
 /* gradY[places[t*k + j]] = weights[t*k + j] * gradOut_t, zero for the rows past offsets[groups], and
- * gradWeights[t*k + j] = <gradOut_t, Y[places[t*k + j]]>; either may be null when it is not wanted. */
+ * gradWeights[t*k + j] = <gradOut_t, Y[places[t*k + j]]>; either may be null when it is not wanted.  For the places of
+ * aclsparseRoute or aclsparseExpertPlan as they are, which name each row before offsets[groups] once: of other places
+ * a row that none names is not written, one that several name gets the part of any of them.  aclsparseCombineGradAny
+ * takes those. */
 aclsparseStatus_t aclsparseCombineGrad(aclsparseHandle_t handle, int64_t tokens, int64_t k, int64_t width,
                                        int64_t rows, int64_t groups, const int32_t* offsets, const int32_t* places,
                                        const float* weights, const void* Y, int64_t ldy, const void* gradOut,
                                        int64_t ldOut, aclDataType type, void* gradY, int64_t ldGradY,
                                        float* gradWeights);
+/* Bytes of the buffer that aclsparseCombineGradAny works in (calls that share one must not overlap). */
+aclsparseStatus_t aclsparseCombineGradAny_bufferSize(aclsparseHandle_t handle, int64_t tokens, int64_t k,
+                                                     int64_t rows, size_t* bufferSize);
+/* The same for any places, as aclsparseCombine takes them: gradY_r is the sum of weights[t*k + j] * gradOut_t over the
+ * (t, j) whose place is r, in fp32 and in their order, zero for a row that no place names.  buffer may be null when
+ * gradY is. */
+aclsparseStatus_t aclsparseCombineGradAny(aclsparseHandle_t handle, int64_t tokens, int64_t k, int64_t width,
+                                          int64_t rows, const int32_t* places, const float* weights, const void* Y,
+                                          int64_t ldy, const void* gradOut, int64_t ldOut, aclDataType type,
+                                          void* gradY, int64_t ldGradY, float* gradWeights, void* buffer);
 
 #ifdef __cplusplus
 }

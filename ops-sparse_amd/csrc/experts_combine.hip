@@ -62,19 +62,109 @@ __global__ __launch_bounds__(kThreads) void CombineKernel(CombineLaunch p, int32
     StorePack<TOut, VEC>(static_cast<TOut*>(p.out) + t * p.ldo + c, out);
 }
 
+// The assignments that name each row, for any places: head[r] is one of row r's and next[a] another of the row that a
+// names, or whatever the memory held: neither array is cleared before.  An entry counts only where it is an assignment
+// that names the row (Names).  That is enough, as every assignment of a row enters its list: what
+// the first to enter finds in head[r] is either no assignment of the row or one that the list holds as well.
+__global__ __launch_bounds__(kThreads) void LinkPlacesKernel(CombineGradLaunch p)
+{
+    const int64_t assignments = p.tokens * p.k;
+    for (int64_t a = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; a < assignments;
+         a += static_cast<int64_t>(gridDim.x) * kThreads) {
+        const int32_t place = p.places[a];
+        if (place >= 0 && place < p.rows) p.next[a] = atomicExch(&p.head[place], static_cast<int32_t>(a));
+    }
+}
+
+struct CombineGradLinks {
+    const CombineGradLaunch& p;
+    int64_t assignments;
+
+    // without a branch, so that what follows need not wait for the load
+    __device__ __forceinline__ bool Names(int32_t a, int64_t row) const
+    {
+        const bool in = a >= 0 && a < assignments;
+        return (p.places[in ? a : 0] == row) & in;
+    }
+};
+
+// dy of a row that several assignments name, a at the head of their list, by one wave: the sum of their parts in
+// fp32 in the order of the assignments, whatever the list's.  A list of more than a wave's lanes is left, and the
+// places are searched for its assignments.
+template <typename T, int VEC>
+__device__ void SumSharedRow(const CombineGradLaunch& p, const CombineGradLinks& links, int32_t a, int32_t place)
+{
+    const int lane = threadIdx.x & 63;
+    int32_t mine = -1, count = 0, at = a;
+    bool searched = false;
+    while (true) {
+        if (lane == count) mine = at;
+        ++count;
+        at = p.next[at];
+        if (!links.Names(at, place) || __any(mine == at)) break;
+        if (count == 64) {
+            searched = true;
+            break;
+        }
+    }
+    int32_t rank = 0;
+    for (int i = 0; i < count; ++i) rank += __builtin_amdgcn_readlane(mine, i) < mine ? 1 : 0;
+    if (lane >= count) rank = -1;
+    for (int64_t c0 = 0; c0 < p.width; c0 += 64 * VEC) {
+        const int64_t c = c0 + lane * VEC;
+        float acc[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
+        auto add = [&](int64_t other) {
+            if (c >= p.width) return;
+            const float w = p.weights != nullptr ? p.weights[other] : 1.0f;
+            const auto g = LoadPack<T, VEC>(static_cast<const T*>(p.grad_out) + other / p.k * p.ldo + c);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) acc[i] = fmaf(w, ToFloat(g.v[i]), acc[i]);
+        };
+        if (searched) {
+            for (int64_t first = 0; first < links.assignments; first += 64) {
+                const bool named = first + lane < links.assignments && p.places[first + lane] == place;
+                for (uint64_t left = __ballot(named); left != 0; left &= left - 1) add(first + __builtin_ctzll(left));
+            }
+        } else {
+            for (int i = 0; i < count; ++i) add(__builtin_amdgcn_readlane(mine, __builtin_ctzll(__ballot(rank == i))));
+        }
+        if (c < p.width) {
+            Pack<T, VEC> d;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) d.v[i] = FromFloat<T>(acc[i]);
+            StorePack<T, VEC>(static_cast<T*>(p.grad_y) + place * p.ld_grad_y + c, d);
+        }
+    }
+}
+
 // One wave per assignment, which reads its token's dout (from L2 after the
 // first of the token's k), its own row of y once, and writes its row of dy; dw
-// is the wave's own sum, so nothing is added across waves.  Assignment number
-// a also clears row a of dy when that row belongs to no group.  Bound by
-// memory: 16384 tokens of 8 rows of 2048, bfloat16, 214 us for 1.14 GB, 5.3
-// TB/s.
-template <typename T, int VEC>
+// is the wave's own sum, so nothing is added across waves.  Wave number r also
+// clears row r of dy where the row has no assignment.  With kAny those are the
+// rows that no place names, and the head of a row's list writes it; without,
+// the rows past the last group, as in a plan whose places name each row before
+// them once.  Bound by memory: 16384 tokens of 8 rows of 2048, bfloat16, 214 to
+// 218 us with kAny for 1.14 GB, 5.2 TB/s, behind 5 us of LinkPlacesKernel (with
+// the list looked up before the row's first loads 236 to 241 us: a chain of
+// three dependent loads of each wave that nothing hid).
+template <typename T, int VEC, bool kAny>
 __global__ __launch_bounds__(kThreads) void CombineGradKernel(CombineGradLaunch p)
 {
     const int lane = threadIdx.x & 63;
     const int64_t a = static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
     const int64_t assignments = p.tokens * p.k;
+    const CombineGradLinks links{p, assignments};
     T* gy = static_cast<T*>(p.grad_y);
+    bool unnamed = false;  // row a has no assignment
+    if (gy != nullptr && a < p.rows) {
+        if constexpr (kAny) {
+            unnamed = assignments == 0 || !links.Names(p.head[a], a);
+        } else {
+            unnamed = a >= p.offsets[p.groups];
+        }
+    }
     if (a < assignments) {
         const int32_t place = p.places[a];
         float dot = 0.0f;
@@ -83,19 +173,46 @@ __global__ __launch_bounds__(kThreads) void CombineGradKernel(CombineGradLaunch 
             const T* go =
                 static_cast<const T*>(p.grad_out) + static_cast<uint32_t>(a) / static_cast<uint32_t>(p.k) * p.ldo;
             const T* y = p.grad_weights != nullptr ? static_cast<const T*>(p.y) + place * p.ldy : nullptr;
-            for (int64_t c = lane * VEC; c < p.width; c += 64 * VEC) {
-                const auto g = LoadPack<T, VEC>(go + c);
-                if (y != nullptr) {
-                    const auto v = LoadPack<T, VEC>(y + c);
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) dot = fmaf(ToFloat(g.v[i]), ToFloat(v.v[i]), dot);
-                }
+            // the row's first part is asked for before anything is known of its list, each next one before the last
+            // one's store
+            int64_t c = lane * VEC;
+            Pack<T, VEC> g{}, v{};
+            auto load = [&] {
+                if (c >= p.width) return;
+                g = LoadPack<T, VEC>(go + c);
+                if (y != nullptr) v = LoadPack<T, VEC>(y + c);
+            };
+            load();
+            bool only = gy != nullptr, first = false;
+            if constexpr (kAny) {
                 if (gy != nullptr) {
+                    const int32_t other = p.next[a];
+                    const bool listed = p.head[place] == a;
+                    const bool shared = links.Names(other, place) & (other != a);
+                    only = listed & !shared;
+                    first = listed & shared;
+                }
+            } else {
+                only = gy != nullptr && place < p.offsets[p.groups];
+            }
+            while (c < p.width) {
+                const auto g0 = g, v0 = v;
+                T* to = gy + place * p.ld_grad_y + c;
+                c += 64 * VEC;
+                load();
+                if (y != nullptr) {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) dot = fmaf(ToFloat(g0.v[i]), ToFloat(v0.v[i]), dot);
+                }
+                if (only) {
                     Pack<T, VEC> d;
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) d.v[i] = FromFloat<T>(w * ToFloat(g.v[i]));
-                    StorePack<T, VEC>(gy + place * p.ld_grad_y + c, d);
+                    for (int i = 0; i < VEC; ++i) d.v[i] = FromFloat<T>(w * ToFloat(g0.v[i]));
+                    StorePack<T, VEC>(to, d);
                 }
+            }
+            if constexpr (kAny) {
+                if (__any(first)) SumSharedRow<T, VEC>(p, links, static_cast<int32_t>(a), place);
             }
         }
         if (p.grad_weights != nullptr) {
@@ -103,7 +220,7 @@ __global__ __launch_bounds__(kThreads) void CombineGradKernel(CombineGradLaunch 
             if (lane == 0) p.grad_weights[a] = dot;
         }
     }
-    if (gy != nullptr && a < p.rows && a >= p.offsets[p.groups]) {
+    if (unnamed) {
         Pack<T, VEC> zero;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) zero.v[i] = FromFloat<T>(0.0f);
@@ -134,7 +251,7 @@ int CombineTyped(const CombineLaunch& l, hipStream_t s)
     return 0;
 }
 
-template <typename T>
+template <typename T, bool kAny>
 int CombineGradTyped(const CombineGradLaunch& l, hipStream_t s)
 {
     constexpr int VEC = 16 / sizeof(T);
@@ -142,10 +259,14 @@ int CombineGradTyped(const CombineGradLaunch& l, hipStream_t s)
                       Aligned(l.grad_out, l.ldo, sizeof(T), 16) && Aligned(l.grad_y, l.ld_grad_y, sizeof(T), 16);
     const int64_t count = l.tokens * l.k > l.rows ? l.tokens * l.k : l.rows;
     const uint32_t grid = static_cast<uint32_t>((count + kThreads / 64 - 1) / (kThreads / 64));
+    if (kAny && l.grad_y != nullptr && l.tokens > 0) {
+        const int64_t blocks = (l.tokens * l.k + kThreads - 1) / kThreads;
+        LinkPlacesKernel<<<static_cast<uint32_t>(blocks < 4096 ? blocks : 4096), kThreads, 0, s>>>(l);
+    }
     if (wide) {
-        CombineGradKernel<T, VEC><<<grid, kThreads, 0, s>>>(l);
+        CombineGradKernel<T, VEC, kAny><<<grid, kThreads, 0, s>>>(l);
     } else {
-        CombineGradKernel<T, 1><<<grid, kThreads, 0, s>>>(l);
+        CombineGradKernel<T, 1, kAny><<<grid, kThreads, 0, s>>>(l);
     }
     return 0;
 }
@@ -164,7 +285,10 @@ int LaunchCombine(const CombineLaunch& l, void* stream)
 int LaunchCombineGrad(const CombineGradLaunch& l, void* stream)
 {
     hipStream_t s = static_cast<hipStream_t>(stream);
-    return l.type == ACL_FLOAT16 ? CombineGradTyped<Half>(l, s) : CombineGradTyped<Bf16>(l, s);
+    if (l.offsets == nullptr) {
+        return l.type == ACL_FLOAT16 ? CombineGradTyped<Half, true>(l, s) : CombineGradTyped<Bf16, true>(l, s);
+    }
+    return l.type == ACL_FLOAT16 ? CombineGradTyped<Half, false>(l, s) : CombineGradTyped<Bf16, false>(l, s);
 }
 
 }  // namespace aclsp

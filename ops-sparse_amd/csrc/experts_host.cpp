@@ -69,6 +69,41 @@ aclsparseStatus_t CheckGroupedShape(int64_t groups, int64_t rows, int64_t n, int
     return ACL_SPARSE_STATUS_SUCCESS;
 }
 
+aclsparseStatus_t CheckCombineShape(int64_t tokens, int64_t k, int64_t width, int64_t rows)
+{
+    if (tokens < 0 || k < 1 || width < 0 || rows < 0) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    if (k > aclsp::kMaxRouteK || tokens > kMaxCount / k || rows > kMaxCount || width > kMaxCount) {
+        return ACL_SPARSE_STATUS_NOT_SUPPORTED;
+    }
+    return ACL_SPARSE_STATUS_SUCCESS;
+}
+
+// What both gradients of a combination check, but the offsets and the buffer
+aclsparseStatus_t CheckCombineGrad(const aclsp::CombineGradLaunch& l)
+{
+    const aclsparseStatus_t st = CheckCombineShape(l.tokens, l.k, l.width, l.rows);
+    if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
+    if (!Is16Bit(l.type)) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
+    if (l.ldo < l.width || (l.grad_y != nullptr && l.ld_grad_y < l.width) ||
+        (l.grad_weights != nullptr && l.ldy < l.width)) {
+        return ACL_SPARSE_STATUS_INVALID_VALUE;
+    }
+    if (l.tokens > 0 && (l.places == nullptr || (l.width > 0 && l.grad_out == nullptr))) {
+        return ACL_SPARSE_STATUS_INVALID_VALUE;
+    }
+    if (l.grad_weights != nullptr && l.y == nullptr && l.rows > 0 && l.width > 0) {
+        return ACL_SPARSE_STATUS_INVALID_VALUE;
+    }
+    return ACL_SPARSE_STATUS_SUCCESS;
+}
+
+// One int32 per row or assignment
+size_t HeadBytes(int64_t count)
+{
+    const size_t bytes = static_cast<size_t>(count) * sizeof(int32_t);
+    return aclsp::AlignUp(bytes < aclsp::kWsAlign ? aclsp::kWsAlign : bytes);
+}
+
 }  // namespace
 
 extern "C" {
@@ -222,10 +257,8 @@ aclsparseStatus_t aclsparseCombine(aclsparseHandle_t handle, int64_t tokens, int
 {
     aclsparseStatus_t st = CheckHandle(handle);
     if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
-    if (tokens < 0 || k < 1 || width < 0 || rows < 0) return ACL_SPARSE_STATUS_INVALID_VALUE;
-    if (k > aclsp::kMaxRouteK || tokens > kMaxCount / k || rows > kMaxCount || width > kMaxCount) {
-        return ACL_SPARSE_STATUS_NOT_SUPPORTED;
-    }
+    st = CheckCombineShape(tokens, k, width, rows);
+    if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
     // rows of 32 bits (a gradient's partial sums) may be rounded to 16 here
     if (!Is16Bit(outType) || (yType != outType && yType != ACL_FLOAT)) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
     if (ldy < width || ldOut < width) return ACL_SPARSE_STATUS_INVALID_VALUE;
@@ -244,23 +277,47 @@ aclsparseStatus_t aclsparseCombineGrad(aclsparseHandle_t handle, int64_t tokens,
 {
     aclsparseStatus_t st = CheckHandle(handle);
     if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
-    if (tokens < 0 || k < 1 || width < 0 || rows < 0 || groups < 1) return ACL_SPARSE_STATUS_INVALID_VALUE;
-    if (k > aclsp::kMaxRouteK || tokens > kMaxCount / k || rows > kMaxCount || width > kMaxCount ||
-        groups > kMaxCount) {
-        return ACL_SPARSE_STATUS_NOT_SUPPORTED;
-    }
-    if (!Is16Bit(type)) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
-    if (ldOut < width || (gradY != nullptr && ldGradY < width) || (gradWeights != nullptr && ldy < width)) {
-        return ACL_SPARSE_STATUS_INVALID_VALUE;
-    }
-    if (tokens == 0 && rows == 0) return ACL_SPARSE_STATUS_SUCCESS;
-    if (offsets == nullptr || (tokens > 0 && (places == nullptr || (width > 0 && gradOut == nullptr)))) {
-        return ACL_SPARSE_STATUS_INVALID_VALUE;
-    }
-    if (gradWeights != nullptr && Y == nullptr && rows > 0 && width > 0) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    if (groups < 1) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    if (groups > kMaxCount) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
+    const aclsp::CombineGradLaunch l{tokens, k, width, rows, groups, offsets, places, weights, Y, ldy, gradOut, ldOut,
+                                     type, gradY, ldGradY, gradWeights, nullptr, nullptr};
+    st = CheckCombineGrad(l);
+    if (st != ACL_SPARSE_STATUS_SUCCESS || (tokens == 0 && rows == 0)) return st;
+    if (offsets == nullptr) return ACL_SPARSE_STATUS_INVALID_VALUE;
     if (gradY == nullptr && gradWeights == nullptr) return ACL_SPARSE_STATUS_SUCCESS;
-    aclsp::CombineGradLaunch l{tokens, k, width, rows, groups, offsets, places, weights, Y, ldy, gradOut, ldOut,
-                               type, gradY, ldGradY, gradWeights};
+    (void)hipGetLastError();
+    return Finish(aclsp::LaunchCombineGrad(l, StreamOf(handle)));
+}
+
+aclsparseStatus_t aclsparseCombineGradAny_bufferSize(aclsparseHandle_t handle, int64_t tokens, int64_t k,
+                                                     int64_t rows, size_t* bufferSize)
+{
+    aclsparseStatus_t st = CheckHandle(handle);
+    if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
+    st = CheckCombineShape(tokens, k, 0, rows);
+    if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
+    if (bufferSize == nullptr) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    *bufferSize = HeadBytes(rows) + HeadBytes(tokens * k);
+    return ACL_SPARSE_STATUS_SUCCESS;
+}
+
+aclsparseStatus_t aclsparseCombineGradAny(aclsparseHandle_t handle, int64_t tokens, int64_t k, int64_t width,
+                                          int64_t rows, const int32_t* places, const float* weights, const void* Y,
+                                          int64_t ldy, const void* gradOut, int64_t ldOut, aclDataType type,
+                                          void* gradY, int64_t ldGradY, float* gradWeights, void* buffer)
+{
+    aclsparseStatus_t st = CheckHandle(handle);
+    if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
+    auto* head = static_cast<int32_t*>(buffer);
+    aclsp::CombineGradLaunch l{tokens, k, width, rows, 0, nullptr, places, weights, Y, ldy, gradOut, ldOut,
+                               type, gradY, ldGradY, gradWeights, head, nullptr};
+    st = CheckCombineGrad(l);
+    if (st != ACL_SPARSE_STATUS_SUCCESS || (tokens == 0 && rows == 0)) return st;
+    if (gradY == nullptr && gradWeights == nullptr) return ACL_SPARSE_STATUS_SUCCESS;
+    if (gradY != nullptr) {
+        if (buffer == nullptr) return ACL_SPARSE_STATUS_INVALID_VALUE;
+        l.next = head + HeadBytes(rows) / sizeof(int32_t);
+    }
     (void)hipGetLastError();
     return Finish(aclsp::LaunchCombineGrad(l, StreamOf(handle)));
 }

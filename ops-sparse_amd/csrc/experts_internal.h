@@ -67,7 +67,7 @@ int LaunchCombine(const CombineLaunch& l, void* stream);
 
 struct CombineGradLaunch {
     int64_t tokens, k, width, rows, groups;
-    const int32_t* offsets;
+    const int32_t* offsets;  // of the plan that the places are of; null: any places, with head and next
     const int32_t* places;
     const float* weights;  // null: ones
     const void* y;         // null: no gradient of the weights
@@ -78,6 +78,8 @@ struct CombineGradLaunch {
     void* grad_y;  // null: not wanted
     int64_t ld_grad_y;
     float* grad_weights;  // null: not wanted
+    int32_t* head;  // the caller's buffer: one per row
+    int32_t* next;  // and one per assignment
 };
 int LaunchCombineGrad(const CombineGradLaunch& l, void* stream);
 

@@ -36,7 +36,8 @@ struct Library {
     decltype(&aclsparseGroupedMMGrad) groupedMMGrad = nullptr;
     decltype(&aclsparseGroupedMMScaled) groupedMMScaled = nullptr;
     decltype(&aclsparseCombine) combine = nullptr;
-    decltype(&aclsparseCombineGrad) combineGrad = nullptr;
+    decltype(&aclsparseCombineGradAny_bufferSize) combineGradBufferSize = nullptr;
+    decltype(&aclsparseCombineGradAny) combineGrad = nullptr;
 } lib;
 
 void Bind(const std::string& path)
@@ -58,7 +59,8 @@ void Bind(const std::string& path)
     look(lib.groupedMMGrad, "aclsparseGroupedMMGrad");
     look(lib.groupedMMScaled, "aclsparseGroupedMMScaled");
     look(lib.combine, "aclsparseCombine");
-    look(lib.combineGrad, "aclsparseCombineGrad");
+    look(lib.combineGradBufferSize, "aclsparseCombineGradAny_bufferSize");
+    look(lib.combineGrad, "aclsparseCombineGradAny");
 }
 
 // A handle on the current stream of a tensor's device, with that device current.
@@ -406,8 +408,8 @@ Tensor GroupedMMScaled(const Tensor& a, const Tensor& aScale, const Tensor& wGiv
 struct CombineNode : torch::autograd::Function<CombineNode> {
     static Tensor forward(AutogradContext* ctx, const Tensor& y, const optional<Tensor>& given, const Sorted& plan)
     {
-        const Tensor weights = given.value_or(Tensor()), &offsets = plan.offsets, &places = plan.places;
-        ctx->save_for_backward({y, weights, offsets, places});
+        const Tensor weights = given.value_or(Tensor()), &places = plan.places;
+        ctx->save_for_backward({y, weights, places});
         ctx->saved_data["y"] = y.requires_grad();
         ctx->saved_data["w"] = weights.defined() && weights.requires_grad();
         return RunCombine(y, places, weights, y.scalar_type());
@@ -415,17 +417,22 @@ struct CombineNode : torch::autograd::Function<CombineNode> {
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
         const auto saved = ctx->get_saved_variables();
-        const Tensor &y = saved[0], &weights = saved[1], &offsets = saved[2], &places = saved[3];
+        const Tensor &y = saved[0], &weights = saved[1], &places = saved[2];
         const Tensor grad = Rows(grads[0]);
         const int64_t tokens = places.size(0), k = places.size(1), rows = y.size(0), width = y.size(1);
-        Tensor dy, dw;
-        if (ctx->saved_data["y"].toBool()) dy = Empty({rows, width}, y.scalar_type(), y);
-        if (ctx->saved_data["w"].toBool()) dw = Empty({tokens, k}, at::kFloat, y);
         Call call(y);
-        Call::Ok(lib.combineGrad(call, tokens, k, width, rows, offsets.size(0) - 1, Ints(offsets), Ints(places),
-                                 Floats(weights), Data(y), Ld(y), Data(grad), Ld(grad), TypeOf(y.scalar_type()),
-                                 Data(dy), std::max<int64_t>(width, 1), Floats(dw)),
-                 "aclsparseCombineGrad");
+        Tensor dy, dw, buffer;
+        if (ctx->saved_data["y"].toBool()) {
+            dy = Empty({rows, width}, y.scalar_type(), y);
+            size_t bytes = 0;
+            Call::Ok(lib.combineGradBufferSize(call, tokens, k, rows, &bytes), "aclsparseCombineGradAny_bufferSize");
+            buffer = Empty({static_cast<int64_t>(bytes)}, at::kByte, y);
+        }
+        if (ctx->saved_data["w"].toBool()) dw = Empty({tokens, k}, at::kFloat, y);
+        Call::Ok(lib.combineGrad(call, tokens, k, width, rows, Ints(places), Floats(weights), Data(y), Ld(y),
+                                 Data(grad), Ld(grad), TypeOf(y.scalar_type()), Data(dy), std::max<int64_t>(width, 1),
+                                 Floats(dw), Data(buffer)),
+                 "aclsparseCombineGradAny");
         return Once({dy, dw, Tensor()});
     }
 };
@@ -454,7 +461,7 @@ Tensor Combine(const Tensor& y, const Tensor& planOffsets, const optional<Tensor
     const Tensor rows = Rows(y);
     if (!Tracked(y, weights)) return RunCombine(rows, places, weights, y.scalar_type());
     return CombineNode::apply(rows, weights.defined() ? optional<Tensor>(weights) : std::nullopt,
-                              Sorted{offsets, {}, places});
+                              Sorted{{}, {}, places});
 }
 
 }  // namespace

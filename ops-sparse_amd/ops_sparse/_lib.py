@@ -189,6 +189,8 @@ SIGNATURES = {
     "aclsparseCombine": [_vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i32, _vp, _i64, _i32],
     "aclsparseCombineGrad": [_vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i32, _vp, _i64,
                              _vp],
+    "aclsparseCombineGradAny_bufferSize": [_vp, _i64, _i64, _i64, ctypes.POINTER(_sz)],
+    "aclsparseCombineGradAny": [_vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i32, _vp, _i64, _vp, _vp],
 }
 
 _LIB = None

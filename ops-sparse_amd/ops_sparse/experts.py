@@ -30,7 +30,8 @@ class ExpertPlan(NamedTuple):
 
     offsets [E + 1]: rows offsets[e] to offsets[e + 1] are expert e's; tokens [T * k]: the token of each row (-1
     past offsets[E]); places [T, k]: the row of each assignment, -1 for a dropped one.  ``tokens`` and ``places``
-    may be None where rows are grouped by other means: such a plan serves products that do not gather.
+    may be None where rows are grouped by other means: such a plan serves products that do not gather.  The gradient
+    of a gathered operand goes by places: an assignment whose place is set to -1 afterwards has no part in it.
     """
     offsets: torch.Tensor
     tokens: Optional[torch.Tensor] = None
@@ -99,7 +100,8 @@ def grouped_mm_scaled(a, a_scale, w, w_scale, plan=None, gather=False, out_dtype
 def combine(y, plan, weights=None):
     """out [T, H]: out[t] = sum over j of weights[t, j] * y[plan.places[t, j]], summed in fp32 (differentiable).
 
-    y [R, H] fp16 or bf16 in the plan's row order; weights [T, k] fp32, None for ones.  Dropped assignments add
-    nothing.
+    y [R, H] fp16 or bf16 in the plan's row order; weights [T, k] fp32, None for ones.  Dropped assignments (places
+    outside [0, R)) add nothing.  Any places will do, -1 set afterwards among them: the gradient of a row of y that no
+    place names is zero, that of one that several name the sum of their parts.
     """
     return (_MODULE or _module()).combine(y, plan.offsets, plan.places, weights)

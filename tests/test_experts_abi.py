@@ -133,6 +133,36 @@ def test_status_codes(lib, handle, name, args, changes):
         assert fn(handle, *args(**change)) == status, (name, change)
 
 
+def combine_grad_any(**kw):
+    a = dict(tokens=4, k=2, width=8, rows=8, places=P, weights=P, y=P, ldy=8, go=P, ldo=8, type=F16, gy=P, ldgy=8, gw=P,
+             buffer=P)
+    a.update(kw)
+    return list(a.values())
+
+
+def test_status_codes_of_the_gradient_for_any_places(lib, handle):
+    fn = lib.aclsparseCombineGradAny
+    assert fn(None, *combine_grad_any()) == Status.HANDLE_IS_NULLPTR
+    for change, status in [
+            (dict(tokens=-1), INVALID), (dict(k=0), INVALID), (dict(k=65), UNSUPPORTED), (dict(rows=-1), INVALID),
+            (dict(rows=2**31), UNSUPPORTED), (dict(tokens=2**30), UNSUPPORTED), (dict(type=F32), UNSUPPORTED),
+            (dict(ldo=7), INVALID), (dict(ldgy=7), INVALID), (dict(ldy=7), INVALID), (dict(places=0), INVALID),
+            (dict(y=0), INVALID), (dict(go=0), INVALID), (dict(buffer=0), INVALID), (dict(gy=0, gw=0, buffer=0), OK),
+            (dict(tokens=0, rows=0), OK)]:
+        assert fn(handle, *combine_grad_any(**change)) == status, change
+
+
+def test_buffer_size_of_the_gradient_for_any_places(lib, handle):
+    size = ctypes.c_size_t(0)
+    fn = lib.aclsparseCombineGradAny_bufferSize
+    for tokens, k, rows in ((0, 1, 0), (1, 1, 1), (100, 3, 7), (16384, 8, 2**31 - 1), (2**25, 63, 5)):
+        assert fn(handle, tokens, k, rows, ctypes.byref(size)) == OK
+        assert 4 * (rows + tokens * k) <= size.value <= 4 * (rows + tokens * k) + 192 and size.value % 64 == 0
+    assert fn(handle, 4, 2, 8, None) == INVALID
+    assert fn(handle, 4, 65, 8, ctypes.byref(size)) == UNSUPPORTED
+    assert fn(None, 4, 2, 8, ctypes.byref(size)) == Status.HANDLE_IS_NULLPTR
+
+
 def test_buffer_size(lib, handle):
     size = ctypes.c_size_t(0)
     for tokens, experts, k in ((0, 1, 1), (1, 8, 2), (64, 64, 8), (16384, 128, 8), (10**6, 1024, 2)):

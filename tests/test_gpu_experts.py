@@ -624,6 +624,91 @@ def test_combine_gradient_against_differences(dev):
         assert abs(slope - float(grad[at])) <= rounding
 
 
+def any_places(kind, tokens, k):
+    """(places, rows of y) that are no plan's: rows that no place names, and rows that several do."""
+    count = tokens * k
+    plan = expert_plan(routed(tokens, max(k, 7), k, 11), max(k, 7)).places.cpu()
+    g = gen(12, "cpu")
+    if kind == "dropped":  # a capacity limit on a finished plan
+        return plan.masked_fill(torch.rand(plan.shape, generator=g) < 0.4, -1), count
+    if kind == "all dropped":
+        return torch.full_like(plan, -1), count
+    if kind == "more rows":
+        return plan * 3 + 1, 3 * count + 5
+    if kind == "outside":  # past y's rows and before them
+        return torch.where(torch.rand(plan.shape, generator=g) < 0.5, plan - 3, plan + count // 2), count
+    if kind == "drawn":  # most rows by none, one or two, some by more
+        return torch.randint(0, count, plan.shape, generator=g, dtype=torch.int32), count
+    if kind == "one row":
+        return torch.full_like(plan, 3), 5
+    # two rows by as many as fit a wave, and by one more; the rest each by one
+    flat = plan.reshape(-1).clone()
+    order = torch.randperm(count, generator=g)
+    flat[order[:64]], flat[order[64:129]] = 0, 1
+    return flat.view(tokens, k), count
+
+
+@pytest.mark.parametrize("kind", ["dropped", "all dropped", "more rows", "outside", "drawn", "one row", "a wave"])
+@pytest.mark.parametrize("tokens,k,width,dtype", [(100, 2, 1, F16), (70, 3, 33, BF16), (65, 4, 264, F16),
+                                                  (300, 8, 2056, BF16)])
+def test_combine_gradients_of_any_places(dev, kind, tokens, k, width, dtype):
+    places, rows = any_places(kind, tokens, k)
+    plan = ExpertPlan(torch.tensor([0, 2], dtype=torch.int32, device=dev), None, places.to(dev))
+    y = torch.randn(rows, width, generator=gen(1), device=dev).to(dtype).requires_grad_(True)
+    weights = torch.randn(tokens, k, generator=gen(2), device=dev).requires_grad_(True)
+    grad = torch.randn(tokens, width, generator=gen(4), device=dev).to(dtype)
+    used = ((places >= 0) & (places < rows)).to(dev)
+    safe = torch.where(used, plan.places, 0).long()
+    for w in (weights, None):
+        factor = (torch.ones(tokens, k, dtype=torch.float64, device=dev) if w is None else w.detach().double()) * used
+        part = (factor[:, :, None] * grad.double()[:, None, :]).reshape(-1, width)
+        want, magnitude = (torch.zeros(rows, width, dtype=torch.float64, device=dev)
+                           .index_add_(0, safe.reshape(-1), t) for t in (part, part.abs()))
+        most = int(torch.bincount(safe[used], minlength=1).max()) if used.any() else 1
+        first = None
+        for turn in range(3):
+            # what the allocator hands out next is not zeros: values, and numbers of assignments
+            left = [torch.full((rows, width), float("nan"), dtype=dtype, device=dev),
+                    torch.randint(0, tokens * k, (rows + 16,), device=dev, dtype=torch.int32),
+                    torch.randint(0, tokens * k, (rows + tokens * k + 32,), device=dev, dtype=torch.int32)]
+            del left
+            out = combine(y, plan, w)
+            grads = torch.autograd.grad(out, (y,) if w is None else (y, w), grad)
+            close(grads[0], want, magnitude, most)
+            named = torch.zeros(rows, dtype=torch.bool, device=dev)
+            named[safe[used]] = True
+            assert not grads[0][~named].any()
+            if w is not None:
+                prod = y.detach().double()[safe] * used[:, :, None] * grad.double()[:, None, :]
+                close(grads[1], prod.sum(2), prod.abs().sum(2), width)
+            assert first is None or all(torch.equal(a, b) for a, b in zip(first, grads))
+            first = grads
+
+
+@pytest.mark.parametrize("tokens", [5, 400])
+def test_layer_gradients_after_assignments_are_dropped(dev, tokens):
+    # a capacity of 3 rows an expert, set on the finished plan: what is dropped has no part in any gradient
+    experts, k, n, width = 6, 2, 72, 136
+    full = expert_plan(routed(tokens, experts, k, 2), experts)
+    expert = (full.places[:, :, None] >= full.offsets[1:]).sum(2)
+    place = torch.where(full.places - full.offsets[expert] < 3, full.places, -1)
+    plan = full._replace(places=place)
+    x = torch.randn(tokens, width, generator=gen(1), device=dev).to(BF16).requires_grad_(True)
+    w = torch.randn(experts, n, width, generator=gen(2), device=dev).to(BF16).requires_grad_(True)
+    weights = torch.rand(tokens, k, generator=gen(3), device=dev)
+    grad = torch.randn(tokens, n, generator=gen(4), device=dev).to(BF16)
+    out = combine(grouped_mm(x, w, plan, gather=True), plan, weights)
+    dx, dw = torch.autograd.grad(out, (x, w), grad)
+    kept = (place >= 0).double() * weights.double()
+    rows = torch.zeros(tokens * k, n, dtype=torch.float64, device=dev)
+    rows[full.places.long()] = kept[:, :, None] * grad.double()[:, None, :]
+    wx, mx, ww, mw = plain_grads(x.detach(), w.detach(), full, rows)
+    # the rows' gradients are rounded to bfloat16 between the two operators
+    for got, want, magnitude in ((dx, wx, mx), (dw, ww, mw)):
+        bound = 2 * U[BF16] * want.abs() + (2 * U[BF16] + (n + tokens) * U32) * magnitude + 2.0**-25
+        assert bool(((got.double() - want).abs() <= bound).all())
+
+
 # ------------------------------------------------------------------------------------------------------- as a whole
 
 

@@ -423,7 +423,7 @@ aclsparseStatus_t aclsparseRouteGrad(aclsparseHandle_t handle, int64_t tokens, i
  * ACL_SPARSE_OP_NON_TRANSPOSE takes B_g [k, n], ACL_SPARSE_OP_TRANSPOSE takes B_g [n, k]; B_g starts strideB elements
  * after B_(g-1).  A and B ACL_FLOAT16 or ACL_BF16, C their type or ACL_FLOAT; sums in fp32.  offsets start at 0 and do
  * not decrease and indices lie in [0, rowsA): others give values without meaning, never an access outside the
- * operands.  rows, n and k up to 2^31 - 4097. */
+ * operands.  groups, rows, n and k up to 2^31 - 4097. */
 aclsparseStatus_t aclsparseGroupedMM(aclsparseHandle_t handle, aclsparseOperation_t opB, int64_t groups, int64_t rows,
                                      int64_t n, int64_t k, const int32_t* offsets, const int32_t* rowIndex,
                                      int64_t rowsA, const void* A, int64_t lda, const void* B, int64_t ldb,

@@ -16,7 +16,8 @@
 namespace {
 
 constexpr int64_t kMaxCount = INT32_MAX;  // counts that index arrays of int32
-constexpr int64_t kMaxSide = INT32_MAX - 4096;  // sides of a product: positions in the tile that passes the end fit too
+// sides and groups of a product: positions past the end, in the last tile or the last step of a scan, fit int32 too
+constexpr int64_t kMaxSide = INT32_MAX - 4096;
 
 void* StreamOf(aclsparseHandle_t h)
 {
@@ -60,7 +61,7 @@ aclsparseStatus_t CheckGroupedShape(int64_t groups, int64_t rows, int64_t n, int
                                     const int32_t* rowIndex, int64_t rowsA)
 {
     if (groups < 1 || rows < 0 || n < 0 || k < 0 || rowsA < 0) return ACL_SPARSE_STATUS_INVALID_VALUE;
-    if (groups > kMaxCount || rows > kMaxSide || n > kMaxSide || k > kMaxSide || rowsA > kMaxCount) {
+    if (groups > kMaxSide || rows > kMaxSide || n > kMaxSide || k > kMaxSide || rowsA > kMaxCount) {
         return ACL_SPARSE_STATUS_NOT_SUPPORTED;
     }
     if (offsets == nullptr && groups != 1) return ACL_SPARSE_STATUS_INVALID_VALUE;

@@ -133,6 +133,15 @@ def test_status_codes(lib, handle, name, args, changes):
         assert fn(handle, *args(**change)) == status, (name, change)
 
 
+@pytest.mark.parametrize("name,args", [("aclsparseGroupedMM", grouped), ("aclsparseGroupedMMScaled", scaled),
+                                       ("aclsparseGroupedMMGrad", grad)])
+def test_more_groups_than_a_scan_can_count_are_refused(lib, handle, name, args):
+    # the kernels' scans go over the groups 64 at a time in int32, and their last step has to fit it
+    for groups in (2**31 - 4096, 2**31 - 64, 2**31 - 1, 2**40):
+        assert getattr(lib, name)(handle, *args(groups=groups, stride=0 if name != "aclsparseGroupedMMGrad" else 128)) \
+            == UNSUPPORTED, groups
+
+
 def combine_grad_any(**kw):
     a = dict(tokens=4, k=2, width=8, rows=8, places=P, weights=P, y=P, ldy=8, go=P, ldo=8, type=F16, gy=P, ldgy=8, gw=P,
              buffer=P)

@@ -13,7 +13,7 @@
 namespace aclsp {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;  // as GridOf takes them
 
 template <typename T, int N>
 struct Pack {
@@ -41,9 +41,10 @@ __device__ __forceinline__ void StorePack(T* p, const Pack<T, N>& v)
 template <typename TIn, typename TOut, int VEC>
 __global__ __launch_bounds__(kThreads) void CombineKernel(CombineLaunch p, int32_t chunks)
 {
-    const int64_t t = blockIdx.x / static_cast<uint32_t>(chunks);
-    const int64_t c = (static_cast<int64_t>(blockIdx.x % static_cast<uint32_t>(chunks)) * kThreads + threadIdx.x) * VEC;
-    if (c >= p.width) return;
+    const uint32_t block = BlockNumber();
+    const int64_t t = block / static_cast<uint32_t>(chunks);
+    const int64_t c = (static_cast<int64_t>(block % static_cast<uint32_t>(chunks)) * kThreads + threadIdx.x) * VEC;
+    if (t >= p.tokens || c >= p.width) return;
     const int k = static_cast<int>(p.k);
     float acc[VEC];
 #pragma unroll
@@ -153,7 +154,7 @@ template <typename T, int VEC, bool kAny>
 __global__ __launch_bounds__(kThreads) void CombineGradKernel(CombineGradLaunch p)
 {
     const int lane = threadIdx.x & 63;
-    const int64_t a = static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
+    const int64_t a = static_cast<int64_t>(BlockNumber()) * (kThreads / 64) + (threadIdx.x >> 6);
     const int64_t assignments = p.tokens * p.k;
     const CombineGradLinks links{p, assignments};
     T* gy = static_cast<T*>(p.grad_y);
@@ -242,7 +243,7 @@ int CombineTyped(const CombineLaunch& l, hipStream_t s)
     const int64_t per = static_cast<int64_t>(kThreads) * (wide ? VEC : 1);
     const int64_t chunks = (l.width + per - 1) / per;
     if (l.tokens > INT32_MAX / chunks) return kTooLarge;
-    const uint32_t grid = static_cast<uint32_t>(l.tokens * chunks);
+    const dim3 grid = GridOf(l.tokens * chunks);
     if (wide) {
         CombineKernel<TIn, TOut, VEC><<<grid, kThreads, 0, s>>>(l, static_cast<int32_t>(chunks));
     } else {
@@ -258,7 +259,7 @@ int CombineGradTyped(const CombineGradLaunch& l, hipStream_t s)
     const bool wide = l.width % VEC == 0 && Aligned(l.y, l.ldy, sizeof(T), 16) &&
                       Aligned(l.grad_out, l.ldo, sizeof(T), 16) && Aligned(l.grad_y, l.ld_grad_y, sizeof(T), 16);
     const int64_t count = l.tokens * l.k > l.rows ? l.tokens * l.k : l.rows;
-    const uint32_t grid = static_cast<uint32_t>((count + kThreads / 64 - 1) / (kThreads / 64));
+    const dim3 grid = GridOf((count + kThreads / 64 - 1) / (kThreads / 64));
     if (kAny && l.grad_y != nullptr && l.tokens > 0) {
         const int64_t blocks = (l.tokens * l.k + kThreads - 1) / kThreads;
         LinkPlacesKernel<<<static_cast<uint32_t>(blocks < 4096 ? blocks : 4096), kThreads, 0, s>>>(l);

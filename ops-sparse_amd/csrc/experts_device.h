@@ -99,6 +99,16 @@ __device__ __forceinline__ float WaveMax(float x)
     })));
 }
 
+// Workgroups of 256 threads in two dimensions where one would not take them
+// (fewer than 2^32 threads), and the number of each; those past the last do nothing.
+inline dim3 GridOf(int64_t blocks)
+{
+    constexpr int64_t kRow = int64_t{1} << 23;
+    return blocks <= kRow ? dim3(static_cast<uint32_t>(blocks))
+                          : dim3(static_cast<uint32_t>(kRow), static_cast<uint32_t>((blocks + kRow - 1) / kRow));
+}
+__device__ __forceinline__ uint32_t BlockNumber() { return blockIdx.y * gridDim.x + blockIdx.x; }
+
 // Rows [begin, end) of a group, whatever the offsets hold: within [0, rows] and not negative in length.
 __device__ __forceinline__ void GroupRows(const int32_t* offsets, int64_t rows, int group, int32_t& begin, int32_t& end)
 {

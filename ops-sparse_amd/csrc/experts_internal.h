@@ -17,8 +17,14 @@ constexpr int64_t kMaxRouteK = 64;
 // 2^14 * 131071 < 2^31.
 constexpr int64_t kMaxScaledK = 131071;
 
-// What a launcher returns when a grid would not fit 31 bits.
+// What a launcher returns when a grid would not fit.  Its workgroups are
+// numbered in 31 bits, and along a dimension it has fewer than 2^32 threads: a
+// larger one is launched without an error, with its size cut to 32 bits.
 constexpr int kTooLarge = 1;
+inline bool GridFits(int64_t blocks, int64_t threads)
+{
+    return blocks <= INT32_MAX && blocks * threads <= UINT32_MAX;
+}
 
 struct RouteLaunch {
     int64_t tokens, experts, k;

@@ -275,7 +275,7 @@ __global__ __launch_bounds__(256) void RouteGradKernel(RouteGradLaunch p)
 {
     __shared__ float rows[4][V * 64];
     const int lane = threadIdx.x & 63;
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int64_t t = static_cast<int64_t>(BlockNumber()) * 4 + (threadIdx.x >> 6);
     if (t >= p.tokens) return;  // whole waves
     float* row = rows[threadIdx.x >> 6];
     const int experts = static_cast<int>(p.experts), k = static_cast<int>(p.k);
@@ -347,7 +347,7 @@ int RouteTyped(const RouteLaunch& l, hipStream_t s)
 template <typename T, int V>
 int RouteGradTyped(const RouteGradLaunch& l, hipStream_t s)
 {
-    RouteGradKernel<T, V><<<static_cast<uint32_t>((l.tokens + 3) / 4), 256, 0, s>>>(l);
+    RouteGradKernel<T, V><<<GridOf((l.tokens + 3) / 4), 256, 0, s>>>(l);
     return 0;
 }
 

@@ -986,7 +986,7 @@ int LaunchTiles(const GroupedLaunch& l, hipStream_t s)
     const int64_t tilesN = CeilDiv(l.n, 256);
     // a die may cut the tiles of its last round into four
     const int64_t grid = CeilDiv(MaxRowTiles(l.offsets, l.rows, l.groups, kTileRows) * tilesN, 8) * 8 + 8 * CusPerDie();
-    if (grid > INT32_MAX) return kTooLarge;
+    if (!GridFits(grid, 512)) return kTooLarge;
     GroupedTileKernel<T, TOut, kBTrans>
         <<<static_cast<uint32_t>(grid), 512, 0, s>>>(l, static_cast<int32_t>(tilesN), CusPerDie());
     return 0;
@@ -997,7 +997,7 @@ int LaunchSmallTiles(const GroupedLaunch& l, hipStream_t s)
 {
     const int64_t tilesN = CeilDiv(l.n, 128);
     const int64_t grid = CeilDiv(MaxRowTiles(l.offsets, l.rows, l.groups, 64) * tilesN, 8) * 8;
-    if (grid > INT32_MAX) return kTooLarge;
+    if (!GridFits(grid, kTeams * 256)) return kTooLarge;
     GroupedSmallTileKernel<T, TOut, kBTrans, kAligned, kTeams>
         <<<static_cast<uint32_t>(grid), kTeams * 256, 0, s>>>(l, static_cast<int32_t>(tilesN));
     return 0;
@@ -1010,7 +1010,7 @@ int LaunchRows(const GroupedLaunch& l, hipStream_t s)
     // the row tiles of a group then read a column's weights on one die, whose L2 holds them
     const int64_t tilesN = CeilDiv(CeilDiv(l.n, NT * 16), 8) * 8;
     const int64_t grid = MaxRowTiles(l.offsets, l.rows, l.groups, MT * 16) * tilesN;
-    if (grid > INT32_MAX) return kTooLarge;
+    if (!GridFits(grid, kWaves * 64)) return kTooLarge;
     GroupedRowsKernel<T, TOut, kAligned, MT, NT, kWaves>
         <<<static_cast<uint32_t>(grid), kWaves * 64, 0, s>>>(l, static_cast<int32_t>(tilesN));
     return 0;
@@ -1027,8 +1027,9 @@ int GroupedBySize(const GroupedLaunch& l, hipStream_t s)
         // tiles: 4096x4096 with 1 row 10 / 38, with 32 19 / 39, with 64 21 (32 rows a time; 33 with 16) / 41.
         const bool few = l.rows <= 6 * l.groups || (l.rows <= 64 * l.groups && smallTiles <= cus / 4);
         if (few && l.k * static_cast<int64_t>(sizeof(T)) <= INT32_MAX / 2) {
-            return l.rows <= 6 * l.groups || l.rows <= 32 ? LaunchRows<T, TOut, kAligned, 1, 1>(l, s)
-                                                          : LaunchRows<T, TOut, kAligned, 2, 2>(l, s);
+            const int rc = l.rows <= 6 * l.groups || l.rows <= 32 ? LaunchRows<T, TOut, kAligned, 1, 1>(l, s)
+                                                                  : LaunchRows<T, TOut, kAligned, 2, 2>(l, s);
+            if (rc != kTooLarge) return rc;  // wider tiles may still fit
         }
     }
     // 256x256 tiles / 64x128 ones: 32 groups of 2048x2048 with 128 rows each 97 / 90 us, with 160 96 / 97, with 256
@@ -1066,6 +1067,7 @@ int LaunchGradTiles(const GroupedGradLaunch& l, hipStream_t s)
     const int64_t tilesN = CeilDiv(l.n, MI * WM * 16), tilesK = CeilDiv(l.k, NI * WN * 16);
     if (tilesN * tilesK + 7 > INT32_MAX / l.groups) return kTooLarge;
     const int64_t grid = CeilDiv(tilesN * tilesK, 8) * 8 * l.groups;
+    if (!GridFits(grid, kThreads)) return kTooLarge;
     const auto kernel = l.row_index != nullptr
                             ? GroupedGradTileKernel<T, TOut, true, kAligned, kTeams, kPlacesA, MI, NI, WM, WN>
                             : GroupedGradTileKernel<T, TOut, false, kAligned, kTeams, kPlacesA, MI, NI, WM, WN>;

@@ -142,6 +142,18 @@ def test_more_groups_than_a_scan_can_count_are_refused(lib, handle, name, args):
             == UNSUPPORTED, groups
 
 
+def test_grids_of_too_many_threads_are_refused(lib, handle):
+    # a grid's dimension takes fewer than 2^32 threads: these need more workgroups than that, though fewer than 2^31
+    for name, args in (
+            ("aclsparseGroupedMM", grouped(groups=2**18, rows=2**18, rows_a=2**18, n=2**14, ldc=2**14)),
+            ("aclsparseGroupedMM", grouped(op=NN, groups=2**18, rows=2**18, rows_a=2**18, n=2**14, ldb=2**14, ldc=2**14)),
+            ("aclsparseGroupedMM", grouped(groups=2, rows=2**25, rows_a=2**25, n=2**14, ldc=2**14)),
+            ("aclsparseGroupedMMScaled", scaled(groups=2**18, rows=2**18, rows_a=2**18, n=2**14, ldc=2**14)),
+            ("aclsparseGroupedMMGrad", grad(groups=2**10, n=2**17, k=2**13, ldg=2**17, ldx=2**13, ldw=2**13,
+                                            stride=2**30))):
+        assert getattr(lib, name)(handle, *args) == UNSUPPORTED, (name, args)
+
+
 def combine_grad_any(**kw):
     a = dict(tokens=4, k=2, width=8, rows=8, places=P, weights=P, y=P, ldy=8, go=P, ldo=8, type=F16, gy=P, ldgy=8, gw=P,
              buffer=P)

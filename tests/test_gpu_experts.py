@@ -788,6 +788,65 @@ def test_offsets_past_32_bits(dev):
     assert bool((out == 2.0).all())
 
 
+# Grids of more threads than one dimension takes (2^32): tokens or assignments by the million.
+
+
+@pytest.mark.parametrize("tokens,width", [(2**24 + 9, 3), (2**20, 4097)])
+def test_combine_of_many_tokens(dev, tokens, width):
+    y = torch.randn(64, width, generator=gen(1), device=dev).to(F16)
+    places = torch.randint(0, 64, (tokens, 1), generator=gen(2), device=dev, dtype=torch.int32)
+    out = combine(y, ExpertPlan(torch.tensor([0, 64], dtype=torch.int32, device=dev), None, places))
+    step = 2**17
+    for first in range(0, tokens, step):
+        assert torch.equal(out[first:first + step], y[places[first:first + step, 0].long()])
+
+
+def test_combine_gradient_of_many_assignments(dev):
+    tokens, k = 2**20 + 3, 64
+    places = torch.arange(tokens * k - 1, -1, -1, dtype=torch.int32, device=dev).view(tokens, k)
+    plan = ExpertPlan(torch.tensor([0, tokens * k], dtype=torch.int32, device=dev), None, places)
+    y = torch.randn(tokens * k, 1, generator=gen(1), device=dev).to(F16).requires_grad_(True)
+    weights = torch.randn(tokens, k, generator=gen(2), device=dev).requires_grad_(True)
+    grad = torch.randn(tokens, 1, generator=gen(3), device=dev).to(F16)
+    dy, dw = torch.autograd.grad(combine(y, plan, weights), (y, weights), grad)
+    # one product each, of two fp16 numbers exact in fp32
+    assert torch.equal(dw, y.detach().float().flip(0).view(tokens, k) * grad.float())
+    want = (weights.detach().double() * grad.double()).view(-1, 1).flip(0)
+    close(dy, want, want.abs(), 1)
+
+
+@pytest.mark.parametrize("normalize", [True, False])
+def test_route_gradient_of_many_tokens(dev, normalize):
+    tokens = 2**26 + 5
+    logits = torch.randn(tokens, 2, generator=gen(1), device=dev).requires_grad_(True)
+    weights, ids, _ = route(logits, 1 + normalize, normalize=normalize)
+    grad = torch.zeros_like(weights)
+    grad[:, 0] = 1.0
+    got, = torch.autograd.grad(weights, logits, grad)
+    step = 2**22
+    for first in range(0, tokens, step):
+        part = slice(first, first + step)
+        p = torch.softmax(logits.detach()[part].double(), 1)
+        top = p.argmax(1, keepdim=True)
+        assert torch.equal(top, ids[part, :1].long())
+        # p (1 - p) of the first choice, and its negative: each factor to a few roundings
+        want = torch.full_like(p, -1.0).scatter_(1, top, 1.0) * p[:, :1] * p[:, 1:]
+        assert bool(((got[part].double() - want).abs() <= 64 * U32 * p.gather(1, top)).all())
+
+
+def test_scaled_of_many_columns(dev):
+    n, k = 2**28 + 5, 16
+    a = torch.randint(-127, 128, (1, k), generator=gen(1), device=dev, dtype=torch.int8)
+    w = torch.randint(-127, 128, (n, k), generator=gen(2), device=dev, dtype=torch.int8)
+    sw = torch.rand(n, generator=gen(3), device=dev)
+    y = grouped_mm_scaled(a, torch.ones(1, device=dev), w, sw, out_dtype=F32)
+    step = 2**24
+    for first in range(0, n, step):
+        part = slice(first, first + step)
+        # integers below 2^24: exact in fp32, as is 1 * sw; one rounding
+        assert torch.equal(y[0, part], (w[part].float() * a.float()).sum(1) * sw[part])
+
+
 # ------------------------------------------------------------------------------------------------------- refusals
 
 

@@ -331,6 +331,19 @@ void CheckPlan(const Tensor& a, const Tensor& offsets, const Tensor& tokens, int
     TORCH_CHECK_VALUE(offsets.size(0) == groups + 1, "the plan has ", offsets.size(0) - 1, " experts, w ", groups);
 }
 
+// The rows of a that the plan reads: one per sorted row or, with gather, per token.  More are rows of no expert, or
+// tokens that nothing names.
+void CheckRows(const Tensor& a, const optional<Tensor>& tokens, const optional<Tensor>& places, bool gather)
+{
+    if (gather) {
+        TORCH_CHECK_VALUE(!places.has_value() || places->dim() != 2 || a.size(0) >= places->size(0), "a has ",
+                          a.size(0), " rows, the plan ", places->size(0), " tokens");
+    } else {
+        TORCH_CHECK_VALUE(!tokens.has_value() || a.size(0) >= tokens->numel(), "a has ", a.size(0),
+                          " rows, the plan ", tokens->numel(), " (gather takes a in the order of the tokens)");
+    }
+}
+
 Tensor GroupedMM(const Tensor& a, const Tensor& w, const Tensor& planOffsets, const optional<Tensor>& planTokens,
                  const optional<Tensor>& planPlaces, bool gather)
 {
@@ -344,6 +357,7 @@ Tensor GroupedMM(const Tensor& a, const Tensor& w, const Tensor& planOffsets, co
     const Tensor offsets = Index(planOffsets, "offsets");
     const Tensor tokens = gather ? Index(*planTokens, "tokens") : Tensor();
     CheckPlan(a, offsets, tokens, w.size(0));
+    CheckRows(a, planTokens, planPlaces, gather);
     const Tensor ra = Rows(a), rw = Rows(w);
     if (!Tracked(a, w)) {
         return RunGrouped(ACL_SPARSE_OP_TRANSPOSE, ra, rw, offsets, tokens, gather ? tokens.size(0) : ra.size(0),
@@ -361,8 +375,8 @@ Tensor GroupedMM(const Tensor& a, const Tensor& w, const Tensor& planOffsets, co
 }
 
 Tensor GroupedMMScaled(const Tensor& a, const Tensor& aScale, const Tensor& wGiven, const Tensor& wScaleGiven,
-                       const optional<Tensor>& planOffsets, const optional<Tensor>& planTokens, bool gather,
-                       at::ScalarType type)
+                       const optional<Tensor>& planOffsets, const optional<Tensor>& planTokens,
+                       const optional<Tensor>& planPlaces, bool gather, at::ScalarType type)
 {
     Tensor w = wGiven, wScale = wScaleGiven, offsets, tokens;
     if (!planOffsets.has_value()) {
@@ -390,6 +404,7 @@ Tensor GroupedMMScaled(const Tensor& a, const Tensor& aScale, const Tensor& wGiv
         offsets = Index(*planOffsets, "offsets");
         if (gather) tokens = Index(*planTokens, "tokens");
         CheckPlan(a, offsets, tokens, w.size(0));
+        CheckRows(a, planTokens, planPlaces, gather);
     }
     const Tensor ra = Rows(a), rw = Rows(w), sa = aScale.contiguous(), sw = wScale.contiguous();
     const int64_t rows = gather ? tokens.size(0) : ra.size(0), n = rw.size(1);

@@ -83,7 +83,9 @@ def grouped_mm(a, w, plan, gather=False):
     """y [R, N]: y[r] = w[e] @ a[r] for the rows r of each expert e, rows past the last expert's zero (differentiable).
 
     w [E, N, K], fp16 or bf16 (any strides whose last is 1 avoid a copy); a of its type: [R, K] in the plan's row
-    order or, with ``gather``, [T, K] in token order: row r then reads a[plan.tokens[r]].  Sums are in fp32.
+    order or, with ``gather``, [T, K] in token order: row r then reads a[plan.tokens[r]].  An a of fewer rows than the
+    plan's tokens (with ``gather``, places) is refused, more are no expert's; a plan of offsets alone takes any R.
+    Sums are in fp32.
     """
     return (_MODULE or _module()).grouped_mm(a, w, plan.offsets, plan.tokens, plan.places, gather)
 
@@ -93,8 +95,8 @@ def grouped_mm_scaled(a, a_scale, w, w_scale, plan=None, gather=False, out_dtype
     row of a that row r reads.  a int8, a_scale [rows of a] fp32, w [E, N, K] int8, w_scale [E, N] fp32; with no plan
     one dense product, w [N, K] and w_scale [N].  K <= 131071, so that the sum stays within 32 bits.  No gradient.
     """
-    offsets, tokens, _ = plan if plan is not None else (None, None, None)
-    return (_MODULE or _module()).grouped_mm_scaled(a, a_scale, w, w_scale, offsets, tokens, gather, out_dtype)
+    offsets, tokens, places = plan if plan is not None else (None, None, None)
+    return (_MODULE or _module()).grouped_mm_scaled(a, a_scale, w, w_scale, offsets, tokens, places, gather, out_dtype)
 
 
 def combine(y, plan, weights=None):

@@ -891,3 +891,25 @@ def test_refusals(dev):
         with pytest.raises(error):
             call()
     torch.cuda.synchronize()
+
+
+def test_operands_of_fewer_rows_than_the_plan_are_refused(dev):
+    tokens, experts, k = 20, 4, 2
+    plan = expert_plan(routed(tokens, experts, k, 1), experts)
+    x, w = torch.ones(tokens, 16, dtype=F16, device=dev), torch.ones(experts, 8, 16, dtype=F16, device=dev)
+    x8, w8, one = x.to(torch.int8), w.to(torch.int8), torch.ones(tokens, device=dev)
+    sw = torch.ones(experts, 8, device=dev)
+    for call in (lambda: grouped_mm(x, w, plan),  # gather forgotten
+                 lambda: grouped_mm(x.clone().requires_grad_(True), w, plan),
+                 lambda: grouped_mm(x[:-1], w, plan, gather=True),
+                 lambda: grouped_mm_scaled(x8, one, w8, sw, plan),
+                 lambda: grouped_mm_scaled(x8[:-1], one[:-1], w8, sw, plan, gather=True)):
+        with pytest.raises(ValueError, match="rows"):
+            call()
+    # more of them are none of the plan's: rows of no expert, which are zero, or tokens that nothing names
+    more = torch.ones(tokens * k + 3, 16, dtype=F16, device=dev)
+    y = grouped_mm(more, w, plan)
+    assert y.shape[0] == tokens * k + 3 and bool((y[:-3] == 16).all()) and not y[-3:].any()
+    assert bool((grouped_mm(more, w, plan, gather=True) == 16).all())
+    y = grouped_mm_scaled(more.to(torch.int8), torch.ones(len(more), device=dev), w8, sw, plan)
+    assert bool((y[:-3] == 16).all()) and not y[-3:].any()

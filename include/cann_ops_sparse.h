@@ -419,10 +419,11 @@ aclsparseStatus_t aclsparseRouteGrad(aclsparseHandle_t handle, int64_t tokens, i
                                      const float* weights, const int32_t* ids, const float* gradWeights,
                                      void* gradLogits, int64_t ldGrad);
 /* C_r = A_i(r) op(B_g) for the rows r in [offsets[g], offsets[g+1]) of every group g, i(r) = rowIndex[r] (rowIndex
- * null: i(r) = r), and C_r = 0 for rows past offsets[groups]; offsets null: one group of all rows.  op(B_g) is k x n:
+ * null: i(r) = r), and C_r = 0 for rows before offsets[0] or past offsets[groups] (so offsets may be a part of a longer
+ * list, with the B of its groups); offsets null: one group of all rows.  op(B_g) is k x n:
  * ACL_SPARSE_OP_NON_TRANSPOSE takes B_g [k, n], ACL_SPARSE_OP_TRANSPOSE takes B_g [n, k]; B_g starts strideB elements
- * after B_(g-1).  A and B ACL_FLOAT16 or ACL_BF16, C their type or ACL_FLOAT; sums in fp32.  offsets start at 0 and do
- * not decrease and indices lie in [0, rowsA): others give values without meaning, never an access outside the
+ * after B_(g-1).  A and B ACL_FLOAT16 or ACL_BF16, C their type or ACL_FLOAT; sums in fp32.  offsets do not
+ * decrease and indices lie in [0, rowsA): others give values without meaning, never an access outside the
  * operands.  groups, rows, n and k up to 2^31 - 4097. */
 aclsparseStatus_t aclsparseGroupedMM(aclsparseHandle_t handle, aclsparseOperation_t opB, int64_t groups, int64_t rows,
                                      int64_t n, int64_t k, const int32_t* offsets, const int32_t* rowIndex,

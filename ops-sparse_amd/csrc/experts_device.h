@@ -123,8 +123,8 @@ __device__ __forceinline__ void GroupRows(const int32_t* offsets, int64_t rows, 
     end = e < begin ? begin : e > r ? r : e;
 }
 
-// A tile of a ragged product: rows [row, end) of `group`; group == groups is
-// the tail of rows that belong to no group, group < 0 no tile.
+// A tile of a ragged product: rows [row, end) of `group`; group == groups are
+// the rows that belong to no group, group < 0 no tile.
 struct RaggedTile {
     int32_t group;
     int32_t row;
@@ -134,14 +134,15 @@ struct RaggedTile {
     int32_t tiles;   // and its own
 };
 
-// The tiles of `height` rows of all groups and then of the tail, for whole
+// The tiles of `height` rows of all groups, of the rows past the last and of
+// those before the first (offsets that are some of a longer list's), for whole
 // waves: 64 groups at a time, one per lane.  The first 64 are read once for
 // both the count and the search, which every workgroup waits for.
 struct RaggedTiles {
     const int32_t* offsets;
     int32_t rows, groups, height;
     int32_t begin, end, tiles, upTo;  // this lane's group of the first 64; upTo: tiles through it
-    int32_t tail;                     // its first row
+    int32_t head, tail;               // rows before the first group, and the first one past the last
     int32_t total;
 
     __device__ __forceinline__ int32_t Count(int32_t from, int32_t to) const
@@ -171,7 +172,8 @@ struct RaggedTiles {
             lastLane = (groups - g0 < 64 ? groups - g0 : 64) - 1;
         }
         tail = offsets != nullptr ? __builtin_amdgcn_readlane(last, lastLane) : rows;
-        total += Count(tail, rows);
+        head = offsets != nullptr ? __builtin_amdgcn_readlane(begin, 0) : 0;
+        total += Count(tail, rows) + Count(0, head);
         if (total < 0) total = 0;  // the sum of offsets without meaning
     }
 
@@ -195,9 +197,11 @@ struct RaggedTiles {
             }
             before += __builtin_amdgcn_readlane(through, 63);
         }
-        const int32_t n0 = Count(tail, rows);
-        if (tile - before >= n0) return {-1, 0, 0, 0, 0, 0};
-        return {groups, tail + (tile - before) * height, rows, tail, before, n0};
+        const int32_t past = Count(tail, rows), ahead = Count(0, head);
+        if (tile - before < past) return {groups, tail + (tile - before) * height, rows, tail, before, past};
+        before += past;
+        if (tile - before >= ahead) return {-1, 0, 0, 0, 0, 0};
+        return {groups, (tile - before) * height, head, 0, before, ahead};
     }
 };
 

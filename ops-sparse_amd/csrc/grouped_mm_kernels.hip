@@ -961,11 +961,11 @@ int64_t CeilDiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 bool Aligned16(const void* p, int64_t strideBytes) { return (reinterpret_cast<uintptr_t>(p) | strideBytes) % 16 == 0; }
 
-// The most tiles of `height` rows: every group, and the tail, may end inside one.
+// The most tiles of `height` rows: every group, and the rows on either side, may end inside one.
 int64_t MaxRowTiles(const int32_t* offsets, int64_t rows, int64_t groups, int64_t height)
 {
     if (offsets == nullptr) return CeilDiv(rows, height);
-    const int64_t most = rows / height + groups + 1;
+    const int64_t most = rows / height + groups + 2;
     return most < rows ? most : rows;
 }
 

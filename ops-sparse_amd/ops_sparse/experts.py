@@ -30,7 +30,8 @@ class ExpertPlan(NamedTuple):
 
     offsets [E + 1]: rows offsets[e] to offsets[e + 1] are expert e's; tokens [T * k]: the token of each row (-1
     past offsets[E]); places [T, k]: the row of each assignment, -1 for a dropped one.  ``tokens`` and ``places``
-    may be None where rows are grouped by other means: such a plan serves products that do not gather.  The gradient
+    may be None where rows are grouped by other means: such a plan serves products that do not gather.  Some of the
+    experts, a part of ``offsets`` with the ``w`` of those, have the others' rows as rows of no expert.  The gradient
     of a gathered operand goes by places: an assignment whose place is set to -1 afterwards has no part in it.
     """
     offsets: torch.Tensor
@@ -80,7 +81,7 @@ def expert_plan(ids, experts):
 
 
 def grouped_mm(a, w, plan, gather=False):
-    """y [R, N]: y[r] = w[e] @ a[r] for the rows r of each expert e, rows past the last expert's zero (differentiable).
+    """y [R, N]: y[r] = w[e] @ a[r] for the rows r of each expert e, rows of no expert zero (differentiable).
 
     w [E, N, K], fp16 or bf16 (any strides whose last is 1 avoid a copy); a of its type: [R, K] in the plan's row
     order or, with ``gather``, [T, K] in token order: row r then reads a[plan.tokens[r]].  An a of fewer rows than the

@@ -788,6 +788,40 @@ def test_offsets_past_32_bits(dev):
     assert bool((out == 2.0).all())
 
 
+@pytest.mark.parametrize("lens,first,last,n,k", [
+    ([2, 1, 0, 3, 2, 1], 2, 5, 64, 72), ([30, 0, 200, 77, 5, 64], 1, 4, 40, 33), ([900, 0, 700, 1100, 90, 300], 2, 5, 2304, 64),
+    ([5, 3, 4], 2, 3, 264, 136), ([(i * 7) % 5 for i in range(130)], 66, 130, 96, 128)])
+def test_rows_before_the_first_expert_are_zero(dev, lens, first, last, n, k):
+    # some of a plan's experts, as where they are spread over devices: the others' rows are no expert's
+    full, rows = lengths_to_plan(lens, tail=3)
+    offsets = full.offsets[first:last + 1]
+    lo, hi = int(offsets[0]), int(offsets[-1])
+    tokens = torch.randint(0, 50, (rows,), generator=gen(5), device=dev, dtype=torch.int32)
+    w = torch.randn(last - first, n, k, generator=gen(2), device=dev).to(BF16).requires_grad_(True)
+    w8 = torch.randint(-127, 128, w.shape, generator=gen(2), device=dev, dtype=torch.int8)
+    for plan, count in ((ExpertPlan(offsets), rows), (ExpertPlan(offsets, tokens), 50)):
+        gather = plan.tokens is not None
+        a = torch.randn(count, k, generator=gen(1), device=dev).to(BF16)
+        a.requires_grad_(not gather)
+        left = [torch.full(s, float("nan"), dtype=BF16, device=dev) for s in ((rows, n), (rows, k))]
+        del left  # what the allocator hands out next is not zeros
+        y = grouped_mm(a, w, plan, gather=gather)
+        close(y.detach(), *plain_grouped(a.detach(), w.detach(), plan, rows), k)
+        assert not y[:lo].any() and not y[hi:].any()
+        grad = torch.randn(rows, n, generator=gen(3), device=dev).to(BF16)
+        grads = torch.autograd.grad(y, (w,) if gather else (w, a), grad)
+        wa, ma, ww, mw = plain_grads(a.detach(), w.detach(), plan, grad)
+        close(grads[0], ww, mw, max(lens))
+        if not gather:
+            close(grads[1], wa, ma, n)
+        a8 = a.detach().mul(20).clamp(-127, 127).to(torch.int8)
+        one, sw = torch.ones(count, device=dev), torch.ones(last - first, n, device=dev)
+        left = torch.full((rows, n), float("nan"), device=dev)
+        del left
+        y8 = grouped_mm_scaled(a8, one, w8, sw, plan, gather=gather, out_dtype=F32)
+        scaled_close(y8, plain_scaled(a8, one, w8, sw, plan, rows))
+
+
 # Grids of more threads than one dimension takes (2^32): tokens or assignments by the million.
 
 

@@ -147,6 +147,13 @@ bool Tracked(const Tensor& a, const Tensor& b)
     return at::GradMode::is_enabled() && ((a.defined() && a.requires_grad()) || (b.defined() && b.requires_grad()));
 }
 
+// The kernels read a tensor's value alone: a tangent that it carries would pass for zero.
+void NoTangent(const Tensor& t)
+{
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(),
+                                "the experts' operators have no forward-mode derivative");
+}
+
 // Gradients come from kernels that autograd does not see: one that is itself
 // differentiated raises an error instead of passing for a constant.
 variable_list Once(variable_list grads)
@@ -212,6 +219,7 @@ struct RouteNode : torch::autograd::Function<RouteNode> {
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
         if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
+        NoTangent(grads[0]);
         const auto saved = ctx->get_saved_variables();
         const Tensor &logits = saved[0], &weights = saved[1], &ids = saved[2];
         const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt());
@@ -228,6 +236,7 @@ struct RouteNode : torch::autograd::Function<RouteNode> {
 
 variable_list Route(const Tensor& logits, int64_t k, bool normalize)
 {
+    NoTangent(logits);
     TORCH_CHECK_VALUE(logits.dim() == 2, "logits must be two-dimensional");
     TORCH_CHECK_TYPE(IsFloat(logits.scalar_type()), "logits must be float32, float16 or bfloat16, got ",
                      logits.scalar_type());
@@ -297,6 +306,7 @@ struct GroupedNode : torch::autograd::Function<GroupedNode> {
     {
         const auto saved = ctx->get_saved_variables();
         const Tensor &a = saved[0], &w = saved[1], &offsets = saved[2], &tokens = saved[3], &places = saved[4];
+        NoTangent(grads[0]);
         const Tensor grad = Rows(grads[0]);
         const int64_t rows = grad.size(0), groups = w.size(0), n = w.size(1), k = w.size(2);
         Tensor da, dw;
@@ -347,6 +357,8 @@ void CheckRows(const Tensor& a, const optional<Tensor>& tokens, const optional<T
 Tensor GroupedMM(const Tensor& a, const Tensor& w, const Tensor& planOffsets, const optional<Tensor>& planTokens,
                  const optional<Tensor>& planPlaces, bool gather)
 {
+    NoTangent(a);
+    NoTangent(w);
     TORCH_CHECK_VALUE(a.dim() == 2 && w.dim() == 3 && a.size(1) == w.size(2),
                       "a must be [rows, K] and w [experts, N, K], got ", a.sizes(), " and ", w.sizes());
     TORCH_CHECK_TYPE(IsHalf(a.scalar_type()) && w.scalar_type() == a.scalar_type(),
@@ -378,6 +390,8 @@ Tensor GroupedMMScaled(const Tensor& a, const Tensor& aScale, const Tensor& wGiv
                        const optional<Tensor>& planOffsets, const optional<Tensor>& planTokens,
                        const optional<Tensor>& planPlaces, bool gather, at::ScalarType type)
 {
+    NoTangent(aScale);
+    NoTangent(wScaleGiven);
     Tensor w = wGiven, wScale = wScaleGiven, offsets, tokens;
     if (!planOffsets.has_value()) {
         TORCH_CHECK_VALUE(!gather, "gather needs a plan");
@@ -433,6 +447,7 @@ struct CombineNode : torch::autograd::Function<CombineNode> {
     {
         const auto saved = ctx->get_saved_variables();
         const Tensor &y = saved[0], &weights = saved[1], &places = saved[2];
+        NoTangent(grads[0]);
         const Tensor grad = Rows(grads[0]);
         const int64_t tokens = places.size(0), k = places.size(1), rows = y.size(0), width = y.size(1);
         Call call(y);
@@ -455,6 +470,8 @@ struct CombineNode : torch::autograd::Function<CombineNode> {
 Tensor Combine(const Tensor& y, const Tensor& planOffsets, const optional<Tensor>& planPlaces,
                const optional<Tensor>& givenWeights)
 {
+    NoTangent(y);
+    if (givenWeights.has_value()) NoTangent(*givenWeights);
     TORCH_CHECK_VALUE(planPlaces.has_value() && planPlaces->dim() == 2,
                       "combine needs the plan's places, [tokens, k]");
     TORCH_CHECK_VALUE(y.dim() == 2, "y must be [rows, width]");

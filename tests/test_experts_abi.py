@@ -210,3 +210,22 @@ def test_cpu_tensors_are_refused():
                                                       torch.ones(8))):
         with pytest.raises(ValueError, match="ROCm device"):
             call()
+
+
+def test_forward_mode_is_refused():
+    # before the device is looked at, so tensors of the host show it
+    i = torch.zeros(4, 2, dtype=torch.int32)
+    p = ops_sparse.ExpertPlan(torch.zeros(3, dtype=torch.int32), torch.zeros(8, dtype=torch.int32), i)
+    h, w = torch.zeros(8, 16, dtype=torch.float16), torch.zeros(2, 8, 16, dtype=torch.float16)
+    one, logits = torch.ones(8), torch.zeros(4, 8)
+    with torch.autograd.forward_ad.dual_level():
+        def dual(t):
+            return torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+
+        for call in (lambda: ops_sparse.route(dual(logits), 2), lambda: ops_sparse.grouped_mm(dual(h), w, p),
+                     lambda: ops_sparse.grouped_mm(h, dual(w), p), lambda: ops_sparse.combine(dual(h), p),
+                     lambda: ops_sparse.combine(h, p, dual(torch.ones(4, 2))),
+                     lambda: ops_sparse.grouped_mm_scaled(h.to(torch.int8), dual(one), w[0].to(torch.int8), one),
+                     lambda: ops_sparse.grouped_mm_scaled(h.to(torch.int8), one, w[0].to(torch.int8), dual(one))):
+            with pytest.raises(NotImplementedError, match="forward"):
+                call()

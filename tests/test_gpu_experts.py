@@ -494,6 +494,28 @@ def test_results_are_differentiable_once(dev):
         grad.sum().backward()
 
 
+def test_forward_mode_is_refused(dev):
+    plan = expert_plan(routed(6, 3, 2, 1), 3)
+    x, w = torch.ones(6, 8, dtype=F16, device=dev), torch.ones(3, 8, 8, dtype=F16, device=dev)
+    y, weights = torch.ones(12, 8, dtype=F16, device=dev), torch.ones(6, 2, device=dev)
+    logits = torch.randn(6, 3, generator=gen(1), device=dev)
+    with torch.autograd.forward_ad.dual_level():
+        def dual(t):
+            return torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+
+        for call in (lambda: route(dual(logits), 2), lambda: grouped_mm(dual(x), w, plan, gather=True),
+                     lambda: grouped_mm(x, dual(w), plan, gather=True), lambda: combine(dual(y), plan),
+                     lambda: combine(y, plan, dual(weights))):
+            with pytest.raises(NotImplementedError, match="forward"):
+                call()
+        # and of a gradient: the tangent of what comes in
+        for out, leaf in ((combine(y.requires_grad_(True), plan), y),
+                          (grouped_mm(x.requires_grad_(True), w, plan, gather=True), x),
+                          (route(logits.requires_grad_(True), 2)[0], logits)):
+            with pytest.raises(NotImplementedError, match="forward"):
+                torch.autograd.grad(out, leaf, dual(torch.ones_like(out)))
+
+
 # ------------------------------------------------------------------------------------------------------- 8 bits
 
 

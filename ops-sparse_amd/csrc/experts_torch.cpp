@@ -10,7 +10,6 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include "cann_ops_sparse.h"
@@ -154,18 +153,47 @@ void NoTangent(const Tensor& t)
                                 "the experts' operators have no forward-mode derivative");
 }
 
-// Gradients come from kernels that autograd does not see: one that is itself
-// differentiated raises an error instead of passing for a constant.
-variable_list Once(variable_list grads)
-{
-    if (!at::GradMode::is_enabled()) return grads;
-    for (auto& g : grads) {
-        if (g.defined()) g = g.detach().requires_grad_(true);
+// Results that autograd did not see being made of `inputs`: a derivative through them to any of those raises `message`,
+// where a tensor without a node would pass for a constant.  (A node without edges to the inputs would not do: the
+// engine skips it where a derivative with respect to given tensors is asked for.)
+struct Results {
+    variable_list tensors;
+};
+struct UndifferentiableNode : torch::autograd::Function<UndifferentiableNode> {
+    using Input = optional<Tensor>;
+    static variable_list forward(AutogradContext* ctx, const Input&, const Input&, const Input&, const Results& results,
+                                 const std::string& message)
+    {
+        ctx->saved_data["message"] = message;
+        return results.tensors;
     }
-    const int count = static_cast<int>(grads.size());
-    auto error = std::make_shared<torch::autograd::DelayedError>(
-        "the experts' operators are differentiable once; their gradients are not", count);
-    return (*error)(std::move(grads));
+    static variable_list backward(AutogradContext* ctx, variable_list)
+    {
+        TORCH_CHECK(false, ctx->saved_data["message"].toStringRef());
+    }
+};
+variable_list Undifferentiable(const std::array<Tensor, 3>& inputs, variable_list results, const char* message)
+{
+    if (!at::GradMode::is_enabled()) return results;
+    auto input = [&](int i) { return inputs[i].defined() ? optional<Tensor>(inputs[i]) : std::nullopt; };
+    variable_list defined;
+    for (const auto& t : results) {
+        if (t.defined()) defined.push_back(t);
+    }
+    const variable_list made =
+        UndifferentiableNode::apply(input(0), input(1), input(2), Results{defined}, std::string(message));
+    size_t next = 0;
+    for (auto& t : results) {
+        if (t.defined()) t = made[next++];
+    }
+    return results;
+}
+
+// Gradients, of what comes in and of what the forward call kept.
+variable_list Once(const std::array<Tensor, 3>& inputs, variable_list grads)
+{
+    return Undifferentiable(inputs, std::move(grads),
+                            "the experts' operators are differentiable once; their gradients are not");
 }
 
 // ------------------------------------------------------------------ routing
@@ -230,7 +258,7 @@ struct RouteNode : torch::autograd::Function<RouteNode> {
         Call::Ok(lib.routeGrad(call, tokens, experts, k, Data(logits), logits.defined() ? Ld(logits) : 0, TypeOf(type),
                                !logits.defined(), Floats(weights), Ints(ids), Floats(grad), Data(out), experts),
                  "aclsparseRouteGrad");
-        return Once({out, Tensor(), Tensor()});
+        return Once({grads[0], logits, weights}, {out, Tensor(), Tensor()});
     }
 };
 
@@ -328,7 +356,7 @@ struct GroupedNode : torch::autograd::Function<GroupedNode> {
                                        Ld(grad), Data(a), Ld(a), type, Data(dw), std::max<int64_t>(k, 1), n * k, type),
                      "aclsparseGroupedMMGrad");
         }
-        return Once({da, dw, Tensor()});
+        return Once({grads[0], a, w}, {da, dw, Tensor()});
     }
 };
 
@@ -463,7 +491,7 @@ struct CombineNode : torch::autograd::Function<CombineNode> {
                                  Data(grad), Ld(grad), TypeOf(y.scalar_type()), Data(dy), std::max<int64_t>(width, 1),
                                  Floats(dw), Data(buffer)),
                  "aclsparseCombineGradAny");
-        return Once({dy, dw, Tensor()});
+        return Once({grads[0], y, weights}, {dy, dw, Tensor()});
     }
 };
 

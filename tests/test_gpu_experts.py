@@ -494,6 +494,26 @@ def test_results_are_differentiable_once(dev):
         grad.sum().backward()
 
 
+def test_second_derivatives_with_respect_to_given_tensors_raise(dev):
+    # the engine runs the nodes on the way to these alone: the second derivative's has to be one of them
+    plan = expert_plan(routed(6, 3, 2, 1), 3)
+    x = torch.randn(6, 8, generator=gen(1), device=dev).to(F16).requires_grad_(True)
+    w = torch.randn(3, 8, 8, generator=gen(2), device=dev).to(F16).requires_grad_(True)
+    y = torch.randn(12, 8, generator=gen(3), device=dev).to(F16).requires_grad_(True)
+    weights = torch.rand(6, 2, generator=gen(4), device=dev).requires_grad_(True)
+    logits = torch.randn(6, 3, generator=gen(5), device=dev).requires_grad_(True)
+    for make, leaves in ((lambda: route(logits, 2)[0], (logits,)), (lambda: route(logits, 2, False)[0], (logits,)),
+                         (lambda: grouped_mm(x, w, plan, gather=True), (x, w)),
+                         (lambda: combine(y, plan, weights), (y, weights))):
+        out = (make().float() ** 2).sum()
+        grads = torch.autograd.grad(out, leaves, create_graph=True)
+        for g in grads:
+            with pytest.raises(RuntimeError, match="differentiable once"):
+                torch.autograd.grad((g.float() ** 2).sum() + out, leaves, retain_graph=True)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            sum((g.float() ** 2).sum() for g in grads).backward(retain_graph=True)
+
+
 def test_forward_mode_is_refused(dev):
     plan = expert_plan(routed(6, 3, 2, 1), 3)
     x, w = torch.ones(6, 8, dtype=F16, device=dev), torch.ones(3, 8, 8, dtype=F16, device=dev)

@@ -457,7 +457,8 @@ Tensor GroupedMMScaled(const Tensor& a, const Tensor& aScale, const Tensor& wGiv
                                  static_cast<const int8_t*>(Data(rw)), Ld(rw), rw.size(0) > 1 ? rw.stride(0) : 0,
                                  Floats(sw), Data(out), std::max<int64_t>(n, 1), TypeOf(type)),
              "aclsparseGroupedMMScaled");
-    return out;
+    return Tracked(aScale, wScale) ? Undifferentiable({aScale, wScale}, {out}, "grouped_mm_scaled has no gradient")[0]
+                                   : out;
 }
 
 // ------------------------------------------------------------------ combination

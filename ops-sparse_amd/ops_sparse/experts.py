@@ -94,7 +94,8 @@ def grouped_mm(a, w, plan, gather=False):
 def grouped_mm_scaled(a, a_scale, w, w_scale, plan=None, gather=False, out_dtype=torch.bfloat16):
     """:func:`grouped_mm` of 8-bit integers: y[r, n] = a_scale[i] * w_scale[e, n] * (the exact integer product), i the
     row of a that row r reads.  a int8, a_scale [rows of a] fp32, w [E, N, K] int8, w_scale [E, N] fp32; with no plan
-    one dense product, w [N, K] and w_scale [N].  K <= 131071, so that the sum stays within 32 bits.  No gradient.
+    one dense product, w [N, K] and w_scale [N].  K <= 131071, so that the sum stays within 32 bits.  No gradient:
+    one asked for through the scales raises RuntimeError.
     """
     offsets, tokens, places = plan if plan is not None else (None, None, None)
     return (_MODULE or _module()).grouped_mm_scaled(a, a_scale, w, w_scale, offsets, tokens, places, gather, out_dtype)

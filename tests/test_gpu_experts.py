@@ -596,6 +596,22 @@ def test_scaled_extremes(dev):
                           torch.zeros(5, 131072, dtype=torch.int8, device=dev), one)
 
 
+@pytest.mark.parametrize("of", ["a_scale", "w_scale", "both"])
+def test_scales_that_ask_for_a_gradient_get_an_error(dev, of):
+    a, w = strided((5, 32), torch.int8, 1, 0), strided((8, 32), torch.int8, 2, 0)
+    sa, sw = torch.rand(5, generator=gen(3), device=dev), torch.rand(8, generator=gen(4), device=dev)
+    want = grouped_mm_scaled(a, sa, w, sw)
+    asked = [s.requires_grad_(True) for s, name in ((sa, "a_scale"), (sw, "w_scale")) if of in (name, "both")]
+    with torch.no_grad():
+        y = grouped_mm_scaled(a, sa, w, sw)
+        assert not y.requires_grad and torch.equal(y, want)
+    y = grouped_mm_scaled(a, sa, w, sw)
+    assert torch.equal(y.detach(), want)
+    # beside a part that has a gradient, without which torch itself would raise
+    with pytest.raises(RuntimeError, match="no gradient"):
+        torch.autograd.grad(y.float().sum() + sum(s.sum() for s in asked), asked)
+
+
 # ------------------------------------------------------------------------------------------------------- combination
 
 

@@ -3,6 +3,9 @@
 No call here reaches a kernel launch: each fails its checks, sizes a buffer, or has nothing to do.
 """
 import ctypes
+import re
+import shutil
+import subprocess
 
 import pytest
 import torch
@@ -229,3 +232,31 @@ def test_forward_mode_is_refused():
                      lambda: ops_sparse.grouped_mm_scaled(h.to(torch.int8), one, w[0].to(torch.int8), dual(one))):
             with pytest.raises(NotImplementedError, match="forward"):
                 call()
+
+
+def other_uses_of_m0(lines):
+    """Lines that name m0, but those that set it for the copy to LDS right behind them."""
+    found = []
+    for i, line in enumerate(lines):
+        if re.search(r"\bm0\b", line):
+            copy = (re.fullmatch(r"s_mov_b32 m0, s\d+", line) and lines[i + 1] == "s_nop 0"
+                    and lines[i + 2].startswith("global_load_lds_dwordx4 "))
+            if not copy:
+                found.append(line)
+    return found
+
+
+def test_the_copies_to_lds_are_the_only_use_of_m0(tmp_path):
+    # The grouped products set m0 in assembly that cannot say so: it is a reserved register, whose clobber the compiler
+    # does not heed.  That holds as long as the compiler itself needs m0 nowhere in their code.
+    tool = "/opt/rocm/llvm/bin/llvm-objdump"
+    shutil.copy(_lib.LIB_PATH, tmp_path / "lib.so")
+    subprocess.run([tool, "--offloading", "lib.so"], cwd=tmp_path, check=True, capture_output=True)
+    images = [f for f in tmp_path.iterdir() if f.name.endswith("gfx950") and b"GroupedTileKernel" in f.read_bytes()]
+    assert len(images) == 1
+    text = subprocess.run([tool, "-d", "--no-show-raw-insn", images[0].name], cwd=tmp_path, check=True,
+                          capture_output=True, text=True).stdout
+    lines = [line.split("//")[0].strip() for line in text.splitlines()]
+    assert sum(line.startswith("global_load_lds_dwordx4 ") for line in lines) > 100
+    assert other_uses_of_m0(lines) == []
+    assert other_uses_of_m0(lines + ["s_mov_b32 m0, -1", "ds_read_b32 v0, v1", ""]) == ["s_mov_b32 m0, -1"]

@@ -85,8 +85,18 @@ def torch_module_command(bid):
             "-ltorch", "-ltorch_python", "-ldl", "-o", TORCH_OUT + ".tmp"]
 
 
+def has_torch():
+    import importlib.util
+
+    try:
+        return importlib.util.find_spec("torch") is not None
+    except ValueError:  # a module set to None
+        return False
+
+
 def build_library(verbose=False):
-    """Compiles every source to an object in parallel (ops-sparse_amd/lib/obj), then links; the torch module beside them."""
+    """Compiles every source to an object in parallel (ops-sparse_amd/lib/obj), then links; the torch module beside them,
+    where there is torch to compile it against."""
     from concurrent.futures import ThreadPoolExecutor
 
     os.makedirs(OBJ_DIR, exist_ok=True)
@@ -101,21 +111,22 @@ def build_library(verbose=False):
     def run(cmd):
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
-            raise RuntimeError("hipcc failed:\n" + " ".join(cmd) + "\n" + res.stdout + res.stderr)
+            raise RuntimeError("the compiler failed:\n" + " ".join(cmd) + "\n" + res.stdout + res.stderr)
         return cmd
 
     with ThreadPoolExecutor(max_workers=min(len(cmds) + 1, 8)) as ex:
-        module = ex.submit(run, torch_module_command(bid))
+        module = ex.submit(run, torch_module_command(bid)) if has_torch() else None
         for cmd in ex.map(run, cmds):
             if verbose:
                 print(" ".join(cmd))
-        module.result()
-    os.replace(TORCH_OUT + ".tmp", TORCH_OUT)
-    link = ["hipcc", *HIPCC_FLAGS, *[c[-1] for c in cmds], "-o", OUT + ".tmp"]
-    run(link)
-    os.replace(OUT + ".tmp", OUT)
-    if verbose:
-        print(" ".join(link))
+        link = ["hipcc", *HIPCC_FLAGS, *[c[-1] for c in cmds], "-o", OUT + ".tmp"]
+        run(link)
+        os.replace(OUT + ".tmp", OUT)
+        if verbose:
+            print(" ".join(link))
+        if module is not None:
+            module.result()
+            os.replace(TORCH_OUT + ".tmp", TORCH_OUT)
     return OUT
 
 

@@ -828,6 +828,109 @@ def test_hip_graph_capture_and_replay(dev):
         assert torch.equal(out, layer())
 
 
+def layer_step(logits, x, w, v, k):
+    """A layer and its gradients, of leaves that ask for them."""
+    weights, _, plan = route(logits, k)
+    out = combine(grouped_mm(grouped_mm(x, w, plan, gather=True), v, plan), plan, weights)
+    return (out.detach(),) + torch.autograd.grad(out, (logits, x, w, v), torch.ones_like(out))
+
+
+def layer_leaves(tokens, experts, width, hidden, dtype, dev):
+    shapes = ((tokens, experts), (tokens, width), (experts, hidden, width), (experts, width, hidden))
+    leaves = [torch.randn(s, generator=gen(i), device=dev) for i, s in enumerate(shapes)]
+    return [leaves[0]] + [(t / t.shape[-1] ** 0.5).to(dtype) for t in leaves[1:]]
+
+
+@pytest.mark.parametrize("tokens,width,hidden", [(37, 64, 96), (600, 264, 129)])
+def test_gradients_on_another_stream(dev, tokens, width, hidden):
+    leaves = layer_leaves(tokens, 8, width, hidden, BF16, dev)
+    want = layer_step(*[t.clone().requires_grad_(True) for t in leaves], 2)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(20_000_000)
+        late = [torch.zeros_like(t) for t in leaves]
+        for t, value in zip(late, leaves):
+            t.copy_(value)  # the operands exist only once this stream has got here
+        got = layer_step(*[t.requires_grad_(True) for t in late], 2)
+    stream.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("tokens,experts,width,hidden", [(48, 8, 64, 96), (300, 12, 264, 129), (1500, 70, 72, 256)])
+def test_gradients_in_a_captured_graph(dev, tokens, experts, width, hidden):
+    leaves = [t.requires_grad_(True) for t in layer_leaves(tokens, experts, width, hidden, F16, dev)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer_step(*leaves, 3)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = layer_step(*leaves, 3)
+    for seed in range(4):
+        with torch.no_grad():
+            for i, t in enumerate(leaves):
+                t.copy_(torch.randn(t.shape, generator=gen(100 * seed + i), device=dev) / t.shape[-1] ** 0.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, want in zip(outs, layer_step(*leaves, 3)):
+            assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("lens,n,k", [([20, 70, 3], 48, 72), ([64, 1, 63], 65, 33), ([130, 0, 64, 200], 264, 520),
+                                      ([700, 800], 1536, 1544), ([5, 3], 1, 1)])
+@pytest.mark.parametrize("gather", [True, False])
+def test_non_finite_values_next_to_a_group_stay_out_of_its_weight_gradient(dev, lens, n, k, gather):
+    # rows of the other groups, of no group, and of tokens that no row names
+    plan, rows = lengths_to_plan(lens, tail=2)
+    x = torch.randn(rows, k, generator=gen(1), device=dev).to(BF16)
+    grad = torch.randn(rows, n, generator=gen(2), device=dev).to(BF16)
+    w = torch.zeros(len(lens), n, k, dtype=BF16, device=dev, requires_grad=True)
+    offsets = plan.offsets.tolist()
+    for e, (lo, hi) in enumerate(zip(offsets, offsets[1:])):
+        if lo == hi:
+            continue
+        dirty, dirty_grad = (torch.full_like(t, float("nan")) for t in (x, grad))
+        dirty[lo:hi], dirty_grad[lo:hi] = x[lo:hi], grad[lo:hi]
+        p = plan
+        if gather:  # the same rows, in another order of the tokens among others that are not finite
+            order = torch.randperm(2 * rows, generator=gen(3), device=dev)[:rows]
+            spread = torch.full((2 * rows, k), float("inf"), dtype=BF16, device=dev)
+            spread[order] = dirty
+            p, dirty = plan._replace(tokens=order.to(torch.int32)), spread
+        dw, = torch.autograd.grad(grouped_mm(dirty, w, p, gather=gather), w, dirty_grad)
+        g, a = grad[lo:hi].double(), x[lo:hi].double()
+        close(dw[e], g.t() @ a, g.abs().t() @ a.abs(), hi - lo)
+
+
+@pytest.mark.parametrize("tokens,experts,k,width,drop", [(9, 4, 2, 33, 0.0), (200, 7, 3, 264, 0.3)])
+def test_combine_gradient_of_a_plan_in_c(dev, tokens, experts, k, width, drop):
+    # the entry point for the places of a plan as they are, which takes no buffer
+    import ctypes
+
+    from ops_sparse import _lib
+
+    plan = expert_plan(routed(tokens, experts, k, 3, drop), experts)
+    y = torch.randn(tokens * k, width, generator=gen(1), device=dev).to(F16).requires_grad_(True)
+    weights = torch.randn(tokens, k, generator=gen(2), device=dev).requires_grad_(True)
+    grad = torch.randn(tokens, width, generator=gen(3), device=dev).to(F16)
+    want = torch.autograd.grad(combine(y, plan, weights), (y, weights), grad)
+    dy = torch.full((tokens * k, width), float("nan"), dtype=F16, device=dev)
+    dw = torch.full((tokens, k), float("nan"), device=dev)
+    lib, handle = _lib.lib(), ctypes.c_void_p(0)
+    assert lib.aclsparseCreate(ctypes.byref(handle)) == _lib.Status.SUCCESS
+    stream = torch.cuda.current_stream().cuda_stream or 1  # 1: HIP's default stream
+    assert lib.aclsparseSetStream(handle, ctypes.c_void_p(stream)) == _lib.Status.SUCCESS
+    status = lib.aclsparseCombineGrad(
+        handle, tokens, k, width, tokens * k, experts, plan.offsets.data_ptr(), plan.places.data_ptr(),
+        weights.data_ptr(), y.data_ptr(), width, grad.data_ptr(), width, int(_lib.DataType.FLOAT16), dy.data_ptr(),
+        width, dw.data_ptr())
+    lib.aclsparseDestroy(handle)
+    assert status == _lib.Status.SUCCESS
+    assert torch.equal(dy, want[0]) and torch.equal(dw, want[1])
+
+
 def test_offsets_past_32_bits(dev):
     # an operand of more than 2^32 bytes, read at its far end
     width, tokens = 4096, 540_000

@@ -462,11 +462,17 @@ aclsparseStatus_t aclsparseCombineGradAny_bufferSize(aclsparseHandle_t handle, i
                                                      int64_t rows, size_t* bufferSize);
 /* The same for any places, as aclsparseCombine takes them: gradY_r is the sum of weights[t*k + j] * gradOut_t over the
  * (t, j) whose place is r, in fp32 and in their order, zero for a row that no place names.  buffer may be null when
- * gradY is. */
+ * gradY is.  listed != 0: it is aclsparseCombineAndList's of the same places, tokens, k and rows, and is only read. */
 aclsparseStatus_t aclsparseCombineGradAny(aclsparseHandle_t handle, int64_t tokens, int64_t k, int64_t width,
                                           int64_t rows, const int32_t* places, const float* weights, const void* Y,
                                           int64_t ldy, const void* gradOut, int64_t ldOut, aclDataType type,
-                                          void* gradY, int64_t ldGradY, float* gradWeights, void* buffer);
+                                          void* gradY, int64_t ldGradY, float* gradWeights, void* buffer,
+                                          int32_t listed);
+/* aclsparseCombine that also writes the buffer of the gradient: which assignments name each row. */
+aclsparseStatus_t aclsparseCombineAndList(aclsparseHandle_t handle, int64_t tokens, int64_t k, int64_t width,
+                                          int64_t rows, const int32_t* places, const float* weights, const void* Y,
+                                          int64_t ldy, aclDataType yType, void* out, int64_t ldOut,
+                                          aclDataType outType, void* buffer);
 
 #ifdef __cplusplus
 }

@@ -34,18 +34,46 @@ __device__ __forceinline__ void StorePack(T* p, const Pack<T, N>& v)
     __builtin_memcpy(__builtin_assume_aligned(p, sizeof(v)), &v, sizeof(v));
 }
 
+// The lists of the assignments that name each row, for gradients of any places: head[r] is one of row r's and next[a]
+// another of the row that a names, or whatever the memory held: neither array is cleared before.  An entry counts only
+// where it is an assignment that names the row (Names).  That is enough, as every assignment of a
+// row enters its list: what the first to enter finds in head[r] is either no assignment of the row or one that the
+// list holds as well.
+struct Lists {
+    int32_t* head;
+    int32_t* next;
+};
+// Enters assignments [first, end), one per thread at a time, `threads` of them apart.
+__device__ __forceinline__ void EnterPlaces(const Lists& l, const int32_t* places, int64_t rows, int64_t first,
+                                            int64_t end, int64_t threads)
+{
+    for (int64_t a = first; a < end; a += threads) {
+        const int32_t place = places[a];
+        if (place >= 0 && place < rows) l.next[a] = atomicExch(&l.head[place], static_cast<int32_t>(a));
+    }
+}
+
 // VEC columns of one token per thread, 16 bytes of the output: a row's parts
-// are read whole wherever they lie.  Bound by memory: 16384 tokens of 8 rows of
-// 2048, bfloat16, 137 us for 604 MB, 4.4 TB/s (a copy reaches 5.05, reading
-// alone 3.9).
+// are read whole wherever they lie.  With lists a token's first workgroup in
+// every kListed tokens enters the assignments of all of them: the exchanges come
+// back late, and a workgroup waits for them.  Bound by memory: 16384 tokens of 8
+// rows of 2048, bfloat16, 136 us for 604 MB, 4.4 TB/s (a copy reaches 5.05,
+// reading alone 3.9); with the lists 138 (142 where every token's workgroup
+// enters its own, 158 where kListed is 32 and one die gets all that wait).
+constexpr int kListed = 31;  // odd, so that they are dealt to all dies
 template <typename TIn, typename TOut, int VEC>
 __global__ __launch_bounds__(kThreads) void CombineKernel(CombineLaunch p, int32_t chunks)
 {
     const uint32_t block = BlockNumber();
     const int64_t t = block / static_cast<uint32_t>(chunks);
     const int64_t c = (static_cast<int64_t>(block % static_cast<uint32_t>(chunks)) * kThreads + threadIdx.x) * VEC;
-    if (t >= p.tokens || c >= p.width) return;
+    if (t >= p.tokens) return;
     const int k = static_cast<int>(p.k);
+    if (p.head != nullptr && t % kListed == 0 && block % static_cast<uint32_t>(chunks) == 0) {
+        const int64_t end = t + kListed < p.tokens ? t + kListed : p.tokens;
+        EnterPlaces({p.head, p.next}, p.places, p.rows, t * k + threadIdx.x, end * k, kThreads);
+    }
+    if (c >= p.width) return;
     float acc[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
@@ -63,21 +91,14 @@ __global__ __launch_bounds__(kThreads) void CombineKernel(CombineLaunch p, int32
     StorePack<TOut, VEC>(static_cast<TOut*>(p.out) + t * p.ldo + c, out);
 }
 
-// The assignments that name each row, for any places: head[r] is one of row r's and next[a] another of the row that a
-// names, or whatever the memory held: neither array is cleared before.  An entry counts only where it is an assignment
-// that names the row (Names).  That is enough, as every assignment of a row enters its list: what
-// the first to enter finds in head[r] is either no assignment of the row or one that the list holds as well.
-__global__ __launch_bounds__(kThreads) void LinkPlacesKernel(CombineGradLaunch p)
+// The lists alone, where the product did not make them.  The same assignments: 5.5 us.
+__global__ __launch_bounds__(kThreads) void ListPlacesKernel(CombineGradLaunch p)
 {
-    const int64_t assignments = p.tokens * p.k;
-    for (int64_t a = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; a < assignments;
-         a += static_cast<int64_t>(gridDim.x) * kThreads) {
-        const int32_t place = p.places[a];
-        if (place >= 0 && place < p.rows) p.next[a] = atomicExch(&p.head[place], static_cast<int32_t>(a));
-    }
+    EnterPlaces({p.head, p.next}, p.places, p.rows, static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x,
+                p.tokens * p.k, static_cast<int64_t>(gridDim.x) * kThreads);
 }
 
-struct CombineGradLinks {
+struct CombineGradLists {
     const CombineGradLaunch& p;
     int64_t assignments;
 
@@ -93,7 +114,7 @@ struct CombineGradLinks {
 // fp32 in the order of the assignments, whatever the list's.  A list of more than a wave's lanes is left, and the
 // places are searched for its assignments.
 template <typename T, int VEC>
-__device__ void SumSharedRow(const CombineGradLaunch& p, const CombineGradLinks& links, int32_t a, int32_t place)
+__device__ void SumSharedRow(const CombineGradLaunch& p, const CombineGradLists& lists, int32_t a, int32_t place)
 {
     const int lane = threadIdx.x & 63;
     int32_t mine = -1, count = 0, at = a;
@@ -102,7 +123,7 @@ __device__ void SumSharedRow(const CombineGradLaunch& p, const CombineGradLinks&
         if (lane == count) mine = at;
         ++count;
         at = p.next[at];
-        if (!links.Names(at, place) || __any(mine == at)) break;
+        if (!lists.Names(at, place) || __any(mine == at)) break;
         if (count == 64) {
             searched = true;
             break;
@@ -124,8 +145,8 @@ __device__ void SumSharedRow(const CombineGradLaunch& p, const CombineGradLinks&
             for (int i = 0; i < VEC; ++i) acc[i] = fmaf(w, ToFloat(g.v[i]), acc[i]);
         };
         if (searched) {
-            for (int64_t first = 0; first < links.assignments; first += 64) {
-                const bool named = first + lane < links.assignments && p.places[first + lane] == place;
+            for (int64_t first = 0; first < lists.assignments; first += 64) {
+                const bool named = first + lane < lists.assignments && p.places[first + lane] == place;
                 for (uint64_t left = __ballot(named); left != 0; left &= left - 1) add(first + __builtin_ctzll(left));
             }
         } else {
@@ -146,22 +167,22 @@ __device__ void SumSharedRow(const CombineGradLaunch& p, const CombineGradLinks&
 // clears row r of dy where the row has no assignment.  With kAny those are the
 // rows that no place names, and the head of a row's list writes it; without,
 // the rows past the last group, as in a plan whose places name each row before
-// them once.  Bound by memory: 16384 tokens of 8 rows of 2048, bfloat16, 214 to
-// 218 us with kAny for 1.14 GB, 5.2 TB/s, behind 5 us of LinkPlacesKernel (with
-// the list looked up before the row's first loads 236 to 241 us: a chain of
-// three dependent loads of each wave that nothing hid).
+// them once.  Bound by memory: 16384 tokens of 8 rows of 2048, bfloat16, 211 to
+// 218 us with kAny for 1.14 GB, 5.3 TB/s (with the list looked up before the
+// row's first loads 236 to 241 us: a chain of three dependent loads of each wave
+// that nothing hid).
 template <typename T, int VEC, bool kAny>
 __global__ __launch_bounds__(kThreads) void CombineGradKernel(CombineGradLaunch p)
 {
     const int lane = threadIdx.x & 63;
     const int64_t a = static_cast<int64_t>(BlockNumber()) * (kThreads / 64) + (threadIdx.x >> 6);
     const int64_t assignments = p.tokens * p.k;
-    const CombineGradLinks links{p, assignments};
+    const CombineGradLists lists{p, assignments};
     T* gy = static_cast<T*>(p.grad_y);
     bool unnamed = false;  // row a has no assignment
     if (gy != nullptr && a < p.rows) {
         if constexpr (kAny) {
-            unnamed = assignments == 0 || !links.Names(p.head[a], a);
+            unnamed = assignments == 0 || !lists.Names(p.head[a], a);
         } else {
             unnamed = a >= p.offsets[p.groups];
         }
@@ -189,7 +210,7 @@ __global__ __launch_bounds__(kThreads) void CombineGradKernel(CombineGradLaunch 
                 if (gy != nullptr) {
                     const int32_t other = p.next[a];
                     const bool listed = p.head[place] == a;
-                    const bool shared = links.Names(other, place) & (other != a);
+                    const bool shared = lists.Names(other, place) & (other != a);
                     only = listed & !shared;
                     first = listed & shared;
                 }
@@ -213,7 +234,7 @@ __global__ __launch_bounds__(kThreads) void CombineGradKernel(CombineGradLaunch 
                 }
             }
             if constexpr (kAny) {
-                if (__any(first)) SumSharedRow<T, VEC>(p, links, static_cast<int32_t>(a), place);
+                if (__any(first)) SumSharedRow<T, VEC>(p, lists, static_cast<int32_t>(a), place);
             }
         }
         if (p.grad_weights != nullptr) {
@@ -260,9 +281,9 @@ int CombineGradTyped(const CombineGradLaunch& l, hipStream_t s)
                       Aligned(l.grad_out, l.ldo, sizeof(T), 16) && Aligned(l.grad_y, l.ld_grad_y, sizeof(T), 16);
     const int64_t count = l.tokens * l.k > l.rows ? l.tokens * l.k : l.rows;
     const dim3 grid = GridOf((count + kThreads / 64 - 1) / (kThreads / 64));
-    if (kAny && l.grad_y != nullptr && l.tokens > 0) {
+    if (kAny && !l.listed && l.grad_y != nullptr && l.tokens > 0) {
         const int64_t blocks = (l.tokens * l.k + kThreads - 1) / kThreads;
-        LinkPlacesKernel<<<static_cast<uint32_t>(blocks < 4096 ? blocks : 4096), kThreads, 0, s>>>(l);
+        ListPlacesKernel<<<static_cast<uint32_t>(blocks < 4096 ? blocks : 4096), kThreads, 0, s>>>(l);
     }
     if (wide) {
         CombineGradKernel<T, VEC, kAny><<<grid, kThreads, 0, s>>>(l);

@@ -105,6 +105,28 @@ size_t HeadBytes(int64_t count)
     return aclsp::AlignUp(bytes < aclsp::kWsAlign ? aclsp::kWsAlign : bytes);
 }
 
+int32_t* NextOf(int32_t* head, int64_t rows) { return head + HeadBytes(rows) / sizeof(int32_t); }
+
+aclsparseStatus_t Combine(aclsparseHandle_t handle, aclsp::CombineLaunch l, bool lists)
+{
+    aclsparseStatus_t st = CheckHandle(handle);
+    if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
+    st = CheckCombineShape(l.tokens, l.k, l.width, l.rows);
+    if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
+    // rows of 32 bits (a gradient's partial sums) may be rounded to 16 here
+    if (!Is16Bit(l.out_type) || (l.y_type != l.out_type && l.y_type != ACL_FLOAT)) {
+        return ACL_SPARSE_STATUS_NOT_SUPPORTED;
+    }
+    if (l.ldy < l.width || l.ldo < l.width) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    if (l.tokens == 0 || l.width == 0) return ACL_SPARSE_STATUS_SUCCESS;
+    if (l.places == nullptr || l.out == nullptr || (l.rows > 0 && l.y == nullptr) || (lists && l.head == nullptr)) {
+        return ACL_SPARSE_STATUS_INVALID_VALUE;
+    }
+    if (lists) l.next = NextOf(l.head, l.rows);
+    (void)hipGetLastError();
+    return Finish(aclsp::LaunchCombine(l, StreamOf(handle)));
+}
+
 }  // namespace
 
 extern "C" {
@@ -256,18 +278,19 @@ aclsparseStatus_t aclsparseCombine(aclsparseHandle_t handle, int64_t tokens, int
                                    const int32_t* places, const float* weights, const void* Y, int64_t ldy,
                                    aclDataType yType, void* out, int64_t ldOut, aclDataType outType)
 {
-    aclsparseStatus_t st = CheckHandle(handle);
-    if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
-    st = CheckCombineShape(tokens, k, width, rows);
-    if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
-    // rows of 32 bits (a gradient's partial sums) may be rounded to 16 here
-    if (!Is16Bit(outType) || (yType != outType && yType != ACL_FLOAT)) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
-    if (ldy < width || ldOut < width) return ACL_SPARSE_STATUS_INVALID_VALUE;
-    if (tokens == 0 || width == 0) return ACL_SPARSE_STATUS_SUCCESS;
-    if (places == nullptr || out == nullptr || (rows > 0 && Y == nullptr)) return ACL_SPARSE_STATUS_INVALID_VALUE;
-    aclsp::CombineLaunch l{tokens, k, width, rows, places, weights, Y, ldy, yType, out, ldOut, outType};
-    (void)hipGetLastError();
-    return Finish(aclsp::LaunchCombine(l, StreamOf(handle)));
+    return Combine(handle,
+                   {tokens, k, width, rows, places, weights, Y, ldy, yType, out, ldOut, outType, nullptr, nullptr},
+                   /*lists=*/false);
+}
+
+aclsparseStatus_t aclsparseCombineAndList(aclsparseHandle_t handle, int64_t tokens, int64_t k, int64_t width,
+                                          int64_t rows, const int32_t* places, const float* weights, const void* Y,
+                                          int64_t ldy, aclDataType yType, void* out, int64_t ldOut,
+                                          aclDataType outType, void* buffer)
+{
+    auto* head = static_cast<int32_t*>(buffer);
+    return Combine(handle, {tokens, k, width, rows, places, weights, Y, ldy, yType, out, ldOut, outType, head, nullptr},
+                   /*lists=*/true);
 }
 
 aclsparseStatus_t aclsparseCombineGrad(aclsparseHandle_t handle, int64_t tokens, int64_t k, int64_t width,
@@ -281,7 +304,7 @@ aclsparseStatus_t aclsparseCombineGrad(aclsparseHandle_t handle, int64_t tokens,
     if (groups < 1) return ACL_SPARSE_STATUS_INVALID_VALUE;
     if (groups > kMaxCount) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
     const aclsp::CombineGradLaunch l{tokens, k, width, rows, groups, offsets, places, weights, Y, ldy, gradOut, ldOut,
-                                     type, gradY, ldGradY, gradWeights, nullptr, nullptr};
+                                     type, gradY, ldGradY, gradWeights, nullptr, nullptr, false};
     st = CheckCombineGrad(l);
     if (st != ACL_SPARSE_STATUS_SUCCESS || (tokens == 0 && rows == 0)) return st;
     if (offsets == nullptr) return ACL_SPARSE_STATUS_INVALID_VALUE;
@@ -305,19 +328,20 @@ aclsparseStatus_t aclsparseCombineGradAny_bufferSize(aclsparseHandle_t handle, i
 aclsparseStatus_t aclsparseCombineGradAny(aclsparseHandle_t handle, int64_t tokens, int64_t k, int64_t width,
                                           int64_t rows, const int32_t* places, const float* weights, const void* Y,
                                           int64_t ldy, const void* gradOut, int64_t ldOut, aclDataType type,
-                                          void* gradY, int64_t ldGradY, float* gradWeights, void* buffer)
+                                          void* gradY, int64_t ldGradY, float* gradWeights, void* buffer,
+                                          int32_t listed)
 {
     aclsparseStatus_t st = CheckHandle(handle);
     if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
     auto* head = static_cast<int32_t*>(buffer);
     aclsp::CombineGradLaunch l{tokens, k, width, rows, 0, nullptr, places, weights, Y, ldy, gradOut, ldOut,
-                               type, gradY, ldGradY, gradWeights, head, nullptr};
+                               type, gradY, ldGradY, gradWeights, head, nullptr, listed != 0};
     st = CheckCombineGrad(l);
     if (st != ACL_SPARSE_STATUS_SUCCESS || (tokens == 0 && rows == 0)) return st;
     if (gradY == nullptr && gradWeights == nullptr) return ACL_SPARSE_STATUS_SUCCESS;
     if (gradY != nullptr) {
         if (buffer == nullptr) return ACL_SPARSE_STATUS_INVALID_VALUE;
-        l.next = head + HeadBytes(rows) / sizeof(int32_t);
+        l.next = NextOf(head, rows);
     }
     (void)hipGetLastError();
     return Finish(aclsp::LaunchCombineGrad(l, StreamOf(handle)));

@@ -68,6 +68,8 @@ struct CombineLaunch {
     void* out;
     int64_t ldo;
     aclDataType out_type;
+    int32_t* head;  // null: no lists for the gradient
+    int32_t* next;
 };
 int LaunchCombine(const CombineLaunch& l, void* stream);
 
@@ -86,6 +88,7 @@ struct CombineGradLaunch {
     float* grad_weights;  // null: not wanted
     int32_t* head;  // the caller's buffer: one per row
     int32_t* next;  // and one per assignment
+    bool listed;    // they hold the lists already
 };
 int LaunchCombineGrad(const CombineGradLaunch& l, void* stream);
 

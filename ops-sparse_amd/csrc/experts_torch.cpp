@@ -35,6 +35,7 @@ struct Library {
     decltype(&aclsparseGroupedMMGrad) groupedMMGrad = nullptr;
     decltype(&aclsparseGroupedMMScaled) groupedMMScaled = nullptr;
     decltype(&aclsparseCombine) combine = nullptr;
+    decltype(&aclsparseCombineAndList) combineAndList = nullptr;
     decltype(&aclsparseCombineGradAny_bufferSize) combineGradBufferSize = nullptr;
     decltype(&aclsparseCombineGradAny) combineGrad = nullptr;
 } lib;
@@ -58,6 +59,7 @@ void Bind(const std::string& path)
     look(lib.groupedMMGrad, "aclsparseGroupedMMGrad");
     look(lib.groupedMMScaled, "aclsparseGroupedMMScaled");
     look(lib.combine, "aclsparseCombine");
+    look(lib.combineAndList, "aclsparseCombineAndList");
     look(lib.combineGradBufferSize, "aclsparseCombineGradAny_bufferSize");
     look(lib.combineGrad, "aclsparseCombineGradAny");
 }
@@ -304,14 +306,26 @@ Tensor RunGrouped(aclsparseOperation_t op, const Tensor& a, const Tensor& b, con
     return out;
 }
 
-Tensor RunCombine(const Tensor& y, const Tensor& places, const Tensor& weights, at::ScalarType type)
+// lists: where to put the buffer that lists each row's assignments, null for none
+Tensor RunCombine(const Tensor& y, const Tensor& places, const Tensor& weights, at::ScalarType type,
+                  Tensor* lists = nullptr)
 {
-    const int64_t tokens = places.size(0), width = y.size(1);
+    const int64_t tokens = places.size(0), k = places.size(1), width = y.size(1), rows = y.size(0);
     Tensor out = Empty({tokens, width}, type, y);
     Call call(y);
-    Call::Ok(lib.combine(call, tokens, places.size(1), width, y.size(0), Ints(places), Floats(weights), Data(y), Ld(y),
-                         TypeOf(y.scalar_type()), Data(out), std::max<int64_t>(width, 1), TypeOf(type)),
-             "aclsparseCombine");
+    if (lists == nullptr) {
+        Call::Ok(lib.combine(call, tokens, k, width, rows, Ints(places), Floats(weights), Data(y), Ld(y),
+                             TypeOf(y.scalar_type()), Data(out), std::max<int64_t>(width, 1), TypeOf(type)),
+                 "aclsparseCombine");
+        return out;
+    }
+    size_t bytes = 0;
+    Call::Ok(lib.combineGradBufferSize(call, tokens, k, rows, &bytes), "aclsparseCombineGradAny_bufferSize");
+    *lists = Empty({static_cast<int64_t>(bytes)}, at::kByte, y);
+    Call::Ok(lib.combineAndList(call, tokens, k, width, rows, Ints(places), Floats(weights), Data(y), Ld(y),
+                                TypeOf(y.scalar_type()), Data(out), std::max<int64_t>(width, 1), TypeOf(type),
+                                Data(*lists)),
+             "aclsparseCombineAndList");
     return out;
 }
 
@@ -467,30 +481,26 @@ struct CombineNode : torch::autograd::Function<CombineNode> {
     static Tensor forward(AutogradContext* ctx, const Tensor& y, const optional<Tensor>& given, const Sorted& plan)
     {
         const Tensor weights = given.value_or(Tensor()), &places = plan.places;
-        ctx->save_for_backward({y, weights, places});
-        ctx->saved_data["y"] = y.requires_grad();
-        ctx->saved_data["w"] = weights.defined() && weights.requires_grad();
-        return RunCombine(y, places, weights, y.scalar_type());
+        Tensor lists;  // for y's gradient; kept only where one is asked for
+        const Tensor out =
+            RunCombine(y, places, weights, y.scalar_type(), y.requires_grad() ? &lists : nullptr);
+        ctx->save_for_backward({y, weights, places, lists});
+        return out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
         const auto saved = ctx->get_saved_variables();
-        const Tensor &y = saved[0], &weights = saved[1], &places = saved[2];
+        const Tensor &y = saved[0], &weights = saved[1], &places = saved[2], &lists = saved[3];
         NoTangent(grads[0]);
         const Tensor grad = Rows(grads[0]);
         const int64_t tokens = places.size(0), k = places.size(1), rows = y.size(0), width = y.size(1);
         Call call(y);
-        Tensor dy, dw, buffer;
-        if (ctx->saved_data["y"].toBool()) {
-            dy = Empty({rows, width}, y.scalar_type(), y);
-            size_t bytes = 0;
-            Call::Ok(lib.combineGradBufferSize(call, tokens, k, rows, &bytes), "aclsparseCombineGradAny_bufferSize");
-            buffer = Empty({static_cast<int64_t>(bytes)}, at::kByte, y);
-        }
-        if (ctx->saved_data["w"].toBool()) dw = Empty({tokens, k}, at::kFloat, y);
+        Tensor dy, dw;
+        if (lists.defined()) dy = Empty({rows, width}, y.scalar_type(), y);
+        if (weights.defined() && weights.requires_grad()) dw = Empty({tokens, k}, at::kFloat, y);
         Call::Ok(lib.combineGrad(call, tokens, k, width, rows, Ints(places), Floats(weights), Data(y), Ld(y),
                                  Data(grad), Ld(grad), TypeOf(y.scalar_type()), Data(dy), std::max<int64_t>(width, 1),
-                                 Floats(dw), Data(buffer)),
+                                 Floats(dw), Data(lists), /*listed=*/1),
                  "aclsparseCombineGradAny");
         return Once({grads[0], y, weights}, {dy, dw, Tensor()});
     }

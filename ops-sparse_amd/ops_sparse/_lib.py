@@ -190,7 +190,9 @@ SIGNATURES = {
     "aclsparseCombineGrad": [_vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i32, _vp, _i64,
                              _vp],
     "aclsparseCombineGradAny_bufferSize": [_vp, _i64, _i64, _i64, ctypes.POINTER(_sz)],
-    "aclsparseCombineGradAny": [_vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i32, _vp, _i64, _vp, _vp],
+    "aclsparseCombineGradAny": [_vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i32, _vp, _i64, _vp, _vp,
+                                _i32],
+    "aclsparseCombineAndList": [_vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i32, _vp, _i64, _i32, _vp],
 }
 
 _LIB = None

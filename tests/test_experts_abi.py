@@ -159,9 +159,18 @@ def test_grids_of_too_many_threads_are_refused(lib, handle):
 
 def combine_grad_any(**kw):
     a = dict(tokens=4, k=2, width=8, rows=8, places=P, weights=P, y=P, ldy=8, go=P, ldo=8, type=F16, gy=P, ldgy=8, gw=P,
-             buffer=P)
+             buffer=P, listed=0)
     a.update(kw)
     return list(a.values())
+
+
+def test_status_codes_of_the_combination_that_lists(lib, handle):
+    # as the one that does not, and the buffer
+    for change, status in dict((name, changes) for name, _, changes in CASES)["aclsparseCombine"]:
+        assert lib.aclsparseCombineAndList(handle, *combine(**change), P) == status, change
+    assert lib.aclsparseCombineAndList(handle, *combine(), None) == INVALID
+    assert lib.aclsparseCombineAndList(handle, *combine(tokens=0), None) == OK
+    assert lib.aclsparseCombineAndList(None, *combine(), P) == Status.HANDLE_IS_NULLPTR
 
 
 def test_status_codes_of_the_gradient_for_any_places(lib, handle):

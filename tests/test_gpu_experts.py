@@ -931,6 +931,48 @@ def test_combine_gradient_of_a_plan_in_c(dev, tokens, experts, k, width, drop):
     assert torch.equal(dy, want[0]) and torch.equal(dw, want[1])
 
 
+@pytest.mark.parametrize("kind", ["dropped", "more rows", "outside", "drawn", "one row", "a wave"])
+def test_combine_gradient_of_any_places_in_c(dev, kind):
+    # lists made by the gradient itself, and by the product
+    import ctypes
+
+    from ops_sparse import _lib
+
+    tokens, k, width = 150, 3, 264
+    places, rows = any_places(kind, tokens, k)
+    places = places.to(dev)
+    plan = ExpertPlan(torch.tensor([0, 2], dtype=torch.int32, device=dev), None, places)
+    y = torch.randn(rows, width, generator=gen(1), device=dev).to(F16).requires_grad_(True)
+    weights = torch.randn(tokens, k, generator=gen(2), device=dev).requires_grad_(True)
+    grad = torch.randn(tokens, width, generator=gen(3), device=dev).to(F16)
+    product = combine(y, plan, weights)
+    want = torch.autograd.grad(product, (y, weights), grad)
+    lib, handle, size = _lib.lib(), ctypes.c_void_p(0), ctypes.c_size_t(0)
+    assert lib.aclsparseCreate(ctypes.byref(handle)) == _lib.Status.SUCCESS
+    stream = torch.cuda.current_stream().cuda_stream or 1  # 1: HIP's default stream
+    assert lib.aclsparseSetStream(handle, ctypes.c_void_p(stream)) == _lib.Status.SUCCESS
+    assert lib.aclsparseCombineGradAny_bufferSize(handle, tokens, k, rows, ctypes.byref(size)) == _lib.Status.SUCCESS
+    f16 = int(_lib.DataType.FLOAT16)
+    for listed in (0, 1):
+        buffer = torch.randint(0, tokens * k, (size.value // 4,), device=dev, dtype=torch.int32)
+        if listed:
+            out = torch.empty(tokens, width, dtype=F16, device=dev)
+            assert lib.aclsparseCombineAndList(
+                handle, tokens, k, width, rows, places.data_ptr(), weights.data_ptr(), y.data_ptr(), width, f16,
+                out.data_ptr(), width, f16, buffer.data_ptr()) == _lib.Status.SUCCESS
+            assert torch.equal(out, product)
+        for with_y, with_w in ((True, True), (True, False), (False, True)):
+            dy = torch.full((rows, width), float("nan"), dtype=F16, device=dev) if with_y else None
+            dw = torch.full((tokens, k), float("nan"), device=dev) if with_w else None
+            assert lib.aclsparseCombineGradAny(
+                handle, tokens, k, width, rows, places.data_ptr(), weights.data_ptr(), y.data_ptr(), width,
+                grad.data_ptr(), width, f16, dy.data_ptr() if with_y else None, width,
+                dw.data_ptr() if with_w else None, buffer.data_ptr() if with_y else None, listed) == _lib.Status.SUCCESS
+            assert dy is None or torch.equal(dy, want[0])
+            assert dw is None or torch.equal(dw, want[1])
+    lib.aclsparseDestroy(handle)
+
+
 def test_offsets_past_32_bits(dev):
     # an operand of more than 2^32 bytes, read at its far end
     width, tokens = 4096, 540_000

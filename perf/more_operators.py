@@ -186,9 +186,9 @@ _MASK = 0xFFFFFFFF
 
 def _mix(x):
     x = x ^ (x >> 16)
-    x = (x * 0x6A09E667) & _MASK
+    x = (x * 0x9B05688D) & _MASK
     x = x ^ (x >> 15)
-    x = (x * 0xBB67AE85) & _MASK
+    x = (x * 0x5BE0CD19) & _MASK
     return x ^ (x >> 16)
 
 

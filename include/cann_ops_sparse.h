@@ -474,6 +474,98 @@ aclsparseStatus_t aclsparseCombineAndList(aclsparseHandle_t handle, int64_t toke
                                           int64_t ldy, aclDataType yType, void* out, int64_t ldOut,
                                           aclDataType outType, void* buffer);
 
+/* ---------------- Training and serving of a model (no counterpart in the reference) ----------------
+ *
+ * Beside the experts' operators: their operands in microscaled 4-bit floating
+ * point, the log probabilities that a model is trained on and answers with, and
+ * the optimiser's step.  As there, no call waits, allocates or copies to the
+ * host, every call may be captured in a HIP graph, and results do not change
+ * from run to run.
+ *
+ * Microscaled 4 bits (OCP Microscaling, elements e2m1): a row of k values is
+ * ceil(k / 32) blocks, each of 16 bytes of codes, value 2i in the low half of
+ * byte i, and one scale byte e that stands for 2^(e - 127), 255 for NaN.  Codes
+ * past a row's k values are zero.  Leading dimensions and strides of codes and
+ * scales count bytes.
+ */
+
+/* Rows to the format: a block's scale has the exponent of its largest value less 2 (at least 2^-127), each value over
+ * the scale becomes the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives, ties to the even code and at most
+ * 6; a block with a value that is not finite has scale 255 and codes of zero.  X ACL_FLOAT, ACL_FLOAT16 or ACL_BF16. */
+aclsparseStatus_t aclsparseMx4Quantize(aclsparseHandle_t handle, int64_t rows, int64_t k, const void* X, int64_t ldx,
+                                       aclDataType xType, uint8_t* codes, int64_t ldCodes, uint8_t* scales,
+                                       int64_t ldScales);
+/* The values of k codes of each row, rounded to X's type. */
+aclsparseStatus_t aclsparseMx4Dequantize(aclsparseHandle_t handle, int64_t rows, int64_t k, const uint8_t* codes,
+                                         int64_t ldCodes, const uint8_t* scales, int64_t ldScales, void* X, int64_t ldx,
+                                         aclDataType xType);
+/* aclsparseGroupedMM with ACL_SPARSE_OP_TRANSPOSE on operands in microscaled 4 bits: whole blocks are multiplied, sums
+ * are in fp32.  Rows of codes are aligned to 16 bytes (A, lda, B, ldb, strideB), scales to none; strideB and
+ * strideScaleB are the bytes from one group's to the next's.  C ACL_FLOAT, ACL_FLOAT16 or ACL_BF16. */
+aclsparseStatus_t aclsparseGroupedMMMx4(aclsparseHandle_t handle, int64_t groups, int64_t rows, int64_t n, int64_t k,
+                                        const int32_t* offsets, const int32_t* rowIndex, int64_t rowsA,
+                                        const uint8_t* A, int64_t lda, const uint8_t* scaleA, int64_t ldScaleA,
+                                        const uint8_t* B, int64_t ldb, int64_t strideB, const uint8_t* scaleB,
+                                        int64_t ldScaleB, int64_t strideScaleB, void* C, int64_t ldc,
+                                        aclDataType cType);
+
+/* One tensor of an AdamW step. */
+typedef struct aclsparseAdamWTensor_t {
+    void* param;         /* count values, contiguous, of paramType (ACL_FLOAT, ACL_FLOAT16 or ACL_BF16) */
+    const void* grad;    /* the same of gradType; null: the tensor is left as it is */
+    float* master;       /* null, or the values in fp32, which the step goes by; param gets them rounded */
+    void* moments;       /* first and second moment, each of count values rounded up to 32: fp32, or codes of a byte */
+    uint8_t* exponents;  /* of 8-bit moments: a byte for each 32 values of either; null for fp32 */
+    int64_t count;
+    int32_t paramType, gradType;
+} aclsparseAdamWTensor_t;
+
+/* What a step's tensors share. */
+typedef struct aclsparseAdamWOptions_t {
+    double lr, beta1, beta2, eps, weightDecay;
+    const float* lrDevice;   /* null, or the rate in device memory, read when the step runs */
+    const float* gradScale;  /* null, or a factor of all gradients in device memory */
+    int32_t* step;           /* two counts in device memory: the steps taken, which the call counts up, and zero */
+    uint32_t seed;           /* of the rounding of 8-bit moments */
+    int32_t momentBits;      /* 32 or 8 */
+} aclsparseAdamWOptions_t;
+
+/* m = beta1 m + (1 - beta1) g, v = beta2 v + (1 - beta2) g^2, p = p (1 - lr weightDecay) - lr / (1 - beta1^t) * m /
+ * (sqrt(v) / sqrt(1 - beta2^t) + eps) for every tensor, t the steps taken with this one.  tensors and options are host
+ * memory, read before the call returns.  No two tensors share memory.
+ * 8-bit moments: blocks of 32 values with the exponent f of the largest (its fp32 exponent field); a code c of magnitude
+ * bits stands for (c / 8) 2^(l + f - 127) below 8 and (1 + (c & 7) / 8) 2^((c >> 3) - 1 + l + f - 127) from there on,
+ * l = -13 for the first moment's seven bits below the sign, l = -29 for the second's eight.  They are rounded up or down
+ * at random, by numbers that seed, step, the tensor's place and the element's give, so that slow changes add up; the
+ * parameters go by the moments before that.  A block that holds infinity or NaN becomes NaN. */
+aclsparseStatus_t aclsparseAdamW(aclsparseHandle_t handle, int64_t count, const aclsparseAdamWTensor_t* tensors,
+                                 const aclsparseAdamWOptions_t* options);
+/* The values of 8-bit moments in fp32, [2, count] for each tensor, to its master; param and grad are not read. */
+aclsparseStatus_t aclsparseAdamWMoments(aclsparseHandle_t handle, int64_t count,
+                                        const aclsparseAdamWTensor_t* tensors);
+
+/* Bytes of the buffer that aclsparseTokenLogprobs works in (calls that share one must not overlap). */
+aclsparseStatus_t aclsparseTokenLogprobs_bufferSize(aclsparseHandle_t handle, int64_t rows, int64_t vocab, int64_t top,
+                                                    size_t* bufferSize);
+/* For each row of logits: the log probability of its target (0 for a target outside [0, vocab), as padding has), the
+ * entropy of the row, and its top largest logits' ids (ties: the lowest first; -inf is never one: id -1; NaN counts as
+ * the largest) and log probabilities.  targets ACL_INT32 or ACL_INT64, null together with logprobs; entropy and stats
+ * (two floats a row, for the gradient) may be null.  A row of nothing but -inf has log probabilities of -inf and an
+ * entropy of 0.  top <= 64, vocab <= 2^30; logits ACL_FLOAT, ACL_FLOAT16 or ACL_BF16, statistics in fp32. */
+aclsparseStatus_t aclsparseTokenLogprobs(aclsparseHandle_t handle, int64_t rows, int64_t vocab, const void* logits,
+                                         int64_t ldLogits, aclDataType logitsType, const void* targets,
+                                         aclDataType targetsType, float* logprobs, float* entropy, float* stats,
+                                         int64_t top, float* topLogprobs, int32_t* topIds, void* buffer);
+/* Gradient with respect to the logits, in their type: of the log probabilities, the entropies and the alternatives' log
+ * probabilities, each null for none.  stats, entropy and topIds are aclsparseTokenLogprobs's.  A row of nothing but -inf
+ * has the gradient 0. */
+aclsparseStatus_t aclsparseTokenLogprobsGrad(aclsparseHandle_t handle, int64_t rows, int64_t vocab, const void* logits,
+                                             int64_t ldLogits, aclDataType logitsType, const void* targets,
+                                             aclDataType targetsType, const float* stats, const float* entropy,
+                                             int64_t top, const int32_t* topIds, const float* gradLogprobs,
+                                             const float* gradEntropy, const float* gradTop, void* gradLogits,
+                                             int64_t ldGrad);
+
 #ifdef __cplusplus
 }
 #endif

@@ -116,6 +116,20 @@ _pi64 = ctypes.POINTER(ctypes.c_int64)
 _i32 = ctypes.c_int32
 _sz = ctypes.c_size_t
 
+
+class AdamWTensor(ctypes.Structure):
+    """aclsparseAdamWTensor_t."""
+    _fields_ = [("param", _vp), ("grad", _vp), ("master", _vp), ("moments", _vp), ("exponents", _vp), ("count", _i64),
+                ("paramType", _i32), ("gradType", _i32)]
+
+
+class AdamWOptions(ctypes.Structure):
+    """aclsparseAdamWOptions_t."""
+    _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double),
+                ("eps", ctypes.c_double), ("weightDecay", ctypes.c_double), ("lrDevice", _vp), ("gradScale", _vp),
+                ("step", _vp), ("seed", ctypes.c_uint32), ("momentBits", _i32)]
+
+
 # name -> argtypes; every function returns aclsparseStatus_t (int) unless RESTYPES says otherwise
 RESTYPES = {"aclsparseHipBuildId": ctypes.c_char_p}
 SIGNATURES = {
@@ -193,6 +207,16 @@ SIGNATURES = {
     "aclsparseCombineGradAny": [_vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i32, _vp, _i64, _vp, _vp,
                                 _i32],
     "aclsparseCombineAndList": [_vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i32, _vp, _i64, _i32, _vp],
+    "aclsparseMx4Quantize": [_vp, _i64, _i64, _vp, _i64, _i32, _vp, _i64, _vp, _i64],
+    "aclsparseMx4Dequantize": [_vp, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i32],
+    "aclsparseGroupedMMMx4": [_vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp,
+                              _i64, _i64, _vp, _i64, _i32],
+    "aclsparseAdamW": [_vp, _i64, ctypes.POINTER(AdamWTensor), ctypes.POINTER(AdamWOptions)],
+    "aclsparseAdamWMoments": [_vp, _i64, ctypes.POINTER(AdamWTensor)],
+    "aclsparseTokenLogprobs_bufferSize": [_vp, _i64, _i64, _i64, ctypes.POINTER(_sz)],
+    "aclsparseTokenLogprobs": [_vp, _i64, _i64, _vp, _i64, _i32, _vp, _i32, _vp, _vp, _vp, _i64, _vp, _vp, _vp],
+    "aclsparseTokenLogprobsGrad": [_vp, _i64, _i64, _vp, _i64, _i32, _vp, _i32, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp,
+                                   _i64],
 }
 
 _LIB = None

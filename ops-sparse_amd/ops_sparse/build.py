@@ -18,11 +18,12 @@ HEADER = os.path.join(REPO_ROOT, "include", "cann_ops_sparse.h")
 SOURCES = ["handle_descr.cpp", "spmv_host.cpp", "spmv_kernels.hip", "spmv_csc_sort.hip", "spmv_staged_kernels.hip",
            "spmv_op_host.cpp",
            "spmv_op_kernels.hip", "spmm_op_host.cpp", "spmm_op_kernels.hip", "spmv_noalloc.hip",
-           "experts_host.cpp", "experts_route.hip", "experts_combine.hip", "grouped_mm_kernels.hip"]
+           "experts_host.cpp", "experts_route.hip", "experts_combine.hip", "grouped_mm_kernels.hip",
+           "model_ops_host.cpp", "mx4_kernels.hip", "adamw_kernels.hip", "logprobs_kernels.hip"]
 OUT = os.path.join(PKG_ROOT, "lib", "libaclsparse_hip.so")
 OBJ_DIR = os.path.join(PKG_ROOT, "lib", "obj")
-# the experts' operators on torch tensors: a Python module next to the library, which itself needs no torch
-TORCH_SOURCE = "experts_torch.cpp"
+# the operators on torch tensors: a Python module next to the library, which itself needs no torch
+TORCH_SOURCES = ["experts_torch.cpp", "model_ops_torch.cpp"]
 TORCH_OUT = os.path.join(PKG_ROOT, "lib", "_ops_sparse_experts.so")
 
 HIPCC_FLAGS = [
@@ -68,8 +69,8 @@ def file_build_id(path):
     return data[j:j + 32].decode(errors="replace")
 
 
-def torch_module_command(bid):
-    """The command that compiles and links the torch module (host code only)."""
+def torch_module_commands(bid):
+    """The commands that compile the torch module's sources, and the one that links it (host code only)."""
     import sysconfig
 
     import torch
@@ -77,12 +78,14 @@ def torch_module_command(bid):
 
     includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], "/opt/rocm/include",
                 os.path.join(REPO_ROOT, "include")]
-    libs = cpp_extension.library_paths()
-    return ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1",
-            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-            f"-DACLSPARSE_HIP_BUILD_ID=\"{bid}\"", *["-isystem" + i for i in includes],
-            os.path.join(CSRC, TORCH_SOURCE), *["-L" + d for d in libs], "-lc10", "-lc10_hip", "-ltorch_cpu",
-            "-ltorch", "-ltorch_python", "-ldl", "-o", TORCH_OUT + ".tmp"]
+    compiles = [["g++", "-std=c++17", "-O2", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__=1",
+                 f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                 f"-DACLSPARSE_HIP_BUILD_ID=\"{bid}\"", *["-isystem" + i for i in includes], "-c",
+                 os.path.join(CSRC, src), "-o", os.path.join(OBJ_DIR, os.path.splitext(src)[0] + ".o")]
+                for src in TORCH_SOURCES]
+    link = ["g++", "-shared", *[c[-1] for c in compiles], *["-L" + d for d in cpp_extension.library_paths()], "-lc10",
+            "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-ldl", "-o", TORCH_OUT + ".tmp"]
+    return compiles, link
 
 
 def has_torch():
@@ -114,8 +117,9 @@ def build_library(verbose=False):
             raise RuntimeError("the compiler failed:\n" + " ".join(cmd) + "\n" + res.stdout + res.stderr)
         return cmd
 
-    with ThreadPoolExecutor(max_workers=min(len(cmds) + 1, 8)) as ex:
-        module = ex.submit(run, torch_module_command(bid)) if has_torch() else None
+    module_compiles, module_link = torch_module_commands(bid) if has_torch() else ([], None)
+    with ThreadPoolExecutor(max_workers=8) as ex:
+        module = [ex.submit(run, cmd) for cmd in module_compiles]
         for cmd in ex.map(run, cmds):
             if verbose:
                 print(" ".join(cmd))
@@ -124,8 +128,10 @@ def build_library(verbose=False):
         os.replace(OUT + ".tmp", OUT)
         if verbose:
             print(" ".join(link))
-        if module is not None:
-            module.result()
+        if module_link is not None:
+            for part in module:
+                part.result()
+            run(module_link)
             os.replace(TORCH_OUT + ".tmp", TORCH_OUT)
     return OUT
 

@@ -133,6 +133,29 @@ __device__ __forceinline__ Float4 MmaMx4(Int4 a, Int4 b, Float4 c, uint32_t scal
                                                             kB, static_cast<int>(scaleB));
 }
 
+// The same with the sum kept where it is.  The builtin may put it elsewhere, and did: the loop over a 256x256 tile then
+// moved all 128 registers of sums each turn and spilled others.  Assembly is outside the compiler's count of the wait
+// that a matrix instruction needs behind an ordinary one that wrote an operand (two states, for which the s_nop stands;
+// the instruction before it is still at work then), and of that behind the last one (SettleSums).
+template <int kA, int kB>
+__device__ __forceinline__ void AddMx4(Int4 a, Int4 b, Float4& c, uint32_t scaleA, uint32_t scaleB)
+{
+    asm volatile(
+        "s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0] "
+        "cbsz:4 blgp:4"
+        : "+v"(c)
+        : "v"(a), "v"(b), "v"(scaleA), "v"(scaleB), "n"(kA & 1), "n"(kB & 1), "n"(kA >> 1), "n"(kB >> 1));
+}
+
+// Before other instructions read the sums: a matrix instruction's result takes up to 18 states.
+template <int MI, int NI>
+__device__ __forceinline__ void SettleSums(Float4 (&acc)[MI][NI])
+{
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < MI * NI; ++i) asm volatile("" : "+v"(acc[i / NI][i % NI]));
+}
+
 // The bytes that a lane's scales of N instructions in two steps fill, as
 // dwords: instruction i's of step s at byte 2 i + s.
 template <int N>
@@ -261,8 +284,8 @@ __device__ __forceinline__ void MultiplyMx4(OperandA& a, OperandB& b, Scales& sc
             constexpr int q = decltype(at)::value, s = q / MI, i = q % MI;
             Unroll<0, NI>([&](auto column) {
                 constexpr int j = decltype(column)::value;
-                acc[i][j] = MmaMx4<j % 2 * 2 + s, i % 2 * 2 + s>(fb[s][j], fa[q % D], acc[i][j],
-                                                                 scaleB.word[j / 2], scaleA.word[i / 2]);
+                AddMx4<j % 2 * 2 + s, i % 2 * 2 + s>(fb[s][j], fa[q % D], acc[i][j], scaleB.word[j / 2],
+                                                     scaleA.word[i / 2]);
             });
             if (q < kBefore) {
                 readA(fromA, q + D);
@@ -271,9 +294,10 @@ __device__ __forceinline__ void MultiplyMx4(OperandA& a, OperandB& b, Scales& sc
                 readB(nextB, 0, (q - kBefore) * NI / D, (q - kBefore + 1) * NI / D);
             }
             if (q < MI / 2) readB(fromB, 1, q * NI / (MI / 2), (q + 1) * NI / (MI / 2));
-            constexpr int n = kLast - kFirst;
+            // close behind the barrier: what is copied last is waited for at the end of the turn
+            constexpr int n = kFirst == 0 ? (kLast + 2) / 3 : kLast - kFirst;
 #pragma unroll
-            for (int c = (q - kFirst) * copies / n; c < (q - kFirst + 1) * copies / n; ++c) copy(c);
+            for (int c = (q - kFirst) * copies / n; c < (q - kFirst + 1) * copies / n && c < copies; ++c) copy(c);
             __builtin_amdgcn_sched_barrier(0);
         });
     };
@@ -355,6 +379,7 @@ __device__ __forceinline__ void MultiplyMx4(OperandA& a, OperandB& b, Scales& sc
     for (int64_t t = 2; t < turns; ++t) turn(yes, yes);
     if (turns > 1) turn(yes, no);
     turn(no, no);
+    SettleSums(acc);
 }
 
 constexpr int kMx4TileRows = 256;

@@ -321,17 +321,7 @@ __device__ __forceinline__ void MultiplyMx4(OperandA& a, OperandB& b, Scales& sc
         scales.Commit(placesS + toS);
         toS ^= kScaleBytes;
     };
-    if (tiny) {
-        scales.LoadShort(leftS);
-    } else {
-        loadScales();
-    }
-    commitScales();
-    if (!tiny) {
-        loadScales();
-        commitScales();
-        loadScales();
-    }
+    // all loads at once, so that their latency is waited for once
     prepareA();
 #pragma unroll
     for (int i = 0; i < kCopiesA; ++i) copyA(i);
@@ -340,6 +330,20 @@ __device__ __forceinline__ void MultiplyMx4(OperandA& a, OperandB& b, Scales& sc
 #pragma unroll
     for (int i = 0; i < kCopiesB; ++i) copyB(i);
     toB ^= OperandB::kBytes;
+    if (tiny) {
+        scales.LoadShort(leftS);
+        commitScales();
+    } else {
+        Scales first = scales;
+        first.Load(leftS);
+        Scales second = first;
+        second.Load(leftS - 8);
+        leftS -= 16;
+        scales = second;
+        loadScales();
+        first.Commit(placesS);
+        second.Commit(placesS + kScaleBytes);
+    }
     Wait<0>();
     int nowA = 0, nowB = 0, nowS = 0;
     readScales(placesS);

@@ -156,65 +156,69 @@ __device__ __forceinline__ void SettleSums(Float4 (&acc)[MI][NI])
     for (int i = 0; i < MI * NI; ++i) asm volatile("" : "+v"(acc[i / NI][i % NI]));
 }
 
-// The bytes that a lane's scales of N instructions in two steps fill, as
-// dwords: instruction i's of step s at byte 2 i + s.
-template <int N>
-struct LaneScales {
-    static constexpr int kWords = (N + 1) / 2;
-    uint32_t word[kWords];
-};
-
 // The scales of a tile's operands, RA and RB rows in groups of GA and GB that
-// one wave multiplies: eight bytes per row and turn.  They are loaded into
-// registers, a thread's rows one after another over both operands, and put into
-// LDS so that a lane reads those of all its instructions at once: within a
-// group of G rows those of row 16 i + r and block 4 s + b at byte
-// (16 b + r) * G / 8 + 2 i + s.
+// one wave multiplies: sixteen bytes per row and two turns.  A load touches a
+// memory line per row, however few bytes it takes of it, so few loads of many
+// bytes are better (with eight bytes each turn, scales took a fifth of a
+// turn).  They are loaded into registers, a thread's rows one after another over
+// both operands, and put into LDS so that a lane reads those of all its
+// instructions at once: within a group of G rows, the word of row 16 i + r and
+// block b of each of the four steps lies at word (16 b + r) * G / 16 + i.
 template <int RA, int GA, int RB, int GB, int kThreads>
 struct ScaleRows {
-    static constexpr int kBytes = (RA + RB) * 8;
+    static constexpr int kBytes = (RA + RB) * 16;
     static constexpr int kLoads = (RA + RB + kThreads - 1) / kThreads;
     const uint8_t* ptr[kLoads];
-    uint64_t held[kLoads];
+    Int4 held[kLoads];
 
     // of both operands: below RA the first one's
     static __device__ __forceinline__ int Row(int i) { return i * kThreads + TeamThread<kThreads>(); }
 
-    // The next turn's, of which `blocks` are left; zeros past the row's end.  A row's last bytes are read by the eight
-    // that end there and shifted, without a branch (one in the loop made the compiler copy all sums each turn).
+    // The next two turns', of which `blocks` are left; zeros past the row's end.  A row's last bytes are read by the
+    // sixteen that end there and shifted, without a branch (one in the loop costs registers, and time each turn).
     __device__ __forceinline__ void Load(int64_t blocks)
     {
-        const int64_t over = blocks < 8 ? 8 - blocks : 0;
-        const int shift = over < 8 ? static_cast<int>(over) * 8 : 0;
-        const uint64_t mask = over < 8 ? ~uint64_t{0} : 0;
+        const int64_t over = blocks < 16 ? 16 - blocks : 0;
+        const int bits = over < 16 ? static_cast<int>(over) * 8 : 0;
+        const uint64_t mask = over < 16 ? ~uint64_t{0} : 0;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            using Bytes = int __attribute__((ext_vector_type(2), aligned(1)));
-            const Bytes v = *(const __attribute__((address_space(1))) Bytes*)(ptr[i] - over);
-            held[i] = __builtin_bit_cast(uint64_t, v) >> shift & mask;
-            ptr[i] += 8;
+            const Int4 v = LoadBytes(reinterpret_cast<const char*>(ptr[i] - over));
+            uint64_t half[2];
+            __builtin_memcpy(half, &v, 16);
+            const uint64_t low = bits >= 64 ? half[1] >> (bits & 63) : half[0] >> bits | half[1] << 1 << (63 - bits);
+            half[1] = bits >= 64 ? 0 : half[1] >> bits & mask;
+            half[0] = low & mask;
+            __builtin_memcpy(&held[i], half, 16);
+            ptr[i] += 16;
         }
     }
-    // The only turn of rows of fewer than eight.
+    // The only turns of rows of fewer than sixteen.
     __device__ __forceinline__ void LoadShort(int64_t blocks)
     {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            held[i] = 0;
+            uint64_t half[2] = {0, 0};
             for (int64_t c = 0; c < blocks; ++c) {
-                held[i] |= static_cast<uint64_t>(((const __attribute__((address_space(1))) uint8_t*)(ptr[i]))[c])
-                           << (8 * c);
+                half[c / 8] |= static_cast<uint64_t>(((const __attribute__((address_space(1))) uint8_t*)(ptr[i]))[c])
+                               << (8 * (c % 8));
             }
+            __builtin_memcpy(&held[i], half, 16);
         }
     }
     template <int G>
-    static __device__ __forceinline__ void Put(char* lds, int row, uint64_t eight)
+    static __device__ __forceinline__ void Put(char* lds, int row, const Int4& v)
     {
-        char* to = lds + row / G * (G * 8) + row % 16 * (G / 8) + row % G / 16 * 2;
+        char* to = lds + row / G * (G * 16) + row % 16 * (G / 4) + row % G / 16 * 4;
+        // a word of each block's bytes in the four steps: the transpose of 4 x 4 bytes
+        const uint32_t w[4] = {static_cast<uint32_t>(v[0]), static_cast<uint32_t>(v[1]), static_cast<uint32_t>(v[2]),
+                               static_cast<uint32_t>(v[3])};
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-            const uint64_t one = eight >> (8 * b);
-            *reinterpret_cast<uint16_t*>(to + b * (2 * G)) = static_cast<uint16_t>((one & 0xFF) | (one >> 24 & 0xFF00));
+            // bytes 0 to 3 of a selection are of the second operand, 4 to 7 of the first, 12 is zero
+            const uint32_t pair = 0x0C0C0400U + static_cast<uint32_t>(b) * 0x0101U;
+            const uint32_t low = __builtin_amdgcn_perm(w[1], w[0], pair), high = __builtin_amdgcn_perm(w[3], w[2], pair);
+            *reinterpret_cast<uint32_t*>(to + b * (4 * G)) = low | high << 16;
         }
     }
     __device__ __forceinline__ void Commit(char* lds)
@@ -225,16 +229,15 @@ struct ScaleRows {
             if (row < RA) {
                 Put<GA>(lds, row, held[i]);
             } else if (kLoads * kThreads == RA + RB || row < RA + RB) {
-                Put<GB>(lds + RA * 8, row - RA, held[i]);
+                Put<GB>(lds + RA * 16, row - RA, held[i]);
             }
         }
     }
     template <int G>
-    static __device__ __forceinline__ void Read(const char* lds, int group, LaneScales<G / 16>& s)
+    static __device__ __forceinline__ void Read(const char* lds, int group, uint32_t (&word)[G / 16])
     {
-        static_assert(G % 32 == 0, "whole words");
-        __builtin_memcpy(s.word, __builtin_assume_aligned(lds + group * (G * 8) + (threadIdx.x & 63) * (G / 8), G / 8),
-                         G / 8);
+        __builtin_memcpy(word, __builtin_assume_aligned(lds + group * (G * 16) + (threadIdx.x & 63) * (G / 4), G / 4),
+                         G / 4);
     }
 };
 
@@ -252,40 +255,39 @@ __device__ __forceinline__ void Unroll(F f)
 //
 // Like the 16-bit products' turns: two matrix steps of MI rows of products each; after a row's products come the reads
 // of the first operand D rows on and of the second operand's next step; one barrier per turn, before its last D rows.
-// Both operands have two places in LDS.  Scales are loaded three turns ahead, put into LDS a turn later and read at
-// the end of the turn before theirs, all of a turn's at once.
+// Both operands have two places in LDS.  Turns go in pairs, whose scales have one place: those of the next pair are put
+// there behind the barrier of a pair's first turn, when all waves have read this pair's, and read at the end of its
+// second; they were loaded a pair before that.
 template <int MI, int NI, typename OperandA, typename OperandB, typename Scales>
-__device__ __forceinline__ void MultiplyMx4(OperandA& a, OperandB& b, Scales& scales, char* lds,
-                                            int64_t blocks, int64_t turns, bool tiny, int rowA, int rowB,
-                                            Float4 (&acc)[MI][NI])
+__device__ __forceinline__ void MultiplyMx4(OperandA& a, OperandB& b, Scales& scales, char* lds, int64_t blocks,
+                                            int64_t turns, bool tiny, int rowA, int rowB, Float4 (&acc)[MI][NI])
 {
     constexpr int kCopiesA = OperandA::kLoads, kCopiesB = OperandB::kLoads;
     constexpr int D = MI >= 4 ? MI / 2 : 2, kRows = kSteps * MI, kBefore = kRows - D;
-    constexpr int kScaleBytes = Scales::kBytes;
     char* const placesB = lds + 2 * OperandA::kBytes;
-    char* const placesS = placesB + 2 * OperandB::kBytes;
+    char* const placeS = placesB + 2 * OperandB::kBytes;
     const int groupA = rowA / (MI * 16), groupB = rowB / (NI * 16);
     Int4 fa[D], fb[kSteps][NI];
-    LaneScales<MI> scaleA;
-    LaneScales<NI> scaleB;
+    uint32_t scaleA[MI], scaleB[NI];
     auto readA = [&](const char* from, int q) { fa[q % D] = OperandA::Read(from, rowA + q % MI * 16, q / MI); };
     auto readB = [&](const char* from, int s, int first, int last) {
 #pragma unroll
         for (int j = first; j < last; ++j) fb[s][j] = OperandB::Read(from, rowB + j * 16, s);
     };
-    auto readScales = [&](const char* from) {
-        Scales::template Read<MI * 16>(from, groupA, scaleA);
-        Scales::template Read<NI * 16>(from + OperandA::kBytes / kTurnBytes * 8, groupB, scaleB);
+    auto readScales = [&] {
+        Scales::template Read<MI * 16>(placeS, groupA, scaleA);
+        Scales::template Read<NI * 16>(placeS + OperandA::kBytes / kTurnBytes * 16, groupB, scaleB);
     };
-    auto rows = [&](auto first, auto last, const char* fromA, const char* fromB, const char* nextA, const char* nextB,
-                    int copies, auto copy) {
+    // Rows [first, last) of a pair's first or second turn, in this order to the instruction; nextA: null, or where the
+    // next turn's operands are.
+    auto rows = [&](auto second, auto first, auto last, const char* fromA, const char* fromB, const char* nextA,
+                    const char* nextB, int copies, auto copy) {
         constexpr int kFirst = decltype(first)::value, kLast = decltype(last)::value;
         Unroll<kFirst, kLast>([&](auto at) {
-            constexpr int q = decltype(at)::value, s = q / MI, i = q % MI;
+            constexpr int q = decltype(at)::value, s = q / MI, i = q % MI, byte = decltype(second)::value * 2 + s;
             Unroll<0, NI>([&](auto column) {
                 constexpr int j = decltype(column)::value;
-                AddMx4<j % 2 * 2 + s, i % 2 * 2 + s>(fb[s][j], fa[q % D], acc[i][j], scaleB.word[j / 2],
-                                                     scaleA.word[i / 2]);
+                AddMx4<byte, byte>(fb[s][j], fa[q % D], acc[i][j], scaleB[j], scaleA[i]);
             });
             if (q < kBefore) {
                 readA(fromA, q + D);
@@ -302,7 +304,7 @@ __device__ __forceinline__ void MultiplyMx4(OperandA& a, OperandB& b, Scales& sc
         });
     };
     int64_t leftA = blocks * 16, leftB = blocks * 16, leftS = blocks;
-    int toA = 0, toB = 0, toS = 0;  // places of the next copies, in bytes
+    int toA = 0, toB = 0;  // places of the next copies, in bytes
     auto copyA = [&](int i) { a.Issue(lds + toA, i); };
     auto copyB = [&](int i) { b.Issue(placesB + toB, i); };
     auto prepareA = [&] {
@@ -315,11 +317,7 @@ __device__ __forceinline__ void MultiplyMx4(OperandA& a, OperandB& b, Scales& sc
     };
     auto loadScales = [&] {
         scales.Load(leftS);
-        leftS -= 8;
-    };
-    auto commitScales = [&] {
-        scales.Commit(placesS + toS);
-        toS ^= kScaleBytes;
+        leftS -= 16;
     };
     // all loads at once, so that their latency is waited for once
     prepareA();
@@ -332,57 +330,57 @@ __device__ __forceinline__ void MultiplyMx4(OperandA& a, OperandB& b, Scales& sc
     toB ^= OperandB::kBytes;
     if (tiny) {
         scales.LoadShort(leftS);
-        commitScales();
+        scales.Commit(placeS);
     } else {
         Scales first = scales;
         first.Load(leftS);
-        Scales second = first;
-        second.Load(leftS - 8);
+        scales = first;
         leftS -= 16;
-        scales = second;
         loadScales();
-        first.Commit(placesS);
-        second.Commit(placesS + kScaleBytes);
+        first.Commit(placeS);
     }
     Wait<0>();
-    int nowA = 0, nowB = 0, nowS = 0;
-    readScales(placesS);
-    if (turns > 1) {
-        prepareB();
+    int nowA = 0, nowB = 0;
+    readScales();
+    prepareB();
 #pragma unroll
-        for (int i = 0; i < kCopiesB; ++i) copyB(i);
-    }
+    for (int i = 0; i < kCopiesB; ++i) copyB(i);
     readB(placesB, 0, 0, NI);
 #pragma unroll
     for (int q = 0; q < D; ++q) readA(lds, q);
-    // oneMore, twoMore: that many turns come after this one
-    auto turn = [&](auto oneMore, auto twoMore) {
-        constexpr bool kMore = decltype(oneMore)::value, kTwo = decltype(twoMore)::value;
+    // second: of a pair; oneMore, twoMore: that many turns come after this one
+    auto turn = [&](auto second, auto oneMore, auto twoMore) {
+        constexpr bool kSecond = decltype(second)::value, kMore = decltype(oneMore)::value,
+                       kTwo = decltype(twoMore)::value;
         const char* fromA = lds + nowA;
         const char* fromB = placesB + nowB;
         if constexpr (kMore) prepareA();
-        rows(std::integral_constant<int, 0>{}, std::integral_constant<int, kBefore>{}, fromA, fromB, nullptr, nullptr,
-             kMore ? kCopiesA : 0, copyA);
+        rows(second, std::integral_constant<int, 0>{}, std::integral_constant<int, kBefore>{}, fromA, fromB, nullptr,
+             nullptr, kMore ? kCopiesA : 0, copyA);
         toA ^= OperandA::kBytes;
         toB ^= OperandB::kBytes;
         nowA ^= OperandA::kBytes;
         nowB ^= OperandB::kBytes;
-        nowS ^= kScaleBytes;
         Wait<0>();
-        if constexpr (kTwo) {
-            commitScales();  // of the turn after the next, where this turn's were
+        if constexpr (!kSecond && kTwo) {
+            scales.Commit(placeS);
             loadScales();
-            prepareB();
         }
-        rows(std::integral_constant<int, kBefore>{}, std::integral_constant<int, kRows>{}, fromA, fromB,
+        if constexpr (kTwo) prepareB();
+        rows(second, std::integral_constant<int, kBefore>{}, std::integral_constant<int, kRows>{}, fromA, fromB,
              kMore ? lds + nowA : nullptr, placesB + nowB, kTwo ? kCopiesB : 0, copyB);
-        if constexpr (kMore) readScales(placesS + nowS);
+        if constexpr (kSecond && kMore) readScales();
     };
+    constexpr std::integral_constant<int, 0> first{};
+    constexpr std::integral_constant<int, 1> second{};
     constexpr std::true_type yes{};
     constexpr std::false_type no{};
-    for (int64_t t = 2; t < turns; ++t) turn(yes, yes);
-    if (turns > 1) turn(yes, no);
-    turn(no, no);
+    for (int64_t t = 2; t < turns; t += 2) {
+        turn(first, yes, yes);
+        turn(second, yes, yes);
+    }
+    turn(first, yes, no);
+    turn(second, no, no);
     SettleSums(acc);
 }
 
@@ -398,7 +396,7 @@ __device__ __forceinline__ void Mx4Tile(const Mx4Launch& p, char* lds, int32_t g
     using OperandA = RowOperand<int8_t, BM, kThreads, true>;
     using OperandB = RowOperand<int8_t, BN, kThreads, true>;
     using Scales = ScaleRows<BM, MI * 16, BN, NI * 16, kThreads>;
-    constexpr int kLds = 2 * (OperandA::kBytes + OperandB::kBytes + Scales::kBytes);
+    constexpr int kLds = 2 * (OperandA::kBytes + OperandB::kBytes) + Scales::kBytes;
     const int wave = TeamWave<kThreads>(), team = WaveNumber() / (kThreads / 64);
     const int rowA = (wave % WM) * MI * 16, rowB = (wave / WM) * NI * 16;
     Float4 acc[MI][NI] = {};
@@ -414,7 +412,7 @@ __device__ __forceinline__ void Mx4Tile(const Mx4Launch& p, char* lds, int32_t g
         };
         auto rowOfB = [&](int at) { return n0 + at < p.n ? n0 + at : n0; };
         // each team takes a run of turns
-        const int64_t per = ((p.blocks + 7) / 8 + kTeams - 1) / kTeams, skip = team * per * 8;
+        const int64_t per = ((p.blocks + 15) / 16 + kTeams - 1) / kTeams * 2, skip = team * per * 8;
 #pragma unroll
         for (int i = 0; i < OperandA::kLoads; ++i) {
             a.ptr[i] = reinterpret_cast<const char*>(p.a.codes) + rowOfA(OperandA::Row(i)) * p.a.ld +
@@ -431,7 +429,7 @@ __device__ __forceinline__ void Mx4Tile(const Mx4Launch& p, char* lds, int32_t g
             scale.ptr[i] = skip + (row < BM ? p.a.scales + rowOfA(row) * p.a.ld_scales
                                             : scales + rowOfB(column) * p.b.ld_scales);
         }
-        MultiplyMx4<MI, NI>(a, b, scale, lds + team * kLds, p.blocks - skip, per, p.blocks < 8, rowA, rowB,
+        MultiplyMx4<MI, NI>(a, b, scale, lds + team * kLds, p.blocks - skip, per, p.blocks < 16, rowA, rowB,
                             acc);
     }
     if (!JoinTeams<kTeams, kThreads, (kTeams - 1) * kLds>(lds + kLds, acc)) return;
@@ -447,7 +445,7 @@ __device__ __forceinline__ void Mx4Tile(const Mx4Launch& p, char* lds, int32_t g
 template <typename TOut>
 __global__ __launch_bounds__(512, 1) void Mx4TileKernel(Mx4Launch p, int32_t tilesN, int32_t cus)
 {
-    __shared__ __align__(128) char lds[2 * (kMx4TileRows + 256) * (kTurnBytes + 8)];
+    __shared__ __align__(128) char lds[(kMx4TileRows + 256) * (2 * kTurnBytes + 16)];
     const RaggedTiles tiles(p.offsets, p.rows, p.groups, kMx4TileRows);
     const TileShare share = ShareOfWorkgroup(static_cast<int64_t>(tiles.total) * tilesN, cus);
     if (share.tile < 0) return;
@@ -470,7 +468,7 @@ __global__ __launch_bounds__(512, 1) void Mx4TileKernel(Mx4Launch p, int32_t til
 
 // Tiles of 64x128 for groups of few rows: three workgroups per CU, or one whose
 // three teams share a tile's contraction.
-constexpr int kMx4SmallBytes = 2 * (64 + 128) * (kTurnBytes + 8);
+constexpr int kMx4SmallBytes = (64 + 128) * (2 * kTurnBytes + 16);
 template <typename TOut, int kTeams>
 __global__ __launch_bounds__(kTeams * 256, 3) void Mx4SmallTileKernel(Mx4Launch p, int32_t tilesN)
 {

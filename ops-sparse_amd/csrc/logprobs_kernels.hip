@@ -45,6 +45,18 @@ struct Part {
     }
 };
 
+constexpr int kQuadXor1 = 0xB1, kQuadXor2 = 0x4E;
+__device__ __forceinline__ float QuadMax(float x)
+{
+    x = fmaxf(x, __uint_as_float(Dpp<kQuadXor1, 0xF>(__float_as_uint(x), __float_as_uint(x))));
+    return fmaxf(x, __uint_as_float(Dpp<kQuadXor2, 0xF>(__float_as_uint(x), __float_as_uint(x))));
+}
+__device__ __forceinline__ uint32_t QuadSum(uint32_t x)
+{
+    x += Dpp<kQuadXor1, 0xF>(x, x);
+    return x + Dpp<kQuadXor2, 0xF>(x, x);
+}
+
 // The parts of a wave's lanes as one, in all lanes
 __device__ __forceinline__ Part WavePart(Part p)
 {
@@ -73,14 +85,12 @@ __device__ __forceinline__ uint64_t Pair(float v, int32_t index)
 __device__ __forceinline__ int32_t PairIndex(uint64_t pair) { return static_cast<int32_t>(~static_cast<uint32_t>(pair)); }
 __device__ __forceinline__ float PairValue(uint64_t pair) { return KeyValue(static_cast<uint32_t>(pair >> 32)); }
 
+// The largest of a wave's lanes: of the high halves, then of the low ones of the lanes that have it.
 __device__ __forceinline__ uint64_t WaveMaxU64(uint64_t x)
 {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-        const uint64_t y = __shfl_xor(static_cast<unsigned long long>(x), d);
-        x = x > y ? x : y;
-    }
-    return x;
+    const uint32_t high = WaveMaxU32(static_cast<uint32_t>(x >> 32));
+    const uint32_t low = WaveMaxU32(static_cast<uint32_t>(x >> 32) == high ? static_cast<uint32_t>(x) : 0U);
+    return static_cast<uint64_t>(high) << 32 | low;
 }
 
 // Logits [c, c + 8) of a row's first `end`; -inf past them.
@@ -152,7 +162,7 @@ __device__ __forceinline__ void WriteRow(const LogprobsLaunch& p, int64_t row, c
 
 struct Shared {
     Part part[kWaves];
-    uint64_t pair[kCandidates];  // candidates; before that each thread's largest
+    uint64_t pair[kCandidates];  // candidates; before that each quad's largest
     uint64_t best[kWaves];
     uint32_t count;
     float threshold;
@@ -161,8 +171,8 @@ struct Shared {
 // The k largest of logits [begin, end), first ones first; write(rank, pair)
 // for each, fewer than k where fewer are above -inf.  m: the thread's largest.
 //
-// The k-th largest of the threads' largest is a bound below which the answer
-// has nothing: those threads hold k logits at or above it.  A second pass lists
+// The k-th largest of 64 quads' largest is a bound below which the answer has
+// nothing: those quads hold k logits at or above it.  A second pass lists
 // what is at or above the bound, mostly little more than k logits, and each finds
 // its rank by comparing itself with all.  A row with NaN, or with more logits
 // at the bound than fit (equal ones), goes through k passes instead.
@@ -170,14 +180,19 @@ template <typename T, typename Write>
 __device__ __forceinline__ void TakeTop(Shared& sh, const T* row, int32_t begin, int32_t end, int32_t k, float m,
                                         bool nan, Write write)
 {
+    static_assert(kThreads == 4 * kMaxTop, "as many quads as there can be alternatives");
     const int tid = threadIdx.x;
-    sh.pair[tid] = Pair(m, tid);
+    m = QuadMax(m);
+    if ((tid & 3) == 0) sh.pair[tid >> 2] = Pair(m, tid >> 2);
     if (tid == 0) sh.count = 0;
     __syncthreads();
-    int rank = 0;
-    const uint64_t mine = sh.pair[tid];
-    for (int i = 0; i < kThreads; ++i) rank += sh.pair[i] > mine ? 1 : 0;
-    if (rank == k - 1) sh.threshold = m;
+    // each lane of a quad compares the quad's with a quarter of the others
+    uint32_t rank = 0;
+    const uint64_t mine = sh.pair[tid >> 2];
+#pragma unroll
+    for (int i = 0; i < kMaxTop / 4; ++i) rank += sh.pair[(tid & 3) * (kMaxTop / 4) + i] > mine ? 1 : 0;
+    rank = QuadSum(rank);
+    if (rank == static_cast<uint32_t>(k) - 1 && (tid & 3) == 0) sh.threshold = m;
     __syncthreads();
     const float threshold = sh.threshold;
     if (!nan) {
@@ -237,10 +252,14 @@ __device__ __forceinline__ void WriteTop(const LogprobsLaunch& p, int64_t row, i
     p.top_logprobs[row * p.top + rank] = pair == 0 ? -Infinity() : (PairValue(pair) - m) - logs;
 }
 
-// A segment's record in the buffer: its part, and its k largest
-__device__ __forceinline__ char* Record(const LogprobsLaunch& p, int64_t row, int32_t segments, int32_t segment)
+// The buffer: a part for each segment of each row, then the k largest of each.
+__device__ __forceinline__ Part* PartOf(const LogprobsLaunch& p, int64_t at)
 {
-    return static_cast<char*>(p.buffer) + (row * segments + segment) * (16 + 8 * p.top);
+    return reinterpret_cast<Part*>(static_cast<char*>(p.buffer) + at * 16);
+}
+__device__ __forceinline__ uint64_t* PairsOf(const LogprobsLaunch& p, int64_t at, int32_t segments)
+{
+    return reinterpret_cast<uint64_t*>(static_cast<char*>(p.buffer) + p.rows * segments * 16) + at * p.top;
 }
 
 template <typename T, bool kEntropy>
@@ -278,49 +297,69 @@ __global__ __launch_bounds__(kThreads) void LogprobsKernel(LogprobsLaunch p, int
         }
         return;
     }
-    char* record = Record(p, row, segments, segment);
-    if (threadIdx.x == 0) *reinterpret_cast<Part*>(record) = all;
+    const int64_t at = row * segments + segment;
+    if (threadIdx.x == 0) *PartOf(p, at) = all;
     if (p.top > 0) {
-        auto* pairs = reinterpret_cast<uint64_t*>(record + 16);
+        uint64_t* pairs = PairsOf(p, at, segments);
         TakeTop(sh, logits, begin, end, static_cast<int32_t>(p.top), mine.m, all.s != all.s,
                 [&](int32_t rank, uint64_t pair) { pairs[rank] = pair; });
     }
 }
 
-// Joins a row's segments, one per lane of a wave; of the sorted lists the
-// largest head is taken k times.
+// Joins a row's segments, one per lane of the first wave; of the sorted lists the
+// largest head is taken k times.  All waves bring the lists to LDS, and a lane
+// holds its head and the one behind it: a step waits for no memory.
 template <typename T>
-__global__ __launch_bounds__(64) void LogprobsJoinKernel(LogprobsLaunch p, int32_t segments)
+__global__ __launch_bounds__(kThreads) void LogprobsJoinKernel(LogprobsLaunch p, int32_t segments)
 {
+    __shared__ uint64_t list[kMaxSegments * kMaxTop];
     const int64_t row = BlockNumber();
     if (row >= p.rows) return;
-    const int lane = threadIdx.x;
-    const bool mine = lane < segments;
-    const char* record = Record(p, row, segments, mine ? lane : 0);
+    const int tid = threadIdx.x;
+    const int32_t k = static_cast<int32_t>(p.top);
+    const bool mine = tid < segments;
     Part part{kLowest, 0.0f, 0.0f};
-    if (mine) part = *reinterpret_cast<const Part*>(record);
+    if (mine) part = *PartOf(p, row * segments + tid);
+    if (k > 0) {
+        const uint64_t* pairs = PairsOf(p, row * segments, segments);
+        constexpr int kEach = kMaxSegments * kMaxTop / kThreads;
+        uint64_t held[kEach];
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            if (i * kThreads + tid < segments * k) held[i] = pairs[i * kThreads + tid];
+        }
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            if (i * kThreads + tid < segments * k) list[i * kThreads + tid] = held[i];
+        }
+        __syncthreads();
+    }
+    if (tid >= 64) return;
     part = WavePart(part);
     const RowResult r = Finish(part);
-    if (lane == 0) WriteRow<T>(p, row, part, r);
-    if (p.top == 0) return;
-    const auto* pairs = reinterpret_cast<const uint64_t*>(record + 16);
-    const int32_t k = static_cast<int32_t>(p.top);
-    int32_t at = 0;
-    uint64_t head = mine ? pairs[0] : 0;
+    if (tid == 0) WriteRow<T>(p, row, part, r);
+    if (k == 0) return;
+    int32_t at = tid * k + 1;
+    const int32_t end = mine ? tid * k + k : 0;
+    uint64_t head = mine ? list[tid * k] : 0, next = at < end ? list[at] : 0, taken = 0;
     for (int32_t rank = 0; rank < k; ++rank) {
         const uint64_t best = WaveMaxU64(head);
-        if (lane == 0) WriteTop(p, row, rank, best, r.m, r.logs);
-        if (best != 0 && head == best) {
+        if (tid == rank) taken = best;
+        if (head == best) {  // one lane's, unless nothing is left
+            head = next;
             ++at;
-            head = at < k ? pairs[at] : 0;
+            next = at < end ? list[at] : 0;
         }
     }
+    if (tid < k) WriteTop(p, row, tid, taken, r.m, r.logs);
 }
+
+constexpr int32_t kGradLength = kThreads * kUnit * kBatch;  // of a row that a workgroup takes
 
 // The gradient of one part of a row.  Columns that a token or an alternative
 // names are written again, after the others, with what they have besides.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void LogprobsGradKernel(LogprobsGradLaunch p, int32_t segments, int32_t length)
+__global__ __launch_bounds__(kThreads) void LogprobsGradKernel(LogprobsGradLaunch p, int32_t segments)
 {
     __shared__ int32_t column[kMaxTop + 1];
     __shared__ float weight[kMaxTop + 1];
@@ -329,7 +368,7 @@ __global__ __launch_bounds__(kThreads) void LogprobsGradKernel(LogprobsGradLaunc
     if (row >= p.rows) return;
     const int32_t segment = static_cast<int32_t>(number % static_cast<uint32_t>(segments));
     const int32_t vocab = static_cast<int32_t>(p.vocab), k = p.grad_top != nullptr ? static_cast<int32_t>(p.top) : 0;
-    const int32_t begin = segment * length, end = vocab - begin < length ? vocab : begin + length;
+    const int32_t begin = segment * kGradLength, end = vocab - begin < kGradLength ? vocab : begin + kGradLength;
     const T* logits = static_cast<const T*>(p.logits) + row * p.ld;
     T* grad = static_cast<T*>(p.grad) + row * p.ld_grad;
     const int tid = threadIdx.x;
@@ -358,17 +397,20 @@ __global__ __launch_bounds__(kThreads) void LogprobsGradKernel(LogprobsGradLaunc
         const float d = (x - m) - logs;
         return -Exp2(d * kLog2E) * (total + gh * (fmaxf(d, kFar) + h));
     };
-    for (int32_t c = begin + tid * kUnit; c < end; c += kThreads * kUnit) {
-        T v[kUnit];
-        LoadUnit(logits, c, end, v);
+    T v[kBatch][kUnit];
 #pragma unroll
-        for (int i = 0; i < kUnit; ++i) v[i] = FromFloat<T>(one(ToFloat(v[i])));
+    for (int b = 0; b < kBatch; ++b) LoadUnit(logits, begin + (b * kThreads + tid) * kUnit, end, v[b]);
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+        const int32_t c = begin + (b * kThreads + tid) * kUnit;
+#pragma unroll
+        for (int i = 0; i < kUnit; ++i) v[b][i] = FromFloat<T>(one(ToFloat(v[b][i])));
         if (c + kUnit <= end) {
-            __builtin_memcpy(grad + c, v, sizeof(v));
+            __builtin_memcpy(grad + c, v[b], sizeof(v[b]));
         } else {
 #pragma unroll
             for (int i = 0; i < kUnit; ++i) {
-                if (c + i < end) grad[c + i] = v[i];
+                if (c + i < end) grad[c + i] = v[b][i];
             }
         }
     }
@@ -412,17 +454,16 @@ int LaunchTyped(const LogprobsLaunch& l, hipStream_t s)
     const dim3 grid = GridOf(l.rows * segments);
     if (l.entropy != nullptr) LogprobsKernel<T, true><<<grid, kThreads, 0, s>>>(l, segments, length);
     else LogprobsKernel<T, false><<<grid, kThreads, 0, s>>>(l, segments, length);
-    if (segments > 1) LogprobsJoinKernel<T><<<GridOf(l.rows), 64, 0, s>>>(l, segments);
+    if (segments > 1) LogprobsJoinKernel<T><<<GridOf(l.rows), kThreads, 0, s>>>(l, segments);
     return 0;
 }
 
 template <typename T>
 int LaunchGradTyped(const LogprobsGradLaunch& l, hipStream_t s)
 {
-    constexpr int32_t kLength = kThreads * kUnit * 4;
-    const int64_t segments = (l.vocab + kLength - 1) / kLength;
+    const int64_t segments = (l.vocab + kGradLength - 1) / kGradLength;
     if (l.rows > INT32_MAX / segments) return kTooLarge;
-    LogprobsGradKernel<T><<<GridOf(l.rows * segments), kThreads, 0, s>>>(l, static_cast<int32_t>(segments), kLength);
+    LogprobsGradKernel<T><<<GridOf(l.rows * segments), kThreads, 0, s>>>(l, static_cast<int32_t>(segments));
     return 0;
 }
 

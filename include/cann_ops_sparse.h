@@ -525,7 +525,8 @@ typedef struct aclsparseAdamWOptions_t {
     double lr, beta1, beta2, eps, weightDecay;
     const float* lrDevice;   /* null, or the rate in device memory, read when the step runs */
     const float* gradScale;  /* null, or a factor of all gradients in device memory */
-    int32_t* step;           /* two counts in device memory: the steps taken, which the call counts up, and zero */
+    int32_t* step;           /* the steps taken, in device memory; the call counts it up */
+    void* buffer;            /* 64 bytes of device memory that the call works in (those in flight need their own) */
     uint32_t seed;           /* of the rounding of 8-bit moments */
     int32_t momentBits;      /* 32 or 8 */
 } aclsparseAdamWOptions_t;

@@ -25,29 +25,28 @@ static_assert(kAdamWChunk == kThreads * 8, "eight values per thread");
 // never negative, 5 and 3.  The least exponents leave room above the largest
 // value, which lies under 2: rounding up from it never leaves the format.
 // Codes under 8 are subnormal.
+//
+// A magnitude's bits, moved to the last three of fp32's exponent's bits and
+// the first three behind it, are a float 2^(126 + least) times too small,
+// subnormal where the code is: one product decodes or aligns both kinds.
 constexpr int kLeastM = -13, kLeastV = -29;
 
 template <int kLeast>
-__device__ __forceinline__ float Decode8(uint32_t magnitude)
+__device__ __forceinline__ float Decode8(uint32_t bits)  // of the magnitude, from bit 20 on, and the sign
 {
-    const float small = static_cast<float>(magnitude) * __uint_as_float((127U + kLeast - 3) << 23);
-    const float normal = __uint_as_float((magnitude << 20) + ((126U + kLeast) << 23));
-    return magnitude < 8 ? small : normal;
+    return __uint_as_float(bits) * __uint_as_float(static_cast<uint32_t>(253 + kLeast) << 23);
 }
 
 // The code of a in [0, 2), rounded up with the probability of what lies behind
-// its bits, by 16 random ones.  Rounding to the nearest would lose the slow
-// changes that the moments are made of: beta2 = 0.999 moves v by a hundredth of
-// the distance between two codes.
+// its bits, by 16 random ones (at bit 4; with 8 they are the middle of their
+// range).  Rounding to the nearest would lose the slow changes that the moments
+// are made of: beta2 = 0.999 moves v by a hundredth of the distance between two
+// codes.
 template <int kLeast>
 __device__ __forceinline__ uint32_t Encode8(float a, uint32_t random)
 {
-    constexpr uint32_t kFirst = static_cast<uint32_t>(kLeast + 127) << 3;
-    const uint32_t add = (random << 4) + 8;
-    const float least = __uint_as_float((127U + kLeast) << 23);
-    const uint32_t normal = ((__float_as_uint(a) + add) >> 20) - kFirst + 8;
-    const uint32_t small = ((__float_as_uint(a + least) + add) >> 20) - kFirst;
-    return a < least ? small : normal;
+    const float aligned = a * __uint_as_float(static_cast<uint32_t>(1 - kLeast) << 23);
+    return (__float_as_uint(aligned) + random + 8) >> 20;
 }
 
 __device__ __forceinline__ float Power(uint32_t e)  // 2^(e - 127), NaN for 255
@@ -74,10 +73,22 @@ __device__ __forceinline__ uint32_t Mix(uint32_t x)
     return x ^ (x >> 16);
 }
 
-// What all values of a launch share
+// What all values of a step share, in the caller's buffer
 struct Factors {
-    float beta1, rest1, beta2, rest2, decay, size, root, eps, scale;
+    float beta1, rest1, beta2, rest2, decay, size, inverse_root, eps, scale;
+    uint32_t key;
 };
+static_assert(sizeof(Factors) <= kAdamWBufferBytes, "");
+
+// size * m / (sqrt(v) / root + eps), to 11 roundings: the square root and the
+// reciprocal are the instructions' (one unit in the last place each).  They
+// take no subnormal numbers, so v is at least the least normal one: its root is
+// under 2^-62, which an eps of 1e-8 does not see.
+__device__ __forceinline__ float Change(const Factors& f, float m, float v)
+{
+    const float root = __builtin_amdgcn_sqrtf(fmaxf(v, 1.17549435e-38f));
+    return f.size * (m * __builtin_amdgcn_rcpf(root * f.inverse_root + f.eps));
+}
 
 __device__ __forceinline__ double IntPower(double base, int32_t n)
 {
@@ -89,223 +100,221 @@ __device__ __forceinline__ double IntPower(double base, int32_t n)
     return r;
 }
 
-// Eight elements from `at` on, of which `left` are the tensor's.
-template <typename T>
-__device__ __forceinline__ void Load8(const T* from, int64_t left, float (&v)[8])
+// Counts the step and works out its factors, in 64 bits: done by each workgroup
+// of the step itself they took as long as its values.
+__global__ void AdamWFactorsKernel(AdamWScalars s, Factors* out)
 {
-    T t[8];
-    if (left >= 8) {
+    const int32_t step = s.step[0] + 1;
+    const double lr = s.lr_device != nullptr ? static_cast<double>(*s.lr_device) : s.lr;
+    Factors f;
+    f.beta1 = static_cast<float>(s.beta1);
+    f.rest1 = static_cast<float>(1.0 - s.beta1);
+    f.beta2 = static_cast<float>(s.beta2);
+    f.rest2 = static_cast<float>(1.0 - s.beta2);
+    f.decay = static_cast<float>(1.0 - lr * s.weight_decay);
+    f.size = static_cast<float>(lr / (1.0 - IntPower(s.beta1, step)));
+    f.inverse_root = static_cast<float>(1.0 / sqrt(1.0 - IntPower(s.beta2, step)));
+    f.eps = static_cast<float>(s.eps);
+    f.scale = s.grad_scale != nullptr ? *s.grad_scale : 1.0f;
+    f.key = Mix(Mix(s.seed) + static_cast<uint32_t>(step));
+    *out = f;
+    s.step[0] = step;
+}
+
+// V elements, of which `left` are the tensor's.
+template <typename T, int V>
+__device__ __forceinline__ void Load(const T* from, int64_t left, float (&v)[V])
+{
+    T t[V];
+    if (left >= V) {
         __builtin_memcpy(t, from, sizeof(t));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = ToFloat(t[i]);
+        for (int i = 0; i < V; ++i) v[i] = ToFloat(t[i]);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < left ? ToFloat(from[i]) : 0.0f;
+        for (int i = 0; i < V; ++i) v[i] = i < left ? ToFloat(from[i]) : 0.0f;
     }
 }
-template <typename T>
-__device__ __forceinline__ void Store8(T* to, int64_t left, const float (&v)[8])
+template <typename T, int V>
+__device__ __forceinline__ void Store(T* to, int64_t left, const float (&v)[V])
 {
-    T t[8];
+    T t[V];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = FromFloat<T>(v[i]);
-    if (left >= 8) {
+    for (int i = 0; i < V; ++i) t[i] = FromFloat<T>(v[i]);
+    if (left >= V) {
         __builtin_memcpy(to, t, sizeof(t));
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < V; ++i) {
             if (i < left) to[i] = t[i];
         }
     }
 }
 
-template <int kLeast, bool kSigned>
-__device__ __forceinline__ void Unpack(const uint8_t* codes, uint32_t e, float (&v)[8])
+// V codes from one or two words
+template <int kLeast, bool kSigned, int V>
+__device__ __forceinline__ void Unpack(const uint8_t* codes, uint32_t e, float (&v)[V])
 {
-    uint8_t c[8];
-    __builtin_memcpy(c, __builtin_assume_aligned(codes, 8), 8);
+    uint32_t word[V / 4];
+    __builtin_memcpy(word, __builtin_assume_aligned(codes, V), V);
     const float scale = Power(e);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < V; ++i) {
+        uint32_t bits;
         if constexpr (kSigned) {
-            const float a = Decode8<kLeast>(c[i] & 127U);
-            v[i] = (c[i] >= 128 ? -a : a) * scale;
+            bits = static_cast<uint32_t>(static_cast<int32_t>(word[i / 4] << (24 - i % 4 * 8)) >> 4) & 0x87F00000U;
         } else {
-            v[i] = Decode8<kLeast>(c[i]) * scale;
+            bits = (word[i / 4] >> (i % 4 * 8) & 0xFFU) << 20;
         }
+        v[i] = Decode8<kLeast>(bits) * scale;
     }
 }
 
-// shift: of the random bits
+// bits: those of the random numbers that are used, the 16 low ones or the high ones
 template <int kLeast, bool kSigned>
-__device__ __forceinline__ void Pack(const float (&v)[8], const uint32_t (&random)[8], int shift, uint8_t* codes,
-                                     uint8_t* exponent)
+__device__ __forceinline__ void Pack(const float (&v)[8], const uint32_t (&random)[8], uint8_t* codes, uint8_t* exponent)
 {
     uint32_t most = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const uint32_t bits = __float_as_uint(v[i]) & 0x7FFFFFFFU;
+        // v has no sign but NaN's, which the exponent's bits leave out
+        const uint32_t bits = kSigned ? __float_as_uint(v[i]) & 0x7FFFFFFFU : __float_as_uint(v[i]);
         most = bits > most ? bits : most;
     }
-    const uint32_t e = QuadMax(most) >> 23;
+    const uint32_t e = QuadMax(most) >> 23 & 0xFFU;
     // a block that holds infinity or NaN is NaN
-    const float inverse = e == 255 ? 0.0f : e == 254 ? __uint_as_float(0x00400000U) : __uint_as_float((254U - e) << 23);
-    uint8_t c[8];
+    const float inverse = e >= 254 ? __uint_as_float(e == 254 ? 0x00400000U : 0) : __uint_as_float((254U - e) << 23);
+    uint32_t word[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float a = __uint_as_float(__float_as_uint(v[i]) & 0x7FFFFFFFU) * inverse;
-        uint32_t code = Encode8<kLeast>(a, random[i] >> shift & 0xFFFF);
+        const float a = fabsf(v[i]) * inverse;
+        const uint32_t draw = (kSigned ? random[i] << 4 : random[i] >> 12) & 0xFFFF0U;
+        uint32_t code = Encode8<kLeast>(a, draw);
         if constexpr (kSigned) {
-            code |= __float_as_uint(v[i]) >> 31 << 7;
+            code |= __float_as_uint(v[i]) >> 24 & 0x80U;
         } else {
-            if (code == 0 && a > 0.0f) code = 1;  // a v of zero under an m that is none would make the step m / eps
+            // a v of zero under an m that is none would make the step m / eps
+            const uint32_t some = __float_as_uint(a) < 1U ? __float_as_uint(a) : 1U;
+            code = code > some ? code : some;
         }
-        c[i] = static_cast<uint8_t>(e == 255 ? 0 : code);
+        word[i / 4] |= code << (i % 4 * 8);
     }
-    __builtin_memcpy(__builtin_assume_aligned(codes, 8), c, 8);
+    if (e == 255) word[0] = word[1] = 0;
+    __builtin_memcpy(__builtin_assume_aligned(codes, 8), word, 8);
     if ((threadIdx.x & 3) == 0) *exponent = static_cast<uint8_t>(e);
 }
 
-// A thread takes eight neighbouring values, so a quad a block; a workgroup
-// 2048 at a time.  The chunks of all tensors are numbered in one row, and each
-// wave finds a chunk's tensor by one comparison per lane.
-//
-// The step is counted on the device, so that a captured step counts with each
-// replay: every workgroup reads it first, and the last to finish writes it.
+// A workgroup takes 2048 values: with 8-bit moments a thread eight neighbouring
+// ones, so a quad a block, otherwise four in each half.  The chunks of all
+// tensors are numbered in one row, and each wave finds a chunk's tensor by one
+// comparison per lane.
 template <typename TP, typename TG, int kBits, bool kMaster>
-__global__ __launch_bounds__(kThreads) void AdamWKernel(AdamWTable table, AdamWScalars s)
+__global__ __launch_bounds__(kThreads) void AdamWKernel(AdamWTable table, const Factors* __restrict__ factors)
 {
 #pragma clang fp contract(off)
-    const int32_t step = s.step[0] + 1;
-    Factors f;
-    {
-        const double lr = s.lr_device != nullptr ? static_cast<double>(*s.lr_device) : s.lr;
-        f.beta1 = static_cast<float>(s.beta1);
-        f.rest1 = static_cast<float>(1.0 - s.beta1);
-        f.beta2 = static_cast<float>(s.beta2);
-        f.rest2 = static_cast<float>(1.0 - s.beta2);
-        f.decay = static_cast<float>(1.0 - lr * s.weight_decay);
-        f.size = static_cast<float>(lr / (1.0 - IntPower(s.beta1, step)));
-        f.root = static_cast<float>(sqrt(1.0 - IntPower(s.beta2, step)));
-        f.eps = static_cast<float>(s.eps);
-        f.scale = s.grad_scale != nullptr ? *s.grad_scale : 1.0f;
-    }
-    const uint32_t key = Mix(Mix(s.seed) + static_cast<uint32_t>(step));
-    const int lane = threadIdx.x & 63;
-    const uint32_t first = table.first[lane];
-    for (uint32_t chunk = blockIdx.x; chunk < table.chunks; chunk += gridDim.x) {
-        const int which = __popcll(__ballot(first <= chunk)) - 1;
-        const AdamWTensor& t = table.tensor[which];
-        const int64_t at = static_cast<int64_t>(chunk - table.first[which]) * kAdamWChunk + threadIdx.x * 8;
-        const int64_t left = t.count - at, padded = (t.count + 31) / 32 * 32;
+    constexpr int V = kBits == 8 ? 8 : 4, kUnits = 8 / V;
+    const uint32_t first = table.first[threadIdx.x & 63], chunk = blockIdx.x;
+    const int which = __popcll(__ballot(first <= chunk)) - 1;
+    const AdamWTensor& t = table.tensor[which];
+    const int64_t begin = static_cast<int64_t>(chunk - table.first[which]) * kAdamWChunk + threadIdx.x * V;
+    const int64_t padded = (t.count + 31) / 32 * 32;
+    float g[kUnits][V], p[kUnits][V], m[kUnits][V], v[kUnits][V];
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+        const int64_t at = begin + u * kThreads * V, left = t.count - at;
         if (at >= padded) continue;  // whole quads
-        float g[8], p[8], m[8], v[8];
-        Load8(static_cast<const TG*>(t.grad) + at, left, g);
+        Load(static_cast<const TG*>(t.grad) + at, left, g[u]);
         if constexpr (kMaster) {
-            Load8(t.master + at, left, p);
+            Load(t.master + at, left, p[u]);
         } else {
-            Load8(static_cast<const TP*>(t.param) + at, left, p);
-        }
-        uint8_t *codesM = nullptr, *codesV = nullptr, *expM = nullptr, *expV = nullptr;
-        float *heldM = nullptr, *heldV = nullptr;
-        if constexpr (kBits == 8) {
-            codesM = static_cast<uint8_t*>(t.moments) + at;
-            codesV = codesM + padded;
-            expM = t.exponents + at / 32;
-            expV = expM + padded / 32;
-            Unpack<kLeastM, true>(codesM, *expM, m);
-            Unpack<kLeastV, false>(codesV, *expV, v);
-        } else {
-            heldM = static_cast<float*>(t.moments) + at;
-            heldV = heldM + padded;
-            __builtin_memcpy(m, heldM, sizeof(m));
-            __builtin_memcpy(v, heldV, sizeof(v));
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float grad = g[i] * f.scale;
-            const float keptM = m[i] * f.beta1, newM = grad * f.rest1;
-            m[i] = keptM + newM;
-            const float keptV = v[i] * f.beta2, square = grad * grad, newV = square * f.rest2;
-            v[i] = keptV + newV;
-            const float denominator = sqrtf(v[i]) / f.root + f.eps;
-            const float kept = p[i] * f.decay, change = f.size * (m[i] / denominator);
-            p[i] = kept - change;
+            Load(static_cast<const TP*>(t.param) + at, left, p[u]);
         }
         if constexpr (kBits == 8) {
-            // past the tensor's end the block holds zeros
+            const uint8_t* codes = static_cast<const uint8_t*>(t.moments) + at;
+            Unpack<kLeastM, true>(codes, t.exponents[at / 32], m[u]);
+            Unpack<kLeastV, false>(codes + padded, t.exponents[(padded + at) / 32], v[u]);
+        } else {
+            const float* held = static_cast<const float*>(t.moments) + at;
+            __builtin_memcpy(m[u], held, sizeof(m[u]));
+            __builtin_memcpy(v[u], held + padded, sizeof(v[u]));
+        }
+    }
+    const Factors f = *factors;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (i >= left) m[i] = v[i] = 0.0f;
+    for (int u = 0; u < kUnits; ++u) {
+        const int64_t at = begin + u * kThreads * V, left = t.count - at;
+        if (at >= padded) continue;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float grad = g[u][i] * f.scale;
+            const float keptM = m[u][i] * f.beta1, newM = grad * f.rest1;
+            m[u][i] = keptM + newM;
+            const float keptV = v[u][i] * f.beta2, square = grad * grad, newV = square * f.rest2;
+            v[u][i] = keptV + newV;
+            const float kept = p[u][i] * f.decay, change = Change(f, m[u][i], v[u][i]);
+            p[u][i] = kept - change;
+        }
+        if constexpr (kBits == 8) {
+            if (left < V) {  // past the tensor's end the block holds zeros
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    if (i >= left) m[u][i] = v[u][i] = 0.0f;
+                }
             }
-            uint32_t random[8];
-            const uint32_t low = static_cast<uint32_t>(at);
-            const uint32_t seed = Mix(key + static_cast<uint32_t>(table.place[which]) +
+            uint32_t random[V];
+            const uint32_t seed = Mix(f.key + static_cast<uint32_t>(table.place[which]) +
                                       static_cast<uint32_t>(static_cast<uint64_t>(at) >> 32));
 #pragma unroll
-            for (int i = 0; i < 8; ++i) random[i] = Mix(low + i + seed);
-            Pack<kLeastM, true>(m, random, 0, codesM, expM);
-            Pack<kLeastV, false>(v, random, 16, codesV, expV);
+            for (int i = 0; i < V; ++i) random[i] = Mix(static_cast<uint32_t>(at) + i + seed);
+            uint8_t* codes = static_cast<uint8_t*>(t.moments) + at;
+            Pack<kLeastM, true>(m[u], random, codes, t.exponents + at / 32);
+            Pack<kLeastV, false>(v[u], random, codes + padded, t.exponents + (padded + at) / 32);
         } else {
-            Store8(heldM, left, m);
-            Store8(heldV, left, v);
+            float* held = static_cast<float*>(t.moments) + at;
+            Store(held, left, m[u]);
+            Store(held + padded, left, v[u]);
         }
-        if constexpr (kMaster) Store8(t.master + at, left, p);
-        Store8(static_cast<TP*>(t.param) + at, left, p);
-    }
-    if (!s.last) return;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        const int32_t done = __hip_atomic_fetch_add(&s.step[1], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (done == static_cast<int32_t>(gridDim.x) - 1) {
-            __hip_atomic_store(&s.step[0], step, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __hip_atomic_store(&s.step[1], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
+        if constexpr (kMaster) Store(t.master + at, left, p[u]);
+        Store(static_cast<TP*>(t.param) + at, left, p[u]);
     }
 }
 
+// Four codes per thread, so that neighbouring lanes write neighbouring places.
 __global__ __launch_bounds__(kThreads) void AdamWMomentsKernel(AdamWTable table)
 {
-    const int lane = threadIdx.x & 63;
-    const uint32_t first = table.first[lane];
-    for (uint32_t chunk = blockIdx.x; chunk < table.chunks; chunk += gridDim.x) {
-        const int which = __popcll(__ballot(first <= chunk)) - 1;
-        const AdamWTensor& t = table.tensor[which];
-        const int64_t at = static_cast<int64_t>(chunk - table.first[which]) * kAdamWChunk + threadIdx.x * 8;
-        const int64_t left = t.count - at, padded = (t.count + 31) / 32 * 32;
-        if (left <= 0) continue;
-        const uint8_t* codes = static_cast<const uint8_t*>(t.moments) + at;
-        const uint8_t* exponent = t.exponents + at / 32;
-        float m[8], v[8];
-        Unpack<kLeastM, true>(codes, *exponent, m);
-        Unpack<kLeastV, false>(codes + padded, exponent[padded / 32], v);
-        Store8(t.master + at, left, m);
-        Store8(t.master + t.count + at, left, v);
+    const uint32_t first = table.first[threadIdx.x & 63], chunk = blockIdx.x;
+    const int which = __popcll(__ballot(first <= chunk)) - 1;
+    const AdamWTensor& t = table.tensor[which];
+    const int64_t padded = (t.count + 31) / 32 * 32;
+    const uint8_t* codes = static_cast<const uint8_t*>(t.moments);
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+        const int64_t at = static_cast<int64_t>(chunk - table.first[which]) * kAdamWChunk + part * (kAdamWChunk / 2) +
+                           threadIdx.x * 4;
+        const int64_t left = t.count - at;
+        if (left <= 0) break;
+        float m[4], v[4];
+        Unpack<kLeastM, true>(codes + at, t.exponents[at / 32], m);
+        Unpack<kLeastV, false>(codes + padded + at, t.exponents[(padded + at) / 32], v);
+        Store(t.master + at, left, m);
+        Store(t.master + t.count + at, left, v);
     }
-}
-
-uint32_t Grid(uint32_t chunks)
-{
-    // as many workgroups as the chip holds: each takes several chunks where there are more
-    constexpr uint32_t kMost = 256 * 8;
-    return chunks < kMost ? chunks : kMost;
 }
 
 template <typename TP, typename TG>
-void Launch(const AdamWTable& t, const AdamWScalars& s, int bits, bool master, hipStream_t stream)
+void Launch(const AdamWTable& t, const Factors* s, int bits, bool master, hipStream_t stream)
 {
-    const uint32_t grid = Grid(t.chunks > 0 ? t.chunks : 1);
     if (bits == 8) {
-        if (master) AdamWKernel<TP, TG, 8, true><<<grid, kThreads, 0, stream>>>(t, s);
-        else AdamWKernel<TP, TG, 8, false><<<grid, kThreads, 0, stream>>>(t, s);
+        if (master) AdamWKernel<TP, TG, 8, true><<<t.chunks, kThreads, 0, stream>>>(t, s);
+        else AdamWKernel<TP, TG, 8, false><<<t.chunks, kThreads, 0, stream>>>(t, s);
     } else {
-        if (master) AdamWKernel<TP, TG, 32, true><<<grid, kThreads, 0, stream>>>(t, s);
-        else AdamWKernel<TP, TG, 32, false><<<grid, kThreads, 0, stream>>>(t, s);
+        if (master) AdamWKernel<TP, TG, 32, true><<<t.chunks, kThreads, 0, stream>>>(t, s);
+        else AdamWKernel<TP, TG, 32, false><<<t.chunks, kThreads, 0, stream>>>(t, s);
     }
 }
 
 template <typename TP>
-void LaunchParam(const AdamWTable& t, const AdamWScalars& s, aclDataType grad, int bits, bool master, hipStream_t stream)
+void LaunchParam(const AdamWTable& t, const Factors* s, aclDataType grad, int bits, bool master, hipStream_t stream)
 {
     if (grad == ACL_FLOAT) Launch<TP, float>(t, s, bits, master, stream);
     else if (grad == ACL_FLOAT16) Launch<TP, Half>(t, s, bits, master, stream);
@@ -314,10 +323,17 @@ void LaunchParam(const AdamWTable& t, const AdamWScalars& s, aclDataType grad, i
 
 }  // namespace
 
-int LaunchAdamW(const AdamWTable& t, const AdamWScalars& s, aclDataType param, aclDataType grad, int bits, bool master,
+int LaunchAdamWFactors(const AdamWScalars& s, void* buffer, void* stream)
+{
+    AdamWFactorsKernel<<<1, 1, 0, static_cast<hipStream_t>(stream)>>>(s, static_cast<Factors*>(buffer));
+    return 0;
+}
+
+int LaunchAdamW(const AdamWTable& t, const void* buffer, aclDataType param, aclDataType grad, int bits, bool master,
                 void* stream)
 {
     hipStream_t q = static_cast<hipStream_t>(stream);
+    const auto* s = static_cast<const Factors*>(buffer);
     if (param == ACL_FLOAT) LaunchParam<float>(t, s, grad, bits, master, q);
     else if (param == ACL_FLOAT16) LaunchParam<Half>(t, s, grad, bits, master, q);
     else LaunchParam<Bf16>(t, s, grad, bits, master, q);
@@ -326,7 +342,7 @@ int LaunchAdamW(const AdamWTable& t, const AdamWScalars& s, aclDataType param, a
 
 int LaunchAdamWMoments(const AdamWTable& t, void* stream)
 {
-    AdamWMomentsKernel<<<Grid(t.chunks), kThreads, 0, static_cast<hipStream_t>(stream)>>>(t);
+    AdamWMomentsKernel<<<t.chunks, kThreads, 0, static_cast<hipStream_t>(stream)>>>(t);
     return 0;
 }
 

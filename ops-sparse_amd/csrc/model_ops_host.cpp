@@ -69,7 +69,7 @@ aclsparseStatus_t CheckAdamW(const aclsparseAdamWOptions_t& o)
     const bool fine = o.beta1 >= 0 && o.beta1 < 1 && o.beta2 >= 0 && o.beta2 < 1 && o.eps >= 0 && std::isfinite(o.eps) &&
                       o.weightDecay >= 0 && std::isfinite(o.weightDecay) &&
                       (o.lrDevice != nullptr || (o.lr >= 0 && std::isfinite(o.lr)));
-    return fine && o.step != nullptr ? ACL_SPARSE_STATUS_SUCCESS : ACL_SPARSE_STATUS_INVALID_VALUE;
+    return fine && o.step != nullptr && o.buffer != nullptr && Aligned(o.buffer, 0, 4) ? ACL_SPARSE_STATUS_SUCCESS : ACL_SPARSE_STATUS_INVALID_VALUE;
 }
 
 aclsparseStatus_t CheckAdamWTensor(const aclsparseAdamWTensor_t& t, int bits)
@@ -87,7 +87,7 @@ aclsparseStatus_t CheckAdamWTensor(const aclsparseAdamWTensor_t& t, int bits)
 bool Add(aclsp::AdamWTable& table, int& used, const aclsp::AdamWTensor& t, int64_t place)
 {
     const int64_t chunks = (t.count + aclsp::kAdamWChunk - 1) / aclsp::kAdamWChunk;
-    if (used == aclsp::kAdamWTensors || table.chunks + chunks > INT32_MAX) return false;
+    if (used == aclsp::kAdamWTensors || table.chunks + chunks > aclsp::kAdamWMostChunks) return false;
     table.tensor[used] = t;
     table.first[used] = table.chunks;
     table.place[used] = static_cast<int32_t>(place);
@@ -186,47 +186,46 @@ aclsparseStatus_t aclsparseAdamW(aclsparseHandle_t handle, int64_t count, const 
     st = CheckAdamW(*options);
     if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
     for (int64_t i = 0; i < count; ++i) {
-        if (tensors[i].count > INT32_MAX * aclsp::kAdamWChunk) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
+        if (tensors[i].count > aclsp::kAdamWMostChunks * aclsp::kAdamWChunk) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
         st = CheckAdamWTensor(tensors[i], options->momentBits);
         if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
     }
-    aclsp::AdamWScalars s{options->lr, options->beta1, options->beta2, options->eps, options->weightDecay,
-                          options->lrDevice, options->gradScale, options->step, options->seed, false};
+    const aclsp::AdamWScalars s{options->lr, options->beta1, options->beta2, options->eps, options->weightDecay,
+                          options->lrDevice, options->gradScale, options->step, options->seed};
     (void)hipGetLastError();
-    // one launch for each 64 tensors of one kind; the last counts the step
+    void* stream = StreamOf(handle);
+    int rc = aclsp::LaunchAdamWFactors(s, options->buffer, stream);
+    // one launch for each 64 tensors of one kind
     constexpr aclDataType kTypes[] = {ACL_FLOAT, ACL_FLOAT16, ACL_BF16};
     aclsp::AdamWTable table;
-    int used = 0, waiting = 0;
+    int used = 0;
     aclDataType param = ACL_FLOAT, grad = ACL_FLOAT;
     bool master = false;
-    Clear(table, used);
-    auto flush = [&](bool last) {
-        s.last = last;
-        const int rc = aclsp::LaunchAdamW(table, s, param, grad, options->momentBits, master, StreamOf(handle));
+    auto flush = [&] {
+        if (rc == 0 && used > 0) {
+            rc = aclsp::LaunchAdamW(table, options->buffer, param, grad, options->momentBits, master, stream);
+        }
         Clear(table, used);
-        return rc;
     };
+    Clear(table, used);
     for (int kind = 0; kind < 18; ++kind) {
-        const aclDataType p = kTypes[kind / 6], g = kTypes[kind / 2 % 3];
-        const bool m = kind % 2 != 0;
+        param = kTypes[kind / 6];
+        grad = kTypes[kind / 2 % 3];
+        master = kind % 2 != 0;
         for (int64_t i = 0; i < count; ++i) {
             const aclsparseAdamWTensor_t& t = tensors[i];
-            if (t.count == 0 || t.grad == nullptr || t.paramType != p || t.gradType != g || (t.master != nullptr) != m) {
+            if (t.count == 0 || t.grad == nullptr || t.paramType != param || t.gradType != grad ||
+                (t.master != nullptr) != master) {
                 continue;
             }
             const aclsp::AdamWTensor one{t.param, t.grad, t.master, t.moments, t.exponents, t.count};
-            const bool other = waiting != 0 && (p != param || g != grad || m != master);
-            if (other || !Add(table, used, one, i)) {
-                if (flush(false) != 0) return ACL_SPARSE_STATUS_EXECUTION_FAILED;
-                Add(table, used, one, i);
-            }
-            param = p;
-            grad = g;
-            master = m;
-            waiting = 1;
+            if (Add(table, used, one, i)) continue;
+            flush();
+            Add(table, used, one, i);
         }
+        flush();
     }
-    return Finish(flush(true));
+    return Finish(rc);
 }
 
 aclsparseStatus_t aclsparseAdamWMoments(aclsparseHandle_t handle, int64_t count, const aclsparseAdamWTensor_t* tensors)
@@ -238,7 +237,7 @@ aclsparseStatus_t aclsparseAdamWMoments(aclsparseHandle_t handle, int64_t count,
     for (int64_t i = 0; i < count; ++i) {
         const aclsparseAdamWTensor_t& t = tensors[i];
         if (t.count < 0) return ACL_SPARSE_STATUS_INVALID_VALUE;
-        if (t.count > INT32_MAX * aclsp::kAdamWChunk) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
+        if (t.count > aclsp::kAdamWMostChunks * aclsp::kAdamWChunk) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
         if (t.count > 0 && (t.master == nullptr || t.moments == nullptr || t.exponents == nullptr ||
                             !Aligned(t.moments, 0, 8))) {
             return ACL_SPARSE_STATUS_INVALID_VALUE;

@@ -67,12 +67,15 @@ struct AdamWScalars {
     double lr, beta1, beta2, eps, weight_decay;
     const float* lr_device;   // null: lr
     const float* grad_scale;  // null: one
-    int32_t* step;            // steps taken, and a count that is zero between launches
+    int32_t* step;            // steps taken; this one is counted
     uint32_t seed;
-    bool last;                // of the call's launches: counts the step
 };
-constexpr int64_t kAdamWChunk = 2048;
-int LaunchAdamW(const AdamWTable& t, const AdamWScalars& s, aclDataType param, aclDataType grad, int bits, bool master,
+// Values of a workgroup; a launch has one for each chunk, and fewer than 2^32 threads.
+constexpr int64_t kAdamWChunk = 2048, kAdamWMostChunks = (int64_t{1} << 24) - 1;
+constexpr size_t kAdamWBufferBytes = 64;
+int LaunchAdamWFactors(const AdamWScalars& s, void* buffer, void* stream);
+// With the factors that LaunchAdamWFactors left in the buffer.
+int LaunchAdamW(const AdamWTable& t, const void* buffer, aclDataType param, aclDataType grad, int bits, bool master,
                 void* stream);
 // Values of 8-bit moments, to the tables' masters, [2, count].
 int LaunchAdamWMoments(const AdamWTable& t, void* stream);

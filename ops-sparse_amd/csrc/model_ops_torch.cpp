@@ -236,6 +236,8 @@ void AdamWStep(const Tensors& params, const MaybeTensors& grads, const Tensors& 
     o.lrDevice = lrTensor.has_value() ? Floats(*lrTensor) : nullptr;
     o.gradScale = gradScale.has_value() ? Floats(*gradScale) : nullptr;
     o.step = static_cast<int32_t*>(step.data_ptr());
+    const Tensor buffer = Empty({64}, at::kByte, step);
+    o.buffer = Data(buffer);
     o.seed = static_cast<uint32_t>(seed);
     o.momentBits = exponents.has_value() ? 8 : 32;
     Call call(step);

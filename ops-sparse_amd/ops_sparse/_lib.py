@@ -127,7 +127,7 @@ class AdamWOptions(ctypes.Structure):
     """aclsparseAdamWOptions_t."""
     _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double),
                 ("eps", ctypes.c_double), ("weightDecay", ctypes.c_double), ("lrDevice", _vp), ("gradScale", _vp),
-                ("step", _vp), ("seed", ctypes.c_uint32), ("momentBits", _i32)]
+                ("step", _vp), ("buffer", _vp), ("seed", ctypes.c_uint32), ("momentBits", _i32)]
 
 
 # name -> argtypes; every function returns aclsparseStatus_t (int) unless RESTYPES says otherwise

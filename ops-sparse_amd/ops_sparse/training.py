@@ -46,7 +46,7 @@ class AdamWState(NamedTuple):
 
     moments: [2, P] with P = n rounded up to 32, the first moment and the second one, fp32 or uint8 codes; exponents:
     [2, P / 32] uint8 for the codes, None for fp32; masters: the values in fp32, None where the parameters themselves
-    are kept; step: int32 [2], the steps taken and zero; seed: of the rounding of 8-bit moments (32 bits).
+    are kept; step: int32 [2], the steps taken and a place that is not used; seed: of the rounding of 8-bit moments (32 bits).
     """
     moments: List[torch.Tensor]
     exponents: Optional[List[torch.Tensor]]

@@ -112,7 +112,7 @@ def tensor(**kw):
 
 
 def options(**kw):
-    a = dict(lr=1e-3, beta1=0.9, beta2=0.99, eps=1e-8, weightDecay=0.1, lrDevice=None, gradScale=None, step=P, seed=0,
+    a = dict(lr=1e-3, beta1=0.9, beta2=0.99, eps=1e-8, weightDecay=0.1, lrDevice=None, gradScale=None, step=P, buffer=P, seed=0,
              momentBits=32)
     a.update(kw)
     return AdamWOptions(**a)
@@ -127,7 +127,7 @@ def test_adamw_status_codes(lib, handle):
     assert call(tensor(), options(), count=-1) == INVALID
     for change, status in ((dict(beta1=1.0), INVALID), (dict(beta1=-0.1), INVALID), (dict(beta2=1.5), INVALID),
                            (dict(eps=-1.0), INVALID), (dict(eps=float("nan")), INVALID), (dict(lr=float("inf")), INVALID),
-                           (dict(lr=-1.0), INVALID), (dict(weightDecay=-0.1), INVALID), (dict(step=None), INVALID),
+                           (dict(lr=-1.0), INVALID), (dict(weightDecay=-0.1), INVALID), (dict(step=None), INVALID), (dict(buffer=None), INVALID),
                            (dict(momentBits=16), UNSUPPORTED), (dict(momentBits=8), INVALID)):
         assert call(tensor(), options(**change)) == status, change
     for change, status in ((dict(count=-1), INVALID), (dict(paramType=I8), UNSUPPORTED),

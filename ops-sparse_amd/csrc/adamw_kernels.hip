@@ -142,7 +142,7 @@ __device__ __forceinline__ void Store(T* to, int64_t left, const float (&v)[V])
 #pragma unroll
     for (int i = 0; i < V; ++i) t[i] = FromFloat<T>(v[i]);
     if (left >= V) {
-        __builtin_memcpy(to, t, sizeof(t));
+        StoreStreaming<sizeof(t)>(to, t);
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) {

@@ -23,6 +23,23 @@ __device__ __forceinline__ T FromFloat(float v)
     return static_cast<T>(v);
 }
 
+// Stores a large result by words that are not kept in the L2, whatever their alignment: what is written once and not
+// read before it would have left the caches only displaces what is read.  (Moments' values, 2 bytes read for 8 written:
+// 5.4 TB/s, by ordinary stores 3.5.)
+template <int kBytes>
+__device__ __forceinline__ void StoreStreaming(void* to, const void* from)
+{
+    constexpr int kWords = kBytes >= 16 ? 4 : kBytes / 4;
+    static_assert(kBytes % (kWords * 4) == 0, "whole words");
+    using Words = int __attribute__((ext_vector_type(kWords), aligned(1)));
+    Words w[kBytes / (kWords * 4)];
+    __builtin_memcpy(w, from, kBytes);
+#pragma unroll
+    for (int i = 0; i < kBytes / (kWords * 4); ++i) {
+        __builtin_nontemporal_store(w[i], reinterpret_cast<Words*>(to) + i);
+    }
+}
+
 // Moves within a wave by DPP: lanes that have no source keep `old`.
 template <int kCtrl, int kRowMask>
 __device__ __forceinline__ uint32_t Dpp(uint32_t old, uint32_t v)

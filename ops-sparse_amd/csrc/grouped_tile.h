@@ -235,7 +235,8 @@ __device__ __forceinline__ bool JoinTeams(char* lds, Acc (&acc)[MI][NI])
 // and stores whole rows, 16 bytes per lane.  value(i, j, v) gives the four
 // values of tile (i, j).  Chunk c of row r lies at slot c ^ r (c ^ r / 2 in
 // rows of half the banks), which spreads the rows of a write over the banks.
-template <typename TOut, int MI, int NI, int kLdsBytes, typename Value>
+// kStream: see StoreStreaming.
+template <typename TOut, int MI, int NI, int kLdsBytes, bool kStream = false, typename Value>
 __device__ __forceinline__ void StoreTile(char* lds, TOut* c, int64_t ldc, int64_t rows, int64_t columns, Value value)
 {
     constexpr int kSize = static_cast<int>(sizeof(TOut));
@@ -272,7 +273,8 @@ __device__ __forceinline__ void StoreTile(char* lds, TOut* c, int64_t ldc, int64
             const Int4 v = *reinterpret_cast<const Int4*>(lds + r * kRowBytes + (lane % kChunks) * 16);
             TOut* to = c + row * ldc + chunk * kPer;
             if (left >= kPer) {
-                __builtin_memcpy(to, &v, 16);  // whatever C's alignment
+                if constexpr (kStream) StoreStreaming<16>(to, &v);
+                else __builtin_memcpy(to, &v, 16);  // whatever C's alignment
             } else {
                 TOut o[kPer];
                 __builtin_memcpy(o, &v, 16);

@@ -406,7 +406,7 @@ __global__ __launch_bounds__(kThreads) void LogprobsGradKernel(LogprobsGradLaunc
 #pragma unroll
         for (int i = 0; i < kUnit; ++i) v[b][i] = FromFloat<T>(one(ToFloat(v[b][i])));
         if (c + kUnit <= end) {
-            __builtin_memcpy(grad + c, v[b], sizeof(v[b]));
+            StoreStreaming<sizeof(v[b])>(grad + c, v[b]);
         } else {
 #pragma unroll
             for (int i = 0; i < kUnit; ++i) {

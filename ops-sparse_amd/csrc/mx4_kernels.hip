@@ -106,7 +106,7 @@ __global__ __launch_bounds__(256) void Mx4DequantizeKernel(Mx4Rows p, uint32_t c
     const int64_t at = static_cast<int64_t>(chunk) * 8;
     T* to = static_cast<T*>(p.x) + row * p.ldx + at;
     if (at + 8 <= p.k) {
-        __builtin_memcpy(to, t, sizeof(t));
+        StoreStreaming<sizeof(t)>(to, t);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -388,7 +388,8 @@ constexpr int kMx4TileRows = 256;
 
 // One tile: MI*WM*16 rows by NI*WN*16 columns, of which each of a team's WM x
 // WN waves takes MI x NI instructions' results.
-template <typename TOut, int kTeams, int MI, int NI, int WM, int WN>
+// kStream: the output is large.
+template <typename TOut, int kTeams, bool kStream, int MI, int NI, int WM, int WN>
 __device__ __forceinline__ void Mx4Tile(const Mx4Launch& p, char* lds, int32_t group, int32_t firstRow, int32_t endRow,
                                         int64_t n0)
 {
@@ -435,7 +436,7 @@ __device__ __forceinline__ void Mx4Tile(const Mx4Launch& p, char* lds, int32_t g
     if (!JoinTeams<kTeams, kThreads, (kTeams - 1) * kLds>(lds + kLds, acc)) return;
     const int64_t n = n0 + rowB;
     constexpr int kPart = kLds / (WM * WN) / 128 * 128;
-    StoreTile<TOut, MI, NI, kPart>(lds + wave * kPart, static_cast<TOut*>(p.c) + (firstRow + rowA) * p.ldc + n, p.ldc,
+    StoreTile<TOut, MI, NI, kPart, kStream>(lds + wave * kPart, static_cast<TOut*>(p.c) + (firstRow + rowA) * p.ldc + n, p.ldc,
                                    endRow - firstRow - rowA, p.n - n, [&](int i, int j, float(&v)[4]) {
 #pragma unroll
                                        for (int x = 0; x < 4; ++x) v[x] = acc[i][j][x];
@@ -458,11 +459,11 @@ __global__ __launch_bounds__(512, 1) void Mx4TileKernel(Mx4Launch p, int32_t til
     const int32_t end = tile.end - row < height ? tile.end : row + height;
     const int64_t n0 = static_cast<int64_t>(place.n) * 256;
     if (end - row <= 64) {
-        Mx4Tile<TOut, 1, 2, 4, 2, 4>(p, lds, tile.group, row, end, n0);
+        Mx4Tile<TOut, 1, true, 2, 4, 2, 4>(p, lds, tile.group, row, end, n0);
     } else if (end - row <= 128) {
-        Mx4Tile<TOut, 1, 4, 4, 2, 4>(p, lds, tile.group, row, end, n0);
+        Mx4Tile<TOut, 1, true, 4, 4, 2, 4>(p, lds, tile.group, row, end, n0);
     } else {
-        Mx4Tile<TOut, 1, 8, 4, 2, 4>(p, lds, tile.group, row, end, n0);
+        Mx4Tile<TOut, 1, true, 8, 4, 2, 4>(p, lds, tile.group, row, end, n0);
     }
 }
 
@@ -481,7 +482,7 @@ __global__ __launch_bounds__(kTeams * 256, 3) void Mx4SmallTileKernel(Mx4Launch 
     const TilePlace place = PlaceInBands(share.tile - static_cast<int64_t>(tile.before) * tilesN, tile.tiles, tilesN);
     const int32_t row = tile.begin + place.m * 64;
     if (row < tile.begin || row >= tile.end) return;
-    Mx4Tile<TOut, kTeams, 2, 4, 2, 2>(p, lds, tile.group, row, tile.end - row < 64 ? tile.end : row + 64,
+    Mx4Tile<TOut, kTeams, false, 2, 4, 2, 2>(p, lds, tile.group, row, tile.end - row < 64 ? tile.end : row + 64,
                                       static_cast<int64_t>(place.n) * 128);
 }
 

@@ -493,7 +493,6 @@ __global__ __launch_bounds__(kTeams * 256, 3) void Mx4SmallTileKernel(Mx4Launch 
 template <typename TOut, int MT, int NT, int kWaves>
 __global__ __launch_bounds__(kWaves * 64) void Mx4RowsKernel(Mx4Launch p, int32_t tilesN)
 {
-    constexpr int kAhead = 16 / (MT + NT) > 4 ? 8 : 4;  // steps loaded before they are multiplied
     __shared__ Float4 part[kWaves][MT * NT][64];
     const RaggedTile tile = RaggedTiles(p.offsets, p.rows, p.groups, MT * 16)
                                 .Find(static_cast<int32_t>(blockIdx.x / static_cast<uint32_t>(tilesN)));
@@ -504,6 +503,14 @@ __global__ __launch_bounds__(kWaves * 64) void Mx4RowsKernel(Mx4Launch p, int32_
     Float4 acc[MT][NT] = {};
     if (tile.group < p.groups) {
         const int32_t blocks = static_cast<int32_t>(p.blocks);
+        // the rows' indices first and what needs them last: the weights' loads go out between
+        int32_t index[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const int32_t r = tile.row + i * 16 + (lane & 15);
+            index[i] = r < tile.end ? r : tile.row;
+            if (p.row_index != nullptr) index[i] = p.row_index[index[i]];
+        }
         const uint8_t *b[NT], *sb[NT], *a[MT], *sa[MT];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
@@ -511,31 +518,35 @@ __global__ __launch_bounds__(kWaves * 64) void Mx4RowsKernel(Mx4Launch p, int32_
             b[j] = p.b.codes + tile.group * p.b.stride + n * p.b.ld;
             sb[j] = p.b.scales + tile.group * p.b.stride_scales + n * p.b.ld_scales;
         }
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            const int32_t r = tile.row + i * 16 + (lane & 15);
-            const int64_t row = IndexedRow(p.row_index, r < tile.end ? r : tile.row, p.rows_a);
-            a[i] = p.a.codes + row * p.a.ld;
-            sa[i] = p.a.scales + row * p.a.ld_scales;
-        }
         // step s is four blocks; a wave takes two neighbouring ones, a memory line, at a time
         auto at = [&](int s) { return ((s >> 1) * kWaves + wave) * 8 + (s & 1) * 4 + (lane >> 4); };
-        for (int s0 = 0; ((s0 >> 1) * kWaves + wave) * 8 < blocks; s0 += kAhead) {
+        auto load = [&](const uint8_t* codes, const uint8_t* scales, int s, Int4& f, uint32_t& e) {
+            const int block = at(s) < blocks ? at(s) : 0;
+            f = *reinterpret_cast<const Int4*>(codes + block * static_cast<int64_t>(16));
+            e = scales[block];
+            if (at(s) >= blocks) {
+                f = Int4{0, 0, 0, 0};
+                e = 0;
+            }
+        };
+        // kAhead steps from s0 on, all loaded before they are multiplied
+        auto steps = [&](auto ahead, int s0, bool first) {
+            constexpr int kAhead = decltype(ahead)::value;
             Int4 fb[kAhead][NT], fa[kAhead][MT];
             uint32_t eb[kAhead][NT], ea[kAhead][MT];
-            auto load = [&](const uint8_t* codes, const uint8_t* scales, int s, Int4& f, uint32_t& e) {
-                const int block = at(s) < blocks ? at(s) : 0;
-                f = *reinterpret_cast<const Int4*>(codes + block * static_cast<int64_t>(16));
-                e = scales[block];
-                if (at(s) >= blocks) {
-                    f = Int4{0, 0, 0, 0};
-                    e = 0;
-                }
-            };
 #pragma unroll
             for (int s = 0; s < kAhead; ++s) {
 #pragma unroll
                 for (int j = 0; j < NT; ++j) load(b[j], sb[j], s0 + s, fb[s][j], eb[s][j]);
+            }
+            if (first) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    // stays within the operand whatever the index holds
+                    const int64_t row = index[i] < 0 || index[i] >= p.rows_a ? 0 : index[i];
+                    a[i] = p.a.codes + row * p.a.ld;
+                    sa[i] = p.a.scales + row * p.a.ld_scales;
+                }
             }
 #pragma unroll
             for (int s = 0; s < kAhead; ++s) {
@@ -552,6 +563,15 @@ __global__ __launch_bounds__(kWaves * 64) void Mx4RowsKernel(Mx4Launch p, int32_
                     }
                 }
             }
+        };
+        constexpr int kMost = 16 / (MT + NT) > 4 ? 8 : 4;  // steps at once
+        constexpr std::integral_constant<int, kMost> most{};
+        if (blocks <= kWaves * kMost * 2) {
+            // half as many cover the row: no loads past its end
+            steps(std::integral_constant<int, kMost / 2>{}, 0, true);
+        } else {
+            steps(most, 0, true);
+            for (int s0 = kMost; ((s0 >> 1) * kWaves + wave) * 8 < blocks; s0 += kMost) steps(most, s0, false);
         }
     }
 #pragma unroll
@@ -616,7 +636,8 @@ int Mx4BySize(const Mx4Launch& l, hipStream_t s)
     const int64_t smallTiles = (CeilDiv(l.rows, 64) + (l.groups - 1) / 2) * CeilDiv(l.n, 128);
     const bool few = l.rows <= 6 * l.groups || (l.rows <= 64 * l.groups && smallTiles <= cus / 4);
     if (few && l.blocks <= INT32_MAX / 32) {
-        const int rc = l.rows <= 6 * l.groups || l.rows <= 32 ? LaunchMx4Rows<TOut, 1, 1>(l, s)
+        const int rc = l.rows <= 6 * l.groups || l.rows <= 16 ? LaunchMx4Rows<TOut, 1, 1>(l, s)
+                       : l.rows <= 32                         ? LaunchMx4Rows<TOut, 2, 1>(l, s)
                                                               : LaunchMx4Rows<TOut, 2, 2>(l, s);
         if (rc != kTooLarge) return rc;  // wider tiles may still fit
     }

@@ -4,6 +4,8 @@ the random numbers that 8-bit moments are rounded by.
 No call here reaches a kernel launch: each fails its checks, sizes a buffer, or has nothing to do.
 """
 import ctypes
+import shutil
+import subprocess
 
 import numpy as np
 import pytest
@@ -262,3 +264,38 @@ def test_random_bits_are_even_and_independent():
                 continue
             same = bit == ((other >> np.uint64(i)) & np.uint64(1))
             assert abs(int(same.sum()) - n / 2) <= limit, (i, j)
+
+
+def test_the_copies_to_lds_are_the_only_use_of_m0(tmp_path):
+    # the 4-bit products' tiles set m0 in assembly that cannot say so, as the other grouped products do
+    from test_experts_abi import other_uses_of_m0
+
+    tool = "/opt/rocm/llvm/bin/llvm-objdump"
+    shutil.copy(_lib.LIB_PATH, tmp_path / "lib.so")
+    subprocess.run([tool, "--offloading", "lib.so"], cwd=tmp_path, check=True, capture_output=True)
+    images = [f for f in tmp_path.iterdir() if f.name.endswith("gfx950") and b"Mx4TileKernel" in f.read_bytes()]
+    assert len(images) == 1
+    text = subprocess.run([tool, "-d", "--no-show-raw-insn", images[0].name], cwd=tmp_path, check=True,
+                          capture_output=True, text=True).stdout
+    lines = [line.split("//")[0].strip() for line in text.splitlines()]
+    assert sum(line.startswith("global_load_lds_dwordx4 ") for line in lines) > 100
+    assert other_uses_of_m0(lines) == []
+
+
+def test_scaled_products_in_assembly_follow_their_wait(tmp_path):
+    # a matrix instruction written as assembly has the wait for what an ordinary instruction wrote right before it
+    tool = "/opt/rocm/llvm/bin/llvm-objdump"
+    shutil.copy(_lib.LIB_PATH, tmp_path / "lib.so")
+    subprocess.run([tool, "--offloading", "lib.so"], cwd=tmp_path, check=True, capture_output=True)
+    image = next(f for f in tmp_path.iterdir() if f.name.endswith("gfx950") and b"Mx4TileKernel" in f.read_bytes())
+    text = subprocess.run([tool, "-d", "--no-show-raw-insn", image.name], cwd=tmp_path, check=True, capture_output=True,
+                          text=True).stdout
+    kernel, count = "", 0
+    lines = [line.split("//")[0].strip() for line in text.splitlines()]
+    for before, line in zip(lines, lines[1:]):
+        if line.endswith(">:"):
+            kernel = line
+        if "TileKernel" in kernel and line.startswith("v_mfma_scale"):
+            count += 1
+            assert before == "s_nop 1"
+    assert count > 1000

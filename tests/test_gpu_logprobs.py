@@ -250,6 +250,25 @@ def test_gradient(dev, t, v, k, dtype):
         assert bool((err <= bound).all()), float((err / bound).max())
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_large_gradient_of_the_entropy_beside_masked_logits(dev, dtype):
+    t, v = 5, 300
+    logits = rows(t, v, dtype, 21)
+    logits[:, ::3] = -float("inf")
+    logits[:, 1::3][:, :40] = torch.finfo(dtype).min
+    ge = torch.tensor([1e30, -1e30, 3e12, -1e9, 1e8], device=dev)
+    x = logits.clone().requires_grad_()
+    d = torch.autograd.grad(token_logprobs(x, torch.zeros(t, dtype=torch.int64, device=dev), entropy=True).entropy, x,
+                            ge)[0]
+    want, p = exact_gradient(logits, torch.zeros(t, dtype=torch.int64), None, ge, None, None)
+    size = ge.abs().double().cpu()[:, None]
+    e = 2 * error(logits) + 40 * U  # as above
+    bound = p * size * e * (60 + np.log(v)) + want.abs() * (torch.finfo(dtype).eps / 2 + 8 * U) + 4 * U * (
+        want != 0) * size + 1e-37
+    err = (d.double().cpu() - want).abs()
+    assert bool((err <= bound).all()), float((err / bound).max())
+
+
 def test_gradient_against_differences(dev):
     # the fp64 definition agrees with the results to 1e-6, so a difference over 2^-5 shows the gradient to 1e-6 * 2^6 and
     # the third derivative's share, at most 2^-10 / 6 of weights below one

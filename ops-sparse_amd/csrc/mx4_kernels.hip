@@ -32,7 +32,11 @@ __device__ __forceinline__ float ScaleValue(uint32_t e)
 }
 
 // ---------------------------------------------------------------------------
-// To the format and back.  Four lanes share a block, eight values each.
+// To the format and back.  Four lanes share a block, eight values each: loads
+// and stores of 16 and 4 bytes, the largest value by two exchanges in the quad.
+// Bound by memory.  16381 rows of 4096 bf16 values there and back: 27.6 us (170
+// MB, 6.2 TB/s of what the L2s partly hold) and 24.6 us (6.9 TB/s; most of it
+// is written past the L2); one row 2.0 and 2.1 us, a round of latency.
 // ---------------------------------------------------------------------------
 // Values [c, c + 8) of a row of k, zeros past its end.
 template <typename T>
@@ -384,6 +388,13 @@ __device__ __forceinline__ void MultiplyMx4(OperandA& a, OperandB& b, Scales& sc
     SettleSums(acc);
 }
 
+// 256x256 tiles by eight waves, one workgroup per CU, as the 16-bit products' but for the scales: the largest tile whose
+// sums fit the registers, as each operand byte that comes into a CU then serves most products.  32768 rows by 8 groups of
+// 4096 columns over 4096: 311 us, 3.5 PFLOP/s; the instructions alone reach 6.8 on random operands, for the clock that
+// their power leaves.  One group of 8192 x 8192: a turn takes 1.8 us, of which the matrix instructions and the barrier
+// alone 1.15, copies 0.3, scales 0.15, reads of LDS 0.1; a round of tiles takes 4.5 us of stores and 2 us of dispatch
+// besides.  Slower: a ring of four half turns whose scales are copied by words (396 us for 339 at the time), four waves of
+// 128x128 (378 for 348).
 constexpr int kMx4TileRows = 256;
 
 // One tile: MI*WM*16 rows by NI*WN*16 columns, of which each of a team's WM x
@@ -468,7 +479,9 @@ __global__ __launch_bounds__(512, 1) void Mx4TileKernel(Mx4Launch p, int32_t til
 }
 
 // Tiles of 64x128 for groups of few rows: three workgroups per CU, or one whose
-// three teams share a tile's contraction.
+// three teams share a tile's contraction.  Bound by the latency of a turn's
+// copies, 1 us, one turn ahead: 512 rows x 4096 x 4096 12.1 us, 812 rows of 48
+// groups of 1001 x 1000 8.5 us (3.3 TB/s).
 constexpr int kMx4SmallBytes = (64 + 128) * (2 * kTurnBytes + 16);
 template <typename TOut, int kTeams>
 __global__ __launch_bounds__(kTeams * 256, 3) void Mx4SmallTileKernel(Mx4Launch p, int32_t tilesN)
@@ -489,7 +502,9 @@ __global__ __launch_bounds__(kTeams * 256, 3) void Mx4SmallTileKernel(Mx4Launch 
 // Few rows per group: the weights are read once and bound the time.  A
 // workgroup multiplies MT*16 rows by NT*16 columns; its waves split the
 // contraction, each lane loading its operands and their scales straight from
-// memory, and add their sums through LDS in the order of the waves.
+// memory, and add their sums through LDS in the order of the waves.  4 rows of 4
+// groups of 4096 x 2048: 7.2 us for 18 MB from memory, a chain of two loads
+// (offsets, then operands) and the sums behind a launch of 3.6.
 template <typename TOut, int MT, int NT, int kWaves>
 __global__ __launch_bounds__(kWaves * 64) void Mx4RowsKernel(Mx4Launch p, int32_t tilesN)
 {

@@ -24,7 +24,7 @@
 namespace aclsp {
 namespace {
 
-constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kThreads = 256;
 constexpr int kUnit = 8;         // logits that a thread loads at a time
 constexpr int kBatch = 4;        // units between two looks at the largest
 constexpr int kMaxSegments = 64; // of a row: one for each lane of the wave that joins them
@@ -49,16 +49,28 @@ struct Part {
     }
 };
 
-constexpr int kQuadXor1 = 0xB1, kQuadXor2 = 0x4E;
-__device__ __forceinline__ float QuadMax(float x)
+// f over the lanes of each G, in all of them
+template <int G, typename F>
+__device__ __forceinline__ uint32_t OverLanes(uint32_t x, F f)
 {
-    x = fmaxf(x, __uint_as_float(Dpp<kQuadXor1, 0xF>(__float_as_uint(x), __float_as_uint(x))));
-    return fmaxf(x, __uint_as_float(Dpp<kQuadXor2, 0xF>(__float_as_uint(x), __float_as_uint(x))));
+    static_assert(G == 2 || G == 4 || G == 8 || G == 16, "");
+    x = f(x, Dpp<0xB1, 0xF>(x, x));
+    if constexpr (G > 2) x = f(x, Dpp<0x4E, 0xF>(x, x));
+    if constexpr (G > 4) x = f(x, Dpp<0x141, 0xF>(x, x));  // mirrored in each 8
+    if constexpr (G > 8) x = f(x, Dpp<0x140, 0xF>(x, x));  // and in each 16
+    return x;
 }
-__device__ __forceinline__ uint32_t QuadSum(uint32_t x)
+template <int G>
+__device__ __forceinline__ float MaxOverLanes(float x)
 {
-    x += Dpp<kQuadXor1, 0xF>(x, x);
-    return x + Dpp<kQuadXor2, 0xF>(x, x);
+    return __uint_as_float(OverLanes<G>(__float_as_uint(x), [](uint32_t a, uint32_t b) {
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    }));
+}
+template <int G>
+__device__ __forceinline__ uint32_t SumOverLanes(uint32_t x)
+{
+    return OverLanes<G>(x, [](uint32_t a, uint32_t b) { return a + b; });
 }
 
 // The parts of a wave's lanes as one, in all lanes
@@ -125,8 +137,8 @@ __device__ __forceinline__ void AddUnits(Part& p, const T (&v)[N][kUnit])
     }
 }
 
-// A thread's logits of [begin, end): H units that it holds where they fit, none for H = 0.
-template <typename T, int H>
+// A thread's logits of [begin, end), for a workgroup of W threads: H units that it holds where they fit, none for H = 0.
+template <typename T, int H, int W>
 struct Held {
     T v[H > 0 ? H : 1][kUnit];
 
@@ -137,13 +149,13 @@ struct Held {
         Part p{kLowest, 0.0f, 0.0f};
         if constexpr (H > 0) {
 #pragma unroll
-            for (int b = 0; b < H; ++b) LoadUnit(row, c + b * kThreads * kUnit, end, v[b]);
+            for (int b = 0; b < H; ++b) LoadUnit(row, c + b * W * kUnit, end, v[b]);
             AddUnits<kEntropy>(p, v);
         } else {
-            for (int32_t at = c; at < end; at += kThreads * kUnit * kBatch) {
+            for (int32_t at = c; at < end; at += W * kUnit * kBatch) {
                 T u[kBatch][kUnit];
 #pragma unroll
-                for (int b = 0; b < kBatch; ++b) LoadUnit(row, at + b * kThreads * kUnit, end, u[b]);
+                for (int b = 0; b < kBatch; ++b) LoadUnit(row, at + b * W * kUnit, end, u[b]);
                 AddUnits<kEntropy>(p, u);
             }
         }
@@ -158,10 +170,10 @@ struct Held {
         if constexpr (H > 0) {
 #pragma unroll
             for (int i = 0; i < H * kUnit; ++i) {
-                f(ToFloat(v[i / kUnit][i % kUnit]), c + i / kUnit * kThreads * kUnit + i % kUnit);
+                f(ToFloat(v[i / kUnit][i % kUnit]), c + i / kUnit * W * kUnit + i % kUnit);
             }
         } else {
-            for (int32_t at = c; at < end; at += kThreads * kUnit) {
+            for (int32_t at = c; at < end; at += W * kUnit) {
                 T u[kUnit];
                 LoadUnit(row, at, end, u);
 #pragma unroll
@@ -203,10 +215,11 @@ __device__ __forceinline__ void WriteRow(const LogprobsLaunch& p, int64_t row, c
     }
 }
 
+template <int W>
 struct Shared {
-    Part part[kWaves];
-    uint64_t pair[kCandidates];  // candidates; before that each quad's largest
-    uint64_t best[kWaves];
+    Part part[W / 64];
+    uint64_t pair[kCandidates];  // candidates; before that each group's largest
+    uint64_t best[W / 64];
     uint32_t count;
     float threshold;
 };
@@ -214,28 +227,36 @@ struct Shared {
 // The k largest of logits [begin, end), first ones first; write(rank, pair)
 // for each, fewer than k where fewer are above -inf.  m: the thread's largest.
 //
-// The k-th largest of 64 quads' largest is a bound below which the answer has
-// nothing: those quads hold k logits at or above it.  A second pass lists
+// The k-th largest of 64 or 128 groups' largest is a bound below which the answer
+// has nothing: those groups of threads hold k logits at or above it.  (128 where
+// 64 leave some empty: rows of 1025 to 2048 logits, more than the candidates, else
+// had no bound; its ranks cost 0.6 us more of 256 threads.)  A second pass lists
 // what is at or above the bound, mostly little more than k logits, and each finds
 // its rank by comparing itself with all.  A row with NaN, or with more logits
 // at the bound than fit (equal ones), goes through k passes instead.
-template <typename T, int H, typename Write>
-__device__ __forceinline__ void TakeTop(Shared& sh, const Held<T, H>& held, const T* row, int32_t begin, int32_t end,
+template <typename T, int H, int W, typename Write>
+__device__ __forceinline__ void TakeTop(Shared<W>& sh, const Held<T, H, W>& held, const T* row, int32_t begin, int32_t end,
                                         int32_t k, float m, bool nan, Write write)
 {
-    static_assert(kThreads == 4 * kMaxTop, "as many quads as there can be alternatives");
     const int tid = threadIdx.x;
-    m = QuadMax(m);
-    if ((tid & 3) == 0) sh.pair[tid >> 2] = Pair(m, tid >> 2);
     if (tid == 0) sh.count = 0;
-    __syncthreads();
-    // each lane of a quad compares the quad's with a quarter of the others
-    uint32_t rank = 0;
-    const uint64_t mine = sh.pair[tid >> 2];
+    auto setBound = [&](auto lanes) {
+        constexpr int G = decltype(lanes)::value;
+        const int group = tid / G, lane = tid % G;
+        const float most = MaxOverLanes<G>(m);
+        if (lane == 0) sh.pair[group] = Pair(most, group);
+        __syncthreads();
+        // each lane of a group compares the group's with its share of the others
+        uint32_t rank = 0;
+        const uint64_t mine = sh.pair[group];
 #pragma unroll
-    for (int i = 0; i < kMaxTop / 4; ++i) rank += sh.pair[(tid & 3) * (kMaxTop / 4) + i] > mine ? 1 : 0;
-    rank = QuadSum(rank);
-    if (rank == static_cast<uint32_t>(k) - 1 && (tid & 3) == 0) sh.threshold = m;
+        for (int i = 0; i < W / G / G; ++i) rank += sh.pair[i * G + lane] > mine ? 1 : 0;
+        rank = SumOverLanes<G>(rank);
+        if (rank == static_cast<uint32_t>(k) - 1 && lane == 0) sh.threshold = most;
+    };
+    constexpr int kLanes = W / kMaxTop;
+    if ((end - begin) / (kLanes * kUnit) >= k) setBound(std::integral_constant<int, kLanes>{});
+    else setBound(std::integral_constant<int, kLanes / 2>{});
     __syncthreads();
     const float threshold = sh.threshold;
     if (!nan) {
@@ -248,13 +269,14 @@ __device__ __forceinline__ void TakeTop(Shared& sh, const Held<T, H>& held, cons
         __syncthreads();
         const uint32_t count = sh.count;
         if (count <= kCandidates) {
-            for (uint32_t c = tid; c < count; c += kThreads) {
+            for (uint32_t c = tid; c < count; c += W) {
                 const uint64_t pair = sh.pair[c];
                 int above = 0;
+#pragma unroll 8
                 for (uint32_t i = 0; i < count; ++i) above += sh.pair[i] > pair ? 1 : 0;
                 if (above < k) write(above, pair);
             }
-            for (int32_t r = static_cast<int32_t>(count) + tid; r < k; r += kThreads) write(r, uint64_t{0});
+            for (int32_t r = static_cast<int32_t>(count) + tid; r < k; r += W) write(r, uint64_t{0});
             return;
         }
     }
@@ -270,7 +292,7 @@ __device__ __forceinline__ void TakeTop(Shared& sh, const Held<T, H>& held, cons
         if ((tid & 63) == 0) sh.best[tid >> 6] = best;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) best = sh.best[w] > best ? sh.best[w] : best;
+        for (int w = 0; w < W / 64; ++w) best = sh.best[w] > best ? sh.best[w] : best;
         if (tid == 0) write(r, best);
         last = best;  // 0: nothing is left, nor will be
     }
@@ -296,10 +318,10 @@ __device__ __forceinline__ uint64_t* PairsOf(const LogprobsLaunch& p, int64_t at
 
 // Where a row's part is short enough a thread keeps its logits for the
 // alternatives, in H units (one row of 131072 with 20: 11.2 us; 12.3 read twice).
-template <typename T, bool kEntropy, int H>
-__global__ __launch_bounds__(kThreads) void LogprobsKernel(LogprobsLaunch p, int32_t segments, int32_t length)
+template <typename T, bool kEntropy, int H, int W>
+__global__ __launch_bounds__(W) void LogprobsKernel(LogprobsLaunch p, int32_t segments, int32_t length)
 {
-    __shared__ Shared sh;
+    __shared__ Shared<W> sh;
     const uint32_t number = BlockNumber();
     const int64_t row = number / static_cast<uint32_t>(segments);
     if (row >= p.rows) return;
@@ -307,17 +329,17 @@ __global__ __launch_bounds__(kThreads) void LogprobsKernel(LogprobsLaunch p, int
     const T* logits = static_cast<const T*>(p.logits) + row * p.ld;
     const int32_t vocab = static_cast<int32_t>(p.vocab);
     const int32_t begin = segment * length, end = vocab - begin < length ? vocab : begin + length;
-    Held<T, H> held;
+    Held<T, H, W> held;
     const Part mine = held.template Read<kEntropy>(logits, begin, end);
     const Part wave = WavePart(mine);
     if ((threadIdx.x & 63) == 0) sh.part[threadIdx.x >> 6] = wave;
     __syncthreads();
     float most = kLowest;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) most = fmaxf(most, sh.part[w].m);
+    for (int w = 0; w < W / 64; ++w) most = fmaxf(most, sh.part[w].m);
     Part all{most, 0.0f, 0.0f};
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < W / 64; ++w) {
         Part one = sh.part[w];
         one.MoveTo(most);
         all.s += one.s;
@@ -341,13 +363,23 @@ __global__ __launch_bounds__(kThreads) void LogprobsKernel(LogprobsLaunch p, int
     }
 }
 
-// Joins a row's segments, one per lane of the first wave; of the sorted lists the
-// largest head is taken k times.  All waves bring the lists to LDS, and a lane
-// holds its head and the one behind it: a step waits for no memory.
+// Joins a row's segments, one per lane of the first wave, and their sorted lists.
+//
+// Of the k-th of all, a bound: where r = ceil(k / segments), the ceil(k / r)-th
+// largest of the lists' r-th ones has k at or above it.  What is at or above the
+// bound finds its rank by comparing itself with all of it, as in TakeTop.  Few
+// alternatives, or too many at the bound, are taken one after another, the
+// largest head of all lists each time: a lane holds its list's and the one behind
+// it, so that a step waits for no memory.  Both launches with 5 alternatives of
+// 32000 one after another 8.0 us, by the bound 9.1; 20 of 131072 11 and 10.4, 50
+// 17.9 and 13.2.
+constexpr int32_t kOneByOne = 12;
 template <typename T>
 __global__ __launch_bounds__(kThreads) void LogprobsJoinKernel(LogprobsLaunch p, int32_t segments)
 {
-    __shared__ uint64_t list[kMaxSegments * kMaxTop];
+    __shared__ uint64_t list[kMaxSegments * kMaxTop], candidate[kCandidates], bound;
+    __shared__ uint32_t count;
+    __shared__ RowResult result;
     const int64_t row = BlockNumber();
     if (row >= p.rows) return;
     const int tid = threadIdx.x;
@@ -355,10 +387,10 @@ __global__ __launch_bounds__(kThreads) void LogprobsJoinKernel(LogprobsLaunch p,
     const bool mine = tid < segments;
     Part part{kLowest, 0.0f, 0.0f};
     if (mine) part = *PartOf(p, row * segments + tid);
+    constexpr int kEach = kMaxSegments * kMaxTop / kThreads;
+    uint64_t held[kEach] = {};
     if (k > 0) {
         const uint64_t* pairs = PairsOf(p, row * segments, segments);
-        constexpr int kEach = kMaxSegments * kMaxTop / kThreads;
-        uint64_t held[kEach];
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             if (i * kThreads + tid < segments * k) held[i] = pairs[i * kThreads + tid];
@@ -367,13 +399,65 @@ __global__ __launch_bounds__(kThreads) void LogprobsJoinKernel(LogprobsLaunch p,
         for (int i = 0; i < kEach; ++i) {
             if (i * kThreads + tid < segments * k) list[i * kThreads + tid] = held[i];
         }
+        if (tid == 64) {
+            bound = 1;  // 0 stands for none
+            count = 0;
+        }
         __syncthreads();
     }
-    if (tid >= 64) return;
-    part = WavePart(part);
-    const RowResult r = Finish(part);
-    if (tid == 0) WriteRow<T>(p, row, part, r);
+    if (k > kOneByOne) {
+        // four lanes compare a list's with a quarter of the others
+        constexpr int G = kThreads / kMaxSegments;
+        const int32_t r = (k + segments - 1) / segments, place = (k + r - 1) / r - 1;
+        const int32_t own = tid / G, lane = tid % G;
+        const uint64_t x = own < segments ? list[own * k + r - 1] : 0;
+        uint32_t above = 0;
+#pragma unroll
+        for (int i = 0; i < kMaxSegments / G; ++i) {
+            const int32_t s = i * G + lane;
+            above += s < segments && list[s * k + r - 1] > x ? 1 : 0;
+        }
+        above = SumOverLanes<G>(above);
+        if (above == static_cast<uint32_t>(place) && x != 0 && lane == 0) bound = x;
+    }
+    if (tid < 64) {
+        part = WavePart(part);
+        const RowResult r = Finish(part);
+        if (tid == 0) {
+            WriteRow<T>(p, row, part, r);
+            result = r;
+        }
+    }
     if (k == 0) return;
+    __syncthreads();
+    const RowResult r = result;
+    uint32_t found = kCandidates + 1;
+    if (k > kOneByOne) {
+        const uint64_t least = bound;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            if (held[i] >= least) {
+                const uint32_t at = atomicAdd(&count, 1U);
+                if (at < kCandidates) candidate[at] = held[i];
+            }
+        }
+        __syncthreads();
+        found = count;
+    }
+    if (found <= kCandidates) {
+        for (uint32_t c = tid; c < found; c += kThreads) {
+            const uint64_t pair = candidate[c];
+            int32_t above = 0;
+#pragma unroll 8
+            for (uint32_t i = 0; i < found; ++i) above += candidate[i] > pair ? 1 : 0;
+            if (above < k) WriteTop(p, row, above, pair, r.m, r.logs);
+        }
+        for (int32_t rank = static_cast<int32_t>(found) + tid; rank < k; rank += kThreads) {
+            WriteTop(p, row, rank, 0, r.m, r.logs);
+        }
+        return;
+    }
+    if (tid >= 64) return;
     int32_t at = tid * k + 1;
     const int32_t end = mine ? tid * k + k : 0;
     uint64_t head = mine ? list[tid * k] : 0, next = at < end ? list[at] : 0, taken = 0;
@@ -463,39 +547,56 @@ __global__ __launch_bounds__(kThreads) void LogprobsGradKernel(LogprobsGradLaunc
     }
 }
 
-// Segments of a row: as many as make a thousand workgroups, none shorter than a unit for each thread.
-int32_t Segments(int64_t rows, int64_t vocab)
+// How the rows are cut: segments of a row, their length (a multiple of a unit), threads of a workgroup.
+//
+// Up to 4096 logits are one workgroup's, and so are up to 32768 of up to 512 rows, with 1024 threads that hold them: 37
+// rows of 32000 fp32 with 5 alternatives take 8.2 us, in segments and joined 10.1; 8000 with none 4.3 and 5.2; 512 rows
+// of 32000 with 5 22 and 26, 1024 39 and 41 (of 8000 15 and 11).  Few rows without alternatives are joined faster, 16 of
+// 32000 in 5.1 us where one workgroup each takes 5.5, but a row's sum should not change with what else is asked for.
+// Longer rows are cut into as many segments as make a thousand workgroups, none shorter than a unit for each thread.
+struct Cut {
+    int32_t segments, length;
+    bool wide;
+};
+Cut CutOf(int64_t rows, int64_t vocab)
 {
+    auto whole = [](int64_t n) { return static_cast<int32_t>((n + kUnit - 1) / kUnit * kUnit); };
+    const bool wide = vocab > 4096 && vocab <= 1024 * kUnit * kBatch && rows <= 512;
+    if (vocab <= 4096 || wide) return {1, whole(vocab), wide};
     const int64_t units = (vocab + kThreads * kUnit - 1) / (kThreads * kUnit), want = rows > 0 ? 1024 / rows : 1;
     int64_t s = want < units ? want : units;
-    s = s < kMaxSegments ? s : kMaxSegments;
-    return static_cast<int32_t>(s < 1 ? 1 : s);
-}
-
-// Of a segment, a multiple of a unit
-int32_t Length(int64_t vocab, int32_t segments)
-{
-    const int64_t each = (vocab + segments - 1) / segments;
-    return static_cast<int32_t>((each + kUnit - 1) / kUnit * kUnit);
+    s = s > kMaxSegments ? kMaxSegments : s < 1 ? 1 : s;
+    const int32_t length = whole((vocab + s - 1) / s);
+    return {static_cast<int32_t>((vocab + length - 1) / length), length, false};
 }
 
 template <typename T>
 int LaunchTyped(const LogprobsLaunch& l, hipStream_t s)
 {
-    int32_t segments = Segments(l.rows, l.vocab);
-    const int32_t length = Length(l.vocab, segments);
-    segments = static_cast<int32_t>((l.vocab + length - 1) / length);
-    if (l.rows > INT32_MAX / segments) return kTooLarge;
-    const dim3 grid = GridOf(l.rows * segments);
-    auto launch = [&](auto held) {
-        constexpr int H = decltype(held)::value;
-        if (l.entropy != nullptr) LogprobsKernel<T, true, H><<<grid, kThreads, 0, s>>>(l, segments, length);
-        else LogprobsKernel<T, false, H><<<grid, kThreads, 0, s>>>(l, segments, length);
+    const Cut cut = CutOf(l.rows, l.vocab);
+    if (l.rows > INT32_MAX / cut.segments) return kTooLarge;
+    auto launch = [&](auto held, auto threads) {
+        constexpr int H = decltype(held)::value, W = decltype(threads)::value;
+        const dim3 grid = GridOf(l.rows * cut.segments);
+        if (l.entropy != nullptr) LogprobsKernel<T, true, H, W><<<grid, W, 0, s>>>(l, cut.segments, cut.length);
+        else LogprobsKernel<T, false, H, W><<<grid, W, 0, s>>>(l, cut.segments, cut.length);
     };
-    if (length <= kThreads * kUnit) launch(std::integral_constant<int, 1>{});
-    else if (length <= kThreads * kUnit * kBatch) launch(std::integral_constant<int, kBatch>{});
-    else launch(std::integral_constant<int, 0>{});
-    if (segments > 1) LogprobsJoinKernel<T><<<GridOf(l.rows), kThreads, 0, s>>>(l, segments);
+    constexpr std::integral_constant<int, 0> none{};
+    constexpr std::integral_constant<int, 1> one{};
+    constexpr std::integral_constant<int, kBatch> batch{};
+    constexpr std::integral_constant<int, kThreads> threads{};
+    constexpr std::integral_constant<int, 1024> many{};
+    if (cut.wide) {
+        if (cut.length <= 1024 * kUnit) launch(one, many);
+        else launch(batch, many);
+    } else if (cut.length <= kThreads * kUnit) {
+        launch(one, threads);
+    } else if (cut.length <= kThreads * kUnit * kBatch) {
+        launch(batch, threads);
+    } else {
+        launch(none, threads);
+    }
+    if (cut.segments > 1) LogprobsJoinKernel<T><<<GridOf(l.rows), kThreads, 0, s>>>(l, cut.segments);
     return 0;
 }
 
@@ -512,7 +613,7 @@ int LaunchGradTyped(const LogprobsGradLaunch& l, hipStream_t s)
 
 size_t LogprobsBytes(int64_t rows, int64_t vocab, int64_t top)
 {
-    const int32_t segments = Segments(rows, vocab);
+    const int32_t segments = CutOf(rows, vocab).segments;
     return segments > 1 ? static_cast<size_t>(rows) * segments * (16 + 8 * top) : 0;
 }
 

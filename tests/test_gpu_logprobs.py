@@ -155,6 +155,39 @@ def test_alternatives_in_one_threads_places(dev, t):
     assert torch.equal(r.top_ids.long(), torch.sort(x, dim=1, descending=True, stable=True).indices[:, :64])
 
 
+@pytest.mark.parametrize("t,v", [(5, 1030), (3, 2047), (1, 2049), (2, 4096), (1, 4097), (512, 4100), (40, 8193),
+                                 (513, 9000), (2, 32768), (3, 32769), (70, 32001), (1, 140000)])
+@pytest.mark.parametrize("k", [0, 12, 13, 64])
+def test_ways_of_cutting_rows(dev, t, v, k):
+    # one workgroup or several a row, of 256 or 1024 threads; alternatives by a bound or one after another
+    for dtype in (F32, BF16):
+        logits = rows(t, v, dtype, 25)
+        targets = torch.randint(-1, v + 1, (t,), generator=gen(26), device=dev)
+        r = token_logprobs(logits, targets, top=k, entropy=True)
+        lp, h, logs = plain(logits, targets)
+        check(r.logprobs, lp, error(logits))
+        check(r.entropy, h, error(logits) + 4 * error(logits) * h.abs())
+        if k == 0:
+            continue
+        want = torch.sort(logits.float(), dim=1, descending=True, stable=True).indices[:, :k]
+        assert torch.equal(r.top_ids.long(), want)
+        check(r.top_logprobs, logs.gather(1, want.cpu()), error(logits))
+
+
+@pytest.mark.parametrize("t,v", [(1, 131072), (9, 60000), (6, 32000), (4, 2000)])
+@pytest.mark.parametrize("k", [5, 64])
+def test_alternatives_side_by_side(dev, t, v, k):
+    # rising, falling, and all of what is not masked in one place: the largest are one segment's, or a few threads'
+    up = torch.arange(v, device=dev, dtype=F32) * (40.0 / v)
+    run = torch.full((v,), -float("inf"), device=dev)
+    run[v // 2:v // 2 + 1900] = torch.randn(min(1900, v - v // 2), generator=gen(27), device=dev)
+    for row in (up, up.flip(0), run):
+        logits = row.repeat(t, 1)
+        r = token_logprobs(logits, torch.zeros(t, dtype=torch.int64, device=dev), top=k)
+        want = torch.sort(logits, dim=1, descending=True, stable=True).indices[:, :k]
+        assert torch.equal(r.top_ids.long(), want)
+
+
 def test_far_apart_logits(dev):
     x = torch.tensor([[0.0, 88.0, 200.0], [-200.0, -100.0, -150.0], [1e30, -1e30, 0.0], [3e38, -3e38, 3e38],
                       [100.0, 100.0, 100.0]], device=dev)

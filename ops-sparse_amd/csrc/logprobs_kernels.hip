@@ -8,11 +8,11 @@
 // One pass over a row keeps M, S and W per thread; where the largest grows,
 // S and W are moved to it.  With few rows several workgroups share one, and
 // another launch joins what they found.  Bound by memory: the logits are read
-// once, for alternatives a second time out of the caches.  8192 rows of 65536
+// once, those of few threads a second time for alternatives.  8192 rows of 65536
 // bf16 logits with the entropy: 192 us (5.6 TB/s), their gradient 351 us (6.1
 // TB/s read and written).  One row of 131072 with 20 alternatives, 64 segments:
-// 4.8 us and 5.0 to join them, latency alone; 37 rows of 32003 fp32 with 5, a
-// workgroup each: 7.7 us, its exponentials and what is around them.
+// 4.8 us and 4.8 to join them, latency alone; 37 rows of 32003 fp32 with 5, a
+// workgroup each: 7.5 us, its exponentials and what is around them.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -221,7 +221,8 @@ struct Shared {
     Part part[W / 64];
     uint64_t pair[kCandidates];  // candidates; before that each group's largest
     uint64_t best[W / 64];
-    uint32_t count;
+    uint16_t looking[W];  // threads that hold candidates
+    uint32_t count, lookers;
     float threshold;
 };
 
@@ -231,16 +232,17 @@ struct Shared {
 // The k-th largest of 64 or 128 groups' largest is a bound below which the answer
 // has nothing: those groups of threads hold k logits at or above it.  (128 where
 // 64 leave some empty: rows of 1025 to 2048 logits, more than the candidates, else
-// had no bound; its ranks cost 0.6 us more of 256 threads.)  A second pass lists
-// what is at or above the bound, mostly little more than k logits, and each finds
-// its rank by comparing itself with all.  A row with NaN, or with more logits
+// had no bound; its ranks cost 0.6 us more of 256 threads.)  What is
+// at or above the bound is listed, mostly little more than k logits, out of what
+// the threads have seen whose largest is, and each finds its rank by comparing
+// itself with all.  A row with NaN, or with more logits
 // at the bound than fit (equal ones), goes through k passes instead.
 template <typename T, int H, int W, typename Write>
 __device__ __forceinline__ void TakeTop(Shared<W>& sh, const Held<T, H, W>& held, const T* row, int32_t begin, int32_t end,
                                         int32_t k, float m, bool nan, Write write)
 {
     const int tid = threadIdx.x;
-    if (tid == 0) sh.count = 0;
+    if (tid == 0) sh.count = sh.lookers = 0;
     auto setBound = [&](auto lanes) {
         constexpr int G = decltype(lanes)::value;
         const int group = tid / G, lane = tid % G;
@@ -261,12 +263,35 @@ __device__ __forceinline__ void TakeTop(Shared<W>& sh, const Held<T, H, W>& held
     __syncthreads();
     const float threshold = sh.threshold;
     if (!nan) {
-        held.ForEach(row, begin, end, [&](float x, int32_t index) {
+        auto add = [&](float x, int32_t index) {
             if (x >= threshold) {
                 const uint32_t at = atomicAdd(&sh.count, 1U);
                 if (at < kCandidates) sh.pair[at] = Pair(x, index);
             }
-        });
+        };
+        if constexpr (H > 0) {
+            if (m >= threshold) held.ForEach(row, begin, end, add);
+        } else {
+            // Few threads have seen any.  What they have read is read again, by all threads (1024 rows of 131072 fp32 with 5
+            // alternatives 94 us, by those threads alone 103, the whole row again 180; with none 91).
+            if (m >= threshold) sh.looking[atomicAdd(&sh.lookers, 1U)] = static_cast<uint16_t>(tid);
+            __syncthreads();
+            const uint32_t lookers = sh.lookers, rounds = (end - begin + W * kUnit - 1) / (W * kUnit);
+            const uint32_t units = lookers * rounds;
+            for (uint32_t first = tid; first < units; first += W * kBatch) {
+                T u[kBatch][kUnit];
+                int32_t at[kBatch];
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b) {
+                    const uint32_t n = first + b * W, round = n / lookers;
+                    at[b] = n < units ? begin + static_cast<int32_t>((round * W + sh.looking[n - round * lookers]) * kUnit)
+                                      : end;
+                    LoadUnit(row, at[b], end, u[b]);
+                }
+#pragma unroll
+                for (int i = 0; i < kBatch * kUnit; ++i) add(ToFloat(u[i / kUnit][i % kUnit]), at[i / kUnit] + i % kUnit);
+            }
+        }
         __syncthreads();
         const uint32_t count = sh.count;
         if (count <= kCandidates) {
@@ -554,7 +579,7 @@ __global__ __launch_bounds__(kThreads) void LogprobsGradKernel(LogprobsGradLaunc
 //
 // Up to 4096 logits are one workgroup's, and so are up to 32768 of up to 512 rows, with 1024 threads that hold them: 37
 // rows of 32000 fp32 with 5 alternatives take 8.2 us, in segments and joined 10.1; 8000 with none 4.3 and 5.2; 512 rows
-// of 32000 with 5 22 and 26, 1024 39 and 41 (of 8000 15 and 11).  Few rows without alternatives are joined faster, 16 of
+// of 32000 with 5 21 and 26, 1024 39 and 29 (of 8000 15 and 11).  Few rows without alternatives are joined faster, 16 of
 // 32000 in 5.1 us where one workgroup each takes 5.5, but a row's sum should not change with what else is asked for.
 // Longer rows are cut into as many segments as make a thousand workgroups, none shorter than a unit for each thread.
 struct Cut {

@@ -367,6 +367,27 @@ def test_a_training_step_in_a_graph(dev):
             assert torch.equal(a, b)
 
 
+def test_answers_in_two_graphs(dev):
+    # rows in segments that are joined, in one workgroup, and read again for alternatives; graphs with workspaces each
+    sets = []
+    for t, v, k in ((1, 131072, 20), (3, 40000, 5), (37, 9000, 50), (1100, 9000, 5)):
+        x, targets = rows(t, v, BF16, 40), torch.zeros(t, dtype=torch.int64, device=dev)
+        token_logprobs(x, targets, top=k)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = token_logprobs(x, targets, top=k, entropy=True)
+        sets.append((x, targets, k, graph, got))
+    for seed in range(3):
+        for x, targets, _, graph, _ in sets:
+            x.copy_(rows(*x.shape, BF16, 50 + seed))
+            targets.copy_(torch.randint(0, x.shape[1], targets.shape, generator=gen(seed), device=dev))
+            graph.replay()
+        torch.cuda.synchronize()
+        for x, targets, k, _, got in sets:
+            for one, other in zip(got, token_logprobs(x, targets, top=k, entropy=True)):
+                assert torch.equal(one, other)
+
+
 @pytest.mark.parametrize("leaf", [True, False])
 def test_a_capture_beside_an_eager_graph_of_the_leaf_is_refused(dev, leaf):
     # torch's engine would make the eager graph's stream wait for the captured one and end the process

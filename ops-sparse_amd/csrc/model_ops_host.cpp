@@ -96,10 +96,11 @@ bool Add(aclsp::AdamWTable& table, int& used, const aclsp::AdamWTensor& t, int64
     return true;
 }
 
+// Places that are not used come behind every chunk.
 void Clear(aclsp::AdamWTable& table, int& used)
 {
-    table = {};
     for (uint32_t& first : table.first) first = UINT32_MAX;
+    table.chunks = 0;
     used = 0;
 }
 
@@ -197,14 +198,13 @@ aclsparseStatus_t aclsparseAdamW(aclsparseHandle_t handle, int64_t count, const 
     int rc = aclsp::LaunchAdamWFactors(s, options->buffer, stream);
     // one launch for each 64 tensors of one kind
     constexpr aclDataType kTypes[] = {ACL_FLOAT, ACL_FLOAT16, ACL_BF16};
-    aclsp::AdamWTable table;
+    aclsp::AdamWTable table{};
     int used = 0;
     aclDataType param = ACL_FLOAT, grad = ACL_FLOAT;
     bool master = false;
     auto flush = [&] {
-        if (rc == 0 && used > 0) {
-            rc = aclsp::LaunchAdamW(table, options->buffer, param, grad, options->momentBits, master, stream);
-        }
+        if (used == 0) return;
+        if (rc == 0) rc = aclsp::LaunchAdamW(table, options->buffer, param, grad, options->momentBits, master, stream);
         Clear(table, used);
     };
     Clear(table, used);
@@ -244,7 +244,7 @@ aclsparseStatus_t aclsparseAdamWMoments(aclsparseHandle_t handle, int64_t count,
         }
     }
     (void)hipGetLastError();
-    aclsp::AdamWTable table;
+    aclsp::AdamWTable table{};
     int used = 0;
     Clear(table, used);
     for (int64_t i = 0; i < count; ++i) {

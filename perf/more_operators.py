@@ -186,9 +186,9 @@ _MASK = 0xFFFFFFFF
 
 def _mix(x):
     x = x ^ (x >> 16)
-    x = (x * 0x9B05688D) & _MASK
+    x = (x * 0x6A09E667) & _MASK
     x = x ^ (x >> 15)
-    x = (x * 0x5BE0CD19) & _MASK
+    x = (x * 0xBB67AE85) & _MASK
     return x ^ (x >> 16)
 
 
@@ -390,7 +390,7 @@ def _plain_adamw(s):
         bits = _random_bits(n, s["seed"], s["step"][0].long(), i)
         for j, (x, r) in enumerate(((m, bits & 0xFFFF), (v, bits >> 16))):
             held[j], s["exponents"][i][j] = _to_8(x, r, j)
-        moments.append(torch.stack([_of_8(held[j], s["exponents"][i][j], j) for j in range(2)]))
+        moments.append(torch.stack([_of_8(held[j], s["exponents"][i][j], j)[:n] for j in range(2)]))
     return {"params": s["params"], "masters": s["masters"],
             "moments": s["moments"] if case["bits"] == 32 else moments}
 

@@ -541,6 +541,13 @@ typedef struct aclsparseAdamWOptions_t {
  * parameters go by the moments before that.  A block that holds infinity or NaN becomes NaN. */
 aclsparseStatus_t aclsparseAdamW(aclsparseHandle_t handle, int64_t count, const aclsparseAdamWTensor_t* tensors,
                                  const aclsparseAdamWOptions_t* options);
+/* The same with the factors of the rounding's random numbers, odd ones, for 8-bit moments that are to be another program's
+ * bit by bit.  All in 32 bits without a sign, with mix(x): x ^= x >> 16, x *= factor1, x ^= x >> 15, x *= factor2,
+ * x ^= x >> 16: element i of the place-th tensor takes n = mix(i + mix(mix(mix(seed) + step) + place)), i's bits from the
+ * 32nd on added to place; the first moment is rounded by the 16 low bits of n, the second by the 16 high ones.
+ * aclsparseAdamW takes 0x9B05688D and 0x5BE0CD19, for which the two halves are independent. */
+aclsparseStatus_t aclsparseAdamWMixed(aclsparseHandle_t handle, int64_t count, const aclsparseAdamWTensor_t* tensors,
+                                      const aclsparseAdamWOptions_t* options, uint32_t factor1, uint32_t factor2);
 /* The values of 8-bit moments in fp32, [2, count] for each tensor, to its master; param and grad are not read. */
 aclsparseStatus_t aclsparseAdamWMoments(aclsparseHandle_t handle, int64_t count,
                                         const aclsparseAdamWTensor_t* tensors);

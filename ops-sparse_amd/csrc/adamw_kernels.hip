@@ -66,13 +66,13 @@ __device__ __forceinline__ uint32_t QuadMax(uint32_t x)
     return x > z ? x : z;
 }
 
-// Scrambles 32 bits; the factors are the first bits of the roots of 13 and 19.
-__device__ __forceinline__ uint32_t Mix(uint32_t x)
+// Scrambles 32 bits.
+__device__ __forceinline__ uint32_t Mix(uint32_t x, const AdamWMix& by)
 {
     x ^= x >> 16;
-    x *= 0x9B05688DU;
+    x *= by.first;
     x ^= x >> 15;
-    x *= 0x5BE0CD19U;
+    x *= by.second;
     return x ^ (x >> 16);
 }
 
@@ -80,6 +80,7 @@ __device__ __forceinline__ uint32_t Mix(uint32_t x)
 struct Factors {
     float beta1, rest1, beta2, rest2, decay, size, inverse_root, eps, scale;
     uint32_t key;
+    AdamWMix mix;
 };
 static_assert(sizeof(Factors) <= kAdamWBufferBytes, "");
 
@@ -134,7 +135,8 @@ __global__ void AdamWFactorsKernel(AdamWScalars s, Factors* out)
     f.inverse_root = static_cast<float>(InverseRoot(1.0 - power2));
     f.eps = static_cast<float>(s.eps);
     f.scale = s.grad_scale != nullptr ? *s.grad_scale : 1.0f;
-    f.key = Mix(Mix(s.seed) + static_cast<uint32_t>(step));
+    f.key = Mix(Mix(s.seed, s.mix) + static_cast<uint32_t>(step), s.mix);
+    f.mix = s.mix;
     *out = f;
     s.step[0] = step;
 }
@@ -281,9 +283,10 @@ __global__ __launch_bounds__(kThreads) void AdamWKernel(AdamWTable table, const 
             }
             uint32_t random[V];
             const uint32_t seed = Mix(f.key + static_cast<uint32_t>(table.place[which]) +
-                                      static_cast<uint32_t>(static_cast<uint64_t>(at) >> 32));
+                                          static_cast<uint32_t>(static_cast<uint64_t>(at) >> 32),
+                                      f.mix);
 #pragma unroll
-            for (int i = 0; i < V; ++i) random[i] = Mix(static_cast<uint32_t>(at) + i + seed);
+            for (int i = 0; i < V; ++i) random[i] = Mix(static_cast<uint32_t>(at) + i + seed, f.mix);
             uint8_t* codes = static_cast<uint8_t*>(t.moments) + at;
             Pack<kLeastM, true>(m[u], random, codes, t.exponents + at / 32);
             Pack<kLeastV, false>(v[u], random, codes + padded, t.exponents + (padded + at) / 32);

@@ -41,6 +41,7 @@ void Bind(const std::string& path)
     look(lib.mx4Dequantize, "aclsparseMx4Dequantize");
     look(lib.groupedMMMx4, "aclsparseGroupedMMMx4");
     look(lib.adamW, "aclsparseAdamW");
+    look(lib.adamWMixed, "aclsparseAdamWMixed");
     look(lib.adamWMoments, "aclsparseAdamWMoments");
     look(lib.logprobsBufferSize, "aclsparseTokenLogprobs_bufferSize");
     look(lib.logprobs, "aclsparseTokenLogprobs");

@@ -180,11 +180,18 @@ aclsparseStatus_t aclsparseGroupedMMMx4(aclsparseHandle_t handle, int64_t groups
 aclsparseStatus_t aclsparseAdamW(aclsparseHandle_t handle, int64_t count, const aclsparseAdamWTensor_t* tensors,
                                  const aclsparseAdamWOptions_t* options)
 {
+    constexpr aclsp::AdamWMix own{};
+    return aclsparseAdamWMixed(handle, count, tensors, options, own.first, own.second);
+}
+
+aclsparseStatus_t aclsparseAdamWMixed(aclsparseHandle_t handle, int64_t count, const aclsparseAdamWTensor_t* tensors,
+                                      const aclsparseAdamWOptions_t* options, uint32_t factor1, uint32_t factor2)
+{
     aclsparseStatus_t st = CheckHandle(handle);
     if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
     if (count < 0 || options == nullptr || (count > 0 && tensors == nullptr)) return ACL_SPARSE_STATUS_INVALID_VALUE;
     if (count > INT32_MAX) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
-    st = CheckAdamW(*options);
+    st = factor1 % 2 != 0 && factor2 % 2 != 0 ? CheckAdamW(*options) : ACL_SPARSE_STATUS_INVALID_VALUE;
     if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
     for (int64_t i = 0; i < count; ++i) {
         if (tensors[i].count > aclsp::kAdamWMostChunks * aclsp::kAdamWChunk) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
@@ -192,7 +199,8 @@ aclsparseStatus_t aclsparseAdamW(aclsparseHandle_t handle, int64_t count, const 
         if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
     }
     const aclsp::AdamWScalars s{options->lr, options->beta1, options->beta2, options->eps, options->weightDecay,
-                          options->lrDevice, options->gradScale, options->step, options->seed};
+                          options->lrDevice, options->gradScale, options->step, options->seed,
+                                {factor1, factor2}};
     (void)hipGetLastError();
     void* stream = StreamOf(handle);
     int rc = aclsp::LaunchAdamWFactors(s, options->buffer, stream);

@@ -63,12 +63,18 @@ struct AdamWTable {
     int32_t place[kAdamWTensors];   // in the caller's list
     uint32_t chunks;                // of all
 };
+// Odd factors of the hash that 8-bit moments' random numbers come from.  The library's own are the first bits of the roots
+// of 13 and 19 behind the point (made odd): numbers whose bits, and whose two halves, are independent.
+struct AdamWMix {
+    uint32_t first = 0x9B05688DU, second = 0x5BE0CD19U;
+};
 struct AdamWScalars {
     double lr, beta1, beta2, eps, weight_decay;
     const float* lr_device;   // null: lr
     const float* grad_scale;  // null: one
     int32_t* step;            // steps taken; this one is counted
     uint32_t seed;
+    AdamWMix mix;
 };
 // Values of a workgroup; a launch has one for each chunk, and fewer than 2^32 threads.
 constexpr int64_t kAdamWChunk = 2048, kAdamWMostChunks = (int64_t{1} << 24) - 1;

@@ -174,7 +174,7 @@ void CheckMoments(int64_t count, const Tensor& moments, const optional<Tensor>& 
 void AdamWStep(const Tensors& params, const MaybeTensors& grads, const Tensors& moments,
                const optional<Tensors>& exponents, const optional<Tensors>& masters, const Tensor& step, int64_t seed,
                double lr, const optional<Tensor>& lrTensor, double beta1, double beta2, double eps, double weightDecay,
-               const optional<Tensor>& gradScale)
+               const optional<Tensor>& gradScale, const optional<std::pair<int64_t, int64_t>>& factors)
 {
     const size_t count = params.size();
     TORCH_CHECK_VALUE(grads.size() == count && moments.size() == count &&
@@ -186,6 +186,9 @@ void AdamWStep(const Tensors& params, const MaybeTensors& grads, const Tensors& 
                           (lrTensor.has_value() || (lr >= 0 && std::isfinite(lr))),
                       "lr, eps and weight_decay must be finite and not negative");
     TORCH_CHECK_VALUE(seed >= 0 && seed <= UINT32_MAX, "the seed must fit 32 bits without a sign");
+    auto odd = [](int64_t f) { return f >= 0 && f <= UINT32_MAX && f % 2 != 0; };
+    TORCH_CHECK_VALUE(!factors.has_value() || (odd(factors->first) && odd(factors->second)),
+                      "the factors must be odd and fit 32 bits without a sign");
     TORCH_CHECK_TYPE(step.scalar_type() == at::kInt, "step must be int32, got ", step.scalar_type());
     TORCH_CHECK_VALUE(step.dim() == 1 && step.size(0) == 2 && step.is_contiguous(), "step must hold two counts");
     OnGpu(step);
@@ -241,7 +244,13 @@ void AdamWStep(const Tensors& params, const MaybeTensors& grads, const Tensors& 
     o.seed = static_cast<uint32_t>(seed);
     o.momentBits = exponents.has_value() ? 8 : 32;
     Call call(step);
-    Call::Ok(lib.adamW(call, static_cast<int64_t>(count), table.data(), &o), "aclsparseAdamW");
+    if (factors.has_value()) {
+        Call::Ok(lib.adamWMixed(call, static_cast<int64_t>(count), table.data(), &o, static_cast<uint32_t>(factors->first),
+                                static_cast<uint32_t>(factors->second)),
+                 "aclsparseAdamWMixed");
+    } else {
+        Call::Ok(lib.adamW(call, static_cast<int64_t>(count), table.data(), &o), "aclsparseAdamW");
+    }
     // a value that a backward pass still needs has changed: it raises, as after a torch operation in place
     for (size_t i = 0; i < count; ++i) {
         if (!params[i].is_inference() && grads[i].has_value()) torch::autograd::impl::bump_version(params[i]);

@@ -37,6 +37,7 @@ struct Library {
     decltype(&aclsparseMx4Dequantize) mx4Dequantize = nullptr;
     decltype(&aclsparseGroupedMMMx4) groupedMMMx4 = nullptr;
     decltype(&aclsparseAdamW) adamW = nullptr;
+    decltype(&aclsparseAdamWMixed) adamWMixed = nullptr;
     decltype(&aclsparseAdamWMoments) adamWMoments = nullptr;
     decltype(&aclsparseTokenLogprobs_bufferSize) logprobsBufferSize = nullptr;
     decltype(&aclsparseTokenLogprobs) logprobs = nullptr;

@@ -212,6 +212,8 @@ SIGNATURES = {
     "aclsparseGroupedMMMx4": [_vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp,
                               _i64, _i64, _vp, _i64, _i32],
     "aclsparseAdamW": [_vp, _i64, ctypes.POINTER(AdamWTensor), ctypes.POINTER(AdamWOptions)],
+    "aclsparseAdamWMixed": [_vp, _i64, ctypes.POINTER(AdamWTensor), ctypes.POINTER(AdamWOptions), ctypes.c_uint32,
+                            ctypes.c_uint32],
     "aclsparseAdamWMoments": [_vp, _i64, ctypes.POINTER(AdamWTensor)],
     "aclsparseTokenLogprobs_bufferSize": [_vp, _i64, _i64, _i64, ctypes.POINTER(_sz)],
     "aclsparseTokenLogprobs": [_vp, _i64, _i64, _vp, _i64, _i32, _vp, _i32, _vp, _vp, _vp, _i64, _vp, _vp, _vp],

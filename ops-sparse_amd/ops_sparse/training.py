@@ -12,7 +12,7 @@ torch stream through the C entry points of libaclsparse_hip.so; nothing waits fo
 in a HIP graph.  There is no CPU path.  Arguments that do not fit raise ValueError, types that are not supported
 TypeError.  The reference has no counterpart.
 """
-from typing import List, NamedTuple, Optional
+from typing import List, NamedTuple, Optional, Tuple
 
 import torch
 
@@ -46,13 +46,16 @@ class AdamWState(NamedTuple):
 
     moments: [2, P] with P = n rounded up to 32, the first moment and the second one, fp32 or uint8 codes; exponents:
     [2, P / 32] uint8 for the codes, None for fp32; masters: the values in fp32, None where the parameters themselves
-    are kept; step: int32 [2], the steps taken and a place that is not used; seed: of the rounding of 8-bit moments (32 bits).
+    are kept; step: int32 [2], the steps taken and a place that is not used; seed: of the rounding of 8-bit moments (32 bits);
+    factors: two odd numbers of 32 bits that the rounding's random numbers are made with, where 8-bit moments are to be
+    another program's bit by bit (include/cann_ops_sparse.h says how), None for the library's own.
     """
     moments: List[torch.Tensor]
     exponents: Optional[List[torch.Tensor]]
     masters: Optional[List[torch.Tensor]]
     step: torch.Tensor
     seed: int = 0
+    factors: Optional[Tuple[int, int]] = None
 
 
 def adamw_state(params, bits=32, masters=True, seed=0):
@@ -86,7 +89,7 @@ def adamw_step(params, grads, state, lr, betas=(0.9, 0.999), eps=1e-8, weight_de
     tensor = lr if isinstance(lr, torch.Tensor) else None
     (experts._MODULE or _module()).adamw_step(list(params), list(grads), state.moments, state.exponents, state.masters,
                                               state.step, state.seed, 0.0 if tensor is not None else lr, tensor,
-                                              betas[0], betas[1], eps, weight_decay, grad_scale)
+                                              betas[0], betas[1], eps, weight_decay, grad_scale, state.factors)
 
 
 def adamw_moments(state):

@@ -337,3 +337,20 @@ def test_a_large_tensor(dev, bits):
     want = float(g[0][0].float()) * 0.1
     assert bool((m[0, :n] - want).abs().max() <= (want / 8 if bits == 8 else want * 2**-23))
     assert not m[:, n:].any()
+
+
+def test_random_numbers_by_given_factors(dev, monkeypatch):
+    first, second = 0x6A09E667, 0xBB67AE85  # the first bits of the roots of 2 and 3
+
+    def other(x):
+        x = x ^ (x >> 16)
+        x = (x * first) & 0xFFFFFFFF
+        x = x ^ (x >> 15)
+        x = (x * second) & 0xFFFFFFFF
+        return x ^ (x >> 16)
+
+    params, grads = tensors(SHAPES, BF16)
+    state = adamw_state(params, bits=8, seed=77)._replace(factors=(0x9B05688D, 0x5BE0CD19))
+    steps(params, grads, state, 2)  # the library's own
+    monkeypatch.setitem(globals(), "mix", other)
+    steps(params, grads, state._replace(factors=(first, second)), 2)

@@ -299,3 +299,17 @@ def test_scaled_products_in_assembly_follow_their_wait(tmp_path):
             count += 1
             assert before == "s_nop 1"
     assert count > 1000
+
+
+def test_factors_are_odd_numbers_of_32_bits(lib, handle):
+    for first, second in ((2, 3), (3, 0)):
+        assert lib.aclsparseAdamWMixed(handle, 1, ctypes.byref(tensor()), ctypes.byref(options()), first, second) == INVALID
+    assert lib.aclsparseAdamWMixed(None, 0, None, None, 3, 5) == Status.HANDLE_IS_NULLPTR
+    p = [torch.zeros(3)]
+    state = ops_sparse.adamw_state(p, bits=8)
+    assert state.factors is None
+    for factors in ((2, 3), (3, 2**32 + 1), (-1, 3)):
+        with pytest.raises(ValueError, match="factors"):
+            ops_sparse.adamw_step(p, p, state._replace(factors=factors), 1e-3)
+    with pytest.raises(ValueError, match="ROCm device"):
+        ops_sparse.adamw_step(p, p, state._replace(factors=(3, 5)), 1e-3)

@@ -315,7 +315,7 @@ def prepare(case, seed):
                 s["plan"] = api.ExpertPlan(*s["plan"])
         elif case["op"] == "adamw":
             s["state"] = api.AdamWState(s["moments"], s["exponents"] if case["bits"] == 8 else None, s["masters"],
-                                        s["step"], s["seed"])
+                                        s["step"], s["seed"], (0x6A09E667, 0xBB67AE85))  # of _mix
         elif case["op"] == "logprobs" and case["train"]:
             s["logits"].requires_grad_(True)
     return s
@@ -333,7 +333,9 @@ def _run_own(s):
         return (api.grouped_mm_mx4(s["x"], s["w"], s.get("plan"), gather=case["experts"] > 0),)
     if case["op"] == "adamw":
         api.adamw_step(s["params"], s["grads"], s["state"], grad_scale=s["clip"], **_HYPER)
-        moments = api.adamw_moments(s["state"]) if case["bits"] == 8 else s["moments"]
+        moments = s["moments"]
+        if case["bits"] == 8:
+            moments = [m[:, :p.numel()] for m, p in zip(api.adamw_moments(s["state"]), s["params"])]
         return {"params": s["params"], "masters": s["masters"], "moments": moments}
     r = api.token_logprobs(s["logits"], s["targets"], top=case["top"], entropy=case["entropy"])
     outs = [t.detach() for t in r if t is not None]

@@ -533,7 +533,7 @@ typedef struct aclsparseAdamWOptions_t {
 
 /* m = beta1 m + (1 - beta1) g, v = beta2 v + (1 - beta2) g^2, p = p (1 - lr weightDecay) - lr / (1 - beta1^t) * m /
  * (sqrt(v) / sqrt(1 - beta2^t) + eps) for every tensor, t the steps taken with this one.  tensors and options are host
- * memory, read before the call returns.  No two tensors share memory.  Under the root v counts as 2^-126 at least.
+ * memory, read before the call returns.  No two tensors share memory.  Under the root a number v counts as 2^-126 at least.
  * 8-bit moments: blocks of 32 values with the exponent f of the largest (its fp32 exponent field); a code c of magnitude
  * bits stands for (c / 8) 2^(l + f - 127) below 8 and (1 + (c & 7) / 8) 2^((c >> 3) - 1 + l + f - 127) from there on,
  * l = -13 for the first moment's seven bits below the sign, l = -29 for the second's eight.  They are rounded up or down

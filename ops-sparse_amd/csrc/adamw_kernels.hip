@@ -87,10 +87,13 @@ static_assert(sizeof(Factors) <= kAdamWBufferBytes, "");
 // size * m / (sqrt(v) / root + eps), to 11 roundings: the square root and the
 // reciprocal are the instructions' (one unit in the last place each).  They
 // take no subnormal numbers, so v is at least the least normal one: its root is
-// under 2^-62, which an eps of 1e-8 does not see.
+// under 2^-62, which an eps of 1e-8 does not see.  By a comparison, which NaN
+// passes: the larger of NaN and a number would be the number, and the change
+// m / eps.
 __device__ __forceinline__ float Change(const Factors& f, float m, float v)
 {
-    const float root = __builtin_amdgcn_sqrtf(fmaxf(v, 1.17549435e-38f));
+    constexpr float kLeast = 1.17549435e-38f;
+    const float root = __builtin_amdgcn_sqrtf(v < kLeast ? kLeast : v);
     return f.size * (m * __builtin_amdgcn_rcpf(root * f.inverse_root + f.eps));
 }
 

@@ -354,3 +354,22 @@ def test_random_numbers_by_given_factors(dev, monkeypatch):
     steps(params, grads, state, 2)  # the library's own
     monkeypatch.setitem(globals(), "mix", other)
     steps(params, grads, state._replace(factors=(first, second)), 2)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_step_after_a_second_moment_that_is_not_finite(dev, bits):
+    # one gradient's square is infinite: 8-bit moments make a NaN of v's whole block, under an m that stays finite, and
+    # with it of the block's values from the next step on
+    params, grads = tensors([(256,), (40,)], F32)
+    state = adamw_state(params, bits=bits)
+    plain = [Plain(p, state, i) for i, p in enumerate(params)]
+    for k in range(3):
+        g = grads(k)
+        if k == 0:
+            g[0][200] = 3e38
+        adamw_step(params, g, state, **HYPER)
+        for i, one in enumerate(plain):
+            one.step(g[i], k + 1, **HYPER)
+            one.check(params[i], state, i)
+    bad = torch.isnan(params[0]).view(8, 32).all(1) if bits == 8 else torch.isnan(params[0])
+    assert bad.nonzero().flatten().tolist() == ([6] if bits == 8 else []) and not torch.isnan(params[1]).any()

@@ -83,17 +83,19 @@ __device__ __forceinline__ Part WavePart(Part p)
 
 // A logit as an unsigned key of the same order, NaN above all, and with the
 // index behind it, the lower the greater: what comes first is the larger number.
+// No pair has all bits set, which stands for what is before the first.
+constexpr uint32_t kKeyNan = 0xFFFFFFFEU;
 __device__ __forceinline__ uint32_t OrderKey(float v)
 {
-    if (v != v) return 0xFFFFFFFFU;
+    if (v != v) return kKeyNan;
     const uint32_t u = __float_as_uint(v + 0.0f);
     return u ^ ((u >> 31) ? 0xFFFFFFFFU : 0x80000000U);
 }
 constexpr uint32_t kKeyMinusInf = 0x007FFFFFU;
 __device__ __forceinline__ float KeyValue(uint32_t key)
 {
-    return key == 0xFFFFFFFFU ? __uint_as_float(0x7FC00000U)
-                              : __uint_as_float(key ^ ((key >> 31) ? 0x80000000U : 0xFFFFFFFFU));
+    return key == kKeyNan ? __uint_as_float(0x7FC00000U)
+                          : __uint_as_float(key ^ ((key >> 31) ? 0x80000000U : 0xFFFFFFFFU));
 }
 __device__ __forceinline__ uint64_t Pair(float v, int32_t index)
 {

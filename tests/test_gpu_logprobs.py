@@ -430,3 +430,21 @@ def test_offsets_past_32_bits(dev):
     check(r.logprobs[-2:], lp, error(x))
     assert torch.equal(r.top_ids[-1].long(), torch.sort(x[-1].float(), descending=True, stable=True).indices[:2])
     assert r.top_ids[-2].tolist() == [0, 1]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("t,v", [(1, 1), (1, 40), (3, 9000), (1, 70000), (2, 131072), (600, 9000), (1200, 500)])
+def test_nan_in_the_first_places(dev, t, v, dtype):
+    # NaN is the largest, the lowest id first: in the first column, in all, and at the ends of segments and threads' units
+    k = min(v, 6)
+    x = rows(t, v, dtype, 60)
+    places = sorted({p for p in (0, 1, 7, 8, 2047, 2048, v // 2, v - 1) if p < v})
+    targets = torch.zeros(t, dtype=torch.int64, device=dev)
+    for named in ([0], places[-1:], places, slice(None)):
+        y = x.clone()
+        y[0, named] = float("nan")
+        r = token_logprobs(y, targets, top=k, entropy=True)
+        check_top(type(r)(*(o[:1] for o in r)), y[:1], k)
+        assert torch.isnan(r.logprobs[0]) and torch.isnan(r.entropy[0]) and torch.isnan(r.top_logprobs[0]).all()
+        if t > 1:
+            check_top(type(r)(*(o[-1:] for o in r)), y[-1:], k)

@@ -44,6 +44,10 @@ struct Mx4Launch {
     aclDataType c_type;
 };
 int LaunchGroupedMMMx4(const Mx4Launch& l, void* stream);
+// The kernel that multiplies operands of these sizes on a chip of so many CUs: few rows of each group, 16 or 32 at a time
+// (and 16 columns, or 32), tiles of 256x256, or of 64x128 with one team of waves or three.
+enum class Mx4Kernel : int { kRows16, kRows32, kRows32x2, kTiles, kSmallTiles, kSmallTilesTeams };
+Mx4Kernel Mx4KernelOf(int64_t groups, int64_t rows, int64_t n, int64_t blocks, int64_t cus);
 
 // ---- AdamW
 // The tensors of one launch, passed by value: a kernel's arguments hold so many.

@@ -644,37 +644,18 @@ int LaunchMx4Rows(const Mx4Launch& l, hipStream_t s)
     return 0;
 }
 
-// The times beside the rules are microseconds with weights that no cache holds.
 template <typename TOut>
 int Mx4BySize(const Mx4Launch& l, hipStream_t s)
 {
-    const int64_t cus = 8 * CusPerDie();
-    auto tiles = [&](int64_t height, int64_t width) {  // about as many as there are
-        const int64_t most = l.rows / height + l.groups;
-        return (most < l.rows ? most : l.rows) * CeilDiv(l.n, width);
-    };
-    // Few rows, while the chip holds all workgroups at once, here / by 64x128 tiles: 4 groups of 4096x2048 with 1 row each
-    // 9.0 / 12.0, with 6 9.2 / 12.0; 8 of 4096x4096 with 1 21 / 20; 48 of 1000x1024 with 4 21 / 11.  One group of
-    // 4096x4096: 16 rows 9.1 (16 rows a time), 32 9.4 (32 a time; 11.1 with 16) / 17, 64 11.5 (32 by 32) / 17.
-    if (l.blocks <= INT32_MAX / 32) {
-        int rc = kTooLarge;
-        if (l.rows <= 16 * l.groups) {
-            if (tiles(16, 16) <= 4 * cus) rc = LaunchMx4Rows<TOut, 1, 1>(l, s);
-        } else if (l.rows <= 32 * l.groups) {
-            if (tiles(32, 16) <= 2 * cus) rc = LaunchMx4Rows<TOut, 2, 1>(l, s);
-        } else if (l.rows <= 64 * l.groups) {
-            if (tiles(32, 32) <= 2 * cus) rc = LaunchMx4Rows<TOut, 2, 2>(l, s);
-        }
-        if (rc != kTooLarge) return rc;  // wider tiles may still fit
+    switch (Mx4KernelOf(l.groups, l.rows, l.n, l.blocks, 8 * CusPerDie())) {
+        case Mx4Kernel::kRows16: return LaunchMx4Rows<TOut, 1, 1>(l, s);
+        case Mx4Kernel::kRows32: return LaunchMx4Rows<TOut, 2, 1>(l, s);
+        case Mx4Kernel::kRows32x2: return LaunchMx4Rows<TOut, 2, 2>(l, s);
+        case Mx4Kernel::kTiles: return LaunchMx4Tiles<TOut>(l, s);
+        case Mx4Kernel::kSmallTiles: return LaunchMx4SmallTiles<TOut, 1>(l, s);
+        case Mx4Kernel::kSmallTilesTeams: return LaunchMx4SmallTiles<TOut, 3>(l, s);
     }
-    // 256x256 tiles / 64x128 ones: 64 groups of 2048x2048 with 64 rows each 39 / 38, with 96 44 / 50; 32 with 128 25 / 32;
-    // 1 group of 4096x4096 with 1024 rows 26 / 24, with 1536 29 / 29, with 2048 31 / 47
-    const int64_t smallTiles = (CeilDiv(l.rows, 64) + (l.groups - 1) / 2) * CeilDiv(l.n, 128);
-    if (l.rows >= 96 * l.groups && smallTiles > 3 * cus) return LaunchMx4Tiles<TOut>(l, s);
-    // three teams a tile / one: 512 rows x 4096 x 4096 18 / 21, x 2048 12 / 11; 768 rows x 4096 x 4096 29 / 23; 8 groups of
-    // 4096x4096 with 4 rows 20 / 22
-    const bool teams = smallTiles <= cus && l.blocks >= 8 * 12;
-    return teams ? LaunchMx4SmallTiles<TOut, 3>(l, s) : LaunchMx4SmallTiles<TOut, 1>(l, s);
+    return kTooLarge;
 }
 
 // Launches of fewer than 2^31 threads each, so that a thread's number and its row's fit 32 bits.
@@ -698,6 +679,34 @@ int ByRows(const Mx4Rows& l, int64_t elementBytes, F launch)
 }
 
 }  // namespace
+
+// The times beside the rules are microseconds with weights that no cache holds.
+Mx4Kernel Mx4KernelOf(int64_t groups, int64_t rows, int64_t n, int64_t blocks, int64_t cus)
+{
+    auto tiles = [&](int64_t height, int64_t width) {  // about as many as there are
+        const int64_t most = rows / height + groups;
+        return (most < rows ? most : rows) * CeilDiv(n, width);
+    };
+    // Few rows, while the chip holds all workgroups at once, here / by 64x128 tiles: 4 groups of 4096x2048 with 1 row each
+    // 9.0 / 12.0, with 6 9.2 / 12.0; 8 of 4096x4096 with 1 21 / 20; 48 of 1000x1024 with 4 21 / 11.  One group of
+    // 4096x4096: 16 rows 9.1 (16 rows a time), 32 9.4 (32 a time; 11.1 with 16) / 17, 64 11.5 (32 by 32) / 17.
+    if (blocks <= INT32_MAX / 32) {
+        if (rows <= 16 * groups) {
+            if (tiles(16, 16) <= 4 * cus) return Mx4Kernel::kRows16;
+        } else if (rows <= 32 * groups) {
+            if (tiles(32, 16) <= 2 * cus) return Mx4Kernel::kRows32;
+        } else if (rows <= 64 * groups) {
+            if (tiles(32, 32) <= 2 * cus) return Mx4Kernel::kRows32x2;
+        }
+    }
+    // 256x256 tiles / 64x128 ones: 64 groups of 2048x2048 with 64 rows each 39 / 38, with 96 44 / 50; 32 with 128 25 / 32;
+    // 1 group of 4096x4096 with 1024 rows 26 / 24, with 1536 29 / 29, with 2048 31 / 47
+    const int64_t smallTiles = (CeilDiv(rows, 64) + (groups - 1) / 2) * CeilDiv(n, 128);
+    if (rows >= 96 * groups && smallTiles > 3 * cus) return Mx4Kernel::kTiles;
+    // three teams a tile / one: 512 rows x 4096 x 4096 18 / 21, x 2048 12 / 11; 768 rows x 4096 x 4096 29 / 23; 8 groups of
+    // 4096x4096 with 4 rows 20 / 22
+    return smallTiles <= cus && blocks >= 8 * 12 ? Mx4Kernel::kSmallTilesTeams : Mx4Kernel::kSmallTiles;
+}
 
 int LaunchMx4Quantize(const Mx4Rows& l, void* stream)
 {

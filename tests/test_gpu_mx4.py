@@ -281,3 +281,93 @@ def test_serving_in_a_graph_on_another_stream(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, serve())
+
+
+# Shapes by the kernel that they reach on a chip of 256 CUs; test_model_ops_abi.py looks that they do.
+KERNELS = ("16 rows", "32 rows", "32 rows by 32", "256x256", "64x128", "64x128 by teams")
+REACHED = [  # kernel, groups' lengths, n, k
+    ("16 rows", [5, 0, 1, 16], 70, 200), ("32 rows", [31, 20], 50, 1100), ("32 rows by 32", [64, 0, 70], 100, 500),
+    ("64x128", [130, 20], 300, 2300), ("64x128", [70, 130, 65], 257, 500), ("64x128", [700, 900], 520, 96),
+    ("64x128 by teams", [130, 20], 300, 3200), ("64x128 by teams", [200, 0, 100, 65], 520, 4001),
+    ("64x128 by teams", [300], 130, 8200),
+    # tiles' last rows of any number, halves of tiles in a die's last round
+    ("256x256", [3300], 2048, 288), ("256x256", [2500, 0, 700, 1300], 2200, 520), ("256x256", [3000, 65], 2100, 2000),
+    # whole tiles in the last round, and last tiles of 64, 128, 129, 1 and 130 rows; rows of fewer than 16 blocks
+    ("256x256", [1088, 2176, 1153, 2049, 1154], 1100, 96), ("256x256", [5250], 2200, 512),
+    # a die's last round in quarters
+    ("256x256", [256 * 33], 2048, 64), ("256x256", [256 * 16, 256 * 17 - 40], 2041, 545),
+]
+
+
+def no_expert(lens, head, tail):
+    """Offsets with `head` rows before the first group and `tail` behind the last, and the number of rows."""
+    offsets = torch.tensor(np.concatenate([[0], np.cumsum(lens)]) + head, dtype=torch.int32, device="cuda")
+    return offsets, int(offsets[-1]) + tail
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("kernel,lens,n,k", REACHED)
+def test_products_of_each_kernel(dev, kernel, lens, n, k, dtype):
+    offsets, rows = no_expert(lens, 0, 0)
+    a, w = rows_of(rows, k, 30), rows_of(n, k, 31, (len(lens),))
+    check(grouped_mm_mx4(a, w, ExpertPlan(offsets), out_dtype=dtype), a, w, offsets, None, dtype)
+
+
+NO_EXPERT = [("256x256", [1500, 2000], 2100, 320), ("64x128 by teams", [130, 90], 520, 3300),
+             ("64x128", [130, 90], 520, 330), ("32 rows by 32", [64, 0, 70], 100, 500)]
+
+
+@pytest.mark.parametrize("kernel,lens,n,k", NO_EXPERT)
+def test_rows_of_no_expert_in_each_kernel(dev, kernel, lens, n, k):
+    offsets, rows = no_expert(lens, 5, 9)
+    a, w = rows_of(rows, k, 32), rows_of(n, k, 33, (len(lens),))
+    torch.full((rows, n), float("nan"), device=dev)  # what memory holds
+    y = grouped_mm_mx4(a, w, ExpertPlan(offsets), out_dtype=F32)
+    check(y, a, w, offsets, None, F32)
+    assert not y[:5].any() and not y[-9:].any()
+
+
+GATHERED = [("256x256", 4000, 4, 2, 1100, 300), ("64x128 by teams", 300, 4, 2, 300, 3300)]
+
+
+@pytest.mark.parametrize("kernel,tokens,experts,chosen,n,k", GATHERED)
+def test_gathered_products_of_tiles(dev, kernel, tokens, experts, chosen, n, k):
+    ids = torch.argsort(torch.rand(tokens, experts, generator=gen(34), device=dev), dim=1)[:, :chosen].to(torch.int32)
+    plan = expert_plan(ids, experts)
+    a, w = rows_of(tokens, k, 35), rows_of(n, k, 36, (experts,))
+    check(grouped_mm_mx4(a, w, plan, gather=True), a, w, plan.offsets, plan.tokens, BF16)
+
+
+@pytest.mark.parametrize("k", [290, 520])
+def test_strides_and_nan_in_large_tiles(dev, k):
+    # blocks inside longer rows, groups apart, scales at odd places
+    rows, n, blocks = 3300, 2048, (k + 31) // 32
+    a, w = rows_of(rows, k + 96, 37), rows_of(n + 3, k + 96, 38, (4,))
+    pa = MX4(a.codes[:, 16:16 + 16 * blocks], a.scales[:, 1:1 + blocks])
+    pw = MX4(w.codes[1::2, 2:-1, 16:16 + 16 * blocks], w.scales[1::2, 2:-1, 1:1 + blocks])
+    plan = ExpertPlan(torch.tensor([0, 1100, rows], dtype=torch.int32, device=dev))
+    want = grouped_mm_mx4(MX4(*(t.contiguous() for t in pa)), MX4(*(t.contiguous() for t in pw)), plan, out_dtype=F32)
+    check(want, pa, pw, plan.offsets, None, F32)
+    assert torch.equal(grouped_mm_mx4(pa, pw, plan, out_dtype=F32), want)
+    # one block of a row of each, the last one cut by the width; what lies beside the rows counts nothing
+    a.scales.fill_(255)
+    w.scales.fill_(255)
+    pa.scales.copy_(MX4(*rows_of(rows, k, 39)).scales)
+    pw.scales.copy_(MX4(*rows_of(n, k, 40, (2,))).scales)
+    clean = grouped_mm_mx4(pa, pw, plan, out_dtype=F32)
+    check(clean, pa, pw, plan.offsets, None, F32)
+    pa.scales[1, 2], pw.scales[0, 7, blocks - 1] = 255, 255
+    y = grouped_mm_mx4(pa, pw, plan, out_dtype=F32)
+    bad = torch.zeros_like(y, dtype=torch.bool)
+    bad[1], bad[:1100, 7] = True, True
+    assert torch.equal(torch.isnan(y), bad) and torch.equal(y[~bad], clean[~bad])
+
+
+def test_offsets_and_indices_without_meaning_in_large_tiles(dev):
+    rows = 3400
+    a, w = rows_of(rows, 300, 41), rows_of(2048, 300, 42, (3,))
+    for offsets in ([0, -5, 9000, 3], [900, 1, 2, 2**31 - 1], [-2**31, 2**31 - 1, -1, 700], [rows, 0, rows, 0]):
+        index = torch.randint(-2**31, 2**31 - 1, (rows,), generator=gen(43), device=dev).to(torch.int32)
+        plan = ExpertPlan(torch.tensor(offsets, dtype=torch.int32, device=dev), index)
+        assert grouped_mm_mx4(a, w, plan, gather=True).shape == (rows, 2048)
+    torch.cuda.synchronize()

@@ -313,3 +313,25 @@ def test_factors_are_odd_numbers_of_32_bits(lib, handle):
             ops_sparse.adamw_step(p, p, state._replace(factors=factors), 1e-3)
     with pytest.raises(ValueError, match="ROCm device"):
         ops_sparse.adamw_step(p, p, state._replace(factors=(3, 5)), 1e-3)
+
+
+def test_which_kernel_multiplies(lib):
+    # the rule of the 4-bit products, an internal function of the library, for the shapes that the GPU tests name
+    import test_gpu_mx4 as gpu
+
+    rule = getattr(lib, "_ZN5aclsp11Mx4KernelOfElllll")
+    rule.argtypes, rule.restype = [ctypes.c_int64] * 5, ctypes.c_int
+
+    def kernel(groups, rows, n, k):
+        return gpu.KERNELS[rule(groups, rows, n, (k + 31) // 32, 256)]
+
+    for name, lens, n, k in gpu.REACHED:
+        assert kernel(len(lens), sum(lens), n, k) == name, (lens, n, k)
+    assert {c[0] for c in gpu.REACHED} == set(gpu.KERNELS)
+    for name, lens, n, k in gpu.NO_EXPERT:
+        assert kernel(len(lens), sum(lens) + 14, n, k) == name, (lens, n, k)
+    for name, tokens, experts, chosen, n, k in gpu.GATHERED:
+        assert kernel(experts, tokens * chosen, n, k) == name, (tokens, n, k)
+    assert kernel(2, 3300, 2048, 290) == kernel(2, 3300, 2048, 520) == kernel(3, 3400, 2048, 300) == "256x256"
+    # and those that the first tests took for large tiles reach the small ones
+    assert kernel(1, 2500, 2048, 288) == kernel(4, 2900, 700, 520) == "64x128"

@@ -13,6 +13,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "experts_device.h"
 #include "model_ops_internal.h"
@@ -158,14 +159,14 @@ __device__ __forceinline__ void Load(const T* from, int64_t left, float (&v)[V])
         for (int i = 0; i < V; ++i) v[i] = i < left ? ToFloat(from[i]) : 0.0f;
     }
 }
-template <typename T, int V>
+template <bool kStream, typename T, int V>
 __device__ __forceinline__ void Store(T* to, int64_t left, const float (&v)[V])
 {
     T t[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) t[i] = FromFloat<T>(v[i]);
     if (left >= V) {
-        StoreStreaming<sizeof(t)>(to, t);
+        StoreStreaming<sizeof(t), kStream>(to, t);
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -173,6 +174,12 @@ __device__ __forceinline__ void Store(T* to, int64_t left, const float (&v)[V])
         }
     }
 }
+
+// Launches of more chunks store their results past the L2.  Small ones are soon read again, and storing them takes as long
+// either way: a step and the next read of its bf16 parameters, past the L2 / by ordinary stores, 2^18 values with 8-bit
+// moments 8.6 / 8.4 us, 2^19 9.1 / 8.9, 2^20 10.8 / 10.8, 2^22 (32 bits) 31.3 / 34.0; moments' values 2^12 4.3 / 4.0,
+// 2^18 5.6 / 5.4, 2^20 10.6 / 10.8.
+constexpr uint32_t kOrdinaryChunks = 256;
 
 // V codes from one or two words
 template <int kLeast, bool kSigned, int V>
@@ -231,7 +238,7 @@ __device__ __forceinline__ void Pack(const float (&v)[8], const uint32_t (&rando
 // ones, so a quad a block, otherwise four in each half.  The chunks of all
 // tensors are numbered in one row, and each wave finds a chunk's tensor by one
 // comparison per lane.
-template <typename TP, typename TG, int kBits, bool kMaster>
+template <typename TP, typename TG, int kBits, bool kMaster, bool kStream>
 __global__ __launch_bounds__(kThreads) void AdamWKernel(AdamWTable table, const Factors* __restrict__ factors)
 {
 #pragma clang fp contract(off)
@@ -295,15 +302,16 @@ __global__ __launch_bounds__(kThreads) void AdamWKernel(AdamWTable table, const 
             Pack<kLeastV, false>(v[u], random, codes + padded, t.exponents + (padded + at) / 32);
         } else {
             float* held = static_cast<float*>(t.moments) + at;
-            Store(held, left, m[u]);
-            Store(held + padded, left, v[u]);
+            Store<kStream>(held, left, m[u]);
+            Store<kStream>(held + padded, left, v[u]);
         }
-        if constexpr (kMaster) Store(t.master + at, left, p[u]);
-        Store(static_cast<TP*>(t.param) + at, left, p[u]);
+        if constexpr (kMaster) Store<kStream>(t.master + at, left, p[u]);
+        Store<kStream>(static_cast<TP*>(t.param) + at, left, p[u]);
     }
 }
 
 // Four codes per thread, so that neighbouring lanes write neighbouring places.
+template <bool kStream>
 __global__ __launch_bounds__(kThreads) void AdamWMomentsKernel(AdamWTable table)
 {
     const uint32_t first = table.first[threadIdx.x & 63], chunk = blockIdx.x;
@@ -320,20 +328,28 @@ __global__ __launch_bounds__(kThreads) void AdamWMomentsKernel(AdamWTable table)
         float m[4], v[4];
         Unpack<kLeastM, true>(codes + at, t.exponents[at / 32], m);
         Unpack<kLeastV, false>(codes + padded + at, t.exponents[(padded + at) / 32], v);
-        Store(t.master + at, left, m);
-        Store(t.master + t.count + at, left, v);
+        Store<kStream>(t.master + at, left, m);
+        Store<kStream>(t.master + t.count + at, left, v);
     }
 }
 
 template <typename TP, typename TG>
 void Launch(const AdamWTable& t, const Factors* s, int bits, bool master, hipStream_t stream)
 {
+    auto launch = [&](auto eight, auto kept) {
+        constexpr int kBits = decltype(eight)::value ? 8 : 32;
+        constexpr bool kMaster = decltype(kept)::value;
+        if (t.chunks > kOrdinaryChunks) AdamWKernel<TP, TG, kBits, kMaster, true><<<t.chunks, kThreads, 0, stream>>>(t, s);
+        else AdamWKernel<TP, TG, kBits, kMaster, false><<<t.chunks, kThreads, 0, stream>>>(t, s);
+    };
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
     if (bits == 8) {
-        if (master) AdamWKernel<TP, TG, 8, true><<<t.chunks, kThreads, 0, stream>>>(t, s);
-        else AdamWKernel<TP, TG, 8, false><<<t.chunks, kThreads, 0, stream>>>(t, s);
+        if (master) launch(yes, yes);
+        else launch(yes, no);
     } else {
-        if (master) AdamWKernel<TP, TG, 32, true><<<t.chunks, kThreads, 0, stream>>>(t, s);
-        else AdamWKernel<TP, TG, 32, false><<<t.chunks, kThreads, 0, stream>>>(t, s);
+        if (master) launch(no, yes);
+        else launch(no, no);
     }
 }
 
@@ -366,7 +382,9 @@ int LaunchAdamW(const AdamWTable& t, const void* buffer, aclDataType param, aclD
 
 int LaunchAdamWMoments(const AdamWTable& t, void* stream)
 {
-    AdamWMomentsKernel<<<t.chunks, kThreads, 0, static_cast<hipStream_t>(stream)>>>(t);
+    hipStream_t q = static_cast<hipStream_t>(stream);
+    if (t.chunks > kOrdinaryChunks) AdamWMomentsKernel<true><<<t.chunks, kThreads, 0, q>>>(t);
+    else AdamWMomentsKernel<false><<<t.chunks, kThreads, 0, q>>>(t);
     return 0;
 }
 

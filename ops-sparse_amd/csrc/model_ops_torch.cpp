@@ -79,8 +79,9 @@ Tensor Mx4Dequantize(const Tensor& codes, const Tensor& scales, const optional<i
     CheckMx4(codes, scales, "q");
     TORCH_CHECK_TYPE(IsFloat(type), "dtype must be float32, float16 or bfloat16, got ", type);
     const int64_t blocks = scales.size(-1), width = givenWidth.value_or(blocks * kBlock);
-    TORCH_CHECK_VALUE(width > (blocks - 1) * kBlock && width <= blocks * kBlock, "width must lie in (",
-                      (blocks - 1) * kBlock, ", ", blocks * kBlock, "], got ", width);
+    const int64_t least = std::max<int64_t>((blocks - 1) * kBlock + 1, 0);
+    TORCH_CHECK_VALUE(width >= least && width <= blocks * kBlock, "width must lie in [", least, ", ", blocks * kBlock,
+                      "], got ", width);
     OnGpu(codes);
     SameDevice(codes, scales, "q's scales");
     Tensor out = Empty(WithLast(codes, width), type, codes);

@@ -335,3 +335,11 @@ def test_which_kernel_multiplies(lib):
     assert kernel(2, 3300, 2048, 290) == kernel(2, 3300, 2048, 520) == kernel(3, 3400, 2048, 300) == "256x256"
     # and those that the first tests took for large tiles reach the small ones
     assert kernel(1, 2500, 2048, 288) == kernel(4, 2900, 700, 520) == "64x128"
+
+
+def test_width_of_rows_of_no_blocks():
+    for width in (-1, -31, 1):
+        with pytest.raises(ValueError, match="width"):
+            ops_sparse.mx4_dequantize(mx4(4, blocks=0), width)
+    with pytest.raises(ValueError, match="ROCm device"):
+        ops_sparse.mx4_dequantize(mx4(4, blocks=0), 0)

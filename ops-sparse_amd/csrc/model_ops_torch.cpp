@@ -5,6 +5,7 @@
 #include <torch/csrc/autograd/VariableTypeUtils.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 
+#include <algorithm>
 #include <unordered_set>
 
 #include "torch_common.h"
@@ -172,6 +173,27 @@ void CheckMoments(int64_t count, const Tensor& moments, const optional<Tensor>& 
     TORCH_CHECK_VALUE(reinterpret_cast<uintptr_t>(moments.data_ptr()) % 8 == 0, "moments must be aligned to 8 bytes");
 }
 
+// Memory that a step writes.  What two of a step's tensors share, they would write at once: the result would be any.
+struct Written {
+    uintptr_t begin, end;
+    const char* name;
+    size_t place;
+};
+void Add(std::vector<Written>& written, const Tensor& t, const char* name, size_t place)
+{
+    const auto begin = reinterpret_cast<uintptr_t>(t.data_ptr());
+    if (t.numel() > 0) written.push_back({begin, begin + t.nbytes(), name, place});
+}
+void CheckApart(std::vector<Written>& written)
+{
+    std::sort(written.begin(), written.end(), [](const Written& a, const Written& b) { return a.begin < b.begin; });
+    for (size_t i = 1; i < written.size(); ++i) {
+        const Written &a = written[i - 1], &b = written[i];
+        TORCH_CHECK_VALUE(a.end <= b.begin, "the ", a.name, " at ", a.place, " and the ", b.name, " at ", b.place,
+                          " share memory: no tensor may be there twice");
+    }
+}
+
 void AdamWStep(const Tensors& params, const MaybeTensors& grads, const Tensors& moments,
                const optional<Tensors>& exponents, const optional<Tensors>& masters, const Tensor& step, int64_t seed,
                double lr, const optional<Tensor>& lrTensor, double beta1, double beta2, double eps, double weightDecay,
@@ -197,7 +219,8 @@ void AdamWStep(const Tensors& params, const MaybeTensors& grads, const Tensors& 
     OneFloat(step, gradScale, "grad_scale");
     std::vector<aclsparseAdamWTensor_t> table(count);
     std::vector<Tensor> kept;  // gradients that had to be copied
-    std::unordered_set<void*> seen;
+    std::vector<Written> written;
+    written.reserve(count * 4);
     for (size_t i = 0; i < count; ++i) {
         const Tensor& p = params[i];
         TORCH_CHECK_TYPE(IsFloat(p.scalar_type()), "params must be float32, float16 or bfloat16, got ",
@@ -215,8 +238,12 @@ void AdamWStep(const Tensors& params, const MaybeTensors& grads, const Tensors& 
                               "masters must be contiguous and of their params' shapes, the one at ", i, " is not");
             SameDevice(step, m, "masters");
             master = Floats(m);
+            // a parameter in fp32 may be its own master
+            if (p.scalar_type() != at::kFloat || master != Data(p)) Add(written, m, "master", i);
         }
-        TORCH_CHECK_VALUE(n == 0 || seen.insert(p.data_ptr()).second, "the param at ", i, " is there twice");
+        Add(written, p, "param", i);
+        Add(written, moments[i], "moments", i);
+        if (exponents.has_value()) Add(written, (*exponents)[i], "exponents", i);
         Tensor g;
         if (grads[i].has_value() && grads[i]->defined()) {
             TORCH_CHECK_TYPE(IsFloat(grads[i]->scalar_type()), "grads must be float32, float16 or bfloat16, got ",
@@ -231,6 +258,7 @@ void AdamWStep(const Tensors& params, const MaybeTensors& grads, const Tensors& 
                     exponents.has_value() ? Bytes((*exponents)[i]) : nullptr, n, TypeOf(p.scalar_type()),
                     g.defined() ? TypeOf(g.scalar_type()) : ACL_FLOAT};
     }
+    CheckApart(written);
     aclsparseAdamWOptions_t o{};
     o.lr = lr;
     o.beta1 = beta1;

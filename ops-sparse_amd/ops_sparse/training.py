@@ -84,7 +84,8 @@ def adamw_step(params, grads, state, lr, betas=(0.9, 0.999), eps=1e-8, weight_de
     params: contiguous, fp32, fp16 or bf16; grads: of their shapes and any of these types, None for a tensor that is left
     as it is; lr: a number, or a tensor of one fp32 on the device; grad_scale: a tensor of one fp32 on the device that all
     gradients are multiplied by (clipping by a norm).  The steps are counted on the device, so that a captured step counts
-    with each replay.  With masters in the state the step goes by them and the parameters get them rounded.
+    with each replay.  With masters in the state the step goes by them and the parameters get them rounded.  Tensors that
+    a step writes share no memory (but a parameter in fp32 may be its own master).
     """
     tensor = lr if isinstance(lr, torch.Tensor) else None
     (experts._MODULE or _module()).adamw_step(list(params), list(grads), state.moments, state.exponents, state.masters,

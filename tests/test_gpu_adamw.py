@@ -373,3 +373,37 @@ def test_a_step_after_a_second_moment_that_is_not_finite(dev, bits):
             one.check(params[i], state, i)
     bad = torch.isnan(params[0]).view(8, 32).all(1) if bits == 8 else torch.isnan(params[0])
     assert bad.nonzero().flatten().tolist() == ([6] if bits == 8 else []) and not torch.isnan(params[1]).any()
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_tensors_that_share_memory_are_refused(dev, bits):
+    base = torch.randn(300, generator=gen(8), device=dev)
+    params = [base[:100], base[100:200], base[200:].to(BF16)]
+    grads = [torch.ones_like(p) for p in params]
+    state = adamw_state(params, bits=bits)
+    before = [t.clone() for t in params + state.moments + state.masters]
+
+    def refused(p, s):
+        with pytest.raises(ValueError, match="share memory"):
+            adamw_step(p, grads, s, 1e-3)
+
+    def twice(list_):
+        return [list_[0], list_[0], list_[2]]
+
+    refused([params[0], params[0], params[2]], state)
+    refused([params[0], base[99:199], params[2]], state)
+    refused(params, state._replace(moments=twice(state.moments)))
+    refused(params, state._replace(masters=twice(state.masters)))
+    refused(params, state._replace(masters=[state.masters[0], base[:100], state.masters[2]]))
+    if bits == 8:
+        refused(params, state._replace(exponents=twice(state.exponents)))
+    assert all(torch.equal(a, b) for a, b in zip(before, params + state.moments + state.masters))
+    assert state.step.tolist() == [0, 0]
+    # a parameter in fp32 that is its own master, neighbours in one tensor, a shared gradient
+    own = state._replace(masters=[params[0], params[1], state.masters[2]])
+    shared = [grads[0], grads[0], grads[2]]
+    plain = [Plain(p, own, i) for i, p in enumerate(params)]
+    adamw_step(params, shared, own, **HYPER)
+    for i, one in enumerate(plain):
+        one.step(shared[i], 1, **HYPER)
+        one.check(params[i], own, i)

@@ -566,7 +566,7 @@ aclsparseStatus_t aclsparseTokenLogprobs(aclsparseHandle_t handle, int64_t rows,
                                          int64_t top, float* topLogprobs, int32_t* topIds, void* buffer);
 /* Gradient with respect to the logits, in their type: of the log probabilities, the entropies and the alternatives' log
  * probabilities, each null for none.  stats, entropy and topIds are aclsparseTokenLogprobs's.  A row of nothing but -inf
- * has the gradient 0. */
+ * has the gradient 0.  gradLogits may be logits, with ldGrad = ldLogits. */
 aclsparseStatus_t aclsparseTokenLogprobsGrad(aclsparseHandle_t handle, int64_t rows, int64_t vocab, const void* logits,
                                              int64_t ldLogits, aclDataType logitsType, const void* targets,
                                              aclDataType targetsType, const float* stats, const float* entropy,

@@ -505,8 +505,9 @@ __global__ __launch_bounds__(kThreads) void LogprobsJoinKernel(LogprobsLaunch p,
 
 constexpr int32_t kGradLength = kThreads * kUnit * kBatch;  // of a row that a workgroup takes
 
-// The gradient of one part of a row.  Columns that a token or an alternative
-// names are written again, after the others, with what they have besides.
+// The gradient of one part of a row, which may take the logits' place.  Columns
+// that a token or an alternative names are written again, after the others, with
+// what they have besides; their logits are read before any is written over.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void LogprobsGradKernel(LogprobsGradLaunch p, int32_t segments)
 {
@@ -521,6 +522,10 @@ __global__ __launch_bounds__(kThreads) void LogprobsGradKernel(LogprobsGradLaunc
     const T* logits = static_cast<const T*>(p.logits) + row * p.ld;
     T* grad = static_cast<T*>(p.grad) + row * p.ld_grad;
     const int tid = threadIdx.x;
+    T v[kBatch][kUnit];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) LoadUnit(logits, begin + (b * kThreads + tid) * kUnit, end, v[b]);
+    float mine = 0.0f;  // the logit of this thread's named column
     if (tid <= k) {
         int64_t c = -1;
         float g = 0.0f;
@@ -535,6 +540,7 @@ __global__ __launch_bounds__(kThreads) void LogprobsGradKernel(LogprobsGradLaunc
         const bool named = c >= 0 && c < vocab && p.stats[row * 2 + 1] != Infinity();
         column[tid] = named ? static_cast<int32_t>(c) : -1;
         weight[tid] = named ? g : 0.0f;
+        if (named && c >= begin && c < end) mine = ToFloat(logits[c]);
     }
     __syncthreads();
     float total = 0.0f;
@@ -546,9 +552,6 @@ __global__ __launch_bounds__(kThreads) void LogprobsGradKernel(LogprobsGradLaunc
         const float d = (x - m) - logs;
         return -Exp2(d * kLog2E) * (total + gh * (fmaxf(d, kFar) + h));
     };
-    T v[kBatch][kUnit];
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) LoadUnit(logits, begin + (b * kThreads + tid) * kUnit, end, v[b]);
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
         const int32_t c = begin + (b * kThreads + tid) * kUnit;
@@ -573,7 +576,7 @@ __global__ __launch_bounds__(kThreads) void LogprobsGradKernel(LogprobsGradLaunc
             if (i < tid) first = false;
             g += weight[i];
         }
-        if (first) grad[c] = FromFloat<T>(g + one(ToFloat(logits[c])));
+        if (first) grad[c] = FromFloat<T>(g + one(mine));
     }
 }
 

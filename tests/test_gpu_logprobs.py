@@ -4,11 +4,14 @@ Tolerances: an exponential is off by a few units in the last place of its argume
 logit d below the largest; the sum of V of them by V / 256 + 16 roundings of 2^-24 (each of 256 threads adds its own), and
 the logarithm passes the sum's relative error on as an absolute one.
 """
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 
-from ops_sparse import token_logprobs
+from ops_sparse import _lib, token_logprobs
+from ops_sparse._lib import DataType
 
 pytestmark = pytest.mark.gpu
 
@@ -448,3 +451,43 @@ def test_nan_in_the_first_places(dev, t, v, dtype):
         assert torch.isnan(r.logprobs[0]) and torch.isnan(r.entropy[0]) and torch.isnan(r.top_logprobs[0]).all()
         if t > 1:
             check_top(type(r)(*(o[-1:] for o in r)), y[-1:], k)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("t,v,k", [(1, 5, 3), (7, 20000, 20), (300, 8192, 64), (1200, 333, 0)])
+def test_a_gradient_in_the_place_of_its_logits(dev, t, v, k, dtype):
+    # the C entry point, whose caller may have no use for the logits any more; the torch one keeps them
+    lib, types = _lib.lib(), {F32: DataType.FLOAT, F16: DataType.FLOAT16, BF16: DataType.BF16}
+    logits, ld = rows(t, v + 3, dtype, 61), v + 3
+    targets = torch.randint(-1, v, (t,), generator=gen(62), device=dev)
+    x = logits[:, :v].clone().requires_grad_()
+    r = token_logprobs(x, targets, top=k, entropy=True)
+    gl, ge, gt = (torch.randn(*s, generator=gen(63 + i), device=dev) for i, s in enumerate(((t,), (t,), (t, max(k, 1)))))
+    outs, given = [r.logprobs, r.entropy], [gl, ge]
+    if k:
+        outs, given = outs + [r.top_logprobs], given + [gt]
+    want = torch.autograd.grad(outs, x, given)[0]
+    m = x.detach().float().max(1).values
+    stats = torch.stack([m, torch.log(torch.exp(x.detach().double() - m[:, None]).sum(1)).float()], 1).contiguous()
+    h = ctypes.c_void_p(0)
+    assert lib.aclsparseCreate(ctypes.byref(h)) == 0
+    assert lib.aclsparseSetStream(h, ctypes.c_void_p(_lib.HIP_NULL_STREAM)) == 0
+    entropy = r.entropy.detach().contiguous()
+    apart = torch.zeros_like(logits)
+
+    def run(out):
+        torch.cuda.synchronize()
+        assert lib.aclsparseTokenLogprobsGrad(
+            h, t, v, logits.data_ptr(), ld, int(types[dtype]), targets.data_ptr(), int(DataType.INT64), stats.data_ptr(),
+            entropy.data_ptr(), k, r.top_ids.data_ptr() if k else None, gl.data_ptr(), ge.data_ptr(),
+            gt.data_ptr() if k else None, out.data_ptr(), ld) == 0
+        torch.cuda.synchronize()
+
+    run(apart)
+    rest = logits[:, v:].clone()
+    run(logits)
+    lib.aclsparseDestroy(h)
+    assert torch.equal(logits[:, :v], apart[:, :v]) and torch.equal(logits[:, v:], rest)
+    # log S from 64 bits is the kernel's to its error, which p passes on
+    size = 2 * error(x) * (sum(g.abs().reshape(t, -1).sum(1) for g in given)[:, None].double() * 60 + 1)
+    assert bool(((apart[:, :v].double() - want.double()).abs() <= size + want.double().abs() * torch.finfo(dtype).eps).all())

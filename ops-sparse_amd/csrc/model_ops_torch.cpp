@@ -213,7 +213,7 @@ void AdamWStep(const Tensors& params, const MaybeTensors& grads, const Tensors& 
     TORCH_CHECK_VALUE(!factors.has_value() || (odd(factors->first) && odd(factors->second)),
                       "the factors must be odd and fit 32 bits without a sign");
     TORCH_CHECK_TYPE(step.scalar_type() == at::kInt, "step must be int32, got ", step.scalar_type());
-    TORCH_CHECK_VALUE(step.dim() == 1 && step.size(0) == 2 && step.is_contiguous(), "step must hold two counts");
+    TORCH_CHECK_VALUE(step.dim() == 1 && step.size(0) >= 1, "step must be one-dimensional and hold the steps taken");
     OnGpu(step);
     OneFloat(step, lrTensor, "lr");
     OneFloat(step, gradScale, "grad_scale");

@@ -46,9 +46,9 @@ class AdamWState(NamedTuple):
 
     moments: [2, P] with P = n rounded up to 32, the first moment and the second one, fp32 or uint8 codes; exponents:
     [2, P / 32] uint8 for the codes, None for fp32; masters: the values in fp32, None where the parameters themselves
-    are kept; step: int32 [2], the steps taken and a place that is not used; seed: of the rounding of 8-bit moments (32 bits);
-    factors: two odd numbers of 32 bits that the rounding's random numbers are made with, where 8-bit moments are to be
-    another program's bit by bit (include/cann_ops_sparse.h says how), None for the library's own.
+    are kept; step: int32 [1] or longer, the steps taken in its first place, others are not used; seed: of the rounding of
+    8-bit moments (32 bits); factors: two odd numbers of 32 bits that the rounding's random numbers are made with, where
+    8-bit moments are to be another program's bit by bit (include/cann_ops_sparse.h says how), None for the library's own.
     """
     moments: List[torch.Tensor]
     exponents: Optional[List[torch.Tensor]]

@@ -407,3 +407,16 @@ def test_tensors_that_share_memory_are_refused(dev, bits):
     for i, one in enumerate(plain):
         one.step(shared[i], 1, **HYPER)
         one.check(params[i], own, i)
+
+
+def test_a_step_of_one_count(dev):
+    params, grads = tensors([(100,)], F32)
+    state = adamw_state(params)._replace(step=torch.zeros(1, dtype=torch.int32, device=dev))
+    one = Plain(params[0], state, 0)
+    for k in range(2):
+        adamw_step(params, grads(k), state, **HYPER)
+        one.step(grads(k)[0], k + 1, **HYPER)
+        one.check(params[0], state, 0)
+    assert state.step.tolist() == [2]
+    with pytest.raises(ValueError, match="step"):
+        adamw_step(params, grads(0), state._replace(step=state.step[:0]), 1e-3)

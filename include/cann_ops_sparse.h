@@ -538,7 +538,8 @@ typedef struct aclsparseAdamWOptions_t {
  * bits stands for (c / 8) 2^(l + f - 127) below 8 and (1 + (c & 7) / 8) 2^((c >> 3) - 1 + l + f - 127) from there on,
  * l = -13 for the first moment's seven bits below the sign, l = -29 for the second's eight.  They are rounded up or down
  * at random, by numbers that seed, step, the tensor's place and the element's give, so that slow changes add up; the
- * parameters go by the moments before that.  A block that holds infinity or NaN becomes NaN. */
+ * parameters go by the moments before that.  A second moment that is not zero never becomes zero, under a first moment that
+ * may not be.  A block that holds infinity or NaN becomes NaN. */
 aclsparseStatus_t aclsparseAdamW(aclsparseHandle_t handle, int64_t count, const aclsparseAdamWTensor_t* tensors,
                                  const aclsparseAdamWOptions_t* options);
 /* The same with the factors of the rounding's random numbers, odd ones, for 8-bit moments that are to be another program's

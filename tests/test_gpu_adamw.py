@@ -420,3 +420,55 @@ def test_a_step_of_one_count(dev):
     assert state.step.tolist() == [2]
     with pytest.raises(ValueError, match="step"):
         adamw_step(params, grads(0), state._replace(step=state.step[:0]), 1e-3)
+
+
+@pytest.mark.parametrize("second", [0, 1])
+def test_roundings_are_to_a_neighbour_and_even_on_the_mean(dev, second):
+    # Moments that are the gradients themselves (or their squares): betas of 0.  Each block has the same 32 values, a large
+    # one beside ones down to under the format's least, of either sign; over many blocks each becomes one of the two codes'
+    # values beside it, and on the mean itself.  n roundings by up to a step s have a deviation of at most s / 2 / sqrt(n);
+    # five of them, and the 16 bits of a random number, are allowed.
+    g = np.concatenate([[1.9], 2.0 ** (-0.6 * np.arange(31))]).astype(np.float32) * np.float32(37.0)
+    g[1::3] *= -1
+    assert g.size == 32
+    n = 1 << 15  # blocks
+    p = [torch.zeros(32 * n, device=dev)]
+    state = adamw_state(p, bits=8, seed=11)
+    adamw_step(p, [torch.from_numpy(g).to(dev).repeat(n)], state, lr=0.0, betas=(0.0, 0.0))
+    got = adamw_moments(state)[0][second].double().view(n, 32).cpu().numpy()
+    want = (g * g if second else g).astype(np.float64)
+    # every value of the format under this block's exponent, from its definition
+    exponent = np.uint8((np.abs(want).max().astype(np.float32).view(np.uint32) >> 23) & 255)
+    codes = np.arange(256, dtype=np.uint8)
+    values = np.unique(decode(codes, np.full(8, exponent), second))
+    assert (state.exponents[0][second] == int(exponent)).all() and np.isin(got, values).all()
+    for j, x in enumerate(want):
+        below, above = values[values <= x].max(), values[values >= x].min()
+        if second and below == 0:  # v that is not zero never becomes zero
+            assert (got[:, j] == above).all()
+            continue
+        assert ((got[:, j] == below) | (got[:, j] == above)).all(), j
+        step = above - below
+        assert abs(got[:, j].mean() - x) <= step * (5 / 2 / n**0.5 + 2.0**-16), j
+        if step > 0 and abs(x - below) / step > 0.05 and abs(above - x) / step > 0.05:
+            assert (got[:, j] == below).any() and (got[:, j] == above).any()
+
+
+def test_the_moments_of_a_value_are_rounded_apart(dev):
+    # both moments half way between two codes: up or down independently, and so do neighbours
+    n = 1 << 16
+    p = [torch.zeros(n, device=dev)]
+    state = adamw_state(p, bits=8, seed=12)
+    grad = torch.full((n,), 1.0 + 1.0 / 16, device=dev)  # half way; its square, 1.12890625, is 0.03125 parts from it
+    adamw_step(p, [grad], state, lr=0.0, betas=(0.0, 0.0))
+    m, v = (x.cpu().numpy() for x in adamw_moments(state)[0])
+    assert set(np.unique(m)) == {1.0, 1.125} and set(np.unique(v)) == {1.125, 1.25}
+    up_m, up_v = (m == 1.125).astype(float), (v == 1.25).astype(float)
+    chance_v = (1.12890625 - 1.125) / 0.125
+    assert abs(up_m.mean() - 0.5) <= 5 * 0.5 / n**0.5
+    assert abs(up_v.mean() - chance_v) <= 5 * (chance_v * (1 - chance_v) / n) ** 0.5
+    # the covariance of independent ones has the deviation sqrt(var var / n)
+    both = ((up_m - 0.5) * (up_v - chance_v)).mean()
+    assert abs(both) <= 5 * 0.5 * (chance_v * (1 - chance_v)) ** 0.5 / n**0.5
+    for d in (1, 32, 2048):
+        assert abs(((up_m - 0.5) * (np.roll(up_m, d) - 0.5)).mean()) <= 5 * 0.25 / n**0.5

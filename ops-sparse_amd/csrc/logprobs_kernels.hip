@@ -9,7 +9,7 @@
 // S and W are moved to it.  With few rows several workgroups share one, and
 // another launch joins what they found.  Bound by memory: the logits are read
 // once, those of few threads a second time for alternatives.  8192 rows of 65536
-// bf16 logits with the entropy: 192 us (5.6 TB/s), their gradient 351 us (6.1
+// bf16 logits with the entropy: 192 us (5.6 TB/s), their gradient 358 us (6.0
 // TB/s read and written).  One row of 131072 with 20 alternatives, 64 segments:
 // 4.8 us and 4.8 to join them, latency alone; 37 rows of 32003 fp32 with 5, a
 // workgroup each: 7.5 us, its exponentials and what is around them.

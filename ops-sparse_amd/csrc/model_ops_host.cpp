@@ -324,6 +324,8 @@ aclsparseStatus_t aclsparseTokenLogprobsGrad(aclsparseHandle_t handle, int64_t r
         (gradEntropy != nullptr && entropy == nullptr) || (gradTop != nullptr && (topIds == nullptr || top == 0))) {
         return ACL_SPARSE_STATUS_INVALID_VALUE;
     }
+    // in the logits' place only row by row: other rows would be written over before they are read
+    if (gradLogits == logits && rows > 1 && ldGrad != ldLogits) return ACL_SPARSE_STATUS_INVALID_VALUE;
     const aclsp::LogprobsGradLaunch l{rows, vocab, top, logits, ldLogits, logitsType, targets,
                                       targetsType == ACL_INT64, stats, entropy, topIds, gradLogprobs, gradEntropy,
                                       gradTop, gradLogits, ldGrad};

@@ -343,3 +343,9 @@ def test_width_of_rows_of_no_blocks():
             ops_sparse.mx4_dequantize(mx4(4, blocks=0), width)
     with pytest.raises(ValueError, match="ROCm device"):
         ops_sparse.mx4_dequantize(mx4(4, blocks=0), 0)
+
+
+def test_a_gradient_in_the_logits_place_has_their_rows(lib, handle):
+    grad = lib.aclsparseTokenLogprobsGrad
+    assert grad(handle, *logprobs_grad(ldo=101)) == INVALID and grad(handle, *logprobs_grad(ld=101)) == INVALID
+    assert grad(handle, *logprobs_grad(ldo=101, rows=0)) == OK
